@@ -67,6 +67,18 @@ SIGNATURES = {
     "edf_layer_norm_backward_add": (I, [P, P, P, P, P, P, P, P, P, P, P, S, I, I, I, I]),
     "edf_heads_split": (I, [P, P, P, L, L, I, I, I, I]),
     "edf_heads_merge": (I, [P, P, P, L, L, I, I, I, I]),
+    "edf_heads_split_rotary": (I, [P, P, P, P, P, P, P, P, P, L, L, I, I, I, I, I, I, F, F, I]),
+    "edf_heads_split_rotary_backward_workspace_bytes": (S, [I]),
+    "edf_heads_split_rotary_backward": (
+        I, [P, P, P, P, P, P, P, P, P, P, P, P, P, S, L, L, I, I, I, I, I, I, F, F, I]),
+    "edf_window_attention": (I, [P, P, P, P, P, P, I, I, I, I, I, I, I, I]),
+    "edf_window_attention_backward_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
+    "edf_window_attention_backward": (
+        I, [P, P, P, P, P, P, P, P, P, P, P, S, I, I, I, I, I, I, I, I]),
+    "edf_paged_extend": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I]),
+    "edf_paged_cache_write": (I, [P, P, P, P, P, P, L, L, I, I, L, I, I]),
+    "edf_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
+    "edf_paged_attention": (I, [P, P, P, P, P, P, P, P, S, I, I, I, I, L, I, I, I, I, I]),
     "edf_embedding_backward_workspace_bytes": (S, [L, L]),
     "edf_embedding_backward": (I, [P, P, P, P, P, S, L, L, I, L, I]),
     "edf_softplus": (I, [P, P, P, L, I]),

@@ -1,0 +1,428 @@
+// Attention of one new token per request over a paged key / value cache, with shared key heads and an
+// optional window with sinks:
+//   o[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(d)) v_j,   key head h / G, G = Hq / Hkv query heads each,
+// over the keys j < len_b (window W > 0: j >= len_b - W or j < sinks), key j in page table[b][j / block].
+// Each key and value is read once for its G query heads: 2 Hkv len d elements a request, 4 G flops per
+// element pair, so the kernel is bound by memory up to about G = 60 in bf16.
+//
+// The visible keys are numbered through (sinks, then the window) and cut into chunks; a workgroup of four
+// waves takes one chunk of one key head, each wave tiles of 32 keys with an online softmax of its own:
+//   S^T [32 keys][16 queries] = K Q^T: MFMA 16x16x32, the K operand straight from its pages (a lane's 8
+//   elements of one key are contiguous), queries padded to 16 columns;
+//   O^T [d][16 queries] += V^T P^T: P^T is the S^T registers (a lane holds keys 4 g .. + 3 of both
+//   16-key halves), V^T comes from a wave-private LDS copy of the tile by transposed reads in that order.
+// A tile's keys and values are loaded into registers while the one before is computed; page numbers are
+// looked up one tile further ahead, one key per lane, and handed around the wave by shuffles.
+// The waves' results are joined in LDS; with more than one chunk the workgroup leaves (O, max, sum) in
+// float32 and a second kernel joins the chunks.
+// float32 runs the same way on the float32 matrix instructions (eight 16x16x4 per 32 elements).
+//
+// Scores, softmax and O are float32; in bf16 P is rounded to bf16 for the matrix product (2^-8 of each
+// term, as the attention of the prompt does), its sum is that of the unrounded values.
+// Keys of a page outside [0, num_blocks) are left out, and a request without keys answers with zeros.
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "edf_abi.hpp"
+#include "edf_common.hpp"
+#include "edf_mfma.hpp"
+
+namespace edf {
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_KEYS = 32;                    // keys per wave tile
+constexpr int PA_STEP = PA_WAVES * PA_KEYS;    // keys per workgroup step
+constexpr int PA_MAX_SPLITS = 256;
+
+struct PagedArgs {
+  const void *q, *kc, *vc;
+  const int *table, *len;
+  void* out;
+  float* part;  // [B Hq][splits][d] outputs, then [B Hq][splits][2] (max in log2 units, sum)
+  float* ml;
+  int B, Hq, Hkv, G, qt, d, width, block, window, sinks, splits, chunk;
+  long num_blocks;
+  float scale_log2;
+};
+
+// 8 consecutive elements of a row, the K / Q operand of one lane for 32 columns of the contraction
+template <typename T> struct Frag;
+template <> struct Frag<bf16> {
+  bf16x8 v;
+  EDF_DEVICE static f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+  }
+  EDF_DEVICE void set(int e, float x) { v[e] = (bf16)x; }
+  EDF_DEVICE void load(const bf16* p) { v = *(const bf16x8*)p; }
+  EDF_DEVICE void zero() { v = bf16x8{}; }
+  EDF_DEVICE void store(bf16* p) const { *(bf16x8*)p = v; }
+};
+template <> struct Frag<float> {
+  f32x4 lo, hi;
+  EDF_DEVICE static f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.lo[e], b.lo[e], c, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.hi[e], b.hi[e], c, 0, 0, 0);
+    return c;
+  }
+  EDF_DEVICE void set(int e, float x) {
+    if (e < 4) lo[e] = x;
+    else hi[e - 4] = x;
+  }
+  EDF_DEVICE void load(const float* p) {
+    lo = *(const f32x4*)p;
+    hi = *(const f32x4*)(p + 4);
+  }
+  EDF_DEVICE void zero() { lo = hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+  EDF_DEVICE void store(float* p) const {
+    *(f32x4*)p = lo;
+    *(f32x4*)(p + 4) = hi;
+  }
+};
+
+// columns col .. col + 7 of a row of d elements, zeros past d.  VEC: whole 16-byte pieces.
+template <typename T, int HD, bool VEC>
+EDF_DEVICE Frag<T> row_frag(const T* row, int col, int d) {
+  Frag<T> f;
+  if constexpr (VEC && sizeof(T) == 2) {
+    f.load(row + min(col, d - 8));
+    if (d < HD && col >= d) f.zero();
+  } else if constexpr (VEC) {
+    f.lo = *(const f32x4*)(row + min(col, d - 4));
+    f.hi = *(const f32x4*)(row + min(col + 4, d - 4));
+    if (d < HD) {
+      if (col >= d) f.lo = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (col + 4 >= d) f.hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = to_f32(row[min(col + e, d - 1)]);
+      f.set(e, col + e < d ? x : 0.0f);
+    }
+  }
+  return f;
+}
+
+template <typename T, int HD>
+struct VTile {  // a wave's 32 x HD value tile in LDS
+  static constexpr int LD = sizeof(T) == 2 ? 0 : HD + 4;
+  static constexpr int ELEMS = sizeof(T) == 2 ? lds_tile_elems<HD>(PA_KEYS) : PA_KEYS * (HD + 4);
+  EDF_DEVICE static int off(int row, int col) {
+    if constexpr (sizeof(T) == 2) return lds_off<HD>(row, col);
+    else return row * LD + col;
+  }
+  // V^T operand: dims 16 dt + i, keys 4 g .. + 3 and 16 + 4 g .. + 3
+  EDF_DEVICE static Frag<T> trans(const T* t, int dt, int g, int i) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      const int row = 4 * g + (i >> 2), col = 16 * dt + 4 * (i & 3);
+      f.v = cat4(lds_read_tr16(t + off(row, col)), lds_read_tr16(t + off(row + 16, col)));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f.lo[e] = t[off(4 * g + e, 16 * dt + i)];
+        f.hi[e] = t[off(16 + 4 * g + e, 16 * dt + i)];
+      }
+    }
+    return f;
+  }
+};
+
+template <typename T, int HD, bool VEC>
+__global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_attn_kernel(PagedArgs a) {
+  constexpr int NKK = HD / 32, NDT = HD / 16;
+  constexpr int CPR = HD / 8, NV = PA_KEYS * CPR / 64;  // 8-element pieces per row, and per lane of a tile
+  using VT = VTile<T, HD>;
+  constexpr int TILE_BYTES = VT::ELEMS * sizeof(T), OUT_BYTES = 16 * (HD + 4) * 4;
+  constexpr int WAVE_BYTES = TILE_BYTES > OUT_BYTES ? TILE_BYTES : OUT_BYTES;
+  __shared__ __attribute__((aligned(16))) char smem[PA_WAVES * WAVE_BYTES];
+  __shared__ float sML[PA_WAVES][16][2];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4, i = l & 15;
+  const int split = blockIdx.x % a.splits;
+  const int bq = blockIdx.x / a.splits;  // (b, key head, query tile)
+  const int qt = bq % a.qt, h = bq / a.qt % a.Hkv, b = bq / a.qt / a.Hkv;
+  const int hq0 = h * a.G + 16 * qt, nq = min(16, a.G - 16 * qt);
+
+  const int len = min(max(a.len[b], 0), a.width * a.block);
+  const int lo = a.window > 0 ? max(0, len - a.window) : 0;
+  const int ns = min(a.sinks, lo);     // sinks outside the window
+  const int nvis = ns + (len - lo);    // visible keys; key n is n + (n >= ns ? lo - ns : 0)
+  const int skip = lo - ns;
+  const int n0 = (int)min((long)split * a.chunk, (long)nvis), n1 = (int)min((long)n0 + a.chunk, (long)nvis);
+
+  const T *Q = (const T*)a.q, *K = (const T*)a.kc, *V = (const T*)a.vc;
+  Frag<T> qf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    qf[kk].zero();
+    if (i < nq)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = 32 * kk + 8 * g + e;
+        qf[kk].set(e, col < a.d ? to_f32(Q[((long)b * a.Hq + hq0 + i) * a.d + col]) : 0.0f);
+      }
+  }
+  f32x4 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, lsum = 0.0f;
+
+  // row of the cache [num_blocks Hkv block] that holds visible key n, or -1; lanes 32 .. 63 repeat 0 .. 31
+  const int* tb = a.table + (long)b * a.width;
+  auto row_of = [&](int nbase) {
+    const int n = nbase + (l & 31);
+    if (n >= n1) return -1;
+    const int key = n + (n >= ns ? skip : 0);
+    const int c = key / a.block;
+    const int page = tb[c];
+    return page >= 0 && page < a.num_blocks ? (page * a.Hkv + h) * a.block + (key - c * a.block) : -1;
+  };
+  Frag<T> kf[2][NKK], vf[NV];
+  auto load_tile = [&](int rows) {  // rows: this lane's key's row; a row of -1 reads row 0 (masked, or zeroed)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const long r = max(__shfl(rows, 16 * t + i), 0);
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) kf[t][kk] = row_frag<T, HD, VEC>(K + r * a.d, 32 * kk + 8 * g, a.d);
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = l + 64 * n;
+      const long r = max(__shfl(rows, c / CPR), 0);
+      vf[n] = row_frag<T, HD, VEC>(V + r * a.d, c % CPR * 8, a.d);
+    }
+  };
+  T* sv = reinterpret_cast<T*>(smem + w * WAVE_BYTES);
+  int nb = n0 + PA_KEYS * w;
+  int rows = row_of(nb);
+  if (nb < n1) load_tile(rows);
+  int rows_next = row_of(nb + PA_STEP);
+  for (; nb < n1; nb += PA_STEP) {
+    const unsigned long long live = __ballot(rows >= 0);  // bit k (and k + 32): key k of the tile
+    // values into LDS; those of absent keys as zeros, since a masked P of 0 would keep a NaN
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = l + 64 * n, row = c / CPR;
+      if (live != ~0ull && !((live >> row) & 1)) vf[n].zero();
+      vf[n].store(sv + VT::off(row, c % CPR * 8));
+    }
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) s[t] = Frag<T>::mma(kf[t][kk], qf[kk], s[t]);
+    }
+    // the next tile's loads go out before this one's softmax
+    rows = rows_next;
+    if (nb + PA_STEP < n1) load_tile(rows);
+    rows_next = row_of(nb + 2 * PA_STEP);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (live != ~0ull) s[t][r] = (live >> (16 * t + 4 * g + r)) & 1 ? s[t][r] : -INFINITY;
+        mx = fmaxf(mx, s[t][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const float mnew = fmaxf(m, mx);
+    const float mns = mnew == -INFINITY ? 0.0f : mnew * a.scale_log2;
+    if (__any(mnew > m)) {
+      const float alpha = fast_exp2(m * a.scale_log2 - mns);
+      lsum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
+    }
+    m = mnew;
+    Frag<T> pf;
+    float rs = 0.0f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = fast_exp2(fmaf(s[t][r], a.scale_log2, -mns));
+        rs += p;
+        pf.set(4 * t + r, p);
+      }
+    rs += __shfl_xor(rs, 16);
+    lsum += rs + __shfl_xor(rs, 32);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = Frag<T>::mma(VT::trans(sv, dt, g, i), pf, o[dt]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+
+  // join the four waves: O^T as [query][dim] rows of HD + 4 floats, then each thread sums its elements
+  float* so = reinterpret_cast<float*>(smem + w * WAVE_BYTES);
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) *(f32x4*)(so + i * (HD + 4) + 16 * dt + 4 * g) = o[dt];
+  if (g == 0) {
+    sML[w][i][0] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+    sML[w][i][1] = lsum;
+  }
+  __syncthreads();
+  for (int e = tid; e < nq * a.d; e += 256) {
+    const int q = e / a.d, c = e - q * a.d;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < PA_WAVES; ++x) mm = fmaxf(mm, sML[x][q][0]);
+    float acc = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int x = 0; x < PA_WAVES; ++x) {
+      const float f = mm == -INFINITY ? 0.0f : fast_exp2(sML[x][q][0] - mm);
+      sum = fmaf(f, sML[x][q][1], sum);
+      acc = fmaf(f, reinterpret_cast<const float*>(smem + x * WAVE_BYTES)[q * (HD + 4) + c], acc);
+    }
+    const long row = (long)b * a.Hq + hq0 + q;
+    if (a.splits == 1) {
+      st((T*)a.out, row * a.d + c, sum > 0.0f ? acc / sum : sum == 0.0f ? 0.0f : sum);
+    } else {
+      const long pr = row * a.splits + split;
+      a.part[pr * a.d + c] = acc;
+      if (c == 0) {
+        a.ml[2 * pr] = mm;
+        a.ml[2 * pr + 1] = sum;
+      }
+    }
+  }
+}
+
+// out[row] = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the row's chunks
+template <typename T>
+__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+  __shared__ float sw[PA_MAX_SPLITS];
+  __shared__ float sr[2];
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float* ml = a.ml + row * a.splits * 2;
+  if (tid < 64) {
+    float mm = -INFINITY;
+    for (int s = tid; s < a.splits; s += 64) mm = fmaxf(mm, ml[2 * s]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+    float sum = 0.0f;
+    for (int s = tid; s < a.splits; s += 64) {
+      const float f = mm == -INFINITY || ml[2 * s] == -INFINITY ? 0.0f : fast_exp2(ml[2 * s] - mm);
+      sw[s] = f;
+      sum = fmaf(f, ml[2 * s + 1], sum);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (tid == 0) sr[0] = sum;
+  }
+  __syncthreads();
+  const float sum = sr[0];
+  for (int c = tid; c < a.d; c += 256) {
+    float acc = 0.0f;
+    for (int s = 0; s < a.splits; ++s) acc = fmaf(sw[s], a.part[(row * a.splits + s) * a.d + c], acc);
+    st((T*)a.out, row * a.d + c, sum > 0.0f ? acc / sum : sum == 0.0f ? 0.0f : sum);
+  }
+}
+
+// Keys per chunk and chunks for the longest request that the table can hold.
+void plan(int B, int Hkv, int qt, long visible, int& chunk, int& splits) {
+  const long wgs = (long)B * Hkv * qt;
+  const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (1536 + wgs - 1) / wgs));
+  long c = (visible + want - 1) / want;
+  c = std::max(2L * PA_STEP, (c + PA_STEP - 1) / PA_STEP * PA_STEP);
+  chunk = (int)std::min(c, 1L << 30);
+  splits = (int)std::max(1L, (visible + chunk - 1) / chunk);
+}
+
+long visible_keys(long width, int block, int window, int sinks) {
+  const long cap = width * block;
+  return window > 0 ? std::min(cap, (long)window + sinks) : cap;
+}
+
+template <typename T, int HD>
+void launch_paged(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
+  if (vec)
+    paged_attn_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
+  else
+    paged_attn_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
+}
+template <typename T>
+void launch_paged_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
+  if (a.d <= 64)
+    launch_paged<T, 64>(s, a, grid, vec);
+  else if (a.d <= 128)
+    launch_paged<T, 128>(s, a, grid, vec);
+  else
+    launch_paged<T, 256>(s, a, grid, vec);
+  if (a.splits > 1) paged_join_kernel<T><<<(unsigned)(a.B * a.Hq), 256, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace edf
+
+extern "C" {
+
+size_t edf_paged_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width,
+                                           int block_size, int window, int sinks) {
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || table_width <= 0 || block_size <= 0 ||
+      window < 0 || sinks < 0)
+    return 0;
+  int chunk, splits;
+  edf::plan(batch, num_kv_heads, (num_heads / num_kv_heads + 15) / 16,
+            edf::visible_keys(table_width, block_size, window, sinks), chunk, splits);
+  return splits == 1 ? 0 : (size_t)batch * num_heads * splits * (head_dim + 2) * sizeof(float);
+}
+
+int edf_paged_attention(void* stream, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
+                        const int32_t* lengths, void* out, void* workspace, size_t workspace_bytes, int batch,
+                        int num_heads, int num_kv_heads, int head_dim, long num_blocks, int block_size,
+                        int table_width, int window, int sinks, int dtype) {
+  using namespace edf;
+  EDF_REQUIRE(batch > 0 && num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && num_blocks > 0 && block_size > 0 &&
+                  table_width > 0,
+              EDF_ERR_INVALID_ARG, "dimensions must be positive");
+  EDF_REQUIRE(valid_dtype(dtype), EDF_ERR_INVALID_ARG, "dtype must be 0 (f32) or 1 (bf16)");
+  EDF_REQUIRE(num_heads % num_kv_heads == 0, EDF_ERR_INVALID_ARG, "num_heads %d is no multiple of num_kv_heads %d",
+              num_heads, num_kv_heads);
+  EDF_REQUIRE(window >= 0 && sinks >= 0, EDF_ERR_INVALID_ARG, "window and sinks must not be negative");
+  EDF_REQUIRE(head_dim <= 256, EDF_ERR_UNSUPPORTED, "head_dim %d > 256 unsupported", head_dim);
+  EDF_REQUIRE((double)num_blocks * block_size * num_kv_heads < 2147483648.0, EDF_ERR_UNSUPPORTED,
+              "the cache has 2^31 or more rows of head_dim");
+  EDF_REQUIRE((long)table_width * block_size < (1L << 30), EDF_ERR_UNSUPPORTED,
+              "table_width x block_size must be below 2^30");
+  EDF_REQUIRE(q && k_cache && v_cache && table && lengths && out, EDF_ERR_INVALID_ARG, "null tensor pointer");
+  PagedArgs a{};
+  a.q = q, a.kc = k_cache, a.vc = v_cache, a.table = table, a.len = lengths, a.out = out;
+  a.B = batch, a.Hq = num_heads, a.Hkv = num_kv_heads, a.G = num_heads / num_kv_heads, a.qt = (a.G + 15) / 16;
+  a.d = head_dim, a.width = table_width, a.block = block_size, a.window = window, a.sinks = sinks;
+  a.num_blocks = num_blocks;
+  a.scale_log2 = LOG2E / sqrtf((float)head_dim);
+  plan(batch, num_kv_heads, a.qt, visible_keys(table_width, block_size, window, sinks), a.chunk, a.splits);
+  const double wgs = (double)batch * num_kv_heads * a.qt * a.splits;
+  EDF_REQUIRE(wgs < 2147483648.0 && (double)batch * num_heads < 2147483648.0, EDF_ERR_UNSUPPORTED,
+              "batch x heads too large for one call");
+  const size_t need = edf_paged_attention_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, table_width,
+                                                          block_size, window, sinks);
+  EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
+              "workspace too small: need %zu bytes", need);
+  a.part = (float*)workspace;
+  a.ml = (float*)workspace + (size_t)batch * num_heads * a.splits * head_dim;
+  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 &&
+                   !(((uintptr_t)k_cache | (uintptr_t)v_cache) & 15);
+  hipStream_t s = as_stream(stream);
+  const unsigned grid = (unsigned)wgs;
+  if (dtype == EDF_BF16)
+    launch_paged_t<bf16>(s, a, grid, vec);
+  else
+    launch_paged_t<float>(s, a, grid, vec);
+  return check_launch("paged attention");
+}
+
+}  // extern "C"

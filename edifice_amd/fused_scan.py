@@ -14,6 +14,7 @@ oracle in ``oracle/``, which the product never calls).
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 import torch.nn.functional as F
@@ -1018,6 +1019,274 @@ def flash_attention(q, k, v, causal: bool = False):
     Scale 1/sqrt(d); causal keeps keys j <= i.  Differentiable (fused HIP backward).
     """
     return _FlashAttention.apply(q, k, v, bool(causal))
+
+
+# ---------------------------------------------------------------------------
+# Attention of a decoder with positions, windows and a paged cache
+# ---------------------------------------------------------------------------
+
+def _here(*ts):
+    """GPU tensors of the current device: the launch goes to its current stream."""
+    cur = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise EdificeHipError("edifice_amd ops need GPU tensors (no CPU fallback)")
+        if cur is None:
+            cur = torch.cuda.current_device()
+        if t.get_device() != cur:
+            raise EdificeHipError(f"tensor on cuda:{t.get_device()}, but the current device is cuda:{cur}")
+
+
+def _i32(name, t, shape):
+    """t as the contiguous int32 GPU tensor of that shape that a kernel indexes by."""
+    if t.dtype != torch.int32:
+        raise EdificeHipError(f"{name} must be int32, got {t.dtype}")
+    _shape(name, t, shape)
+    _here(t)
+    return t.contiguous()
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str = None, factor: float = 1.0,
+                       original_length: int = 0, slow: float = 1.0, fast: float = 32.0, device="cuda"):
+    """Angle per position of each rotated pair, float64 [rotary_dim / 2]: f_i = base^(-2 i / rotary_dim).
+
+    scaling, for contexts ``factor`` times longer than trained on: "linear" divides every f_i by factor;
+    "base" raises the base to base factor^(rotary_dim / (rotary_dim - 2)), which keeps the fastest pair and
+    divides the slowest by factor; "parts" divides the pairs that turn fewer than ``slow`` times over
+    ``original_length`` positions, keeps those that turn more than ``fast`` times and goes linearly between.
+    """
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise EdificeHipError(f"rotary_dim must be even, got {rotary_dim}")
+    if base <= 0 or factor <= 0:
+        raise EdificeHipError("base and factor must be positive")
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-i / rotary_dim) for i in range(0, rotary_dim, 2)]
+    if scaling == "linear":
+        f = [x / factor for x in f]
+    elif scaling == "parts":
+        if original_length <= 0 or fast <= slow:
+            raise EdificeHipError('scaling "parts" needs original_length > 0 and fast > slow')
+        keep = [min(max((original_length * x / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0) for x in f]
+        f = [x / factor * (1 - k) + x * k for x, k in zip(f, keep)]
+    elif scaling not in (None, "base"):
+        raise EdificeHipError(f'unknown scaling {scaling!r} (None, "linear", "base" or "parts")')
+    return torch.tensor(f, dtype=torch.float64, device=device)
+
+
+def _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq, wk):
+    _rank("x", x, 3)
+    bsz, seq, width = x.shape
+    if num_heads <= 0 or num_kv_heads <= 0 or width % (num_heads + 2 * num_kv_heads):
+        raise EdificeHipError(f"split_heads_rotary: last dimension {width} is not (num_heads + 2 num_kv_heads) x "
+                              f"head_dim for {num_heads} and {num_kv_heads} heads")
+    d = width // (num_heads + 2 * num_kv_heads)
+    if (wq is None) != (wk is None):
+        raise EdificeHipError("q_weight and k_weight come together")
+    _here(x, wq, wk, freq)
+    _same(x, wq, wk)
+    _shape("q_weight", wq, (d,))
+    _shape("k_weight", wk, (d,))
+    rot = 0
+    if freq is not None:
+        if freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous() or 2 * freq.numel() > d:
+            raise EdificeHipError("frequencies must be a contiguous float64 tensor of at most head_dim / 2 values")
+        rot = 2 * freq.numel()
+    per_row = 0
+    if positions is not None:
+        per_row = int(positions.dim() == 2)
+        positions = _i32("positions", positions, (bsz, seq) if per_row else (seq,))
+    return bsz, seq, d, rot, positions, per_row
+
+
+class _SplitHeadsRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wq, wk, freq, positions, num_heads, num_kv_heads, eps, interleaved, amplitude):
+        x, wq, wk = x.contiguous(), _c(wq), _c(wk)
+        bsz, seq, d, rot, positions, per_row = _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq, wk)
+        q = x.new_empty((bsz, num_heads, seq, d))
+        k, v = (x.new_empty((bsz, num_kv_heads, seq, d)) for _ in range(2))
+        conf = (bsz, seq, num_heads, num_kv_heads, d, rot, per_row, int(interleaved), float(eps), float(amplitude),
+                dtype_flag(x))
+        if x.numel():
+            nat.call("edf_heads_split_rotary", _stream(), _p(x), _p(freq), _p(positions), _p(wq), _p(wk), _p(q), _p(k),
+                     _p(v), *conf)
+        if ctx is not None:  # None: no gradient is asked for
+            ctx.conf = conf
+            ctx.save_for_backward(x, wq, wk, freq, positions)
+        return q, k, v
+
+    @staticmethod
+    def backward(ctx, dq, dk, dv):
+        x, wq, wk, freq, positions = ctx.saved_tensors
+        g = [t.contiguous().to(x.dtype) for t in (dq, dk, dv)]
+        dx = torch.empty_like(x)
+        dwq, dwk = (None if w is None else torch.zeros_like(w) if not x.numel() else torch.empty_like(w)
+                    for w in (wq, wk))
+        if x.numel():
+            wsb = 0 if wq is None else nat.query("edf_heads_split_rotary_backward_workspace_bytes", ctx.conf[4])
+            ws = _u8(wsb, x)
+            nat.call("edf_heads_split_rotary_backward", _stream(), _p(x), _p(freq), _p(positions), _p(wq), _p(wk),
+                     *(_p(t) for t in g), _p(dx), _p(dwq), _p(dwk), _p(ws), wsb, *ctx.conf)
+        return dx, dwq, dwk, None, None, None, None, None, None, None
+
+
+def _wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def split_heads_rotary(x: torch.Tensor, num_heads: int, num_kv_heads: int, frequencies: torch.Tensor = None,
+                       positions: torch.Tensor = None, q_weight: torch.Tensor = None, k_weight: torch.Tensor = None,
+                       *, eps: float = 1e-6, interleaved: bool = False, amplitude: float = 1.0):
+    """``split_heads`` of a decoder's attention with query / key norms and rotary positions in the same pass.
+
+    x [B, T, (num_heads + 2 num_kv_heads) d] (q | k | v) -> q [B, num_heads, T, d], k, v [B, num_kv_heads, T, d].
+    q_weight, k_weight [d] (both or neither): each query / key head row u becomes u w / sqrt(mean(u^2) + eps).
+    frequencies (``rotary_frequencies``; None: no rotation): pair i of the first 2 len(frequencies) elements then
+    turns by positions[b, t] frequencies[i] and is scaled by ``amplitude``; pairs are (i, i + half), or
+    (2 i, 2 i + 1) when ``interleaved``.  positions: int32 [B, T] or [T] (any value; None: 0 .. T - 1).
+    float32 or bfloat16, float32 inside (angles in float64), head_dim <= 256; differentiable in x and the weights.
+    """
+    args = (x, q_weight, k_weight, frequencies, positions, num_heads, num_kv_heads, eps, interleaved, amplitude)
+    if _wants_grad(x, q_weight, k_weight):
+        return _SplitHeadsRotary.apply(*args)
+    return _SplitHeadsRotary.forward(None, *args)
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        _here(q, k, v)
+        _same(q, k, v)
+        _rank("q", q, 4)
+        _rank("k", k, 4)
+        bsz, nh, seq, hd = q.shape
+        nkv = k.shape[1]
+        if tuple(k.shape) != (bsz, nkv, seq, hd) or v.shape != k.shape or nkv == 0 or nh % nkv:
+            raise EdificeHipError("window_attention needs q [B, H, T, d] and k, v [B, Hkv, T, d] with H a multiple of "
+                                  f"Hkv, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        out = torch.empty_like(q)
+        keep = ctx is not None  # None: no gradient is asked for
+        lse = torch.empty((bsz, nh, seq), dtype=torch.float32, device=q.device) if keep else None
+        conf = (bsz, nh, nkv, seq, hd, window, sinks, dtype_flag(q))
+        nat.call("edf_window_attention", _stream(), _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
+        if keep:
+            ctx.conf = conf
+            ctx.save_for_backward(q, k, v, out, lse)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        dout = dout.contiguous().to(q.dtype)
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        wsb = nat.query("edf_window_attention_backward_workspace_bytes", *ctx.conf)
+        ws = _u8(wsb, q)
+        nat.call("edf_window_attention_backward", _stream(), _p(q), _p(k), _p(v), _p(out), _p(dout), _p(lse), _p(dq),
+                 _p(dk), _p(dv), _p(ws), wsb, *ctx.conf)
+        return dq, dk, dv, None, None
+
+
+def window_attention(q, k, v, window: int, sinks: int = 0):
+    """Causal attention with a sliding window and sinks, with shared key heads: q [B, H, T, d], k, v
+    [B, Hkv, T, d], query head h reads key head h // (H // Hkv).  Query i sees key j when j <= i and
+    (i - j < window or j < sinks); scale 1/sqrt(d).  float32 or bfloat16, head_dim <= 128; differentiable (fused
+    HIP backward, the gradients of shared heads summed in a fixed order).  window >= T is causal attention.
+    Keys and values have to be finite, as those of rows behind a padded batch's ends are."""
+    args = (q, k, v, int(window), int(sinks))
+    if _wants_grad(q, k, v):
+        return _WindowAttention.apply(*args)
+    return _WindowAttention.forward(None, *args)
+
+
+def _cache_dims(k_cache, v_cache, num_kv_heads, d, like):
+    _rank("k_cache", k_cache, 4)
+    blocks, nkv, block, hd = k_cache.shape
+    if v_cache.shape != k_cache.shape or hd != d or (num_kv_heads is not None and nkv != num_kv_heads):
+        raise EdificeHipError(f"k_cache and v_cache must be [num_blocks, Hkv, block_size, {d}], got "
+                              f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    _here(like, k_cache, v_cache)
+    _same(like, k_cache, v_cache)
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise EdificeHipError("edifice_amd ops need contiguous tensors")
+    return blocks, nkv, block
+
+
+def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor, free_blocks: torch.Tensor,
+                 block_size: int, num_tokens: int):
+    """Block tables and slots of a paged cache, on the GPU: request r grows from old_lengths[r] to new_lengths[r].
+
+    table int32 [R, width] is written in place: pages ceil(old / block_size) .. ceil(new / block_size) - 1 of each
+    request are the next entries of free_blocks (int32 [F]), request by request.  Returns (slots, positions, used):
+    slots, positions int32 [R, num_tokens] of tokens old_lengths[r] + t (-1 past new_lengths[r]; slot -1 too where
+    the table or the list of free blocks ended), and used int32 [1], the blocks drawn (more than F when the list
+    was too short).  The caller takes the first ``used`` entries off its list."""
+    _rank("table", table, 2)
+    reqs, width = table.shape
+    if not table.is_contiguous() or table.dtype != torch.int32:
+        raise EdificeHipError("table must be a contiguous int32 tensor")
+    old_lengths = _i32("old_lengths", old_lengths, (reqs,))
+    new_lengths = _i32("new_lengths", new_lengths, (reqs,))
+    _rank("free_blocks", free_blocks, 1)
+    free_blocks = _i32("free_blocks", free_blocks, free_blocks.shape)
+    _here(table)
+    slots, positions = (table.new_empty((reqs, num_tokens)) for _ in range(2))
+    used = table.new_empty((1,))
+    nat.call("edf_paged_extend", _stream(), _p(table), _p(old_lengths), _p(new_lengths), _p(free_blocks), _p(slots),
+             _p(positions), _p(used), reqs, width, free_blocks.numel(), int(block_size), int(num_tokens))
+    return slots, positions, used
+
+
+def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                      v_cache: torch.Tensor) -> None:
+    """Keys and values k, v [B, Hkv, T, d] into the pages k_cache, v_cache [num_blocks, Hkv, block_size, d], in
+    place: token (b, t) into slot slots[b, t] (int32 [B, T], as ``paged_extend`` gives them; -1, or any other slot
+    outside the cache: left out).  Slots have to differ from one another.  Inference only."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_cache, v_cache)):
+        raise EdificeHipError("paged_cache_write has no backward: call it under torch.no_grad()")
+    k, v = k.contiguous(), v.contiguous()
+    _rank("k", k, 4)
+    bsz, nkv, seq, d = k.shape
+    _shape("v", v, k.shape)
+    _here(v)
+    _same(k, v)
+    blocks, _, block = _cache_dims(k_cache, v_cache, nkv, d, k)
+    slots = _i32("slots", slots, (bsz, seq))
+    if k.numel():
+        nat.call("edf_paged_cache_write", _stream(), _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), bsz, seq, nkv,
+                 d, blocks, block, dtype_flag(k))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
+                    lengths: torch.Tensor, *, window: int = 0, sinks: int = 0) -> torch.Tensor:
+    """Attention of one new token per request over a paged cache: q [B, H, d] (or [B, H, 1, d]), k_cache, v_cache
+    [num_blocks, Hkv, block_size, d], table int32 [B, width] (the request's pages in order), lengths int32 [B]
+    (tokens in the cache, the new one among them).  window > 0: only the last ``window`` and the first ``sinks``
+    tokens are seen.  Returns q's shape; a request of length 0 answers with zeros, and pages outside the cache hold
+    no keys.  float32 or bfloat16, head_dim <= 256, scale 1/sqrt(d), H a multiple of Hkv.  Inference only.
+
+    The launch depends on shapes alone (a table as wide as the longest request may get), so a captured call may be
+    replayed after the lengths and the table have changed."""
+    if _wants_grad(q, k_cache, v_cache):
+        raise EdificeHipError("paged_attention has no backward: call it under torch.no_grad()")
+    q = q.contiguous()
+    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
+        raise EdificeHipError(f"q must be [B, H, d] or [B, H, 1, d], got shape {tuple(q.shape)}")
+    bsz, nh, d = q.shape[0], q.shape[1], q.shape[-1]
+    blocks, nkv, block = _cache_dims(k_cache, v_cache, None, d, q)
+    _rank("table", table, 2)
+    width = table.shape[1]
+    table = _i32("table", table, (bsz, width))
+    lengths = _i32("lengths", lengths, (bsz,))
+    out = torch.empty_like(q)
+    wsb = nat.query("edf_paged_attention_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
+    ws = _u8(wsb, q)
+    nat.call("edf_paged_attention", _stream(), _p(q), _p(k_cache), _p(v_cache), _p(table), _p(lengths), _p(out), _p(ws),
+             wsb, bsz, nh, nkv, d, blocks, block, width, window, sinks, dtype_flag(q))
+    return out
 
 
 BETA_PER_ELEMENT, BETA_PER_HEAD = 0, 1

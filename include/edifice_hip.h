@@ -637,6 +637,83 @@ int edf_heads_merge(void* stream, const void* const* parts, void* y, long batch,
                     int num_heads, int head_dim, int dtype);
 
 /* ------------------------------------------------------------------------
+ * Head split with query / key norms and rotary positions in the same pass (the attention blocks; the
+ * reference composes them from Nx operations, lib/edifice/blocks/):
+ *   x [batch, seq, (Hq + 2 Hkv) d] (q | k | v) -> q [batch, Hq, seq, d], k, v [batch, Hkv, seq, d]
+ * For a query or key head row u at position p:  n = u w / sqrt(mean(u^2) + eps) (w = wq or wk [d]; both NULL:
+ * n = u); the first rotary_dim elements in pairs (a, b) turn by the angle p freq[i]:
+ *   y_a = amplitude (n_a cos - n_b sin), y_b = amplitude (n_b cos + n_a sin);  the others stay.
+ * Pairs are (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved != 0.  freq: float64 device array
+ * [rotary_dim / 2]; positions: int32 [batch, seq] (positions_per_row != 0) or [seq], NULL: 0 .. seq - 1.
+ * head_dim <= 256, rotary_dim even and <= head_dim, 0 for norms alone.
+ * The backward takes the forward's x and the gradients of q, k, v; grad_wq / grad_wk [d] (NULL without norms)
+ * are summed in a fixed order through a workspace of edf_heads_split_rotary_backward_workspace_bytes()
+ * (not used, and may be NULL, without norms).
+ * ------------------------------------------------------------------------ */
+int edf_heads_split_rotary(void* stream, const void* x, const double* freq, const int32_t* positions, const void* wq,
+                           const void* wk, void* q, void* k, void* v, long batch, long seq, int num_heads,
+                           int num_kv_heads, int head_dim, int rotary_dim, int positions_per_row, int interleaved,
+                           float eps, float amplitude, int dtype);
+size_t edf_heads_split_rotary_backward_workspace_bytes(int head_dim);
+int edf_heads_split_rotary_backward(void* stream, const void* x, const double* freq, const int32_t* positions,
+                                    const void* wq, const void* wk, const void* grad_q, const void* grad_k,
+                                    const void* grad_v, void* grad_x, void* grad_wq, void* grad_wk, void* workspace,
+                                    size_t workspace_bytes, long batch, long seq, int num_heads, int num_kv_heads,
+                                    int head_dim, int rotary_dim, int positions_per_row, int interleaved, float eps,
+                                    float amplitude, int dtype);
+
+/* ------------------------------------------------------------------------
+ * Causal attention with a sliding window, sinks and shared key heads (no counterpart among the reference's
+ * NIFs; its hybrid models mask a full score matrix, lib/edifice/ssm/hybrid.ex:501-556):
+ *   q, out [batch, num_heads, seq_len, d], k, v [batch, num_kv_heads, seq_len, d]; query head h reads key head
+ *   h / (num_heads / num_kv_heads); query i sees key j when j <= i and (i - j < window or j < sinks);
+ *   scores / sqrt(d).
+ * lse (may be NULL): float32 [batch, num_heads, seq_len] natural-log row sums, required by the backward.
+ * head_dim <= 128, batch x num_heads <= 65535.  Keys and values have to be finite where some query of the same
+ * 64-key tile sees the tile.  The backward's workspace: edf_window_attention_backward_workspace_bytes().
+ * ------------------------------------------------------------------------ */
+int edf_window_attention(void* stream, const void* q, const void* k, const void* v, void* out, float* lse, int batch,
+                         int num_heads, int num_kv_heads, int seq_len, int head_dim, int window, int sinks, int dtype);
+size_t edf_window_attention_backward_workspace_bytes(int batch, int num_heads, int num_kv_heads, int seq_len,
+                                                     int head_dim, int window, int sinks, int dtype);
+int edf_window_attention_backward(void* stream, const void* q, const void* k, const void* v, const void* out,
+                                  const void* grad_out, const float* lse, void* grad_q, void* grad_k, void* grad_v,
+                                  void* workspace, size_t workspace_bytes, int batch, int num_heads,
+                                  int num_kv_heads, int seq_len, int head_dim, int window, int sinks, int dtype);
+
+/* ------------------------------------------------------------------------
+ * Paged key / value cache (inference; no counterpart among the reference's NIFs).  k_cache, v_cache
+ * [num_blocks, num_kv_heads, block_size, d]; table [requests, table_width] int32 names each request's pages in
+ * order, -1: none; slot s = page * block_size + offset names one token's place.
+ *
+ * edf_paged_extend: request r grows from old_lengths[r] to new_lengths[r] tokens (negative ones count as 0;
+ *   new <= old: nothing).  Its pages ceil(old / block_size) .. ceil(new / block_size) - 1 (within the table's
+ *   width) are the next entries of free_blocks [num_free], request by request, and are written into table; past
+ *   the list's end they are -1.  slots, positions [requests, num_tokens]: those of token old_lengths[r] + t, or
+ *   -1 past new_lengths[r]; a token without a page has the position and slot -1.  used [1]: pages drawn, which
+ *   exceeds num_free when the list was too short.
+ * edf_paged_cache_write: rows of k, v [batch, num_kv_heads, seq, d] into the pages by slots [batch, seq]; slots
+ *   outside [0, num_blocks * block_size) are left out.  Slots have to differ from one another.
+ * edf_paged_attention: one query per request, q, out [batch, num_heads, d], over the request's first lengths[b]
+ *   tokens (clamped to [0, table_width * block_size]), of which, with window > 0, the last `window` and the first
+ *   `sinks` are seen.  Pages outside [0, num_blocks) hold no keys; a request that sees none answers with zeros.
+ *   head_dim <= 256.  The grid and the workspace (edf_paged_attention_workspace_bytes()) depend on the shapes
+ *   alone, not on lengths, so a captured call may be replayed after lengths and table have changed.
+ * ------------------------------------------------------------------------ */
+int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, const int32_t* new_lengths,
+                     const int32_t* free_blocks, int32_t* slots, int32_t* positions, int32_t* used, int requests,
+                     int table_width, int num_free, int block_size, int num_tokens);
+int edf_paged_cache_write(void* stream, const void* k, const void* v, const int32_t* slots, void* k_cache,
+                          void* v_cache, long batch, long seq, int num_kv_heads, int head_dim, long num_blocks,
+                          int block_size, int dtype);
+size_t edf_paged_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width,
+                                           int block_size, int window, int sinks);
+int edf_paged_attention(void* stream, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
+                        const int32_t* lengths, void* out, void* workspace, size_t workspace_bytes, int batch,
+                        int num_heads, int num_kv_heads, int head_dim, long num_blocks, int block_size,
+                        int table_width, int window, int sinks, int dtype);
+
+/* ------------------------------------------------------------------------
  * Token-embedding weight gradient (block callers: the language models' input embedding,
  * Axon.embedding, e.g. lib/edifice/generative/show_o.ex:123):
  *   grad_weight[v, :] = sum over positions p with ids[p] == v (ascending p) of grad[p, :]
