@@ -75,7 +75,7 @@ SIGNATURES = {
     "edf_window_attention_backward_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
     "edf_window_attention_backward": (
         I, [P, P, P, P, P, P, P, P, P, P, P, S, I, I, I, I, I, I, I, I]),
-    "edf_paged_extend": (I, [P, P, P, P, P, P, P, P, I, I, I, I, I]),
+    "edf_paged_extend": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I]),
     "edf_paged_cache_write": (I, [P, P, P, P, P, P, L, L, I, I, L, I, I]),
     "edf_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
     "edf_paged_attention": (I, [P, P, P, P, P, P, P, P, S, I, I, I, I, L, I, I, I, I, I]),

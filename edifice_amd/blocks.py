@@ -19,7 +19,8 @@ forward and backward through a block runs the HIP kernels for the recurrence and
                      causal conv, 6 x hidden projection, per-head alpha = mean of sigmoid,
                      swish output gate)
   GQABlock           causal grouped-query attention routed to flash attention
-                     (lib/edifice/blocks/sdpa.ex:74-91) + GELU feed-forward
+                     (lib/edifice/blocks/sdpa.ex:74-91) + GELU feed-forward; with rotary positions,
+                     query / key norms, a window or sinks, and a step over a paged cache
 
 ``build(name, **opts)`` mirrors ``Edifice.build(name, opts)`` for these families and returns
 a model mapping [batch, seq, embed] to the last timestep's hidden state, as the reference's
@@ -259,11 +260,72 @@ class GatedDeltaNetLayer(nn.Module):
         return x + self.out_proj(o.reshape(bsz, seq, hid) * F.silu(gpre))
 
 
-class GQAttention(nn.Module):
-    """Causal grouped-query self-attention on the fused flash kernel; the KV heads are
-    repeated to the query heads before the kernel."""
+class PagedCache:
+    """Keys and values of ``layers`` attention layers for ``requests`` places, in pages shared by all of them.
 
-    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int):
+    k[layer], v[layer] [num_blocks, num_kv_heads, block_size, head_dim]; table [requests, width] and lengths
+    [requests] live on the GPU, and so does the list of free pages: ``extend`` makes room for new tokens without a
+    host synchronisation, and may be captured with the step that follows it."""
+
+    def __init__(self, layers: int, requests: int, max_length: int, num_kv_heads: int, head_dim: int, *,
+                 block_size: int = 16, num_blocks: int | None = None, dtype=torch.bfloat16, device="cuda"):
+        width = -(-max_length // block_size)
+        blocks = requests * width if num_blocks is None else num_blocks
+        self.block_size = block_size
+        shape = (blocks, num_kv_heads, block_size, head_dim)
+        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        i32 = dict(dtype=torch.int32, device=device)
+        self.table = torch.full((requests, width), -1, **i32)
+        self.lengths = torch.zeros(requests, **i32)
+        self.free = torch.arange(blocks, **i32)  # free pages, -1 behind them; the first ``taken`` are in use again
+        self.taken = torch.zeros(1, **i32)
+        self.available = blocks
+        self._old = torch.zeros(requests, **i32)
+
+    def extend(self, num_tokens: int, counts: torch.Tensor = None):
+        """Room for the next counts[r] tokens of each place (int [requests], taken as 0 .. num_tokens; None: num_tokens
+        each): their (slots, positions) [requests, num_tokens], -1 past counts[r].  lengths then holds them."""
+        if counts is not None and tuple(counts.shape) != tuple(self.lengths.shape):
+            raise ValueError(f"counts must be [{self.lengths.numel()}], got {tuple(counts.shape)}")
+        self._old.copy_(self.lengths)
+        self.lengths.add_(num_tokens if counts is None else counts.clamp(0, num_tokens))
+        slots, positions, used = fs.paged_extend(self.table, self._old, self.lengths, self.free, self.block_size,
+                                                 num_tokens, self.taken)
+        self.taken.copy_(used)
+        return slots, positions
+
+    def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+        fs.paged_cache_write(k, v, slots, self.k[layer], self.v[layer])
+
+    def attend(self, layer: int, q: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
+        return fs.paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, window=window, sinks=sinks)
+
+    def exhausted(self) -> bool:
+        """Whether some token found no page: the list of free ones ended, or a table row (waits for the GPU)."""
+        return int(self.taken) > self.available or bool(
+            (self.lengths > self.table.shape[1] * self.block_size).any())
+
+    def release(self, place: int) -> None:
+        """The place's pages back onto the list of free ones, its length 0 (waits for the GPU)."""
+        row = self.table[place]
+        left = torch.cat([self.free[min(int(self.taken), self.available):self.available], row[row >= 0]])
+        self.available = left.numel()
+        self.free.fill_(-1)
+        self.free[:self.available] = left
+        self.taken.zero_()
+        row.fill_(-1)
+        self.lengths[place] = 0
+
+
+class GQAttention(nn.Module):
+    """Causal grouped-query self-attention.  Without the options below it runs on the fused flash kernel, the KV heads
+    repeated to the query heads before it; with one of them on the kernels that take shared KV heads as they are:
+    rotary_dim (positions, pairs (i, i + rotary_dim / 2) of each head; rotary_base), qk_norm (learned query / key norms
+    per head), window (keys seen per query) and sinks (first keys that stay visible)."""
+
+    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, *, rotary_dim: int = 0,
+                 rotary_base: float = 10000.0, qk_norm: bool = False, window: int = 0, sinks: int = 0):
         super().__init__()
         self.num_heads, self.num_kv_heads = num_heads, num_kv_heads
         hd = hidden_size // num_heads
@@ -271,20 +333,41 @@ class GQAttention(nn.Module):
         self.k_proj = Linear(hidden_size, num_kv_heads * hd)
         self.v_proj = Linear(hidden_size, num_kv_heads * hd)
         self.out_proj = Linear(hidden_size, hidden_size)
+        self.window, self.sinks, self.rotary_dim, self.rotary_base = window, sinks, rotary_dim, rotary_base
+        self.q_norm = nn.Parameter(torch.ones(hd)) if qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(hd)) if qk_norm else None
+        self._frequencies = None  # float64 whatever the module is cast to, so not a buffer
+        self.shared = bool(rotary_dim or qk_norm or window or sinks)
+
+    def _stacked(self, x):
+        """q | k | v as one product over the stacked weights: [B, T, (num_heads + 2 num_kv_heads) head_dim]."""
+        projs = (self.q_proj, self.k_proj, self.v_proj)
+        w = torch.cat([m.weight for m in projs], 0)
+        b = None
+        if any(m.bias is not None for m in projs):
+            b = torch.cat([m.bias if m.bias is not None else m.weight.new_zeros(m.weight.shape[0]) for m in projs], 0)
+        return _LinearFn.apply(x, w, b)
+
+    def _heads(self, x, positions=None):
+        if self.rotary_dim and (self._frequencies is None or self._frequencies.device != x.device):
+            self._frequencies = fs.rotary_frequencies(self.rotary_dim, self.rotary_base, device=x.device)
+        return fs.split_heads_rotary(self._stacked(x), self.num_heads, self.num_kv_heads, self._frequencies, positions,
+                                     self.q_norm, self.k_norm)
+
+    def _seen(self, seq):
+        return self.window or seq  # no window: all earlier keys
 
     def forward(self, x):
         bsz, seq, hid = x.shape
         nh, nkv = self.num_heads, self.num_kv_heads
         hd = hid // nh
+        if self.shared:
+            q, k, v = self._heads(x)
+            return self.out_proj(fs.merge_heads(fs.window_attention(q, k, v, self._seen(seq), self.sinks)))
         if nkv == nh:
             # q, k, v as one product over the stacked weights, split into the kernel's head
             # layout in one pass (the backward merges dq, dk, dv into one gradient, no adds)
-            projs = (self.q_proj, self.k_proj, self.v_proj)
-            w = torch.cat([m.weight for m in projs], 0)
-            b = None
-            if any(m.bias is not None for m in projs):
-                b = torch.cat([m.bias if m.bias is not None else m.weight.new_zeros(hid) for m in projs], 0)
-            q, k, v = fs.split_heads(_LinearFn.apply(x, w, b), 3, nh)
+            q, k, v = fs.split_heads(self._stacked(x), 3, nh)
         else:
             q = self.q_proj(x).reshape(bsz, seq, nh, hd).transpose(1, 2).contiguous()
             k = self.k_proj(x).reshape(bsz, seq, nkv, hd).transpose(1, 2)
@@ -294,20 +377,37 @@ class GQAttention(nn.Module):
         o = fs.flash_attention(q, k, v, causal=True)
         return self.out_proj(fs.merge_heads(o))
 
+    def step(self, x, cache: PagedCache, layer: int, slots, positions):
+        """x [places, T, hidden], the tokens that cache.extend just made room for: T = 1 attends over the cache;
+        T > 1 is a prompt into empty places and attends to itself.  Inference (call under torch.no_grad())."""
+        seq = x.shape[1]
+        q, k, v = self._heads(x, positions)
+        cache.write(layer, k, v, slots)
+        if seq == 1:
+            o = cache.attend(layer, q, self.window, self.sinks)
+        else:
+            o = fs.window_attention(q, k, v, self._seen(seq), self.sinks)
+        return self.out_proj(fs.merge_heads(o))
+
 
 class GQABlock(nn.Module):
-    """Pre-norm transformer block: x + attn(norm x), then + ffn_down(gelu(ffn_up(norm x)))."""
+    """Pre-norm transformer block: x + attn(norm x), then + ffn_down(gelu(ffn_up(norm x))); attention options as
+    ``GQAttention``."""
 
-    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, ffn_mult: int = 4):
+    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, ffn_mult: int = 4, **attention):
         super().__init__()
         self.attn_norm = LayerNorm(hidden_size, eps=LN_EPS)
-        self.attn = GQAttention(hidden_size, num_heads, num_kv_heads)
+        self.attn = GQAttention(hidden_size, num_heads, num_kv_heads, **attention)
         self.ffn_norm = LayerNorm(hidden_size, eps=LN_EPS)
         self.ffn_up = Linear(hidden_size, ffn_mult * hidden_size)
         self.ffn_down = Linear(ffn_mult * hidden_size, hidden_size)
 
     def forward(self, x):
         x = x + self.attn(self.attn_norm(x))
+        return x + self.ffn(self.ffn_norm(x))
+
+    def step(self, x, cache: PagedCache, layer: int, slots, positions):
+        x = x + self.attn.step(self.attn_norm(x), cache, layer, slots, positions)
         return x + self.ffn(self.ffn_norm(x))
 
     def ffn(self, n):
@@ -339,6 +439,30 @@ class SequenceModel(nn.Module):
     def forward(self, x):
         return self.sequence(x)[:, -1]
 
+    def paged_cache(self, requests: int, max_length: int, **opts) -> PagedCache:
+        """An empty cache for ``step`` (the "gqa" family): options as ``PagedCache``."""
+        blocks = getattr(self, self._blocks_name)
+        if not all(isinstance(b, GQABlock) for b in blocks):
+            raise ValueError("only models of attention blocks take a paged cache")
+        w = blocks[0].attn.k_proj.weight
+        nkv = blocks[0].attn.num_kv_heads
+        return PagedCache(len(blocks), requests, max_length, nkv, w.shape[0] // nkv,
+                          **{"dtype": w.dtype, "device": w.device, **opts})
+
+    @torch.no_grad()
+    def step(self, x, cache: PagedCache, counts=None):
+        """The next tokens x [requests, T, embed] of a cache's places -> their hidden states [requests, T, hidden]:
+        prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
+        time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text.  A step of one token does not wait
+        for the GPU and may be captured; one of several checks that their places are empty."""
+        if x.shape[1] > 1 and bool((cache.lengths * (1 if counts is None else counts)).any()):
+            raise ValueError("several tokens at once go into empty places only")
+        slots, positions = cache.extend(x.shape[1], counts)
+        h = self.input_projection(x) if hasattr(self, "input_projection") else x
+        for layer, blk in enumerate(getattr(self, self._blocks_name)):
+            h = blk.step(h, cache, layer, slots, positions)
+        return self.final_norm(h) if hasattr(self, "final_norm") else h
+
     def load_reference_weights(self, weights: dict):
         """Load a reference weight file's ``weight.<layer>.<param>`` tensors (PyTorch layout)."""
         sd = {k[len("weight."):]: v for k, v in weights.items() if k.startswith("weight.")}
@@ -353,11 +477,14 @@ class SequenceModel(nn.Module):
 
 def build(name: str, *, embed_size: int, hidden_size: int | None = None, num_layers: int = 2,
           num_heads: int = 4, num_kv_heads: int | None = None, state_size: int = 16, expand_factor: int = 2,
-          conv_size: int = 4, use_short_conv: bool = True) -> SequenceModel:
+          conv_size: int = 4, use_short_conv: bool = True, **attention) -> SequenceModel:
     """``Edifice.build(name, opts)`` for the sequence-mixing families on the fused path.
 
     name: "min_gru", "min_lstm", "mamba", "delta_net", "gated_delta_net" or "gqa".  hidden_size defaults
-    to embed_size; an input projection is added when they differ."""
+    to embed_size; an input projection is added when they differ.  "gqa" takes ``GQAttention``'s options too
+    (rotary_dim, rotary_base, qk_norm, window, sinks)."""
+    if attention and name != "gqa":
+        raise TypeError(f"build({name!r}) takes no {sorted(attention)}")
     hidden = hidden_size or embed_size
     proj = Linear(embed_size, hidden) if hidden != embed_size else None
     if name == "min_gru":
@@ -376,7 +503,7 @@ def build(name: str, *, embed_size: int, hidden_size: int | None = None, num_lay
         return SequenceModel("blocks", [MambaBlock(hidden, state_size, expand_factor, conv_size)
                                         for _ in range(num_layers)], proj, None, residual=True)
     if name == "gqa":
-        return SequenceModel("blocks", [GQABlock(hidden, num_heads, num_kv_heads or num_heads)
+        return SequenceModel("blocks", [GQABlock(hidden, num_heads, num_kv_heads or num_heads, **attention)
                                         for _ in range(num_layers)], proj, LayerNorm(hidden, eps=LN_EPS))
     raise ValueError(f"unknown block family {name!r}")
 

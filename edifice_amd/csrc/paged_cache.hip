@@ -48,7 +48,8 @@ EDF_DEVICE int wave_sum_i(int v) {
 
 __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ table, const int* __restrict__ old_len,
                                                              const int* __restrict__ new_len,
-                                                             const int* __restrict__ free_ids, int* __restrict__ slots,
+                                                             const int* __restrict__ free_ids,
+                                                             const int* __restrict__ taken, int* __restrict__ slots,
                                                              int* __restrict__ positions, int* __restrict__ used, int R,
                                                              int width, int nfree, int block, int tokens) {
   __shared__ int first[PX_ITEMS + 1];  // draws before each of this workgroup's requests
@@ -69,6 +70,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
     __syncthreads();
     return wsum[0] + wsum[1] + wsum[2] + wsum[3];
   };
+  const int start = taken != nullptr ? max(*taken, 0) : 0;  // entries of the list that are gone
   int before = 0;
   for (int r = tid; r < r0; r += PX_NT) before += draws(r);
   before = block_sum(before);
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
   __syncthreads();
   if (lane == 63) wsum[wv] = incl;
   __syncthreads();
-  int at = before + incl - run;
+  int at = start + before + incl - run;
   for (int w = 0; w < wv; ++w) at += wsum[w];
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
     int all = 0;
     for (int r = tid; r < R; r += PX_NT) all += draws(r);
     all = block_sum(all);
-    if (tid == 0) *used = all;
+    if (tid == 0) *used = start + all;
   }
 #pragma unroll
   for (int e = 0; e < PX_ITEMS / PX_NT; ++e) {
@@ -174,17 +176,18 @@ __global__ __launch_bounds__(PW_NT) void paged_write_kernel(const U* __restrict_
 extern "C" {
 
 int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, const int32_t* new_lengths,
-                     const int32_t* free_blocks, int32_t* slots, int32_t* positions, int32_t* used, int requests,
-                     int table_width, int num_free, int block_size, int num_tokens) {
+                     const int32_t* free_blocks, const int32_t* taken, int32_t* slots, int32_t* positions,
+                     int32_t* used, int requests, int table_width, int num_free, int block_size, int num_tokens) {
   using namespace edf;
   EDF_REQUIRE(requests > 0 && table_width > 0 && block_size > 0 && num_tokens > 0 && num_free >= 0,
               EDF_ERR_INVALID_ARG, "dimensions must be positive");
   EDF_REQUIRE((long)requests * num_tokens < (1L << 31), EDF_ERR_UNSUPPORTED, "requests x num_tokens must be below 2^31");
   EDF_REQUIRE(table && old_lengths && new_lengths && (free_blocks || num_free == 0) && slots && positions && used,
               EDF_ERR_INVALID_ARG, "null tensor pointer");
+  EDF_REQUIRE(taken != used, EDF_ERR_INVALID_ARG, "taken and used must be two places: workgroups read one while the other is written");
   const unsigned grid = (unsigned)(((long)requests * num_tokens + PX_ITEMS - 1) / PX_ITEMS);
-  paged_extend_kernel<<<grid, PX_NT, 0, as_stream(stream)>>>(table, old_lengths, new_lengths, free_blocks, slots,
-                                                             positions, used, requests, table_width, num_free,
+  paged_extend_kernel<<<grid, PX_NT, 0, as_stream(stream)>>>(table, old_lengths, new_lengths, free_blocks, taken,
+                                                             slots, positions, used, requests, table_width, num_free,
                                                              block_size, num_tokens);
   return check_launch("paged extend");
 }

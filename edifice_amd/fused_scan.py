@@ -1216,14 +1216,14 @@ def _cache_dims(k_cache, v_cache, num_kv_heads, d, like):
 
 
 def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor, free_blocks: torch.Tensor,
-                 block_size: int, num_tokens: int):
+                 block_size: int, num_tokens: int, taken: torch.Tensor = None):
     """Block tables and slots of a paged cache, on the GPU: request r grows from old_lengths[r] to new_lengths[r].
 
     table int32 [R, width] is written in place: pages ceil(old / block_size) .. ceil(new / block_size) - 1 of each
-    request are the next entries of free_blocks (int32 [F]), request by request.  Returns (slots, positions, used):
-    slots, positions int32 [R, num_tokens] of tokens old_lengths[r] + t (-1 past new_lengths[r]; slot -1 too where
-    the table or the list of free blocks ended), and used int32 [1], the blocks drawn (more than F when the list
-    was too short).  The caller takes the first ``used`` entries off its list."""
+    request are the next entries of free_blocks (int32 [F]), request by request, after its first taken[0] (int32 [1];
+    None: 0).  Returns (slots, positions, used): slots, positions int32 [R, num_tokens] of tokens old_lengths[r] + t
+    (-1 past new_lengths[r]; slot -1 too where the table or the list of free blocks ended), and used int32 [1], the
+    next call's ``taken``: more than F when the list was too short."""
     _rank("table", table, 2)
     reqs, width = table.shape
     if not table.is_contiguous() or table.dtype != torch.int32:
@@ -1232,11 +1232,13 @@ def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: to
     new_lengths = _i32("new_lengths", new_lengths, (reqs,))
     _rank("free_blocks", free_blocks, 1)
     free_blocks = _i32("free_blocks", free_blocks, free_blocks.shape)
+    if taken is not None:
+        taken = _i32("taken", taken, (1,))
     _here(table)
     slots, positions = (table.new_empty((reqs, num_tokens)) for _ in range(2))
     used = table.new_empty((1,))
-    nat.call("edf_paged_extend", _stream(), _p(table), _p(old_lengths), _p(new_lengths), _p(free_blocks), _p(slots),
-             _p(positions), _p(used), reqs, width, free_blocks.numel(), int(block_size), int(num_tokens))
+    nat.call("edf_paged_extend", _stream(), _p(table), _p(old_lengths), _p(new_lengths), _p(free_blocks), _p(taken),
+             _p(slots), _p(positions), _p(used), reqs, width, free_blocks.numel(), int(block_size), int(num_tokens))
     return slots, positions, used
 
 

@@ -688,10 +688,10 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  *
  * edf_paged_extend: request r grows from old_lengths[r] to new_lengths[r] tokens (negative ones count as 0;
  *   new <= old: nothing).  Its pages ceil(old / block_size) .. ceil(new / block_size) - 1 (within the table's
- *   width) are the next entries of free_blocks [num_free], request by request, and are written into table; past
- *   the list's end they are -1.  slots, positions [requests, num_tokens]: those of token old_lengths[r] + t, or
- *   -1 past new_lengths[r]; a token without a page has the position and slot -1.  used [1]: pages drawn, which
- *   exceeds num_free when the list was too short.
+ *   width) are the next entries of free_blocks [num_free], request by request, after the first taken[0] (NULL: 0),
+ *   and are written into table; past the list's end they are -1.  slots, positions [requests, num_tokens]: those of token old_lengths[r] + t, or
+ *   -1 past new_lengths[r]; a token without a page has the position and slot -1.  used [1]: taken[0] plus the
+ *   pages drawn (the next call's taken), which exceeds num_free when the list was too short; not taken itself.
  * edf_paged_cache_write: rows of k, v [batch, num_kv_heads, seq, d] into the pages by slots [batch, seq]; slots
  *   outside [0, num_blocks * block_size) are left out.  Slots have to differ from one another.
  * edf_paged_attention: one query per request, q, out [batch, num_heads, d], over the request's first lengths[b]
@@ -701,8 +701,8 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  *   alone, not on lengths, so a captured call may be replayed after lengths and table have changed.
  * ------------------------------------------------------------------------ */
 int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, const int32_t* new_lengths,
-                     const int32_t* free_blocks, int32_t* slots, int32_t* positions, int32_t* used, int requests,
-                     int table_width, int num_free, int block_size, int num_tokens);
+                     const int32_t* free_blocks, const int32_t* taken, int32_t* slots, int32_t* positions,
+                     int32_t* used, int requests, int table_width, int num_free, int block_size, int num_tokens);
 int edf_paged_cache_write(void* stream, const void* k, const void* v, const int32_t* slots, void* k_cache,
                           void* v_cache, long batch, long seq, int num_kv_heads, int head_dim, long num_blocks,
                           int block_size, int dtype);
