@@ -22,7 +22,23 @@ struct WindowArgs {
   float scale, scale_log2;
 };
 
+constexpr int WINDOW_DMA_T = 1 << 22;  // longest sequence of the DMA kernels: a head's buffer stays below 2^31 bytes
+
 EDF_DEVICE bool window_sees(int q, int key, int W, int S) { return key <= q && (q - key < W || key < S); }
+// the same for key first + c of one query, c a constant after unrolling: three values stay in registers
+struct SeesKey {
+  int rel, out, sink;
+  EDF_DEVICE SeesKey(int q, int first, int W, int S) : rel(q - first), out(q - first - W), sink(S - first) {}
+  EDF_DEVICE bool operator()(int c) const { return c <= rel && (c > out || c < sink); }
+};
+
+// A loop bound in a vector register: branches on it are divergent in the compiler's eyes, which then keeps the
+// bodies of a loop apart (as uniform branches they were merged and spilled: 31 registers in the forward at
+// head_dim 128, 592 us against 345).
+EDF_DEVICE int in_vector_register(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 
 // 8 consecutive contraction elements of one row (or column): the operand of one lane for 16 steps of the
 // contraction (lane half g holds steps 8 g .. 8 g + 7).  In float32 step pairs {e, 8 + e} go through eight

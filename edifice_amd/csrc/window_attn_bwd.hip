@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
   };
   auto tile = [&](int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
-    const int k0 = kt.key0(t);
+    const SeesKey sees(myq, kt.key0(t) + 4 * g, a.W, a.S);
     const T *sk = sK[t & 1], *sv = sV[t & 1];
     f32x16 s[NH], dp[NH];
 #pragma unroll
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float x = fast_exp2(fmaf(s[h][r], a.scale_log2, -lse)) * (dp[h][r] - dd);  // 1 / sqrt(d) at the end
-        if constexpr (MASK) x = window_sees(myq, k0 + h * 32 + d_row(r, g), a.W, a.S) ? x : 0.0f;
+        if constexpr (MASK) x = sees(h * 32 + d_row(r, 0)) ? x : 0.0f;
         s[h][r] = x;
       }
 #pragma unroll
@@ -156,6 +156,121 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
         for (int e = 0; e < 4; ++e)
           if (c + e < d) out[c + e] = from_f32<T>(dq[dt][rb * 4 + e] * a.scale);
       }
+    }
+}
+
+// dQ, bf16 at head_dim 128: tiles by DMA loads, each as two 32-key halves so that one half's S and dP are live;
+// two workgroups per CU, so one wave's exponentials and waits overlap another's products.
+__global__ __launch_bounds__(256, 2) void window_dq128_kernel(WindowArgs a) {
+  constexpr int HD = 128, BN = 64, NKK = HD / 16, NDT = HD / 32;
+  __shared__ __attribute__((aligned(16))) bf16 sR0[2 * BN * HD];  // ring slot: K then V
+  __shared__ __attribute__((aligned(16))) bf16 sR1[2 * BN * HD];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  int xb;
+  long bh;
+  head_block(xb, bh);
+  const int T = a.T;
+  const int q0 = (gridDim.x - 1 - xb) * WB_M, qw = q0 + 32 * w, myq = qw + li;
+  const long qrow = bh * T + min(myq, T - 1), kvbase = bh / a.G * T * HD;
+  const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)T * HD * 2);
+  const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)T * HD * 2);
+
+  bf16x8 qf[NKK], of[NKK];
+  float dd = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    const long at = qrow * HD + kk * 16 + 8 * g;
+    qf[kk] = *(const bf16x8*)((const bf16*)a.q + at);
+    of[kk] = *(const bf16x8*)((const bf16*)a.go + at);
+    const bf16x8 ov = *(const bf16x8*)((const bf16*)a.o + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)ov[e], dd);
+  }
+  dd += __shfl_xor(dd, 32);
+  const float lse = a.lse[qrow] * LOG2E;
+  if (g == 0 && myq < T) a.dd[qrow] = dd;
+  f32x16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
+
+  const int grp = l >> 4, i16 = l & 15;
+  const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
+  const int krow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
+  const int ktr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
+  const KeyTiles<WB_M, BN> kt(q0, T, a.W, a.S);
+  const int whole = in_vector_register(kt.first_whole);
+  auto issue = [&](auto bt, int t) {
+    constexpr int B = decltype(bt)::value;
+    const int k0 = kt.key0(t);
+    stage_hb<BN>(rK, B ? sR1 : sR0, k0, wu, l);
+    stage_hb<BN>(rV, (B ? sR1 : sR0) + BN * HD, k0, wu, l);
+  };
+  auto tile = [&](auto bt, int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const bf16* sK = decltype(bt)::value ? sR1 : sR0;
+    const bf16* sV = sK + BN * HD;
+    const int k0 = kt.key0(t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int kb = k0 + 32 * h;
+      if (MASK && !((kb <= qw + 31 && kb + 32 + a.W > qw + 1) || kb < a.S)) continue;  // no visible pair
+      const SeesKey sees(myq, kb + 4 * g, a.W, a.S);
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        const int off = krow[kk & 1] + hb_row_off<BN>(kk, 32 * h);
+        s = mfma32(*(const bf16x8*)(&sK[off]), qf[kk], s);
+        dp = mfma32(*(const bf16x8*)(&sV[off]), of[kk], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = fast_exp2(fmaf(s[r], a.scale_log2, -lse)) * (dp[r] - dd);
+        if constexpr (MASK) x = sees(d_row(r, 0)) ? x : 0.0f;
+        s[r] = x;
+      }
+      bf16x8 df[2];
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) df[kc][e] = (bf16)s[8 * kc + e];
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+          const int o = hb_tr_off<BN>(dt, kc, 32 * h);
+          dq[dt] = mfma32(cat4(lds_read_tr16(&sK[ktr[0] + o]), lds_read_tr16(&sK[ktr[1] + o])), df[kc], dq[dt]);
+        }
+    }
+  };
+  auto step = [&](auto bt, int t) {
+    const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
+    if (t + 1 < kt.count) issue(ot, t + 1);
+    if (t >= whole) tile(bt, t, std::false_type{});
+    else tile(bt, t, std::true_type{});
+    wait_vm();
+    __syncthreads();
+  };
+  const std::integral_constant<int, 0> b0{};
+  const std::integral_constant<int, 1> b1{};
+  issue(b0, 0);
+  wait_vm();
+  __syncthreads();
+  for (int t = 0; t < kt.count; t += 2) {
+    step(b0, t);
+    if (t + 1 < kt.count) step(b1, t + 1);
+  }
+  if (myq >= T) return;
+  bf16* out = (bf16*)a.dq + qrow * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (bf16)(dq[dt][rb * 4 + e] * a.scale);
+      *(bf16x4*)(out + dt * 32 + 8 * rb + 4 * g) = v;
     }
 }
 
@@ -303,15 +418,20 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
     }
     __syncthreads();
   }
-  if (per > 1) {  // this chunk's sums: [dK | dV][dim][key] of the block
-    float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD);
+  if (per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
+    float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int o = (dt * 32 + d_row(r, g)) * WB_M + 32 * w + li;
-        out[o] = dk[dt][r];
-        out[WB_M * HD + o] = dv[dt][r];
+      for (int rb = 0; rb < 4; ++rb) {
+        f32x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = dk[dt][rb * 4 + e];
+          y[e] = dv[dt][rb * 4 + e];
+        }
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) = x;
+        *(f32x4*)(out + WB_M * HD + dt * 32 + 8 * rb + 4 * g) = y;
       }
     return;
   }
@@ -344,32 +464,204 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
     }
 }
 
-// dK, dV of the blocks that were divided: the chunks' sums added in order.  Grid x: the divided blocks, z: 0
-// dK, 1 dV, y: batch x key head.
+// dK, dV, bf16 at head_dim 128: V is read from an LDS copy of the workgroup's 128 keys (its fragments would not
+// fit 256 registers beside the two accumulators), Q and dO come in 32-query tiles by DMA loads, two workgroups per
+// CU.
+__global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
+  constexpr int HD = 128, BQ = 32, NKK = HD / 16, NDT = HD / 32;
+  __shared__ __attribute__((aligned(16))) bf16 sV[WB_M * HD];
+  __shared__ __attribute__((aligned(16))) bf16 sR0[2 * BQ * HD];  // ring slot: Q then dO
+  __shared__ __attribute__((aligned(16))) bf16 sR1[2 * BQ * HD];
+  __shared__ __attribute__((aligned(16))) float sL0[BQ], sL1[BQ], sD0[BQ], sD1[BQ];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  int xb;
+  long bh;  // batch x key head
+  head_block(xb, bh);
+  const int T = a.T;
+  const bool sink_part = xb < a.nsb * a.c_sink;
+  const int xr = sink_part ? xb : xb - a.nsb * a.c_sink;
+  const int per = sink_part ? a.c_sink : a.c_win, len = sink_part ? a.len_sink : a.len_win;
+  const int kblk = (sink_part ? 0 : a.nsb) + xr / per, chunk = xr % per;
+  const int kb0 = kblk * WB_M, kw = kb0 + 32 * w, mykey = kw + li;
+  int qs, nt;
+  query_tiles<BQ>(kb0, T, a.W, a.S, qs, nt);
+  const int t0 = chunk * len, t1 = min(t0 + len, nt * a.G);
+
+  // keys past the end read zero rows of V: they only feed their own columns, never stored
+  stage_hb<WB_M>(make_rsrc((const bf16*)a.v + bh * T * HD, (unsigned)T * HD * 2), sV, kb0, wu, l);
+  bf16x8 kf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk)
+    kf[kk] = *(const bf16x8*)((const bf16*)a.k + (bh * T + min(mykey, T - 1)) * HD + kk * 16 + 8 * g);
+  f32x16 dk[NDT], dv[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    dk[dt] = zero16();
+    dv[dt] = zero16();
+  }
+  float rl = 0.0f, rd = 0.0f;
+  // Tile t into ring slot B: Q and dO by DMA, row sums and D into registers of the first wave, which publish()
+  // writes to LDS once the tile's loads have landed.
+  auto issue = [&](auto bt, int t) {
+    constexpr int B = decltype(bt)::value;
+    const int h = t / nt, q0 = qs + (t - h * nt) * BQ;
+    const long row = (bh * a.G + h) * T;
+    stage_hb<BQ>(make_rsrc((const bf16*)a.q + row * HD, (unsigned)T * HD * 2), B ? sR1 : sR0, q0, wu, l);
+    stage_hb<BQ>(make_rsrc((const bf16*)a.go + row * HD, (unsigned)T * HD * 2), (B ? sR1 : sR0) + BQ * HD, q0, wu, l);
+    if (tid < BQ) {
+      const long q = row + min(q0 + tid, T - 1);
+      rl = q0 + tid < T ? a.lse[q] : INFINITY;  // a query past the end gets P = 0
+      rd = a.dd[q];
+    }
+  };
+  auto publish = [&](auto bt) {
+    constexpr int B = decltype(bt)::value;
+    wait_vm();
+    if (tid < BQ) {
+      (B ? sL1 : sL0)[tid] = rl * LOG2E;
+      (B ? sD1 : sD0)[tid] = rd;
+    }
+  };
+  const int grp = l >> 4, i16 = l & 15;
+  const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
+  const int qrow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
+  const int vrow[2] = {hb_row_base(li, g, 0) + hb_row_off<WB_M>(0, 32 * w),
+                       hb_row_base(li, g, 1) + hb_row_off<WB_M>(0, 32 * w)};
+  const int qtr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
+  auto subtile = [&](auto bt, int qb, auto masked) {
+    constexpr int B = decltype(bt)::value;
+    constexpr bool MASK = decltype(masked)::value;
+    const bf16* sQ = B ? sR1 : sR0;
+    const bf16* sO = sQ + BQ * HD;
+    // distinct barriers keep the two bodies' equal LDS reads from being hoisted above their branch
+    __builtin_amdgcn_sched_barrier(MASK ? 1 : 2);
+    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const int off = qrow[kk & 1] + hb_row_off<BQ>(kk, 0);
+      const bf16x8 vf = *(const bf16x8*)(&sV[vrow[kk & 1] + hb_row_off<WB_M>(kk, 0)]);
+      s = mfma32(*(const bf16x8*)(&sQ[off]), kf[kk], s);
+      dp = mfma32(*(const bf16x8*)(&sO[off]), vf, dp);
+    }
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const f32x4 lv = *(const f32x4*)(&(B ? sL1 : sL0)[8 * rb + 4 * g]);
+      const f32x4 dv4 = *(const f32x4*)(&(B ? sD1 : sD0)[8 * rb + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 4 + e;
+        float p = fast_exp2(fmaf(s[r], a.scale_log2, -lv[e]));
+        float x = p * (dp[r] - dv4[e]);
+        if constexpr (MASK) {
+          const bool see = window_sees(qb + 8 * rb + 4 * g + e, mykey, a.W, a.S);
+          p = see ? p : 0.0f;
+          x = see ? x : 0.0f;
+        }
+        s[r] = p;
+        dp[r] = x;
+      }
+    }
+    bf16x8 pf[2], df[2];
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pf[kc][e] = (bf16)s[8 * kc + e];
+        df[kc][e] = (bf16)dp[8 * kc + e];
+      }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        const int o = hb_tr_off<BQ>(dt, kc, 0);
+        dv[dt] = mfma32(cat4(lds_read_tr16(&sO[qtr[0] + o]), lds_read_tr16(&sO[qtr[1] + o])), pf[kc], dv[dt]);
+        dk[dt] = mfma32(cat4(lds_read_tr16(&sQ[qtr[0] + o]), lds_read_tr16(&sQ[qtr[1] + o])), df[kc], dk[dt]);
+      }
+  };
+  auto step = [&](auto bt, int t) {
+    const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
+    if (t + 1 < t1) issue(ot, t + 1);
+    const int qb = qs + t % nt * BQ;
+    if (!(qb + 31 < kw || (qb > kw + 30 + a.W && kw >= a.S))) {  // some query sees a key of this wave
+      if (qb >= kw + 31 && qb + 31 - kw < a.W) subtile(bt, qb, std::false_type{});
+      else subtile(bt, qb, std::true_type{});
+    }
+    if (t + 1 < t1) publish(ot);
+    __syncthreads();
+  };
+  const std::integral_constant<int, 0> b0{};
+  const std::integral_constant<int, 1> b1{};
+  if (t0 < t1) {
+    issue(b0, t0);
+    publish(b0);
+  } else {
+    wait_vm();
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; t += 2) {
+    step(b0, t);
+    if (t + 1 < t1) step(b1, t + 1);
+  }
+  if (per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
+    float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) {
+        f32x4 x, y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = dk[dt][rb * 4 + e];
+          y[e] = dv[dt][rb * 4 + e];
+        }
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) = x;
+        *(f32x4*)(out + WB_M * HD + dt * 32 + 8 * rb + 4 * g) = y;
+      }
+    return;
+  }
+  if (mykey >= T) return;
+  const long row = (bh * T + mykey) * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      bf16x4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = (bf16)(dk[dt][rb * 4 + e] * a.scale);
+        y[e] = (bf16)dv[dt][rb * 4 + e];
+      }
+      *(bf16x4*)((bf16*)a.dk + row + dt * 32 + 8 * rb + 4 * g) = x;
+      *(bf16x4*)((bf16*)a.dv + row + dt * 32 + 8 * rb + 4 * g) = y;
+    }
+}
+
+// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  Grid x:
+// pieces of the block's [dK | dV][key][dim], y: the divided blocks from `first` on, z: batch x key head.
 template <typename T, int HD, int BQ>
 __global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx, int first, int per) {
-  __shared__ float t[HD * (WB_M + 1)];
-  const int kblk = first + blockIdx.x, kb0 = kblk * WB_M;
-  const long bh = blockIdx.y;
-  const bool is_v = blockIdx.z;
+  const int kblk = first + blockIdx.y, kb0 = kblk * WB_M;
+  const long bh = blockIdx.z;
   int qs, nt;
   query_tiles<BQ>(kb0, a.T, a.W, a.S, qs, nt);
   const int len = kblk < a.nsb ? a.len_sink : a.len_win;
   const int n = min(per, (nt * a.G + len - 1) / len);  // chunks that hold a tile
   const int x0 = kblk < a.nsb ? kblk * a.c_sink : a.nsb * a.c_sink + (kblk - a.nsb) * a.c_win;
-  const float* in = a.part + (bh * gx + x0) * (2L * WB_M * HD) + (is_v ? WB_M * HD : 0);
-  for (int e = threadIdx.x; e < a.d * WB_M; e += 256) {
-    float s = 0.0f;
-    for (int c = 0; c < n; ++c) s += in[c * (2L * WB_M * HD) + e];
-    t[e / WB_M * (WB_M + 1) + e % WB_M] = is_v ? s : s * a.scale;
-  }
-  __syncthreads();
-  T* out = (T*)(is_v ? a.dv : a.dk) + (bh * a.T + kb0) * a.d;
-  const int rows = min(WB_M, a.T - kb0);
-  for (int e = threadIdx.x; e < rows * a.d; e += 256) {
-    const int key = e / a.d, c = e - key * a.d;
-    out[e] = from_f32<T>(t[c * (WB_M + 1) + key]);
-  }
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const bool is_v = e >= WB_M * HD;
+  const int key = e / HD % WB_M, c = e % HD;
+  if (kb0 + key >= a.T || c >= a.d) return;
+  const float* in = a.part + (bh * gx + x0) * (2L * WB_M * HD) + e;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * WB_M * HD));
+  if (!is_v) s *= a.scale;
+  T* out = (T*)(is_v ? a.dv : a.dk) + (bh * a.T + kb0 + key) * a.d + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < a.d) out[i] = from_f32<T>(s[i]);
 }
 
 constexpr int WB_FILL = 512;  // workgroups of the dK, dV kernel that fill the GPU twice over
@@ -397,27 +689,41 @@ KvPlan kv_plan(int heads, int G, int T, int W, int S, int BQ) {
   return p;
 }
 
-template <typename T, int HD, int BN, int BQ, bool VEC>
-int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
-  const unsigned nb = (unsigned)((a.T + WB_M - 1) / WB_M);
-  window_dq_kernel<T, HD, BN, VEC><<<dim3(nb, BH), 256, 0, s>>>(a);
-  int rc = check_launch("window attention dQ");
-  if (rc) return rc;
+// the dK, dV kernel of the call, its query tiles, and the sums of divided blocks
+template <typename T, int HD, int BQ, typename F>
+int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
   const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, BQ);
   a.nsb = p.nsb, a.c_sink = p.c_sink, a.c_win = p.c_win, a.len_sink = p.len_sink, a.len_win = p.len_win;
   const int gx = p.gx();
-  window_dkdv_kernel<T, HD, BQ, VEC><<<dim3(gx, BHkv), 256, 0, s>>>(a);
-  rc = check_launch("window attention dK, dV");
+  kernel<<<dim3(gx, BHkv), 256, 0, s>>>(a);
+  const int rc = check_launch("window attention dK, dV");
   if (rc) return rc;
   if (p.nsb > 0 && p.c_sink > 1)
-    window_sum_kernel<T, HD, BQ><<<dim3(p.nsb, BHkv, 2), 256, 0, s>>>(a, gx, 0, p.c_sink);
+    window_sum_kernel<T, HD, BQ><<<dim3(2 * WB_M * HD / 1024, p.nsb, BHkv), 256, 0, s>>>(a, gx, 0, p.c_sink);
   if (p.nkb > p.nsb && p.c_win > 1)
-    window_sum_kernel<T, HD, BQ><<<dim3(p.nkb - p.nsb, BHkv, 2), 256, 0, s>>>(a, gx, p.nsb, p.c_win);
+    window_sum_kernel<T, HD, BQ><<<dim3(2 * WB_M * HD / 1024, p.nkb - p.nsb, BHkv), 256, 0, s>>>(a, gx, p.nsb, p.c_win);
   return check_launch("window attention dK, dV sums");
 }
 
+constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles: bf16, and float32 or the DMA kernel
+bool dma_kernels(int d, int T, int dtype, bool vec) { return dtype == EDF_BF16 && vec && d == 128 && T <= WINDOW_DMA_T; }
+
+template <typename T, int HD, int BN, int BQ, bool VEC>
+int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
+  const dim3 grid((a.T + WB_M - 1) / WB_M, BH);
+  constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
+  const bool fast = dma && dma_kernels(a.d, a.T, EDF_BF16, VEC);
+  if (fast) window_dq128_kernel<<<grid, 256, 0, s>>>(a);
+  else window_dq_kernel<T, HD, BN, VEC><<<grid, 256, 0, s>>>(a);
+  const int rc = check_launch("window attention dQ");
+  if (rc) return rc;
+  if constexpr (dma) {
+    if (fast) return launch_dkdv<bf16, 128, BQ_32>(s, a, BHkv, window_dkdv128_kernel);
+  }
+  return launch_dkdv<T, HD, BQ>(s, a, BHkv, window_dkdv_kernel<T, HD, BQ, VEC>);
+}
+
 int pad_width(int d) { return (d + 31) / 32 * 32; }
-constexpr int BQ_BF16 = 64, BQ_F32 = 32;
 
 template <typename T, int BN, int BQ, bool VEC>
 int launch_bwd_d(hipStream_t s, const WindowArgs& a, int BH, int BHkv) {
@@ -440,10 +746,14 @@ size_t edf_window_attention_backward_workspace_bytes(int batch, int num_heads, i
   if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || seq_len <= 0 || head_dim <= 0 || window <= 0 || sinks < 0)
     return 0;
   const int W = std::min(window, seq_len), S = std::min(sinks, seq_len), heads = batch * num_kv_heads;
-  const KvPlan p = kv_plan(heads, num_heads / num_kv_heads, seq_len, W, S, dtype == EDF_BF16 ? BQ_BF16 : BQ_F32);
   const size_t rows = ((size_t)batch * num_heads * seq_len * sizeof(float) + 255) & ~(size_t)255;
-  const bool divided = (p.nsb > 0 && p.c_sink > 1) || (p.nkb > p.nsb && p.c_win > 1);
-  return rows + (divided ? (size_t)heads * p.gx() * 2 * WB_M * pad_width(head_dim) * sizeof(float) : 0);
+  size_t sums = 0;  // of the larger of the plans: which kernel runs also depends on the tensors' alignment
+  for (int bq : {BQ_BF16, BQ_32}) {
+    const KvPlan p = kv_plan(heads, num_heads / num_kv_heads, seq_len, W, S, bq);
+    if ((dtype == EDF_BF16 || bq == BQ_32) && ((p.nsb > 0 && p.c_sink > 1) || (p.nkb > p.nsb && p.c_win > 1)))
+      sums = std::max(sums, (size_t)heads * p.gx() * 2 * WB_M * pad_width(head_dim) * sizeof(float));
+  }
+  return rows + sums;
 }
 
 int edf_window_attention_backward(void* stream, const void* q, const void* k, const void* v, const void* out,
@@ -474,8 +784,8 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
   if (dtype == EDF_BF16)
     return vec ? launch_bwd_d<bf16, 64, BQ_BF16, true>(s, a, BH, BHkv)
                : launch_bwd_d<bf16, 64, BQ_BF16, false>(s, a, BH, BHkv);
-  return vec ? launch_bwd_d<float, 32, BQ_F32, true>(s, a, BH, BHkv)
-             : launch_bwd_d<float, 32, BQ_F32, false>(s, a, BH, BHkv);
+  return vec ? launch_bwd_d<float, 32, BQ_32, true>(s, a, BH, BHkv)
+             : launch_bwd_d<float, 32, BQ_32, false>(s, a, BH, BHkv);
 }
 
 }  // extern "C"
