@@ -4,6 +4,8 @@
 // Query i sees key j when j <= i and (i - j < W or j < S).  Query head h reads key head h / G.
 #pragma once
 
+#include <algorithm>
+
 #include "edf_abi.hpp"
 #include "edf_common.hpp"
 #include "edf_mfma.hpp"
@@ -76,6 +78,27 @@ template <> struct WFrag<float> {
     *(f32x4*)(p + 4) = hi;
   }
   EDF_DEVICE void zero() { lo = hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+};
+
+// N steps use(i, load(i)) with the loads A steps ahead of their use: the barriers keep the compiler from sinking a
+// step's LDS reads to its products, whose wait then idles the matrix core (float32 at head_dim 128, dK and dV of
+// 1x8(4)x4000, window 2000: 886 us without).
+template <int N, int A, typename L, typename U>
+EDF_DEVICE void ahead(L load, U use) {
+  decltype(load(0)) f[A];
+#pragma unroll
+  for (int i = 0; i < A && i < N; ++i) f[i] = load(i);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    use(i, f[i % A]);
+    if (i + A < N) f[i % A] = load(i + A);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <typename T>
+struct Pair {
+  WFrag<T> x, y;
 };
 
 // Columns col .. col + 7 of a row of d <= HD elements in memory, zeros past d.  VEC: d a multiple of 16
@@ -163,5 +186,125 @@ struct KeyTiles {
     return x * BN;
   }
 };
+
+// Query tiles of BQ that see a key of block [k0, k0 + KB): from qs on, n of them per query head.
+template <int KB, int BQ>
+EDF_DEVICE void query_tiles(int k0, int T, int W, int S, int& qs, int& n) {
+  qs = k0;
+  const int end = k0 < S ? T : min(T, k0 + KB - 1 + W);  // one past the last query
+  n = (end - qs + BQ - 1) / BQ;
+}
+
+// The key block of workgroup xb of a dK, dV kernel and its share [t0, t1) of the block's (query head, tile) pairs,
+// nt tiles a head from query qs on; per: workgroups that share the block.
+template <int KB, int BQ>
+struct KeyChunk {
+  int key0, qs, nt, t0, t1, per;
+  EDF_DEVICE KeyChunk(const WindowArgs& a, int xb) {
+    const bool sink = xb < a.nsb * a.c_sink;
+    const int x = sink ? xb : xb - a.nsb * a.c_sink, len = sink ? a.len_sink : a.len_win;
+    per = sink ? a.c_sink : a.c_win;
+    const int blk = (sink ? 0 : a.nsb) + x / per;
+    key0 = blk * KB;
+    query_tiles<KB, BQ>(key0, a.T, a.W, a.S, qs, nt);
+    t0 = x % per * len;
+    t1 = min(t0 + len, nt * a.G);
+  }
+};
+
+// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  Grid x:
+// pieces of the block's [dK | dV][key][dim], y: the divided blocks from `first` on, z: batch x key head.
+template <typename T, int HD, int KB, int BQ>
+__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx, int first, int per) {
+  const int kblk = first + blockIdx.y, kb0 = kblk * KB;
+  const long bh = blockIdx.z;
+  int qs, nt;
+  query_tiles<KB, BQ>(kb0, a.T, a.W, a.S, qs, nt);
+  const int len = kblk < a.nsb ? a.len_sink : a.len_win;
+  const int n = min(per, (nt * a.G + len - 1) / len);  // chunks that hold a tile
+  const int x0 = kblk < a.nsb ? kblk * a.c_sink : a.nsb * a.c_sink + (kblk - a.nsb) * a.c_win;
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const bool is_v = e >= KB * HD;
+  const int key = e / HD % KB, c = e % HD;
+  if (kb0 + key >= a.T || c >= a.d) return;
+  const float* in = a.part + (bh * gx + x0) * (2L * KB * HD) + e;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * KB * HD));
+  if (!is_v) s *= a.scale;
+  T* out = (T*)(is_v ? a.dv : a.dk) + (bh * a.T + kb0 + key) * a.d + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < a.d) out[i] = from_f32<T>(s[i]);
+}
+
+struct KvPlan {
+  int nkb, nsb, c_sink, c_win, len_sink, len_win;
+  int gx() const { return nsb * c_sink + (nkb - nsb) * c_win; }
+  bool divided() const { return (nsb > 0 && c_sink > 1) || (nkb > nsb && c_win > 1); }
+};
+// How many workgroups share the tiles of a block of KB keys.  The GPU runs `slots` workgroups at once, so a call takes
+// about ceil(workgroups / slots) rounds of the longest share, and every workgroup of a divided block costs `join`
+// tiles more for its float32 sums, written and read again: the division with the least of that is taken.  A sink
+// block's tiles are divided into shares no longer than another block's (with many sink keys into longer ones, so
+// that there are not more of them than four rounds).
+inline KvPlan kv_plan(int heads, int G, int T, int W, int S, int KB, int BQ, int slots, int join) {
+  KvPlan best{};
+  double least = 0.0;
+  const int nkb = (T + KB - 1) / KB, nsb = std::min(nkb, (S + KB - 1) / KB);
+  const long n_sink = (long)G * ((T + BQ - 1) / BQ);
+  const long n_win = std::min(n_sink, (long)G * ((KB - 1 + W + BQ - 1) / BQ));
+  for (long c = 1; c <= 64 && c <= n_win; ++c) {
+    KvPlan p{nkb, nsb, 1, 1, 0, 0};
+    p.len_win = (int)((n_win + c - 1) / c);
+    p.c_win = (int)((n_win + p.len_win - 1) / p.len_win);
+    p.len_sink = (int)std::max((long)p.len_win, (n_sink * nsb * heads + 4L * slots - 1) / (4L * slots));
+    p.c_sink = (int)std::max(1L, (n_sink + p.len_sink - 1) / p.len_sink);
+    const double wgs = (double)heads * p.gx(), rounds = std::max(1.0, wgs / slots);
+    // a last round that is not full counts by half of what it lacks: workgroups end at different times
+    const double whole = (double)(long)(rounds + 0.999999);
+    const double cost = 0.5 * (rounds + whole) * (std::max(p.len_win, nsb > 0 ? p.len_sink : 0) + 2.0 +
+                                                  (p.c_win > 1 ? join : 0));
+    if (c == 1 || cost < least) best = p, least = cost;
+  }
+  return best;
+}
+
+inline int window_pad(int d) { return (d + 31) / 32 * 32; }
+
+// workgroups of a dK, dV kernel that run at once (256 CUs; the registers leave one or two a CU)
+template <typename T>
+int kv_slots(int hd) {
+  return sizeof(T) == 4 && hd > 64 ? 256 : 512;
+}
+// the cost of a workgroup's sums in tiles of BQ queries: 8 KB HD bytes written and read again against 8 KB BQ HD
+// flops, at the rates of a CU (about 40 bytes and 250 float32 or 2000 bf16 flops a cycle)
+template <typename T>
+int kv_join(int KB, int BQ) {
+  return sizeof(T) == 4 ? 2 : 16 * 32 / BQ;
+}
+
+// a dK, dV kernel and the sums of the blocks that several of its workgroups share
+template <typename T, int HD, int KB, int BQ, typename F>
+int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
+  const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, KB, BQ, kv_slots<T>(HD), kv_join<T>(KB, BQ));
+  a.nsb = p.nsb, a.c_sink = p.c_sink, a.c_win = p.c_win, a.len_sink = p.len_sink, a.len_win = p.len_win;
+  const int gx = p.gx(), pieces = 2 * KB * HD / 1024;
+  kernel<<<dim3(gx, BHkv), 256, 0, s>>>(a);
+  const int rc = check_launch("window attention dK, dV");
+  if (rc) return rc;
+  if (p.nsb > 0 && p.c_sink > 1)
+    window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, p.nsb, BHkv), 256, 0, s>>>(a, gx, 0, p.c_sink);
+  if (p.nkb > p.nsb && p.c_win > 1)
+    window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, p.nkb - p.nsb, BHkv), 256, 0, s>>>(a, gx, p.nsb, p.c_win);
+  return check_launch("window attention dK, dV sums");
+}
+
+// The narrow kernels (window_narrow.hip): forward, or dQ with D.  They take the calls whose 128-query workgroups would
+// leave the GPU half empty.  Forward, window 256, wide against narrow: 128 wide workgroups bf16 18.8 / 17.5 us
+// (1x32x500x128) and 15.4 / 11.5 (x64), float32 64.8 / 45.5 and 37.1 / 25.7; 192 of them bf16 19.7 / 30.5 (1x16x1500x128)
+// and 15.8 / 14.6, float32 65.8 / 68.2 and 38.5 / 40.8.
+int window_narrow_run(bool backward, hipStream_t s, const WindowArgs& a, int BH, int dtype);
+inline bool window_narrow(int BH, int T, bool vec) { return vec && (long)BH * ((T + 127) / 128) < 160; }
 
 }  // namespace edf

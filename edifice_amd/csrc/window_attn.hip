@@ -28,7 +28,7 @@ constexpr int WA_BM = 128;
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
-  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256;
+  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 2 ? 4 : 1;
   using Tile = WTile<T, HD, BN>;
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
@@ -79,11 +79,10 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
     const T *sk = sK[t & 1], *sv = sV[t & 1];
     f32x16 s[NH];
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      s[h] = zero16();
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) s[h] = WFrag<T>::mma(Tile::row(sk, h * 32 + li, kk * 16 + 8 * g), qf[kk], s[h]);
-    }
+    for (int h = 0; h < NH; ++h) s[h] = zero16();
+    // consecutive products go to different halves' scores
+    ahead<NH * NKK, AHEAD>([&](int i) { return Tile::row(sk, i % NH * 32 + li, i / NH * 16 + 8 * g); },
+                           [&](int i, const WFrag<T>& f) { s[i % NH] = WFrag<T>::mma(f, qf[i / NH], s[i % NH]); });
     float mx = -INFINITY;
 #pragma unroll
     for (int h = 0; h < NH; ++h)
@@ -113,14 +112,13 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
         rs += s[h][r];
       }
     lsum += rs + __shfl_xor(rs, 32);
+    WFrag<T> pf[2 * NH];
 #pragma unroll
-    for (int kc = 0; kc < 2 * NH; ++kc) {
-      WFrag<T> pf;
+    for (int kc = 0; kc < 2 * NH; ++kc)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pf.set(e, s[kc >> 1][8 * (kc & 1) + e]);
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) o[dt] = WFrag<T>::mma(Tile::trans(sv, 16 * kc, dt, l), pf, o[dt]);
-    }
+      for (int e = 0; e < 8; ++e) pf[kc].set(e, s[kc >> 1][8 * (kc & 1) + e]);
+    ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sv, 16 * (i / NDT), i % NDT, l); },
+                               [&](int i, const WFrag<T>& f) { o[i % NDT] = WFrag<T>::mma(f, pf[i / NDT], o[i % NDT]); });
   };
   auto advance = [&](int t) {  // the next tile into the other buffer, the one after it into registers
     if (t + 1 < kt.count) {
@@ -425,6 +423,7 @@ int edf_window_attention(void* stream, const void* q, const void* k, const void*
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15);
   hipStream_t s = as_stream(stream);
   const int BH = batch * num_heads;
+  if (window_narrow(BH, seq_len, vec)) return window_narrow_run(false, s, a, BH, dtype);
   if (dtype == EDF_BF16)
     vec ? launch_fwd<bf16, 64, true>(s, a, BH) : launch_fwd<bf16, 64, false>(s, a, BH);
   else

@@ -30,7 +30,7 @@ constexpr int WB_M = 128;  // queries (dQ) or keys (dK, dV) per workgroup
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
-  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256;
+  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 2 ? 3 : 1;
   using Tile = WTile<T, HD, BN>;
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
@@ -94,12 +94,16 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
     for (int h = 0; h < NH; ++h) {
       s[h] = zero16();
       dp[h] = zero16();
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) {
-        s[h] = WFrag<T>::mma(Tile::row(sk, h * 32 + li, kk * 16 + 8 * g), qf[kk], s[h]);
-        dp[h] = WFrag<T>::mma(Tile::row(sv, h * 32 + li, kk * 16 + 8 * g), of[kk], dp[h]);
-      }
     }
+    ahead<NH * NKK, AHEAD>(
+        [&](int i) {
+          const int row = i / NKK * 32 + li, col = i % NKK * 16 + 8 * g;
+          return Pair<T>{Tile::row(sk, row, col), Tile::row(sv, row, col)};
+        },
+        [&](int i, const Pair<T>& f) {
+          s[i / NKK] = WFrag<T>::mma(f.x, qf[i % NKK], s[i / NKK]);
+          dp[i / NKK] = WFrag<T>::mma(f.y, of[i % NKK], dp[i / NKK]);
+        });
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -108,14 +112,13 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
         if constexpr (MASK) x = sees(h * 32 + d_row(r, 0)) ? x : 0.0f;
         s[h][r] = x;
       }
+    WFrag<T> df[2 * NH];
 #pragma unroll
-    for (int kc = 0; kc < 2 * NH; ++kc) {
-      WFrag<T> df;
+    for (int kc = 0; kc < 2 * NH; ++kc)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) df.set(e, s[kc >> 1][8 * (kc & 1) + e]);
-#pragma unroll
-      for (int dt = 0; dt < NDT; ++dt) dq[dt] = WFrag<T>::mma(Tile::trans(sk, 16 * kc, dt, l), df, dq[dt]);
-    }
+      for (int e = 0; e < 8; ++e) df[kc].set(e, s[kc >> 1][8 * (kc & 1) + e]);
+    ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sk, 16 * (i / NDT), i % NDT, l); },
+                               [&](int i, const WFrag<T>& f) { dq[i % NDT] = WFrag<T>::mma(f, df[i / NDT], dq[i % NDT]); });
   };
   auto advance = [&](int t) {
     if (t + 1 < kt.count) {
@@ -274,18 +277,10 @@ __global__ __launch_bounds__(256, 2) void window_dq128_kernel(WindowArgs a) {
     }
 }
 
-// Query tiles of BQ that see a key of block [k0, k0 + WB_M): from qs on, n of them per query head.
-template <int BQ>
-EDF_DEVICE void query_tiles(int k0, int T, int W, int S, int& qs, int& n) {
-  qs = k0;
-  const int end = k0 < S ? T : min(T, k0 + WB_M - 1 + W);  // one past the last query
-  n = (end - qs + BQ - 1) / BQ;
-}
-
 template <typename T, int HD, int BQ, bool VEC>
 __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32;
-  constexpr int CPR = HD / 8, PIECES = BQ * CPR, CPT = (PIECES + 255) / 256;
+  constexpr int CPR = HD / 8, PIECES = BQ * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 2 ? 3 : 1;
   using Tile = WTile<T, HD, BQ>;
   __shared__ __attribute__((aligned(16))) T sQ[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sO[2][Tile::ELEMS];
@@ -296,15 +291,8 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
   long bh;  // batch x key head
   head_block(xb, bh);
   const int T_ = a.T, d = a.d;
-  // which key block, and which of its chunks of tiles
-  const bool sink_part = xb < a.nsb * a.c_sink;
-  const int xr = sink_part ? xb : xb - a.nsb * a.c_sink;
-  const int per = sink_part ? a.c_sink : a.c_win, len = sink_part ? a.len_sink : a.len_win;
-  const int kblk = (sink_part ? 0 : a.nsb) + xr / per, chunk = xr % per;
-  const int kb0 = kblk * WB_M, kw = kb0 + 32 * w, mykey = kw + li;
-  int qs, nt;
-  query_tiles<BQ>(kb0, T_, a.W, a.S, qs, nt);
-  const int t0 = chunk * len, t1 = min(t0 + len, nt * a.G);  // tiles (query head, tile) of this workgroup
+  const KeyChunk<WB_M, BQ> kc_(a, xb);
+  const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
 
   const T* K = (const T*)a.k + bh * T_ * d;
   const T* V = (const T*)a.v + bh * T_ * d;
@@ -370,11 +358,15 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
       auto subtile = [&](auto masked) {
         constexpr bool MASK = decltype(masked)::value;
         f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-        for (int kk = 0; kk < NKK; ++kk) {
-          s = WFrag<T>::mma(Tile::row(sQ[buf], 32 * sub + li, kk * 16 + 8 * g), kf[kk], s);
-          dp = WFrag<T>::mma(Tile::row(sO[buf], 32 * sub + li, kk * 16 + 8 * g), vf[kk], dp);
-        }
+        ahead<NKK, AHEAD>(
+            [&](int i) {
+              const int row = 32 * sub + li, col = i * 16 + 8 * g;
+              return Pair<T>{Tile::row(sQ[buf], row, col), Tile::row(sO[buf], row, col)};
+            },
+            [&](int i, const Pair<T>& f) {
+              s = WFrag<T>::mma(f.x, kf[i], s);
+              dp = WFrag<T>::mma(f.y, vf[i], dp);
+            });
 #pragma unroll
         for (int rb = 0; rb < 4; ++rb) {
           const f32x4 lv = *(const f32x4*)(&sL[buf][32 * sub + 8 * rb + 4 * g]);
@@ -393,20 +385,23 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
             dp[r] = x;
           }
         }
+        WFrag<T> pf[2], df[2];
 #pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-          WFrag<T> pf, df;
+        for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            pf.set(e, s[8 * kc + e]);
-            df.set(e, dp[8 * kc + e]);
+            pf[kc].set(e, s[8 * kc + e]);
+            df[kc].set(e, dp[8 * kc + e]);
           }
-#pragma unroll
-          for (int dt = 0; dt < NDT; ++dt) {
-            dv[dt] = WFrag<T>::mma(Tile::trans(sO[buf], 32 * sub + 16 * kc, dt, l), pf, dv[dt]);
-            dk[dt] = WFrag<T>::mma(Tile::trans(sQ[buf], 32 * sub + 16 * kc, dt, l), df, dk[dt]);
-          }
-        }
+        ahead<2 * NDT, AHEAD>(
+            [&](int i) {
+              const int r0 = 32 * sub + 16 * (i / NDT);
+              return Pair<T>{Tile::trans(sO[buf], r0, i % NDT, l), Tile::trans(sQ[buf], r0, i % NDT, l)};
+            },
+            [&](int i, const Pair<T>& f) {
+              dv[i % NDT] = WFrag<T>::mma(f.x, pf[i / NDT], dv[i % NDT]);
+              dk[i % NDT] = WFrag<T>::mma(f.y, df[i / NDT], dk[i % NDT]);
+            });
       };
       // every pair visible: the queries lie past the wave's keys and within the window of its first
       if (qb >= kw + 31 && qb + 31 - kw < a.W) subtile(std::false_type{});
@@ -418,7 +413,7 @@ __global__ __launch_bounds__(256, 1) void window_dkdv_kernel(WindowArgs a) {
     }
     __syncthreads();
   }
-  if (per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
+  if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
     float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
@@ -480,14 +475,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
   long bh;  // batch x key head
   head_block(xb, bh);
   const int T = a.T;
-  const bool sink_part = xb < a.nsb * a.c_sink;
-  const int xr = sink_part ? xb : xb - a.nsb * a.c_sink;
-  const int per = sink_part ? a.c_sink : a.c_win, len = sink_part ? a.len_sink : a.len_win;
-  const int kblk = (sink_part ? 0 : a.nsb) + xr / per, chunk = xr % per;
-  const int kb0 = kblk * WB_M, kw = kb0 + 32 * w, mykey = kw + li;
-  int qs, nt;
-  query_tiles<BQ>(kb0, T, a.W, a.S, qs, nt);
-  const int t0 = chunk * len, t1 = min(t0 + len, nt * a.G);
+  const KeyChunk<WB_M, BQ> kc_(a, xb);
+  const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
 
   // keys past the end read zero rows of V: they only feed their own columns, never stored
   stage_hb<WB_M>(make_rsrc((const bf16*)a.v + bh * T * HD, (unsigned)T * HD * 2), sV, kb0, wu, l);
@@ -604,7 +593,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
     step(b0, t);
     if (t + 1 < t1) step(b1, t + 1);
   }
-  if (per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
+  if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
     float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
@@ -638,73 +627,6 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
     }
 }
 
-// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  Grid x:
-// pieces of the block's [dK | dV][key][dim], y: the divided blocks from `first` on, z: batch x key head.
-template <typename T, int HD, int BQ>
-__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx, int first, int per) {
-  const int kblk = first + blockIdx.y, kb0 = kblk * WB_M;
-  const long bh = blockIdx.z;
-  int qs, nt;
-  query_tiles<BQ>(kb0, a.T, a.W, a.S, qs, nt);
-  const int len = kblk < a.nsb ? a.len_sink : a.len_win;
-  const int n = min(per, (nt * a.G + len - 1) / len);  // chunks that hold a tile
-  const int x0 = kblk < a.nsb ? kblk * a.c_sink : a.nsb * a.c_sink + (kblk - a.nsb) * a.c_win;
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;
-  const bool is_v = e >= WB_M * HD;
-  const int key = e / HD % WB_M, c = e % HD;
-  if (kb0 + key >= a.T || c >= a.d) return;
-  const float* in = a.part + (bh * gx + x0) * (2L * WB_M * HD) + e;
-  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * WB_M * HD));
-  if (!is_v) s *= a.scale;
-  T* out = (T*)(is_v ? a.dv : a.dk) + (bh * a.T + kb0 + key) * a.d + c;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (c + i < a.d) out[i] = from_f32<T>(s[i]);
-}
-
-constexpr int WB_FILL = 512;  // workgroups of the dK, dV kernel that fill the GPU twice over
-
-struct KvPlan {
-  int nkb, nsb, c_sink, c_win, len_sink, len_win;
-  int gx() const { return nsb * c_sink + (nkb - nsb) * c_win; }
-};
-// How many workgroups share a key block's tiles: one where the blocks alone fill the GPU, else as many as fill
-// it; a sink block's tiles are divided into chunks no longer than another block's.
-KvPlan kv_plan(int heads, int G, int T, int W, int S, int BQ) {
-  KvPlan p;
-  p.nkb = (T + WB_M - 1) / WB_M;
-  p.nsb = std::min(p.nkb, (S + WB_M - 1) / WB_M);
-  const long n_sink = (long)G * ((T + BQ - 1) / BQ);
-  const long n_win = std::min(n_sink, (long)G * ((WB_M - 1 + W + BQ - 1) / BQ));
-  const long want = std::max(1L, WB_FILL / std::max(1L, (long)p.nkb * heads));
-  p.c_win = (int)std::min(want, n_win);
-  p.len_win = (int)((n_win + p.c_win - 1) / p.c_win);
-  p.c_win = (int)((n_win + p.len_win - 1) / p.len_win);
-  // (many sink keys: no more workgroups, each with its float32 sums, than fill the GPU four times over)
-  const long all = n_sink * p.nsb * heads;
-  p.len_sink = (int)std::max((long)p.len_win, (all + 4 * WB_FILL - 1) / (4 * WB_FILL));
-  p.c_sink = (int)std::max(1L, (n_sink + p.len_sink - 1) / p.len_sink);
-  return p;
-}
-
-// the dK, dV kernel of the call, its query tiles, and the sums of divided blocks
-template <typename T, int HD, int BQ, typename F>
-int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
-  const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, BQ);
-  a.nsb = p.nsb, a.c_sink = p.c_sink, a.c_win = p.c_win, a.len_sink = p.len_sink, a.len_win = p.len_win;
-  const int gx = p.gx();
-  kernel<<<dim3(gx, BHkv), 256, 0, s>>>(a);
-  const int rc = check_launch("window attention dK, dV");
-  if (rc) return rc;
-  if (p.nsb > 0 && p.c_sink > 1)
-    window_sum_kernel<T, HD, BQ><<<dim3(2 * WB_M * HD / 1024, p.nsb, BHkv), 256, 0, s>>>(a, gx, 0, p.c_sink);
-  if (p.nkb > p.nsb && p.c_win > 1)
-    window_sum_kernel<T, HD, BQ><<<dim3(2 * WB_M * HD / 1024, p.nkb - p.nsb, BHkv), 256, 0, s>>>(a, gx, p.nsb, p.c_win);
-  return check_launch("window attention dK, dV sums");
-}
-
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles: bf16, and float32 or the DMA kernel
 bool dma_kernels(int d, int T, int dtype, bool vec) { return dtype == EDF_BF16 && vec && d == 128 && T <= WINDOW_DMA_T; }
 
@@ -713,21 +635,25 @@ int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
   const dim3 grid((a.T + WB_M - 1) / WB_M, BH);
   constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
   const bool fast = dma && dma_kernels(a.d, a.T, EDF_BF16, VEC);
-  if (fast) window_dq128_kernel<<<grid, 256, 0, s>>>(a);
-  else window_dq_kernel<T, HD, BN, VEC><<<grid, 256, 0, s>>>(a);
-  const int rc = check_launch("window attention dQ");
+  int rc = EDF_OK;
+  if (window_narrow(BH, a.T, VEC)) {
+    rc = window_narrow_run(true, s, a, BH, sizeof(T) == 2 ? EDF_BF16 : EDF_F32);
+  } else {
+    if (fast) window_dq128_kernel<<<grid, 256, 0, s>>>(a);
+    else window_dq_kernel<T, HD, BN, VEC><<<grid, 256, 0, s>>>(a);
+    rc = check_launch("window attention dQ");
+  }
   if (rc) return rc;
   if constexpr (dma) {
-    if (fast) return launch_dkdv<bf16, 128, BQ_32>(s, a, BHkv, window_dkdv128_kernel);
+    if (fast) return launch_dkdv<bf16, 128, WB_M, BQ_32>(s, a, BHkv, window_dkdv128_kernel);
   }
-  return launch_dkdv<T, HD, BQ>(s, a, BHkv, window_dkdv_kernel<T, HD, BQ, VEC>);
+  return launch_dkdv<T, HD, WB_M, BQ>(s, a, BHkv, window_dkdv_kernel<T, HD, BQ, VEC>);
 }
 
-int pad_width(int d) { return (d + 31) / 32 * 32; }
 
 template <typename T, int BN, int BQ, bool VEC>
 int launch_bwd_d(hipStream_t s, const WindowArgs& a, int BH, int BHkv) {
-  switch (pad_width(a.d)) {
+  switch (window_pad(a.d)) {
     case 32: return launch_bwd<T, 32, BN, BQ, VEC>(s, a, BH, BHkv);
     case 64: return launch_bwd<T, 64, BN, BQ, VEC>(s, a, BH, BHkv);
     case 96: return launch_bwd<T, 96, BN, BQ, VEC>(s, a, BH, BHkv);
@@ -747,12 +673,17 @@ size_t edf_window_attention_backward_workspace_bytes(int batch, int num_heads, i
     return 0;
   const int W = std::min(window, seq_len), S = std::min(sinks, seq_len), heads = batch * num_kv_heads;
   const size_t rows = ((size_t)batch * num_heads * seq_len * sizeof(float) + 255) & ~(size_t)255;
-  size_t sums = 0;  // of the larger of the plans: which kernel runs also depends on the tensors' alignment
-  for (int bq : {BQ_BF16, BQ_32}) {
-    const KvPlan p = kv_plan(heads, num_heads / num_kv_heads, seq_len, W, S, bq);
-    if ((dtype == EDF_BF16 || bq == BQ_32) && ((p.nsb > 0 && p.c_sink > 1) || (p.nkb > p.nsb && p.c_win > 1)))
-      sums = std::max(sums, (size_t)heads * p.gx() * 2 * WB_M * pad_width(head_dim) * sizeof(float));
-  }
+  // of the largest of the plans that may run: which one does also depends on the tensors' alignment
+  size_t sums = 0;
+  auto need = [&](int kb, int bq) {
+    const int hd = window_pad(head_dim), G = num_heads / num_kv_heads;
+    const KvPlan p = dtype == EDF_BF16
+                         ? kv_plan(heads, G, seq_len, W, S, kb, bq, kv_slots<bf16>(hd), kv_join<bf16>(kb, bq))
+                         : kv_plan(heads, G, seq_len, W, S, kb, bq, kv_slots<float>(hd), kv_join<float>(kb, bq));
+    if (p.divided()) sums = std::max(sums, (size_t)heads * p.gx() * 2 * kb * hd * sizeof(float));
+  };
+  need(WB_M, BQ_32);
+  if (dtype == EDF_BF16) need(WB_M, BQ_BF16);
   return rows + sums;
 }
 
