@@ -6,13 +6,15 @@
 // element pair, so the kernel is bound by memory up to about G = 60 in bf16.
 //
 // The visible keys are numbered through (sinks, then the window) and cut into chunks; a workgroup of four
-// waves takes one chunk of one key head, each wave tiles of 32 keys with an online softmax of its own:
-//   S^T [32 keys][16 queries] = K Q^T: MFMA 16x16x32, the K operand straight from its pages (a lane's 8
-//   elements of one key are contiguous), queries padded to 16 columns;
-//   O^T [d][16 queries] += V^T P^T: P^T is the S^T registers (a lane holds keys 4 g .. + 3 of both
-//   16-key halves), V^T comes from a wave-private LDS copy of the tile by transposed reads in that order.
-// A tile's keys and values are loaded into registers while the one before is computed; page numbers are
-// looked up one tile further ahead, one key per lane, and handed around the wave by shuffles.
+// waves takes one chunk of one key head, each wave tiles of 32 keys (16 where rows are longer than 256 bytes) with an
+// online softmax of its own:
+//   S^T [16 keys][16 queries] = K Q^T: MFMA 16x16x32, queries padded to 16 columns;
+//   O^T [d][16 queries] += V^T P^T: P^T is the S^T registers (a lane holds keys 4 g .. + 3 of each 16),
+//   V^T comes by transposed reads in that order.
+// Both tiles pass through wave-private LDS: whole rows are read from memory, 16 lanes a row (the matrix operands'
+// own pattern, 64-byte pieces of 16 rows, reaches 4.8 TB/s where whole rows reach 5.2), and the loads of the next
+// tile go out as soon as this one's registers are in LDS.  Page numbers are looked up one tile further ahead, one key
+// per lane, and handed around the wave by shuffles.
 // The waves' results are joined in LDS; with more than one chunk the workgroup leaves (O, max, sum) in
 // float32 and a second kernel joins the chunks.
 // float32 runs the same way on the float32 matrix instructions (eight 16x16x4 per 32 elements).
@@ -22,6 +24,7 @@
 // Keys of a page outside [0, num_blocks) are left out, and a request without keys answers with zeros.
 #include <math.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -35,15 +38,14 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 constexpr int PA_WAVES = 4;
-constexpr int PA_KEYS = 32;                    // keys per wave tile
-constexpr int PA_STEP = PA_WAVES * PA_KEYS;    // keys per workgroup step
+constexpr int PA_STEP = 128;                   // chunks are whole steps of four waves' tiles of 32 keys
 constexpr int PA_MAX_SPLITS = 256;
 
 struct PagedArgs {
   const void *q, *kc, *vc;
   const int *table, *len;
   void* out;
-  float* part;  // [B Hq][splits][d] outputs, then [B Hq][splits][2] (max in log2 units, sum)
+  float* part;  // [B Hq][splits][d rounded up to 4] outputs, then [B Hq][splits][2] (max in log2 units, sum)
   float* ml;
   int B, Hq, Hkv, G, qt, d, width, block, window, sinks, splits, chunk;
   long num_blocks;
@@ -86,14 +88,20 @@ template <> struct Frag<float> {
   }
 };
 
-// columns col .. col + 7 of a row of d elements, zeros past d.  VEC: whole 16-byte pieces.
-template <typename T, int HD, bool VEC>
+// How rows are read: element by element, in 16-byte pieces, or in 16-byte pieces with d = HD (no element past d, and
+// the pieces of a row are immediate offsets from one address).
+enum { BY_ELEMENT, BY_PIECE, WHOLE };
+
+// columns col .. col + 7 of a row of d elements, zeros past d
+template <typename T, int HD, int MODE>
 EDF_DEVICE Frag<T> row_frag(const T* row, int col, int d) {
   Frag<T> f;
-  if constexpr (VEC && sizeof(T) == 2) {
+  if constexpr (MODE == WHOLE) {
+    f.load(row + col);
+  } else if constexpr (MODE == BY_PIECE && sizeof(T) == 2) {
     f.load(row + min(col, d - 8));
     if (d < HD && col >= d) f.zero();
-  } else if constexpr (VEC) {
+  } else if constexpr (MODE == BY_PIECE) {
     f.lo = *(const f32x4*)(row + min(col, d - 4));
     f.hi = *(const f32x4*)(row + min(col + 4, d - 4));
     if (d < HD) {
@@ -110,37 +118,57 @@ EDF_DEVICE Frag<T> row_frag(const T* row, int col, int d) {
   return f;
 }
 
-template <typename T, int HD>
-struct VTile {  // a wave's 32 x HD value tile in LDS
-  static constexpr int LD = sizeof(T) == 2 ? 0 : HD + 4;
-  static constexpr int ELEMS = sizeof(T) == 2 ? lds_tile_elems<HD>(PA_KEYS) : PA_KEYS * (HD + 4);
+// A wave's tile of 16 NT rows in LDS: row operands, and the transposed operand of 16 dims and keys 4 g .. + 3 of each
+// 16, with P in the same key order.
+template <typename T, int HD, int NT>
+struct KVTile {
+  static constexpr int ROWS = 16 * NT;
+  static constexpr int ELEMS = sizeof(T) == 2 ? lds_tile_elems<HD>(ROWS) : ROWS * (HD + 4);
   EDF_DEVICE static int off(int row, int col) {
     if constexpr (sizeof(T) == 2) return lds_off<HD>(row, col);
-    else return row * LD + col;
+    else return row * (HD + 4) + col;
   }
-  // V^T operand: dims 16 dt + i, keys 4 g .. + 3 and 16 + 4 g .. + 3
-  EDF_DEVICE static Frag<T> trans(const T* t, int dt, int g, int i) {
+  EDF_DEVICE static Frag<T> row(const T* t, int r, int col) {
     Frag<T> f;
+    f.load(t + off(r, col));
+    return f;
+  }
+  // o += V^T P^T for dims 16 dt + i; p: the lane's 4 NT probabilities
+  EDF_DEVICE static f32x4 pv(const T* t, int dt, int g, int i, const float* p, f32x4 o) {
     if constexpr (sizeof(T) == 2) {
       const int row = 4 * g + (i >> 2), col = 16 * dt + 4 * (i & 3);
-      f.v = cat4(lds_read_tr16(t + off(row, col)), lds_read_tr16(t + off(row + 16, col)));
+      if constexpr (NT == 2) {
+        Frag<T> v, pf;
+        v.v = cat4(lds_read_tr16(t + off(row, col)), lds_read_tr16(t + off(row + 16, col)));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pf.set(e, p[e]);
+        return Frag<T>::mma(v, pf, o);
+      } else {
+        typedef __attribute__((ext_vector_type(4))) short s16x4;
+        bf16x4 pf;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pf[e] = (bf16)p[e];
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, lds_read_tr16(t + off(row, col))),
+                                                         __builtin_bit_cast(s16x4, pf), o, 0, 0, 0);
+      }
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f.lo[e] = t[off(4 * g + e, 16 * dt + i)];
-        f.hi[e] = t[off(16 + 4 * g + e, 16 * dt + i)];
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o = __builtin_amdgcn_mfma_f32_16x16x4f32(t[off(16 * n + 4 * g + e, 16 * dt + i)], p[4 * n + e], o, 0, 0, 0);
+      return o;
     }
-    return f;
   }
 };
 
-template <typename T, int HD, bool VEC>
+template <typename T, int HD, int MODE>
 __global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_attn_kernel(PagedArgs a) {
+  constexpr int NT = HD * sizeof(T) > 256 ? 1 : 2, KEYS = 16 * NT, STEP = PA_WAVES * KEYS;
   constexpr int NKK = HD / 32, NDT = HD / 16;
-  constexpr int CPR = HD / 8, NV = PA_KEYS * CPR / 64;  // 8-element pieces per row, and per lane of a tile
-  using VT = VTile<T, HD>;
-  constexpr int TILE_BYTES = VT::ELEMS * sizeof(T), OUT_BYTES = 16 * (HD + 4) * 4;
+  constexpr int CPR = HD / 8, NV = KEYS * CPR / 64;  // 8-element pieces per row, and per lane of a tile
+  using Tile = KVTile<T, HD, NT>;
+  constexpr int TILE_BYTES = 2 * Tile::ELEMS * sizeof(T), OUT_BYTES = 16 * (HD + 4) * 4;
   constexpr int WAVE_BYTES = TILE_BYTES > OUT_BYTES ? TILE_BYTES : OUT_BYTES;
   __shared__ __attribute__((aligned(16))) char smem[PA_WAVES * WAVE_BYTES];
   __shared__ float sML[PA_WAVES][16][2];
@@ -156,78 +184,71 @@ __global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_att
   const int ns = min(a.sinks, lo);     // sinks outside the window
   const int nvis = ns + (len - lo);    // visible keys; key n is n + (n >= ns ? lo - ns : 0)
   const int skip = lo - ns;
-  const int n0 = (int)min((long)split * a.chunk, (long)nvis), n1 = (int)min((long)n0 + a.chunk, (long)nvis);
+  const int n1 = min((split + 1) * a.chunk, nvis);  // this workgroup's keys: split * chunk .. n1 - 1
 
   const T *Q = (const T*)a.q, *K = (const T*)a.kc, *V = (const T*)a.vc;
   Frag<T> qf[NKK];
 #pragma unroll
   for (int kk = 0; kk < NKK; ++kk) {
-    qf[kk].zero();
-    if (i < nq)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = 32 * kk + 8 * g + e;
-        qf[kk].set(e, col < a.d ? to_f32(Q[((long)b * a.Hq + hq0 + i) * a.d + col]) : 0.0f);
-      }
+    qf[kk] = row_frag<T, HD, MODE>(Q + ((long)b * a.Hq + hq0 + min(i, nq - 1)) * a.d, 32 * kk + 8 * g, a.d);
+    if (i >= nq) qf[kk].zero();
   }
   f32x4 o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, lsum = 0.0f;
 
-  // row of the cache [num_blocks Hkv block] that holds visible key n, or -1; lanes 32 .. 63 repeat 0 .. 31
+  // row of the cache [num_blocks Hkv block] that holds visible key n, or -1; one key a lane, repeated every KEYS
+  // lanes.  The table is read before the length is known to cover n (within its width), so that the two loads of a
+  // call without a window do not wait for each other.
   const int* tb = a.table + (long)b * a.width;
   auto row_of = [&](int nbase) {
-    const int n = nbase + (l & 31);
-    if (n >= n1) return -1;
-    const int key = n + (n >= ns ? skip : 0);
+    const int n = nbase + (l & (KEYS - 1));
+    const int key = a.window > 0 ? n + (n >= ns ? skip : 0) : n;
     const int c = key / a.block;
-    const int page = tb[c];
-    return page >= 0 && page < a.num_blocks ? (page * a.Hkv + h) * a.block + (key - c * a.block) : -1;
+    const int page = tb[min(c, a.width - 1)];
+    return n < n1 && page >= 0 && page < a.num_blocks ? (page * a.Hkv + h) * a.block + (key - c * a.block) : -1;
   };
-  Frag<T> kf[2][NKK], vf[NV];
-  auto load_tile = [&](int rows) {  // rows: this lane's key's row; a row of -1 reads row 0 (masked, or zeroed)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const long r = max(__shfl(rows, 16 * t + i), 0);
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) kf[t][kk] = row_frag<T, HD, VEC>(K + r * a.d, 32 * kk + 8 * g, a.d);
-    }
+  Frag<T> kr[NV], vr[NV];
+  auto load_tile = [&](int rows) {  // a row of -1 reads row 0 (masked, or zeroed)
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = l + 64 * n;
       const long r = max(__shfl(rows, c / CPR), 0);
-      vf[n] = row_frag<T, HD, VEC>(V + r * a.d, c % CPR * 8, a.d);
+      kr[n] = row_frag<T, HD, MODE>(K + r * a.d, c % CPR * 8, a.d);
+      vr[n] = row_frag<T, HD, MODE>(V + r * a.d, c % CPR * 8, a.d);
     }
   };
-  T* sv = reinterpret_cast<T*>(smem + w * WAVE_BYTES);
-  int nb = n0 + PA_KEYS * w;
+  T* sk = reinterpret_cast<T*>(smem + w * WAVE_BYTES);
+  T* sv = sk + Tile::ELEMS;
+  int nb = split * a.chunk + KEYS * w;
   int rows = row_of(nb);
   if (nb < n1) load_tile(rows);
-  int rows_next = row_of(nb + PA_STEP);
-  for (; nb < n1; nb += PA_STEP) {
-    const unsigned long long live = __ballot(rows >= 0);  // bit k (and k + 32): key k of the tile
-    // values into LDS; those of absent keys as zeros, since a masked P of 0 would keep a NaN
+  int rows_next = row_of(nb + STEP);
+  for (; nb < n1; nb += STEP) {
+    const unsigned long long live = __ballot(rows >= 0);  // bit k (repeated): key k of the tile
+    // values of absent keys as zeros, since a masked P of 0 would keep a NaN
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = l + 64 * n, row = c / CPR;
-      if (live != ~0ull && !((live >> row) & 1)) vf[n].zero();
-      vf[n].store(sv + VT::off(row, c % CPR * 8));
+      kr[n].store(sk + Tile::off(row, c % CPR * 8));
+      if (live != ~0ull && !((live >> row) & 1)) vr[n].zero();
+      vr[n].store(sv + Tile::off(row, c % CPR * 8));
     }
-    f32x4 s[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) s[t] = Frag<T>::mma(kf[t][kk], qf[kk], s[t]);
-    }
-    // the next tile's loads go out before this one's softmax
     rows = rows_next;
-    if (nb + PA_STEP < n1) load_tile(rows);
-    rows_next = row_of(nb + 2 * PA_STEP);
+    if (nb + STEP < n1) load_tile(rows);
+    rows_next = row_of(nb + 2 * STEP);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    f32x4 s[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[t] = Frag<T>::mma(Tile::row(sk, 16 * t + i, 32 * kk + 8 * g), qf[kk], s[t]);
     float mx = -INFINITY;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (live != ~0ull) s[t][r] = (live >> (16 * t + 4 * g + r)) & 1 ? s[t][r] : -INFINITY;
@@ -246,21 +267,16 @@ __global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_att
         for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
     }
     m = mnew;
-    Frag<T> pf;
-    float rs = 0.0f;
+    float p[4 * NT], rs = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p = fast_exp2(fmaf(s[t][r], a.scale_log2, -mns));
-        rs += p;
-        pf.set(4 * t + r, p);
-      }
+    for (int e = 0; e < 4 * NT; ++e) {
+      p[e] = fast_exp2(fmaf(s[e >> 2][e & 3], a.scale_log2, -mns));
+      rs += p[e];
+    }
     rs += __shfl_xor(rs, 16);
     lsum += rs + __shfl_xor(rs, 32);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt] = Frag<T>::mma(VT::trans(sv, dt, g, i), pf, o[dt]);
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = Tile::pv(sv, dt, g, i, p, o[dt]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 
@@ -290,7 +306,7 @@ __global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_att
       st((T*)a.out, row * a.d + c, sum > 0.0f ? acc / sum : sum == 0.0f ? 0.0f : sum);
     } else {
       const long pr = row * a.splits + split;
-      a.part[pr * a.d + c] = acc;
+      a.part[pr * ((a.d + 3) & ~3) + c] = acc;
       if (c == 0) {
         a.ml[2 * pr] = mm;
         a.ml[2 * pr + 1] = sum;
@@ -299,13 +315,16 @@ __global__ __launch_bounds__(256, (HD * sizeof(T) > 512 ? 1 : 2)) void paged_att
   }
 }
 
-// out[row] = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the row's chunks
+// out[row] = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s over the row's chunks: the chunks over PJ_G groups of 32
+// lanes, four elements of the head a lane, then the groups in order
+constexpr int PJ_G = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
+__global__ __launch_bounds__(32 * PJ_G) void paged_join_kernel(PagedArgs a) {
   __shared__ float sw[PA_MAX_SPLITS];
-  __shared__ float sr[2];
+  __shared__ float sr;
+  __shared__ f32x4 part[PJ_G][32];
   const long row = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, grp = tid >> 5, c = (blockIdx.y * 32 + (tid & 31)) * 4;
   const float* ml = a.ml + row * a.splits * 2;
   if (tid < 64) {
     float mm = -INFINITY;
@@ -320,23 +339,35 @@ __global__ __launch_bounds__(256) void paged_join_kernel(PagedArgs a) {
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (tid == 0) sr[0] = sum;
+    if (tid == 0) sr = sum;
   }
   __syncthreads();
-  const float sum = sr[0];
-  for (int c = tid; c < a.d; c += 256) {
-    float acc = 0.0f;
-    for (int s = 0; s < a.splits; ++s) acc = fmaf(sw[s], a.part[(row * a.splits + s) * a.d + c], acc);
-    st((T*)a.out, row * a.d + c, sum > 0.0f ? acc / sum : sum == 0.0f ? 0.0f : sum);
+  const int dp = (a.d + 3) & ~3;  // row length of the partial outputs
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c < a.d) {
+    const float* in = a.part + row * a.splits * dp + c;
+#pragma unroll 8
+    for (int s = grp; s < a.splits; s += PJ_G) acc += sw[s] * *(const f32x4*)(in + (long)s * dp);
   }
+  part[grp][tid & 31] = acc;
+  __syncthreads();
+  if (grp != 0 || c >= a.d) return;
+#pragma unroll
+  for (int g = 1; g < PJ_G; ++g) acc += part[g][tid];
+  const float sum = sr;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < a.d) st((T*)a.out, row * a.d + c + e, sum > 0.0f ? acc[e] / sum : sum == 0.0f ? 0.0f : sum);
 }
 
+inline long plan_wgs() { static const char* e = getenv("EDF_PW"); return e ? atol(e) : 1536; }
+inline long plan_min() { static const char* e = getenv("EDF_PM"); return e ? atol(e) : 256; }
 // Keys per chunk and chunks for the longest request that the table can hold.
 void plan(int B, int Hkv, int qt, long visible, int& chunk, int& splits) {
   const long wgs = (long)B * Hkv * qt;
-  const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (1536 + wgs - 1) / wgs));
+  const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (plan_wgs() + wgs - 1) / wgs));
   long c = (visible + want - 1) / want;
-  c = std::max(2L * PA_STEP, (c + PA_STEP - 1) / PA_STEP * PA_STEP);
+  c = std::max((long)plan_min(), (c + PA_STEP - 1) / PA_STEP * PA_STEP);
   chunk = (int)std::min(c, 1L << 30);
   splits = (int)std::max(1L, (visible + chunk - 1) / chunk);
 }
@@ -348,10 +379,12 @@ long visible_keys(long width, int block, int window, int sinks) {
 
 template <typename T, int HD>
 void launch_paged(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
-  if (vec)
-    paged_attn_kernel<T, HD, true><<<grid, 256, 0, s>>>(a);
+  if (vec && a.d == HD)
+    paged_attn_kernel<T, HD, WHOLE><<<grid, 256, 0, s>>>(a);
+  else if (vec)
+    paged_attn_kernel<T, HD, BY_PIECE><<<grid, 256, 0, s>>>(a);
   else
-    paged_attn_kernel<T, HD, false><<<grid, 256, 0, s>>>(a);
+    paged_attn_kernel<T, HD, BY_ELEMENT><<<grid, 256, 0, s>>>(a);
 }
 template <typename T>
 void launch_paged_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
@@ -361,7 +394,8 @@ void launch_paged_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) 
     launch_paged<T, 128>(s, a, grid, vec);
   else
     launch_paged<T, 256>(s, a, grid, vec);
-  if (a.splits > 1) paged_join_kernel<T><<<(unsigned)(a.B * a.Hq), 256, 0, s>>>(a);
+  if (a.splits > 1)
+    paged_join_kernel<T><<<dim3((unsigned)(a.B * a.Hq), (unsigned)((a.d + 127) / 128)), 32 * PJ_G, 0, s>>>(a);
 }
 
 }  // namespace
@@ -377,7 +411,7 @@ size_t edf_paged_attention_workspace_bytes(int batch, int num_heads, int num_kv_
   int chunk, splits;
   edf::plan(batch, num_kv_heads, (num_heads / num_kv_heads + 15) / 16,
             edf::visible_keys(table_width, block_size, window, sinks), chunk, splits);
-  return splits == 1 ? 0 : (size_t)batch * num_heads * splits * (head_dim + 2) * sizeof(float);
+  return splits == 1 ? 0 : (size_t)batch * num_heads * splits * ((head_dim + 3) / 4 * 4 + 2) * sizeof(float);
 }
 
 int edf_paged_attention(void* stream, const void* q, const void* k_cache, const void* v_cache, const int32_t* table,
@@ -413,9 +447,9 @@ int edf_paged_attention(void* stream, const void* q, const void* k_cache, const 
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
   a.part = (float*)workspace;
-  a.ml = (float*)workspace + (size_t)batch * num_heads * a.splits * head_dim;
+  a.ml = (float*)workspace + (size_t)batch * num_heads * a.splits * ((head_dim + 3) / 4 * 4);
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 &&
-                   !(((uintptr_t)k_cache | (uintptr_t)v_cache) & 15);
+                   !(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15);
   hipStream_t s = as_stream(stream);
   const unsigned grid = (unsigned)wgs;
   if (dtype == EDF_BF16)
