@@ -24,7 +24,6 @@
 // Keys of a page outside [0, num_blocks) are left out, and a request without keys answers with zeros.
 #include <math.h>
 #include <stdint.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -39,7 +38,7 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_STEP = 128;                   // chunks are whole steps of four waves' tiles of 32 keys
-constexpr int PA_MAX_SPLITS = 256;
+constexpr int PA_MAX_SPLITS = 255;
 
 struct PagedArgs {
   const void *q, *kc, *vc;
@@ -360,16 +359,23 @@ __global__ __launch_bounds__(32 * PJ_G) void paged_join_kernel(PagedArgs a) {
     if (c + e < a.d) st((T*)a.out, row * a.d + c + e, sum > 0.0f ? acc[e] / sum : sum == 0.0f ? 0.0f : sum);
 }
 
-inline long plan_wgs() { static const char* e = getenv("EDF_PW"); return e ? atol(e) : 1536; }
-inline long plan_min() { static const char* e = getenv("EDF_PM"); return e ? atol(e) : 256; }
-// Keys per chunk and chunks for the longest request that the table can hold.
+// Keys per chunk and chunks for the longest request that the table can hold: about PA_WGS workgroups, so that ragged
+// requests, whose later chunks are empty, still fill the 512 places of the GPU twice, and chunks of at least PA_MIN
+// keys, below which a workgroup's start (length, page, key: three loads that wait for each other) is no longer paid
+// for (16x32(8)x128 ragged to 2000: 23.4 us at 256 keys, 20.1 at 512; 8x8(1)x128 to 30000: 22.3 and 21.6; 32x16(2)x256 to
+// 4096: 42.2 at 256, 36.7 at 384).
+constexpr int PA_WGS = 2560, PA_MIN = 384;
 void plan(int B, int Hkv, int qt, long visible, int& chunk, int& splits) {
   const long wgs = (long)B * Hkv * qt;
-  const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (plan_wgs() + wgs - 1) / wgs));
+  const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (PA_WGS + wgs - 1) / wgs));
   long c = (visible + want - 1) / want;
-  c = std::max((long)plan_min(), (c + PA_STEP - 1) / PA_STEP * PA_STEP);
+  c = std::max((long)PA_MIN, (c + PA_STEP - 1) / PA_STEP * PA_STEP);
   chunk = (int)std::min(c, 1L << 30);
   splits = (int)std::max(1L, (visible + chunk - 1) / chunk);
+  // An odd number, the last one empty if need be: workgroups go round the eight XCDs in turn, and with four chunks a
+  // request all first ones, which are never empty, would fall on two of them (64x32(8)x128 ragged to 4096: 139 us with
+  // four chunks, 123 with three).
+  if (splits % 2 == 0) ++splits;
 }
 
 long visible_keys(long width, int block, int window, int sinks) {

@@ -272,24 +272,29 @@ __global__ __launch_bounds__(RO_NT) void rotary_kernel(RotaryArgs a, int lpr) {
   }
 }
 
-// dw[c] = sum of the partials in order: one workgroup per 32 columns, 32 rows of partials at a time
+// dw[c] = sum of the partials in order: one workgroup per 16 columns, 64 partials at a time
 template <typename T>
 __global__ __launch_bounds__(1024) void rotary_dw_kernel(const float* __restrict__ part, T* dwq, T* dwk, int n, int d) {
-  __shared__ float red[32][33];
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + c;
+  __shared__ float red[64][17];
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  const int col = blockIdx.x * 16 + c;
   float s = 0.0f;
-  if (col < 2 * d)
-    for (int i = r; i < n; i += 32) s += part[(size_t)i * 2 * d + col];
+  if (col < 2 * d) {
+#pragma unroll 8
+    for (int i = r; i < n; i += 64) s += part[(size_t)i * 2 * d + col];
+  }
   red[r][c] = s;
   __syncthreads();
-  if (r == 0 && col < 2 * d) {
-    for (int i = 1; i < 32; ++i) s += red[i][c];
-    if (col < d)
-      dwq[col] = from_f32<T>(s);
-    else
-      dwk[col - d] = from_f32<T>(s);
-  }
+  if (r >= 4 || col >= 2 * d) return;
+#pragma unroll
+  for (int i = 4; i < 64; i += 4) s += red[r + i][c];
+  s += __shfl_xor(s, 16);
+  s += __shfl_xor(s, 32);
+  if (r != 0) return;
+  if (col < d)
+    dwq[col] = from_f32<T>(s);
+  else
+    dwk[col - d] = from_f32<T>(s);
 }
 
 // chunk of C elements: 16 bytes, else 8 (bf16), else one element
@@ -403,7 +408,7 @@ int edf_heads_split_rotary_backward(void* stream, const void* x, const double* f
   unsigned wg = 0;
   rc = rotary_dispatch<true>(s, a, interleaved != 0, dtype, RO_BWD_WG, &wg);
   if (rc || !wq) return rc;
-  const unsigned grid = (unsigned)((2 * head_dim + 31) / 32);
+  const unsigned grid = (unsigned)((2 * head_dim + 15) / 16);
   if (dtype == EDF_BF16)
     rotary_dw_kernel<bf16><<<grid, 1024, 0, s>>>(a.part, (bf16*)grad_wq, (bf16*)grad_wk, (int)wg, head_dim);
   else
