@@ -369,7 +369,12 @@ void plan(int B, int Hkv, int qt, long visible, int& chunk, int& splits) {
   const long wgs = (long)B * Hkv * qt;
   const long want = std::max(1L, std::min((long)PA_MAX_SPLITS, (PA_WGS + wgs - 1) / wgs));
   long c = (visible + want - 1) / want;
-  c = std::max((long)PA_MIN, (c + PA_STEP - 1) / PA_STEP * PA_STEP);
+  // with fewer chunks of PA_MIN keys than CUs, smaller ones, about one a CU (1x8(8)x128 of 600: 11.4 -> 8.5 us), unless one
+  // chunk holds them all (no join: 1x32(8)x128 of 200: 7.1 us, 8.7 in two)
+  const bool few = visible > PA_MIN && wgs * ((visible + PA_MIN - 1) / PA_MIN) < 256;
+  const long least = few ? std::min((long)PA_MIN, (visible * wgs + 255) / 256) : PA_MIN;
+  c = std::max(c, least);
+  c = (c + PA_STEP - 1) / PA_STEP * PA_STEP;
   chunk = (int)std::min(c, 1L << 30);
   splits = (int)std::max(1L, (visible + chunk - 1) / chunk);
   // An odd number, the last one empty if need be: workgroups go round the eight XCDs in turn, and with four chunks a

@@ -28,9 +28,8 @@ namespace edf {
 namespace {
 
 constexpr int RO_NT = 256;
-constexpr int RO_PASSES = 4;      // row passes per tile: a thread's rows in a tile
 constexpr int RO_BWD_WG = 1024;   // backward workgroups at most (each leaves one partial weight gradient)
-constexpr int RO_TABLE = 1024;    // sine table entries (cos, sin) per tile
+constexpr int RO_TABLE = 2048;    // sine table entries (cos, sin) per tile
 
 struct RotaryArgs {
   const char *x, *wq, *wk;
@@ -45,40 +44,30 @@ struct RotaryArgs {
   float eps, amp;
 };
 
+// C elements as they are loaded (16 bytes, 8, or one element) and their float32 values
 template <typename T, int C>
-struct Chunk;
-template <typename T>
-struct Chunk<T, 1> {
-  static EDF_DEVICE void ld(const T* p, float* v) { v[0] = to_f32(p[0]); }
-  static EDF_DEVICE void st(T* p, const float* v) { p[0] = from_f32<T>(v[0]); }
-};
-template <>
-struct Chunk<float, 4> {
-  static EDF_DEVICE void ld(const float* p, float* v) {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-  }
-  static EDF_DEVICE void st(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  }
-};
-template <int C>
-struct ChunkBf16 {
-  typedef __attribute__((ext_vector_type(C))) __bf16 vec;
-  static EDF_DEVICE void ld(const bf16* p, float* v) {
-    const vec u = *reinterpret_cast<const vec*>(p);
+struct Chunk {
+  typedef __attribute__((ext_vector_type(C))) T vec;
+  vec v;
+  EDF_DEVICE void ld(const T* p) { v = *reinterpret_cast<const vec*>(p); }
+  EDF_DEVICE void get(float* f) const {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = (float)u[i];
+    for (int i = 0; i < C; ++i) f[i] = (float)v[i];
   }
-  static EDF_DEVICE void st(bf16* p, const float* v) {
+  static EDF_DEVICE void st(T* p, const float* f) {
     vec u;
 #pragma unroll
-    for (int i = 0; i < C; ++i) u[i] = (bf16)v[i];
+    for (int i = 0; i < C; ++i) u[i] = (T)f[i];
     *reinterpret_cast<vec*>(p) = u;
   }
 };
-template <> struct Chunk<bf16, 4> : ChunkBf16<4> {};
-template <> struct Chunk<bf16, 8> : ChunkBf16<8> {};
+template <typename T>
+struct Chunk<T, 1> {
+  T v;
+  EDF_DEVICE void ld(const T* p) { v = p[0]; }
+  EDF_DEVICE void get(float* f) const { f[0] = to_f32(v); }
+  static EDF_DEVICE void st(T* p, const float* f) { p[0] = from_f32<T>(f[0]); }
+};
 
 // The two chunks of unit j: element offsets a and b (b < 0: the row ends after a).
 template <int C, bool INTER>
@@ -111,9 +100,11 @@ EDF_DEVICE float row_sum_n(float v, int lpr) {
   return v;
 }
 
-// LPR lanes (a power of two) walk a row, NU units each.  A tile is a.tile tokens with all their heads.
+// lpr lanes (a power of two) walk a row, NU units each.  A tile is a.tile tokens with all their heads; a
+// thread's first row of a tile is loaded before the tile's sines are computed (more rows ahead cost more in waves per
+// SIMD than they hide: 8x2048x(8 + 2 4)x128 bf16 normed backward 57.0 us with four, 51.7 with two, 47.8 with one).
 template <typename T, int C, bool INTER, int NU, bool BACK>
-__global__ __launch_bounds__(RO_NT) void rotary_kernel(RotaryArgs a, int lpr) {
+__global__ __launch_bounds__(RO_NT, 4) void rotary_kernel(RotaryArgs a, int lpr) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int H = a.Hq + 2 * a.Hkv, npair = a.units * C;
   float2* sCS = reinterpret_cast<float2*>(smem);                           // [tile][npair]
@@ -136,111 +127,138 @@ __global__ __launch_bounds__(RO_NT) void rotary_kernel(RotaryArgs a, int lpr) {
         sW[(size_t)(which * a.units * 2 + c) * C + e] = o < 0 || o >= a.d ? 0.0f : to_f32(W[o + e]);
     }
   float accq[NU][2 * C] = {}, acck[NU][2 * C] = {};  // BACK: this thread's share of dw
+  int ua[NU], ub[NU];                                // its units' chunks; ua < 0: no unit
+#pragma unroll
+  for (int n = 0; n < NU; ++n) {
+    const int j = j0 + lpr * n;
+    unit_at<C, INTER>(j, a.d, a.rot, ua[n], ub[n]);
+    if (j >= a.units) ua[n] = ub[n] = -1;
+  }
 
-  const long ntile = (a.tokens + a.tile - 1) / a.tile;
-  for (long tl = blockIdx.x; tl < ntile; tl += gridDim.x) {
-    const long tok0 = tl * a.tile;
-    const int nt = (int)min((long)a.tile, a.tokens - tok0);
-    __syncthreads();  // the last tile's sines are read, the weights are written
-    for (int i = tid; i < nt * npair; i += RO_NT) {
-      const int t = i / npair, p = i - t * npair;
-      float2 cs = make_float2(1.0f, 0.0f);
-      if (2 * p < a.rot) {
-        const long tok = tok0 + t;
-        const long b = tok / a.T;
-        const int pp = a.pos ? a.pos[b * a.pos_batch + (tok - b * a.T)] : (int)(tok - b * a.T);
-        double turns = (double)pp * (a.freq[p] * 0.15915494309189535);  // 1 / (2 pi)
-        turns -= rint(turns);
-        float s, c;
-        sincospif(2.0f * (float)turns, &s, &c);
-        cs = make_float2(c * a.amp, s * a.amp);
-      }
-      sCS[i] = cs;
-    }
-    __syncthreads();
+  const int ntile = (int)((a.tokens + a.tile - 1) / a.tile);
+  for (int tl = blockIdx.x; tl < ntile; tl += gridDim.x) {
+    const int tok0 = tl * a.tile, nt = min(a.tile, (int)a.tokens - tok0);
+    const int b0 = tok0 / a.T, p0 = tok0 - b0 * a.T;  // batch row and place of the tile's first token
     int h = (tid / lpr) % H, t = (tid / lpr) / H;
-    for (; t < nt;) {
-      const long tok = tok0 + t;
-      const long b = tok / a.T;
-      const int kind = h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;
-      const int hh = h - (kind == 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv);
-      const long hrow = ((b * (kind == 0 ? a.Hq : a.Hkv) + hh) * a.T + (tok - b * a.T)) * a.d;
-      T* Y = (T*)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + hrow;
-      const long xrow = (tok * H + h) * a.d;
-      float u[NU][2 * C], g[NU][2 * C];
-      float ss = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        const int j = j0 + lpr * n;
-        int oa, ob;
-        unit_at<C, INTER>(j, a.d, a.rot, oa, ob);
-#pragma unroll
-        for (int e = 0; e < 2 * C; ++e) u[n][e] = g[n][e] = 0.0f;
-        if (j < a.units) {
-          if (!BACK || (norm && kind < 2)) {
-            Chunk<T, C>::ld(X + xrow + oa, u[n]);
-            if (ob >= 0) Chunk<T, C>::ld(X + xrow + ob, u[n] + C);
-          }
-          if (BACK) {
-            Chunk<T, C>::ld(Y + oa, g[n]);
-            if (ob >= 0) Chunk<T, C>::ld(Y + ob, g[n] + C);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2 * C; ++e) ss = fmaf(u[n][e], u[n][e], ss);
+    bool fresh = true;  // the tile's sines are still to be computed
+    for (int r0 = 0; r0 < nt * H; r0 += step) {
+      Chunk<T, C> u[NU][2], g[NU][2];
+      const int tt = t;
+      // 0: query head, 1: key, 2: value, -1: past the tile
+      const int kind = t >= nt ? -1 : h < a.Hq ? 0 : h < a.Hq + a.Hkv ? 1 : 2;
+      int b = b0, place = p0 + t;
+      while (place >= a.T) {
+        place -= a.T;
+        ++b;
       }
-      float r = 1.0f;
-      if (norm) r = rsqrtf(row_sum_n(ss, lpr) * inv_d + a.eps);
-      float gx = 0.0f;
+      const int hh = h - (kind <= 0 ? 0 : kind == 1 ? a.Hq : a.Hq + a.Hkv);
+      const long hrow = (((long)b * (kind <= 0 ? a.Hq : a.Hkv) + hh) * a.T + place) * a.d;
+      const long xrow = ((long)(tok0 + t) * H + h) * a.d;
+      if (kind >= 0) {
+        const T* Y = (const T*)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + hrow;
 #pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        const int j = j0 + lpr * n;
-        if (j >= a.units) continue;
-        const float* w = sW + (size_t)(kind * a.units + j) * 2 * C;
-        if constexpr (!BACK) {
-          if (kind < 2) {
-            if (norm)
-#pragma unroll
-              for (int e = 0; e < 2 * C; ++e) u[n][e] *= r * w[e];
-            turn<C, INTER, false>(u[n], sCS + t * npair + j * C);
-          }
-        } else if (kind < 2) {
-          turn<C, INTER, true>(g[n], sCS + t * npair + j * C);
-          if (norm) {
-#pragma unroll
-            for (int e = 0; e < 2 * C; ++e) {
-              u[n][e] *= r;  // xh
-              const float gw = g[n][e] * w[e], dw = g[n][e] * u[n][e];
-              accq[n][e] += kind == 0 ? dw : 0.0f;
-              acck[n][e] += kind == 1 ? dw : 0.0f;
-              gx = fmaf(gw, u[n][e], gx);
-              g[n][e] = gw;
+        for (int n = 0; n < NU; ++n)
+          if (ua[n] >= 0) {
+            if (!BACK || (norm && kind < 2)) {
+              u[n][0].ld(X + xrow + ua[n]);
+              if (ub[n] >= 0) u[n][1].ld(X + xrow + ub[n]);
+            }
+            if (BACK) {
+              g[n][0].ld(Y + ua[n]);
+              if (ub[n] >= 0) g[n][1].ld(Y + ub[n]);
             }
           }
-        }
-      }
-      if (BACK && norm) {
-        gx = row_sum_n(gx, lpr) * inv_d;
-        if (kind < 2)
-#pragma unroll
-          for (int n = 0; n < NU; ++n)
-#pragma unroll
-            for (int e = 0; e < 2 * C; ++e) g[n][e] = r * fmaf(-u[n][e], gx, g[n][e]);
-      }
-#pragma unroll
-      for (int n = 0; n < NU; ++n) {
-        const int j = j0 + lpr * n;
-        if (j >= a.units) continue;
-        int oa, ob;
-        unit_at<C, INTER>(j, a.d, a.rot, oa, ob);
-        T* out = BACK ? (T*)a.dx + xrow : Y;
-        const float* y = BACK ? g[n] : u[n];
-        Chunk<T, C>::st(out + oa, y);
-        if (ob >= 0) Chunk<T, C>::st(out + ob, y + C);
       }
       h += step_h;
       t += step_t;
       if (h >= H) h -= H, ++t;
+      if (fresh) {
+        fresh = false;
+        __syncthreads();  // the last tile's sines are read, the weights are written
+        for (int i = tid; i < nt * npair; i += RO_NT) {
+          const int ti = i / npair, pr = i - ti * npair;
+          float2 cs = make_float2(1.0f, 0.0f);
+          if (2 * pr < a.rot) {
+            int b = b0, place = p0 + ti;
+            while (place >= a.T) {
+              place -= a.T;
+              ++b;
+            }
+            const int pos = a.pos ? a.pos[(long)b * a.pos_batch + place] : place;
+            double turns = (double)pos * (a.freq[pr] * 0.15915494309189535);  // 1 / (2 pi)
+            turns -= rint(turns);
+            float s, c;
+            sincospif(2.0f * (float)turns, &s, &c);
+            cs = make_float2(c * a.amp, s * a.amp);
+          }
+          sCS[i] = cs;
+        }
+        __syncthreads();
+      }
+      if (kind < 0) continue;  // the lanes of a row agree
+      const bool turned = kind < 2;
+      float x[NU][2 * C] = {}, y[NU][2 * C] = {};  // y: BACK, the gradient
+      float ss = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NU; ++n)
+        if (ua[n] >= 0) {
+          if (!BACK || (norm && turned)) {
+            u[n][0].get(x[n]);
+            if (ub[n] >= 0) u[n][1].get(x[n] + C);
+          }
+          if (BACK) {
+            g[n][0].get(y[n]);
+            if (ub[n] >= 0) g[n][1].get(y[n] + C);
+          }
+#pragma unroll
+          for (int e = 0; e < 2 * C; ++e) ss = fmaf(x[n][e], x[n][e], ss);
+        }
+      float r = 1.0f;
+      if (norm) r = rsqrtf(row_sum_n(ss, lpr) * inv_d + a.eps);
+      float gx = 0.0f;
+      if (turned) {
+#pragma unroll
+        for (int n = 0; n < NU; ++n) {
+          if (ua[n] < 0) continue;
+          const int j = j0 + lpr * n;
+          const float* w = sW + (size_t)(kind * a.units + j) * 2 * C;
+          const float2* cs = sCS + tt * npair + j * C;
+          if constexpr (!BACK) {
+            if (norm)
+#pragma unroll
+              for (int e = 0; e < 2 * C; ++e) x[n][e] *= r * w[e];
+            turn<C, INTER, false>(x[n], cs);
+          } else {
+            turn<C, INTER, true>(y[n], cs);
+            if (norm) {
+#pragma unroll
+              for (int e = 0; e < 2 * C; ++e) {
+                x[n][e] *= r;  // xh
+                const float gw = y[n][e] * w[e], dw = y[n][e] * x[n][e];
+                accq[n][e] += kind == 0 ? dw : 0.0f;
+                acck[n][e] += kind == 1 ? dw : 0.0f;
+                gx = fmaf(gw, x[n][e], gx);
+                y[n][e] = gw;
+              }
+            }
+          }
+        }
+        if (BACK && norm) {
+          gx = row_sum_n(gx, lpr) * inv_d;
+#pragma unroll
+          for (int n = 0; n < NU; ++n)
+#pragma unroll
+            for (int e = 0; e < 2 * C; ++e) y[n][e] = r * fmaf(-x[n][e], gx, y[n][e]);
+        }
+      }
+      T* out = BACK ? (T*)a.dx + xrow : (T*)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + hrow;
+#pragma unroll
+      for (int n = 0; n < NU; ++n) {
+        if (ua[n] < 0) continue;
+        const float* f = BACK ? y[n] : x[n];
+        Chunk<T, C>::st(out + ua[n], f);
+        if (ub[n] >= 0) Chunk<T, C>::st(out + ub[n], f + C);
+      }
     }
   }
   if constexpr (BACK) {
@@ -314,7 +332,11 @@ int rotary_launch(hipStream_t s, RotaryArgs a, unsigned max_wg, unsigned* wg) {
   int lpr = 1;
   while (lpr * NU < a.units) lpr <<= 1;
   const int H = a.Hq + 2 * a.Hkv, npair = a.units * C;
-  int tile = std::max(1, RO_PASSES * (RO_NT / lpr) / H);
+  // Forward: two rows a thread and tile (four: 25.6 us for 24.8 at 8x2048x(8 + 2 4)x128 bf16).  Backward: as many, up to
+  // eight, as leave a tile for each of its workgroups, which keep their weight gradients over all their tiles.
+  const int step = RO_NT / lpr;
+  const int passes = BACK ? (int)std::max(1L, std::min(8L, a.tokens * H / ((long)step * RO_BWD_WG))) : 2;
+  int tile = std::max(1, passes * step / H);
   tile = std::min(tile, std::max(1, RO_TABLE / npair));
   a.tile = tile;
   const long ntile = (a.tokens + tile - 1) / tile;
