@@ -1026,25 +1026,28 @@ def flash_attention(q, k, v, causal: bool = False):
 # ---------------------------------------------------------------------------
 
 def _here(*ts):
-    """GPU tensors of the current device: the launch goes to its current stream."""
-    cur = None
+    """Raise unless all of these are tensors on the current GPU; its current stream, which the launch goes to."""
+    dev = -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        d = t.get_device()
+        if d < 0:
             raise EdificeHipError("edifice_amd ops need GPU tensors (no CPU fallback)")
-        if cur is None:
-            cur = torch.cuda.current_device()
-        if t.get_device() != cur:
-            raise EdificeHipError(f"tensor on cuda:{t.get_device()}, but the current device is cuda:{cur}")
+        if dev >= 0 and d != dev:
+            raise EdificeHipError(f"tensors on cuda:{dev} and cuda:{d}")
+        dev = d
+    if dev != torch._C._cuda_getDevice():
+        raise EdificeHipError(f"tensors on cuda:{dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _i32(name, t, shape):
-    """t as the contiguous int32 GPU tensor of that shape that a kernel indexes by."""
+    """t as a contiguous int32 tensor of that shape, which a kernel indexes by."""
     if t.dtype != torch.int32:
         raise EdificeHipError(f"{name} must be int32, got {t.dtype}")
-    _shape(name, t, shape)
-    _here(t)
+    if t.shape != shape:
+        raise EdificeHipError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     return t.contiguous()
 
 
@@ -1085,7 +1088,6 @@ def _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq, wk):
     d = width // (num_heads + 2 * num_kv_heads)
     if (wq is None) != (wk is None):
         raise EdificeHipError("q_weight and k_weight come together")
-    _here(x, wq, wk, freq)
     _same(x, wq, wk)
     _shape("q_weight", wq, (d,))
     _shape("k_weight", wk, (d,))
@@ -1098,20 +1100,22 @@ def _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq, wk):
     if positions is not None:
         per_row = int(positions.dim() == 2)
         positions = _i32("positions", positions, (bsz, seq) if per_row else (seq,))
-    return bsz, seq, d, rot, positions, per_row
+    return bsz, seq, d, rot, positions, per_row, _here(x, wq, wk, freq, positions)
 
 
 class _SplitHeadsRotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wq, wk, freq, positions, num_heads, num_kv_heads, eps, interleaved, amplitude):
         x, wq, wk = x.contiguous(), _c(wq), _c(wk)
-        bsz, seq, d, rot, positions, per_row = _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq, wk)
+        bsz, seq, d, rot, positions, per_row, stream = _rotary_operands(x, num_heads, num_kv_heads, freq, positions, wq,
+                                                                        wk)
         q = x.new_empty((bsz, num_heads, seq, d))
-        k, v = (x.new_empty((bsz, num_kv_heads, seq, d)) for _ in range(2))
+        k = x.new_empty((bsz, num_kv_heads, seq, d))
+        v = torch.empty_like(k)
         conf = (bsz, seq, num_heads, num_kv_heads, d, rot, per_row, int(interleaved), float(eps), float(amplitude),
                 dtype_flag(x))
         if x.numel():
-            nat.call("edf_heads_split_rotary", _stream(), _p(x), _p(freq), _p(positions), _p(wq), _p(wk), _p(q), _p(k),
+            nat.call("edf_heads_split_rotary", stream, _p(x), _p(freq), _p(positions), _p(wq), _p(wk), _p(q), _p(k),
                      _p(v), *conf)
         if ctx is not None:  # None: no gradient is asked for
             ctx.conf = conf
@@ -1159,20 +1163,20 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks):
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-        _here(q, k, v)
+        stream = _here(q, k, v)
         _same(q, k, v)
         _rank("q", q, 4)
         _rank("k", k, 4)
         bsz, nh, seq, hd = q.shape
         nkv = k.shape[1]
-        if tuple(k.shape) != (bsz, nkv, seq, hd) or v.shape != k.shape or nkv == 0 or nh % nkv:
+        if k.shape != (bsz, nkv, seq, hd) or v.shape != k.shape or nkv == 0 or nh % nkv:
             raise EdificeHipError("window_attention needs q [B, H, T, d] and k, v [B, Hkv, T, d] with H a multiple of "
                                   f"Hkv, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
         out = torch.empty_like(q)
         keep = ctx is not None  # None: no gradient is asked for
         lse = torch.empty((bsz, nh, seq), dtype=torch.float32, device=q.device) if keep else None
         conf = (bsz, nh, nkv, seq, hd, window, sinks, dtype_flag(q))
-        nat.call("edf_window_attention", _stream(), _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
+        nat.call("edf_window_attention", stream, _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
         if keep:
             ctx.conf = conf
             ctx.save_for_backward(q, k, v, out, lse)
@@ -1202,13 +1206,12 @@ def window_attention(q, k, v, window: int, sinks: int = 0):
     return _WindowAttention.forward(None, *args)
 
 
-def _cache_dims(k_cache, v_cache, num_kv_heads, d, like):
+def _cache_dims(k_cache, v_cache, d, like):
     _rank("k_cache", k_cache, 4)
     blocks, nkv, block, hd = k_cache.shape
-    if v_cache.shape != k_cache.shape or hd != d or (num_kv_heads is not None and nkv != num_kv_heads):
+    if v_cache.shape != k_cache.shape or hd != d:
         raise EdificeHipError(f"k_cache and v_cache must be [num_blocks, Hkv, block_size, {d}], got "
                               f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    _here(like, k_cache, v_cache)
     _same(like, k_cache, v_cache)
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise EdificeHipError("edifice_amd ops need contiguous tensors")
@@ -1228,17 +1231,18 @@ def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: to
     reqs, width = table.shape
     if not table.is_contiguous() or table.dtype != torch.int32:
         raise EdificeHipError("table must be a contiguous int32 tensor")
+    _rank("free_blocks", free_blocks, 1)
     old_lengths = _i32("old_lengths", old_lengths, (reqs,))
     new_lengths = _i32("new_lengths", new_lengths, (reqs,))
-    _rank("free_blocks", free_blocks, 1)
     free_blocks = _i32("free_blocks", free_blocks, free_blocks.shape)
     if taken is not None:
         taken = _i32("taken", taken, (1,))
-    _here(table)
-    slots, positions = (table.new_empty((reqs, num_tokens)) for _ in range(2))
+    stream = _here(table, old_lengths, new_lengths, free_blocks, taken)
+    slots = table.new_empty((reqs, num_tokens))
+    positions = torch.empty_like(slots)
     used = table.new_empty((1,))
-    nat.call("edf_paged_extend", _stream(), _p(table), _p(old_lengths), _p(new_lengths), _p(free_blocks), _p(taken),
-             _p(slots), _p(positions), _p(used), reqs, width, free_blocks.numel(), int(block_size), int(num_tokens))
+    nat.call("edf_paged_extend", stream, _p(table), _p(old_lengths), _p(new_lengths), _p(free_blocks), _p(taken),
+             _p(slots), _p(positions), _p(used), reqs, width, free_blocks.numel(), block_size, num_tokens)
     return slots, positions, used
 
 
@@ -1247,19 +1251,22 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     """Keys and values k, v [B, Hkv, T, d] into the pages k_cache, v_cache [num_blocks, Hkv, block_size, d], in
     place: token (b, t) into slot slots[b, t] (int32 [B, T], as ``paged_extend`` gives them; -1, or any other slot
     outside the cache: left out).  Slots have to differ from one another.  Inference only."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, k_cache, v_cache)):
+    if _wants_grad(k, v, k_cache, v_cache):
         raise EdificeHipError("paged_cache_write has no backward: call it under torch.no_grad()")
     k, v = k.contiguous(), v.contiguous()
     _rank("k", k, 4)
     bsz, nkv, seq, d = k.shape
-    _shape("v", v, k.shape)
-    _here(v)
+    if v.shape != k.shape:
+        raise EdificeHipError(f"v must have shape {tuple(k.shape)}, got {tuple(v.shape)}")
     _same(k, v)
-    blocks, _, block = _cache_dims(k_cache, v_cache, nkv, d, k)
+    blocks, heads, block = _cache_dims(k_cache, v_cache, d, k)
+    if heads != nkv:
+        raise EdificeHipError(f"k has {nkv} heads, the cache {heads}")
     slots = _i32("slots", slots, (bsz, seq))
+    stream = _here(k, v, slots, k_cache, v_cache)
     if k.numel():
-        nat.call("edf_paged_cache_write", _stream(), _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), bsz, seq, nkv,
-                 d, blocks, block, dtype_flag(k))
+        nat.call("edf_paged_cache_write", stream, _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), bsz, seq, nkv, d,
+                 blocks, block, dtype_flag(k))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -1278,15 +1285,16 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
         raise EdificeHipError(f"q must be [B, H, d] or [B, H, 1, d], got shape {tuple(q.shape)}")
     bsz, nh, d = q.shape[0], q.shape[1], q.shape[-1]
-    blocks, nkv, block = _cache_dims(k_cache, v_cache, None, d, q)
+    blocks, nkv, block = _cache_dims(k_cache, v_cache, d, q)
     _rank("table", table, 2)
     width = table.shape[1]
     table = _i32("table", table, (bsz, width))
     lengths = _i32("lengths", lengths, (bsz,))
+    stream = _here(q, k_cache, v_cache, table, lengths)
     out = torch.empty_like(q)
     wsb = nat.query("edf_paged_attention_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
-    ws = _u8(wsb, q)
-    nat.call("edf_paged_attention", _stream(), _p(q), _p(k_cache), _p(v_cache), _p(table), _p(lengths), _p(out), _p(ws),
+    ws = _u8(wsb, q) if wsb else None
+    nat.call("edf_paged_attention", stream, _p(q), _p(k_cache), _p(v_cache), _p(table), _p(lengths), _p(out), _p(ws),
              wsb, bsz, nh, nkv, d, blocks, block, width, window, sinks, dtype_flag(q))
     return out
 
