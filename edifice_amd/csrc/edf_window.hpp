@@ -213,10 +213,12 @@ struct KeyChunk {
 };
 
 // dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  Grid x:
-// pieces of the block's [dK | dV][key][dim], y: the divided blocks from `first` on, z: batch x key head.
+// pieces of the block's [dK | dV][key][dim], y: the blocks (those of one workgroup are already in place), z: batch x
+// key head.
 template <typename T, int HD, int KB, int BQ>
-__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx, int first, int per) {
-  const int kblk = first + blockIdx.y, kb0 = kblk * KB;
+__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx) {
+  const int kblk = blockIdx.y, kb0 = kblk * KB, per = kblk < a.nsb ? a.c_sink : a.c_win;
+  if (per == 1) return;
   const long bh = blockIdx.z;
   int qs, nt;
   query_tiles<KB, BQ>(kb0, a.T, a.W, a.S, qs, nt);
@@ -292,11 +294,10 @@ int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
   const int gx = p.gx(), pieces = 2 * KB * HD / 1024;
   kernel<<<dim3(gx, BHkv), 256, 0, s>>>(a);
   const int rc = check_launch("window attention dK, dV");
-  if (rc) return rc;
-  if (p.nsb > 0 && p.c_sink > 1)
-    window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, p.nsb, BHkv), 256, 0, s>>>(a, gx, 0, p.c_sink);
-  if (p.nkb > p.nsb && p.c_win > 1)
-    window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, p.nkb - p.nsb, BHkv), 256, 0, s>>>(a, gx, p.nsb, p.c_win);
+  if (rc || !p.divided()) return rc;
+  // divided sink blocks alone are the first ones
+  const int blocks = p.nkb > p.nsb && p.c_win > 1 ? p.nkb : p.nsb;
+  window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, blocks, BHkv), 256, 0, s>>>(a, gx);
   return check_launch("window attention dK, dV sums");
 }
 

@@ -5,8 +5,9 @@
 // (window_narrow).  Rows of whole 16-byte pieces only.
 //
 // Row operands (a lane's 8 elements of one row) come straight from memory, a tile ahead of their use.
-// Transposed operands: in float32 straight from memory too (a 32-lane row piece is 128 contiguous bytes), in bf16
-// through a wave-private LDS copy of the tile and transposed reads.
+// Transposed operands come through a wave-private LDS copy of the tile; the forward in float32 past head_dim 64 reads
+// V^T straight from memory (a 32-lane row piece is 128 contiguous bytes; 1x8(4)x1000x128 window 300: 24.9 us, 29.4 through
+// LDS; at 64 27.1 and 25.8, and dQ 49.8 and 36.9 at 128).
 #include <math.h>
 #include <stdint.h>
 
@@ -21,10 +22,9 @@ constexpr float LN2 = 0.6931471805599453f;
 constexpr int WN_R = 32, WN_WAVES = 4;  // rows per workgroup; waves
 
 // The 32-row tile of a tensor [T, d] at row r0 as a wave reads it.
-template <typename T, int HD>
+template <typename T, int HD, bool LDS>
 struct NTile {
   static constexpr int NKK = HD / 16, NDT = HD / 32;
-  static constexpr bool LDS = sizeof(T) == 2;
   using Tile = WTile<T, HD, WN_R>;
   // rows past the end repeat the last one: their scores are masked
   EDF_DEVICE static void rows(const T* x, int r0, int T_, int d, int l, WFrag<T>* f) {
@@ -102,8 +102,9 @@ constexpr int waves_per_simd(int tensors, int accumulators) {
 template <typename T, int HD>
 __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32;
-  using N = NTile<T, HD>;
-  constexpr int TILE = N::LDS ? N::Tile::ELEMS * (int)sizeof(T) : 0, JOIN = 2 * NDT * 64 * 64;
+  constexpr bool LDS = sizeof(T) == 2 || HD <= 64;
+  using N = NTile<T, HD, LDS>;
+  constexpr int TILE = LDS ? N::Tile::ELEMS * (int)sizeof(T) : 0, JOIN = 2 * NDT * 64 * 64;
   __shared__ __attribute__((aligned(16))) char smem[WN_WAVES * TILE > JOIN ? WN_WAVES * TILE : JOIN];
   __shared__ float sM[WN_WAVES][32], sS[WN_WAVES][32];
 
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
   const T* V = (const T*)a.v + bh / a.G * T_ * d;
   T* sv = reinterpret_cast<T*>(smem + w * TILE);
 
-  WFrag<T> qf[NKK], kf[NKK], vf[N::LDS ? NKK : 1];
+  WFrag<T> qf[NKK], kf[NKK], vf[LDS ? NKK : 1];
   N::rows((const T*)a.q + bh * T_ * d, q0, T_, d, l, qf);
   f32x16 o[NDT];
 #pragma unroll
@@ -126,13 +127,13 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
   const KeyTiles<WN_R, WN_R> kt(q0, T_, a.W, a.S);
   if (w < kt.count) {
     N::rows(K, kt.key0(w), T_, d, l, kf);
-    if constexpr (N::LDS) N::rows(V, kt.key0(w), T_, d, l, vf);
+    if constexpr (LDS) N::rows(V, kt.key0(w), T_, d, l, vf);
   }
   for (int t = w; t < kt.count; t += WN_WAVES) {
     const int k0 = kt.key0(t);
     const SeesKey sees(myq, k0 + 4 * g, a.W, a.S);
-    WFrag<T> vt[N::LDS ? 1 : 2 * NDT];
-    if constexpr (N::LDS) {
+    WFrag<T> vt[LDS ? 1 : 2 * NDT];
+    if constexpr (LDS) {
       N::keep(sv, l, vf);
     } else {
 #pragma unroll
@@ -143,7 +144,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
     for (int kk = 0; kk < NKK; ++kk) s = WFrag<T>::mma(kf[kk], qf[kk], s);
     if (t + WN_WAVES < kt.count) {  // the next tile's loads go out before this one's softmax
       N::rows(K, kt.key0(t + WN_WAVES), T_, d, l, kf);
-      if constexpr (N::LDS) N::rows(V, kt.key0(t + WN_WAVES), T_, d, l, vf);
+      if constexpr (LDS) N::rows(V, kt.key0(t + WN_WAVES), T_, d, l, vf);
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
       rs += s[r];
     }
     lsum += rs + __shfl_xor(rs, 32);
-    if constexpr (N::LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if constexpr (LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
       WFrag<T> pf;
@@ -178,11 +179,11 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
       for (int e = 0; e < 8; ++e) pf.set(e, s[8 * kc + e]);
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
-        if constexpr (N::LDS) o[dt] = WFrag<T>::mma(N::trans(V, sv, k0, T_, d, kc, dt, l), pf, o[dt]);
+        if constexpr (LDS) o[dt] = WFrag<T>::mma(N::trans(V, sv, k0, T_, d, kc, dt, l), pf, o[dt]);
         else o[dt] = WFrag<T>::mma(vt[kc * NDT + dt], pf, o[dt]);
       }
     }
-    if constexpr (N::LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if constexpr (LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   // the waves' maxima, then their sums and outputs in units of the common one
   if (g == 0) sM[w][li] = m;
@@ -204,8 +205,8 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
 template <typename T, int HD>
 __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32;
-  using N = NTile<T, HD>;
-  constexpr int TILE = N::LDS ? N::Tile::ELEMS * (int)sizeof(T) : 0, JOIN = 2 * NDT * 64 * 64;
+  using N = NTile<T, HD, true>;
+  constexpr int TILE = N::Tile::ELEMS * (int)sizeof(T), JOIN = 2 * NDT * 64 * 64;
   __shared__ __attribute__((aligned(16))) char smem[WN_WAVES * TILE > JOIN ? WN_WAVES * TILE : JOIN];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
@@ -242,7 +243,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
   for (int t = w; t < kt.count; t += WN_WAVES) {
     const int k0 = kt.key0(t);
     const SeesKey sees(myq, k0 + 4 * g, a.W, a.S);
-    if constexpr (N::LDS) N::keep(sk, l, kf);
+    N::keep(sk, l, kf);
     f32x16 s = zero16(), dp = zero16();
 #pragma unroll
     for (int kk = 0; kk < NKK; ++kk) {
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
       const float x = fast_exp2(fmaf(s[r], a.scale_log2, -lse)) * (dp[r] - dd);  // 1 / sqrt(d) at the end
       s[r] = sees(d_row(r, 0)) ? x : 0.0f;
     }
-    if constexpr (N::LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int kc = 0; kc < 2; ++kc) {
       WFrag<T> df;
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) dq[dt] = WFrag<T>::mma(N::trans(K, sk, k0, T_, d, kc, dt, l), df, dq[dt]);
     }
-    if constexpr (N::LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   join_waves<NDT>(dq, (f32x16*)smem, w, l);
   if (w == 0 && myq < T_) store_rows_t<T, HD>((T*)a.dq + qrow * d, dq, a.scale, d, g);
