@@ -24,7 +24,7 @@ struct WindowArgs {
   float scale, scale_log2;
 };
 
-constexpr int WINDOW_DMA_T = 1 << 22;  // longest sequence of the DMA kernels: a head's buffer stays below 2^31 bytes
+constexpr int WINDOW_VEC_T = 1 << 22;  // longest sequence of the buffer loads: a head of 512-byte rows stays below 2^31 bytes
 
 EDF_DEVICE bool window_sees(int q, int key, int W, int S) { return key <= q && (q - key < W || key < S); }
 // the same for key first + c of one query, c a constant after unrolling: three values stay in registers
@@ -54,6 +54,14 @@ template <> struct WFrag<bf16> {
   EDF_DEVICE void load(const bf16* p) { v = *(const bf16x8*)p; }
   EDF_DEVICE void store(bf16* p) const { *(bf16x8*)p = v; }
   EDF_DEVICE void zero() { v = bf16x8{}; }
+  // elements e, e + 1 (e even); returns s plus the sum of the pair as rounded, one dot product.  (Taking the pairs out
+  // of the finished vector instead compiles to its first pair four times.)
+  EDF_DEVICE float set2(int e, float x, float y, float s) {
+    const bf16x2 p = __builtin_bit_cast(bf16x2, pack_bf16x2(x, y));
+    v[e] = p[0];
+    v[e + 1] = p[1];
+    return __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{(bf16)1.0f, (bf16)1.0f}, s, false);
+  }
 };
 template <> struct WFrag<float> {
   f32x4 lo, hi;
@@ -78,6 +86,11 @@ template <> struct WFrag<float> {
     *(f32x4*)(p + 4) = hi;
   }
   EDF_DEVICE void zero() { lo = hi = f32x4{0.0f, 0.0f, 0.0f, 0.0f}; }
+  EDF_DEVICE float set2(int e, float x, float y, float s) {
+    set(e, x);
+    set(e + 1, y);
+    return s + (x + y);
+  }
 };
 
 // N steps use(i, load(i)) with the loads A steps ahead of their use: the barriers keep the compiler from sinking a
@@ -125,6 +138,60 @@ EDF_DEVICE WFrag<T> window_row(const T* row, int col, int d) {
   }
   return f;
 }
+
+// A workgroup of 256 threads moves the R-row tile at row r0 of x [T, d] through registers into an LDS tile of HD columns,
+// N pieces of 8 elements a thread; columns past d are zeros, rows past the end zeros or copies of the last (their scores
+// are masked).  VEC: buffer loads, whose range check stands in for comparisons on every piece (a head's T d elements
+// have to stay below 2^31 bytes).
+template <typename T, int HD, int R, bool VEC>
+struct TileLoader {
+  static constexpr int CPR = HD / 8, PIECES = R * CPR, N = (PIECES + 255) / 256;
+  static constexpr bool F32 = sizeof(T) == 4;
+  unsigned lo[VEC ? N : 1], hi[VEC && F32 ? N : 1];  // byte offsets of a piece's 16-byte parts from the tile's first row
+  int tid, d, T_;
+  EDF_DEVICE TileLoader(int tid_, int d_, int t_) : tid(tid_), d(d_), T_(t_) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
+        lo[i] = c < PIECES && col < d ? (unsigned)((row * d + col) * (int)sizeof(T)) : OOB_OFF;
+        if constexpr (F32) hi[i] = c < PIECES && col + 4 < d ? (unsigned)((row * d + col + 4) * (int)sizeof(T)) : OOB_OFF;
+      }
+    }
+  }
+  EDF_DEVICE void load(const T* x, int r0, WFrag<T>* f) const {
+    if constexpr (VEC) {
+      const rsrc_t rs = make_rsrc(x, (unsigned)T_ * (unsigned)d * (unsigned)sizeof(T));
+      const unsigned base = (unsigned)r0 * (unsigned)d * (unsigned)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const u32x4 a = __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(lo[i] + base), 0, 0);
+        if constexpr (F32) {
+          f[i].lo = __builtin_bit_cast(f32x4, a);
+          f[i].hi = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(hi[i] + base), 0, 0));
+        } else {
+          f[i].v = __builtin_bit_cast(bf16x8, a);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
+        if (PIECES % 256 != 0 && c >= PIECES) continue;
+        f[i] = window_row<T, HD, false>(x + (long)min(r0 + row, T_ - 1) * d, col, d);
+      }
+    }
+  }
+  template <typename Tile>
+  EDF_DEVICE void store(T* lds, const WFrag<T>* f) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
+      if (PIECES % 256 != 0 && c >= PIECES) continue;
+      f[i].store(lds + Tile::off(row, col));
+    }
+  }
+};
 
 // A row-major LDS tile of R rows: operand reads along rows, and transposed ones (lane column c, the 8 rows
 // r0 + 4 g + {0 .. 3} and r0 + 8 + 4 g + {0 .. 3}, the order in which an accumulator's registers hold rows).

@@ -10,8 +10,8 @@
 // double-buffered in LDS with the next one on its way in registers.  The partly hidden tiles come first
 // (one loop with the mask), the others after it (one loop without): the order of an online softmax is free.
 //
-// Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), its
-// sum is taken before that.  float32 runs on the float32 matrix instructions.
+// Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and its sum is
+// that of the rounded values.  float32 runs on the float32 matrix instructions.
 #include <math.h>
 #include <stdint.h>
 
@@ -28,7 +28,7 @@ constexpr int WA_BM = 128;
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
-  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 2 ? 4 : 1;
+  constexpr int AHEAD = sizeof(T) == 2 ? 4 : 1;
   using Tile = WTile<T, HD, BN>;
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
@@ -52,26 +52,16 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   float m = -INFINITY, lsum = 0.0f;
 
   const KeyTiles<WA_BM, BN> kt(q0, T_, a.W, a.S);
-  WFrag<T> rk[CPT], rv[CPT];
+  const TileLoader<T, HD, BN, VEC> ld(tid, d, T_);
+  WFrag<T> rk[ld.N], rv[ld.N];
   auto gload = [&](int t) {
     const int k0 = kt.key0(t);
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      const long key = min(k0 + row, T_ - 1);  // rows past the end repeat the last: their scores are masked
-      rk[i] = window_row<T, HD, VEC>(K + key * d, col, d);
-      rv[i] = window_row<T, HD, VEC>(V + key * d, col, d);
-    }
+    ld.load(K, k0, rk);
+    ld.load(V, k0, rv);
   };
   auto sstore = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      rk[i].store(&sK[buf][Tile::off(row, col)]);
-      rv[i].store(&sV[buf][Tile::off(row, col)]);
-    }
+    ld.template store<Tile>(sK[buf], rk);
+    ld.template store<Tile>(sV[buf], rv);
   };
   auto tile = [&](int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
@@ -104,19 +94,16 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
     }
     m = mnew;
     float rs = 0.0f;
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[h][r] = fast_exp2(fmaf(s[h][r], a.scale_log2, -mns));
-        rs += s[h][r];
-      }
-    lsum += rs + __shfl_xor(rs, 32);
     WFrag<T> pf[2 * NH];
 #pragma unroll
     for (int kc = 0; kc < 2 * NH; ++kc)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pf[kc].set(e, s[kc >> 1][8 * (kc & 1) + e]);
+      for (int e = 0; e < 8; e += 2) {
+        const int r = 8 * (kc & 1) + e;
+        rs = pf[kc].set2(e, fast_exp2(fmaf(s[kc >> 1][r], a.scale_log2, -mns)),
+                         fast_exp2(fmaf(s[kc >> 1][r + 1], a.scale_log2, -mns)), rs);
+      }
+    lsum += rs + __shfl_xor(rs, 32);
     ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sv, 16 * (i / NDT), i % NDT, l); },
                                [&](int i, const WFrag<T>& f) { o[i % NDT] = WFrag<T>::mma(f, pf[i / NDT], o[i % NDT]); });
   };
@@ -371,7 +358,7 @@ template <typename T, int BN, bool VEC>
 void launch_fwd(hipStream_t s, const WindowArgs& a, int BH) {
   const dim3 grid((a.T + WA_BM - 1) / WA_BM, BH);
   if constexpr (sizeof(T) == 2 && VEC) {
-    if (a.d == 128 && a.T <= WINDOW_DMA_T) {
+    if (a.d == 128) {
       window_fwd128_kernel<<<grid, 256, 0, s>>>(a);
       return;
     }
@@ -420,7 +407,7 @@ int edf_window_attention(void* stream, const void* q, const void* k, const void*
   a.W = window < seq_len ? window : seq_len, a.S = sinks < seq_len ? sinks : seq_len;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
-  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15);
+  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && seq_len <= WINDOW_VEC_T;
   hipStream_t s = as_stream(stream);
   const int BH = batch * num_heads;
   if (window_narrow(BH, seq_len, vec)) return window_narrow_run(false, s, a, BH, dtype);

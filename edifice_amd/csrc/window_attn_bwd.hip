@@ -30,7 +30,7 @@ constexpr int WB_M = 128;  // queries (dQ) or keys (dK, dV) per workgroup
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
-  constexpr int CPR = HD / 8, PIECES = BN * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 2 ? 3 : 1;
+  constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
   using Tile = WTile<T, HD, BN>;
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
@@ -64,26 +64,16 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
 
   const KeyTiles<WB_M, BN> kt(q0, T_, a.W, a.S);
-  WFrag<T> rk[CPT], rv[CPT];
+  const TileLoader<T, HD, BN, VEC> ld(tid, d, T_);
+  WFrag<T> rk[ld.N], rv[ld.N];
   auto gload = [&](int t) {
     const int k0 = kt.key0(t);
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      const long key = min(k0 + row, T_ - 1);  // rows past the end repeat the last: their P is masked
-      rk[i] = window_row<T, HD, VEC>(K + key * d, col, d);
-      rv[i] = window_row<T, HD, VEC>(V + key * d, col, d);
-    }
+    ld.load(K, k0, rk);
+    ld.load(V, k0, rv);
   };
   auto sstore = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      rk[i].store(&sK[buf][Tile::off(row, col)]);
-      rv[i].store(&sV[buf][Tile::off(row, col)]);
-    }
+    ld.template store<Tile>(sK[buf], rk);
+    ld.template store<Tile>(sV[buf], rv);
   };
   auto tile = [&](int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
@@ -282,7 +272,7 @@ __global__ __launch_bounds__(256, 2) void window_dq128_kernel(WindowArgs a) {
 template <typename T, int HD, int BQ, bool VEC>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) void window_dkdv_kernel(WindowArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32;
-  constexpr int CPR = HD / 8, PIECES = BQ * CPR, CPT = (PIECES + 255) / 256, AHEAD = sizeof(T) == 4 ? 1 : HD == 96 ? 2 : 3;
+  constexpr int AHEAD = sizeof(T) == 4 ? 1 : HD == 96 ? 2 : 3;
   using Tile = WTile<T, HD, BQ>;
   __shared__ __attribute__((aligned(16))) T sQ[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sO[2][Tile::ELEMS];
@@ -311,33 +301,23 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     dk[dt] = zero16();
     dv[dt] = zero16();
   }
-  WFrag<T> rq[CPT], ro[CPT];
+  const TileLoader<T, HD, BQ, VEC> ld(tid, d, T_);
+  WFrag<T> rq[ld.N], ro[ld.N];
   float rl = 0.0f, rd = 0.0f;
   auto gload = [&](int t) {
     const int h = t / nt, q0 = qs + (t - h * nt) * BQ;
     const long base = (bh * a.G + h) * T_;
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      const long q = base + min(q0 + row, T_ - 1);  // rows past the end repeat the last: their P is 0
-      rq[i] = window_row<T, HD, VEC>((const T*)a.q + q * d, col, d);
-      ro[i] = window_row<T, HD, VEC>((const T*)a.go + q * d, col, d);
-    }
+    ld.load((const T*)a.q + base * d, q0, rq);
+    ld.load((const T*)a.go + base * d, q0, ro);
     if (tid < BQ) {
       const long q = base + min(q0 + tid, T_ - 1);
-      rl = q0 + tid < T_ ? a.lse[q] * LOG2E : INFINITY;
+      rl = q0 + tid < T_ ? a.lse[q] * LOG2E : INFINITY;  // a query past the end gets P = 0
       rd = a.dd[q];
     }
   };
   auto sstore = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const int c = tid + 256 * i, row = c / CPR, col = c % CPR * 8;
-      if (PIECES % 256 != 0 && c >= PIECES) continue;
-      rq[i].store(&sQ[buf][Tile::off(row, col)]);
-      ro[i].store(&sO[buf][Tile::off(row, col)]);
-    }
+    ld.template store<Tile>(sQ[buf], rq);
+    ld.template store<Tile>(sO[buf], ro);
     if (tid < BQ) {
       sL[buf][tid] = rl;
       sD[buf][tid] = rd;
@@ -630,13 +610,12 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
 }
 
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles: bf16, and float32 or the DMA kernel
-bool dma_kernels(int d, int T, int dtype, bool vec) { return dtype == EDF_BF16 && vec && d == 128 && T <= WINDOW_DMA_T; }
 
 template <typename T, int HD, int BN, int BQ, bool VEC>
 int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
   const dim3 grid((a.T + WB_M - 1) / WB_M, BH);
   constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
-  const bool fast = dma && dma_kernels(a.d, a.T, EDF_BF16, VEC);
+  const bool fast = dma && a.d == 128;
   int rc = EDF_OK;
   if (window_narrow(BH, a.T, VEC)) {
     rc = window_narrow_run(true, s, a, BH, sizeof(T) == 2 ? EDF_BF16 : EDF_F32);
@@ -711,7 +690,7 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)grad_out |
                          (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
-  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15);
+  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && seq_len <= WINDOW_VEC_T;
   hipStream_t s = as_stream(stream);
   const int BH = batch * num_heads, BHkv = batch * num_kv_heads;
   if (dtype == EDF_BF16)
