@@ -322,7 +322,7 @@ class GQAttention(nn.Module):
     """Causal grouped-query self-attention.  Without the options below it runs on the fused flash kernel, the KV heads
     repeated to the query heads before it; with one of them on the kernels that take shared KV heads as they are:
     rotary_dim (positions, pairs (i, i + rotary_dim / 2) of each head; rotary_base), qk_norm (learned query / key norms
-    per head), window (keys seen per query) and sinks (first keys that stay visible)."""
+    per head), window (keys seen per query) and sinks (first keys that stay visible); head_dim <= 128 then."""
 
     def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, *, rotary_dim: int = 0,
                  rotary_base: float = 10000.0, qk_norm: bool = False, window: int = 0, sinks: int = 0):
@@ -455,11 +455,15 @@ class SequenceModel(nn.Module):
         prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
         time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text.  A step of one token does not wait
         for the GPU and may be captured; one of several checks that their places are empty."""
+        blocks = getattr(self, self._blocks_name)
+        if x.shape[0] != cache.lengths.numel() or len(cache.k) != len(blocks):
+            raise ValueError(f"x of {x.shape[0]} texts and {len(blocks)} layers, a cache of {cache.lengths.numel()} places "
+                             f"and {len(cache.k)} layers")
         if x.shape[1] > 1 and bool((cache.lengths * (1 if counts is None else counts)).any()):
             raise ValueError("several tokens at once go into empty places only")
         slots, positions = cache.extend(x.shape[1], counts)
         h = self.input_projection(x) if hasattr(self, "input_projection") else x
-        for layer, blk in enumerate(getattr(self, self._blocks_name)):
+        for layer, blk in enumerate(blocks):
             h = blk.step(h, cache, layer, slots, positions)
         return self.final_norm(h) if hasattr(self, "final_norm") else h
 

@@ -20,11 +20,12 @@ struct WindowArgs {
   float *lse, *dd;   // [B Hq T]: natural-log row sums; D = rowsum(dO o O) / unscaled
   float* part;       // backward: float32 dK, dV partials of key blocks that several workgroups share
   int T, G, d, W, S;
+  int nx;            // workgroups per head (the grid is one-dimensional: its other axes end at 65535)
   int c_sink, c_win, len_sink, len_win, nsb;  // backward: chunks and tiles per chunk of sink / other key blocks
   float scale, scale_log2;
 };
 
-constexpr int WINDOW_VEC_T = 1 << 22;  // longest sequence of the buffer loads: a head of 512-byte rows stays below 2^31 bytes
+constexpr int WINDOW_VEC_T = (1 << 22) - 1;  // longest sequence of the buffer loads: a head of 512-byte rows below 2^31 bytes
 
 EDF_DEVICE bool window_sees(int q, int key, int W, int S) { return key <= q && (q - key < W || key < S); }
 // the same for key first + c of one query, c a constant after unrolling: three values stay in registers
@@ -33,6 +34,13 @@ struct SeesKey {
   EDF_DEVICE SeesKey(int q, int first, int W, int S) : rel(q - first), out(q - first - W), sink(S - first) {}
   EDF_DEVICE bool operator()(int c) const { return c <= rel && (c > out || c < sink); }
 };
+
+// The (block, head) of this workgroup: the blocks of a head, and so the heads that share keys, on one XCD.
+EDF_DEVICE void window_block(const WindowArgs& a, int& blk, long& head) {
+  const int id = remap_xcd(blockIdx.x, gridDim.x);
+  blk = id % a.nx;
+  head = id / a.nx;
+}
 
 // A loop bound in a vector register: branches on it are divergent in the compiler's eyes, which then keeps the
 // bodies of a loop apart (as uniform branches they were merged and spilled: 31 registers in the forward at
@@ -279,24 +287,25 @@ struct KeyChunk {
   }
 };
 
-// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  Grid x:
-// pieces of the block's [dK | dV][key][dim], y: the blocks (those of one workgroup are already in place), z: batch x
-// key head.
+// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  A workgroup takes
+// one of the pieces of a block's [dK | dV][key][dim]; blocks of one chunk are already in place.
 template <typename T, int HD, int KB, int BQ>
-__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int gx) {
-  const int kblk = blockIdx.y, kb0 = kblk * KB, per = kblk < a.nsb ? a.c_sink : a.c_win;
+__global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int blocks) {
+  constexpr int PIECES = 2 * KB * HD / 1024;
+  const int piece = blockIdx.x % PIECES, kblk = blockIdx.x / PIECES % blocks;
+  const long bh = blockIdx.x / PIECES / blocks;  // batch x key head
+  const int kb0 = kblk * KB, per = kblk < a.nsb ? a.c_sink : a.c_win;
   if (per == 1) return;
-  const long bh = blockIdx.z;
   int qs, nt;
   query_tiles<KB, BQ>(kb0, a.T, a.W, a.S, qs, nt);
   const int len = kblk < a.nsb ? a.len_sink : a.len_win;
   const int n = min(per, (nt * a.G + len - 1) / len);  // chunks that hold a tile
   const int x0 = kblk < a.nsb ? kblk * a.c_sink : a.nsb * a.c_sink + (kblk - a.nsb) * a.c_win;
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 4;
+  const int e = (piece * 256 + threadIdx.x) * 4;
   const bool is_v = e >= KB * HD;
   const int key = e / HD % KB, c = e % HD;
   if (kb0 + key >= a.T || c >= a.d) return;
-  const float* in = a.part + (bh * gx + x0) * (2L * KB * HD) + e;
+  const float* in = a.part + (bh * a.nx + x0) * (2L * KB * HD) + e;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
   for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * KB * HD));
@@ -358,13 +367,14 @@ template <typename T, int HD, int KB, int BQ, typename F>
 int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
   const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, KB, BQ, kv_slots<T>(HD), kv_join<T>(KB, BQ));
   a.nsb = p.nsb, a.c_sink = p.c_sink, a.c_win = p.c_win, a.len_sink = p.len_sink, a.len_win = p.len_win;
-  const int gx = p.gx(), pieces = 2 * KB * HD / 1024;
-  kernel<<<dim3(gx, BHkv), 256, 0, s>>>(a);
+  a.nx = p.gx();
+  const int blocks = p.nkb > p.nsb && p.c_win > 1 ? p.nkb : p.nsb;  // the divided ones, from the first
+  const long wgs = (long)a.nx * BHkv, sums = 2L * KB * HD / 1024 * blocks * BHkv;
+  EDF_REQUIRE(wgs < (1L << 31) && sums < (1L << 31), EDF_ERR_UNSUPPORTED, "batch x heads x seq_len too large for one call");
+  kernel<<<(unsigned)wgs, 256, 0, s>>>(a);
   const int rc = check_launch("window attention dK, dV");
   if (rc || !p.divided()) return rc;
-  // divided sink blocks alone are the first ones
-  const int blocks = p.nkb > p.nsb && p.c_win > 1 ? p.nkb : p.nsb;
-  window_sum_kernel<T, HD, KB, BQ><<<dim3(pieces, blocks, BHkv), 256, 0, s>>>(a, gx);
+  window_sum_kernel<T, HD, KB, BQ><<<(unsigned)sums, 256, 0, s>>>(a, blocks);
   return check_launch("window attention dK, dV sums");
 }
 

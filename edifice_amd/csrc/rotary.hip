@@ -135,9 +135,9 @@ __global__ __launch_bounds__(RO_NT, 4) void rotary_kernel(RotaryArgs a, int lpr)
     if (j >= a.units) ua[n] = ub[n] = -1;
   }
 
-  const int ntile = (int)((a.tokens + a.tile - 1) / a.tile);
-  for (int tl = blockIdx.x; tl < ntile; tl += gridDim.x) {
-    const int tok0 = tl * a.tile, nt = min(a.tile, (int)a.tokens - tok0);
+  const long ntile = (a.tokens + a.tile - 1) / a.tile;
+  for (long tl = blockIdx.x; tl < ntile; tl += gridDim.x) {
+    const int tok0 = (int)(tl * a.tile), nt = min(a.tile, (int)a.tokens - tok0);
     const int b0 = tok0 / a.T, p0 = tok0 - b0 * a.T;  // batch row and place of the tile's first token
     int h = (tid / lpr) % H, t = (tid / lpr) / H;
     bool fresh = true;  // the tile's sines are still to be computed

@@ -36,9 +36,9 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
-  const int q0 = (gridDim.x - 1 - xb) * WA_BM, qw = q0 + 32 * w, myq = qw + li;
+  const int q0 = (a.nx - 1 - xb) * WA_BM, qw = q0 + 32 * w, myq = qw + li;
   const T* Q = (const T*)a.q + bh * T_ * d;
   const T* K = (const T*)a.k + bh / a.G * T_ * d;
   const T* V = (const T*)a.v + bh / a.G * T_ * d;
@@ -166,9 +166,9 @@ __global__ __launch_bounds__(256, 2) void window_fwd128_kernel(WindowArgs a) {
   const int wu = __builtin_amdgcn_readfirstlane(w);
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T = a.T;
-  const int q0 = (gridDim.x - 1 - xb) * WA_BM, qw = q0 + 32 * w, myq = qw + li;
+  const int q0 = (a.nx - 1 - xb) * WA_BM, qw = q0 + 32 * w, myq = qw + li;
   const bf16* Qrow = (const bf16*)a.q + (bh * T + min(myq, T - 1)) * HD;
   const long kvbase = bh / a.G * T * HD;
   // per-head buffer resources: rows past the end read as zeros (their scores are masked)
@@ -355,8 +355,9 @@ __global__ __launch_bounds__(256, 2) void window_fwd128_kernel(WindowArgs a) {
 }
 
 template <typename T, int BN, bool VEC>
-void launch_fwd(hipStream_t s, const WindowArgs& a, int BH) {
-  const dim3 grid((a.T + WA_BM - 1) / WA_BM, BH);
+void launch_fwd(hipStream_t s, WindowArgs a, int BH) {
+  a.nx = (a.T + WA_BM - 1) / WA_BM;
+  const unsigned grid = (unsigned)a.nx * (unsigned)BH;
   if constexpr (sizeof(T) == 2 && VEC) {
     if (a.d == 128) {
       window_fwd128_kernel<<<grid, 256, 0, s>>>(a);
@@ -385,8 +386,9 @@ int window_check(int batch, int num_heads, int num_kv_heads, int seq_len, int he
   EDF_REQUIRE(window > 0 && sinks >= 0, EDF_ERR_INVALID_ARG, "window must be positive and sinks not negative");
   EDF_REQUIRE(sinks <= (1 << 22), EDF_ERR_UNSUPPORTED, "sinks must be at most 2^22");
   EDF_REQUIRE(head_dim <= 128, EDF_ERR_UNSUPPORTED, "head_dim %d > 128 unsupported", head_dim);
-  EDF_REQUIRE(seq_len < (1 << 30), EDF_ERR_UNSUPPORTED, "seq_len must be below 2^30");
-  EDF_REQUIRE((long)batch * num_heads <= 65535, EDF_ERR_UNSUPPORTED, "batch x num_heads must be at most 65535");
+  EDF_REQUIRE(seq_len < (1 << 30) && (long)batch * num_heads < (1L << 31) &&
+                  (double)batch * num_heads * ((seq_len + 31) / 32) < 2147483648.0,
+              EDF_ERR_UNSUPPORTED, "batch x heads x seq_len too large for one call");
   return EDF_OK;
 }
 

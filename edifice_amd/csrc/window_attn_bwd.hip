@@ -38,9 +38,9 @@ __global__ __launch_bounds__(256, 1) void window_dq_kernel(WindowArgs a) {
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
-  const int q0 = (gridDim.x - 1 - xb) * WB_M, qw = q0 + 32 * w, myq = qw + li;
+  const int q0 = (a.nx - 1 - xb) * WB_M, qw = q0 + 32 * w, myq = qw + li;
   const long qrow = bh * T_ + min(myq, T_ - 1);
   const T* K = (const T*)a.k + bh / a.G * T_ * d;
   const T* V = (const T*)a.v + bh / a.G * T_ * d;
@@ -163,9 +163,9 @@ __global__ __launch_bounds__(256, 2) void window_dq128_kernel(WindowArgs a) {
   const int wu = __builtin_amdgcn_readfirstlane(w);
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T = a.T;
-  const int q0 = (gridDim.x - 1 - xb) * WB_M, qw = q0 + 32 * w, myq = qw + li;
+  const int q0 = (a.nx - 1 - xb) * WB_M, qw = q0 + 32 * w, myq = qw + li;
   const long qrow = bh * T + min(myq, T - 1), kvbase = bh / a.G * T * HD;
   const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)T * HD * 2);
   const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)T * HD * 2);
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int xb;
   long bh;  // batch x key head
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
   const KeyChunk<WB_M, BQ> kc_(a, xb);
   const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     __syncthreads();
   }
   if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
-    float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
+    float* out = a.part + (bh * a.nx + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -455,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
   const int wu = __builtin_amdgcn_readfirstlane(w);
   int xb;
   long bh;  // batch x key head
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T = a.T;
   const KeyChunk<WB_M, BQ> kc_(a, xb);
   const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
@@ -576,7 +576,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
     if (t + 1 < t1) step(b1, t + 1);
   }
   if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
-    float* out = a.part + (bh * (long)gridDim.x + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
+    float* out = a.part + (bh * a.nx + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -613,7 +613,8 @@ constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles: bf16, and float32 or th
 
 template <typename T, int HD, int BN, int BQ, bool VEC>
 int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
-  const dim3 grid((a.T + WB_M - 1) / WB_M, BH);
+  a.nx = (a.T + WB_M - 1) / WB_M;
+  const unsigned grid = (unsigned)a.nx * (unsigned)BH;
   constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
   const bool fast = dma && a.d == 128;
   int rc = EDF_OK;

@@ -111,9 +111,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
-  const int q0 = (gridDim.x - 1 - xb) * WN_R, myq = q0 + li;
+  const int q0 = (a.nx - 1 - xb) * WN_R, myq = q0 + li;
   const T* K = (const T*)a.k + bh / a.G * T_ * d;
   const T* V = (const T*)a.v + bh / a.G * T_ * d;
   T* sv = reinterpret_cast<T*>(smem + w * TILE);
@@ -212,9 +212,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int xb;
   long bh;
-  head_block(xb, bh);
+  window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
-  const int q0 = (gridDim.x - 1 - xb) * WN_R, myq = q0 + li;
+  const int q0 = (a.nx - 1 - xb) * WN_R, myq = q0 + li;
   const T* K = (const T*)a.k + bh / a.G * T_ * d;
   const T* V = (const T*)a.v + bh / a.G * T_ * d;
   T* sk = reinterpret_cast<T*>(smem + w * TILE);
@@ -275,8 +275,9 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
 }
 
 template <typename T, int HD>
-void run(bool backward, hipStream_t s, const WindowArgs& a, int BH) {
-  const dim3 grid((a.T + WN_R - 1) / WN_R, BH);
+void run(bool backward, hipStream_t s, WindowArgs a, int BH) {
+  a.nx = (a.T + WN_R - 1) / WN_R;
+  const unsigned grid = (unsigned)a.nx * (unsigned)BH;
   if (backward) narrow_dq_kernel<T, HD><<<grid, 256, 0, s>>>(a);
   else narrow_fwd_kernel<T, HD><<<grid, 256, 0, s>>>(a);
 }

@@ -1151,7 +1151,8 @@ def split_heads_rotary(x: torch.Tensor, num_heads: int, num_kv_heads: int, frequ
     frequencies (``rotary_frequencies``; None: no rotation): pair i of the first 2 len(frequencies) elements then
     turns by positions[b, t] frequencies[i] and is scaled by ``amplitude``; pairs are (i, i + half), or
     (2 i, 2 i + 1) when ``interleaved``.  positions: int32 [B, T] or [T] (any value; None: 0 .. T - 1).
-    float32 or bfloat16, float32 inside (angles in float64), head_dim <= 256; differentiable in x and the weights.
+    float32 or bfloat16 (x and the weights alike), float32 inside (angles in float64), head_dim <= 256; differentiable
+    in x and the weights.
     """
     args = (x, q_weight, k_weight, frequencies, positions, num_heads, num_kv_heads, eps, interleaved, amplitude)
     if _wants_grad(x, q_weight, k_weight):

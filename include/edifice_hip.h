@@ -669,8 +669,8 @@ int edf_heads_split_rotary_backward(void* stream, const void* x, const double* f
  *   h / (num_heads / num_kv_heads); query i sees key j when j <= i and (i - j < window or j < sinks);
  *   scores / sqrt(d).
  * lse (may be NULL): float32 [batch, num_heads, seq_len] natural-log row sums, required by the backward.
- * head_dim <= 128, batch x num_heads <= 65535.  Keys and values have to be finite where some query of the same
- * 64-key tile sees the tile.  The backward's workspace: edf_window_attention_backward_workspace_bytes().
+ * head_dim <= 128, sinks <= 2^22.  Keys and values have to be finite: a value that is not may also reach queries that
+ * do not see its key, where another key of its 64-key tile is seen.  The backward's workspace: edf_window_attention_backward_workspace_bytes().
  * ------------------------------------------------------------------------ */
 int edf_window_attention(void* stream, const void* q, const void* k, const void* v, void* out, float* lse, int batch,
                          int num_heads, int num_kv_heads, int seq_len, int head_dim, int window, int sinks, int dtype);

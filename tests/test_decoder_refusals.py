@@ -53,7 +53,9 @@ def _write(L, B=1, T=1, hkv=1, d=64, blocks=4, block=16, k=P, dtype=1):
     (lambda L: _window(L, window=0), 1, b"window"),
     (lambda L: _window(L, sinks=-1), 1, b"sinks"),
     (lambda L: _window(L, d=129), 2, b"head_dim"),
-    (lambda L: _window(L, B=1 << 16), 2, b"65535"),
+    (lambda L: _window(L, B=1 << 16, hq=1 << 15), 2, b"too large"),
+    (lambda L: _window(L, B=1 << 10, T=1 << 27), 2, b"too large"),
+    (lambda L: _window(L, sinks=(1 << 22) + 1), 2, b"sinks"),
     (lambda L: _window(L, q=None), 1, b"null"),
     (lambda L: _window(L, dtype=3), 1, b"dtype"),
     (lambda L: _window_bwd(L, lse=None), 1, b"lse"),

@@ -134,6 +134,9 @@ def test_prompt_into_a_filled_place_is_refused():
     assert cache.lengths.tolist() == [3, 2]
     with pytest.raises(ValueError):
         cache.extend(1, torch.tensor([1], device="cuda"))
+    with pytest.raises(ValueError):  # texts and places do not match; nothing has moved
+        m.step(x[:1, :1], cache)
+    assert cache.lengths.tolist() == [3, 2]
 
 
 def test_captured_step_replays():

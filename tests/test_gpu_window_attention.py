@@ -45,6 +45,8 @@ CASES = [
     (5, 16, 8, 300, 64, 1000, 0, bf16),
     (10, 8, 2, 150, 80, 64, 1, bf16),
     (10, 8, 8, 140, 96, 33, 20, bf16),
+    (10, 8, 2, 150, 112, 60, 2, bf16),
+    (10, 8, 2, 140, 52, 60, 2, bf16),
     (10, 8, 2, 200, 128, 100, 5, bf16),
     (3, 16, 4, 520, 128, 130, 70, bf16),
     (10, 8, 2, 135, 32, 200, 0, f32),
@@ -134,6 +136,23 @@ def test_causal_window_matches_flash_attention():
     want = fs.flash_attention(q.cuda(), k.cuda(), v.cuda(), causal=True)
     tol = _expected(case, q, k, v, do)["O"][1]
     _within(got, want.cpu().double(), 2 * tol, "flash")
+
+
+def test_many_heads():
+    """More heads than a grid's second axis holds, and sinks whose gradients are divided."""
+    from edifice_amd import fused_scan as fs
+    announce("window_many_heads")
+    B, H, T, d = 1100, 64, 40, 16
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v, do = (torch.randn(B, H, T, d, device="cuda", generator=g) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = fs.window_attention(q, k, v, 7, 2)
+    grads = torch.autograd.grad(out, leaves, do)
+    for b, h in ((0, 0), (1023, 63), (1099, 63)):
+        one = [t.detach()[b:b + 1, h:h + 1].cpu() for t in (q, k, v, do)]
+        exp = _expected((1, 1, 1, T, d, 7, 2, f32), *one)
+        for name, got in zip(("O", "dQ", "dK", "dV"), (out, *grads)):
+            _within(got[b:b + 1, h:h + 1], *exp[name], f"{name} of head {b}, {h}")
 
 
 def test_strided_and_broadcast_inputs():
