@@ -82,17 +82,19 @@ __global__ __launch_bounds__(256, 2) void window_fwd_kernel(WindowArgs a) {
         mx = fmaxf(mx, s[h][r]);
       }
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float mnew = fmaxf(m, mx);
-    const float mns = mnew == -INFINITY ? 0.0f : mnew * a.scale_log2;
-    if (__any(mnew > m)) {  // rescale only when some row maximum grew
-      const float alpha = fast_exp2(m * a.scale_log2 - mns);
+    // O and the sum refer to a maximum that is moved only when a score exceeds it by a factor of 2^8: p <= 256 loses
+    // nothing in float32 or bf16
+    if (__any(mx * a.scale_log2 > m * a.scale_log2 + 8.0f)) {
+      const float mnew = fmaxf(m, mx);
+      const float alpha = fast_exp2(m * a.scale_log2 - (mnew == -INFINITY ? 0.0f : mnew * a.scale_log2));
       lsum *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m = mnew;
     }
-    m = mnew;
+    const float mns = m == -INFINITY ? 0.0f : m * a.scale_log2;
     float rs = 0.0f;
     WFrag<T> pf[2 * NH];
 #pragma unroll
