@@ -52,7 +52,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
                                                              const int* __restrict__ taken, int* __restrict__ slots,
                                                              int* __restrict__ positions, int* __restrict__ used, int R,
                                                              int width, int nfree, int block, int tokens) {
-  __shared__ int first[PX_ITEMS + 1];  // draws before each of this workgroup's requests
+  __shared__ unsigned first[PX_ITEMS];  // list entries gone before each of this workgroup's requests
   __shared__ int wsum[PX_NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const long i0 = (long)blockIdx.x * PX_ITEMS, total = (long)R * tokens;
@@ -70,7 +70,8 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
     __syncthreads();
     return wsum[0] + wsum[1] + wsum[2] + wsum[3];
   };
-  const int start = taken != nullptr ? max(*taken, 0) : 0;  // entries of the list that are gone
+  // entries of the list that are gone; entry numbers are unsigned, so that none past 2^31 looks free
+  const unsigned start = taken != nullptr ? (unsigned)max(*taken, 0) : 0u;
   int before = 0;
   for (int r = tid; r < r0; r += PX_NT) before += draws(r);
   before = block_sum(before);
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
   __syncthreads();
   if (lane == 63) wsum[wv] = incl;
   __syncthreads();
-  int at = start + before + incl - run;
+  unsigned at = start + (unsigned)(before + incl - run);
   for (int w = 0; w < wv; ++w) at += wsum[w];
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
     int all = 0;
     for (int r = tid; r < R; r += PX_NT) all += draws(r);
     all = block_sum(all);
-    if (tid == 0) *used = start + all;
+    if (tid == 0) *used = (int)min(start + (unsigned)all, (unsigned)INT32_MAX);
   }
 #pragma unroll
   for (int e = 0; e < PX_ITEMS / PX_NT; ++e) {
@@ -113,10 +114,11 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
     const int r = (int)(i / tokens), t = (int)(i - (long)r * tokens);
     const int o = max(old_len[r], 0), n = max(new_len[r], 0);
     const Pages pg = pages_of(o, n, block, width);
-    const int base = first[r - r0] - pg.have;  // free-list entry of page c: base + c
+    const unsigned base = first[r - r0];  // free-list entry of page c: base + (c - held)
     auto page_of = [&](int c) {
       if (c < pg.have) return table[(long)r * width + c];
-      return base + c < nfree ? free_ids[base + c] : -1;
+      const unsigned at = base + (unsigned)(c - pg.have);
+      return at < (unsigned)nfree ? free_ids[at] : -1;
     };
     const bool there = n > o && t < n - o;
     const int p = there ? o + t : -1;
@@ -182,6 +184,8 @@ int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, c
   EDF_REQUIRE(requests > 0 && table_width > 0 && block_size > 0 && num_tokens > 0 && num_free >= 0,
               EDF_ERR_INVALID_ARG, "dimensions must be positive");
   EDF_REQUIRE((long)requests * num_tokens < (1L << 31), EDF_ERR_UNSUPPORTED, "requests x num_tokens must be below 2^31");
+  EDF_REQUIRE((long)requests * table_width < (1L << 31), EDF_ERR_UNSUPPORTED,
+              "requests x table_width must be below 2^31");
   EDF_REQUIRE(table && old_lengths && new_lengths && (free_blocks || num_free == 0) && slots && positions && used,
               EDF_ERR_INVALID_ARG, "null tensor pointer");
   EDF_REQUIRE(taken != used, EDF_ERR_INVALID_ARG, "taken and used must be two places: workgroups read one while the other is written");

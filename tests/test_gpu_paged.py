@@ -51,6 +51,26 @@ def test_paged_extend(case):
     assert used.tolist() == [want[3]]
 
 
+@pytest.mark.parametrize("taken", [-3, 2, 5, 2**31 - 1])
+def test_paged_extend_after_a_count(taken):
+    """Entries gone before the call: a negative count is none; past the list, whatever the sum, no page is given."""
+    from edifice_amd import fused_scan as fs
+    announce("paged_extend taken", taken=taken)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    free = [7, 3, 9, 1, 4]
+    table = torch.full((3, 2), -1, dtype=torch.int32, device="cuda")
+    slots, pos, used = fs.paged_extend(table, i32([0, 0, 0]), i32([1, 5, 3]), i32(free), 4, 5, i32([taken]))
+    at = max(taken, 0)
+    pages = [free[at + i] if at + i < len(free) else -1 for i in range(4)]
+    want = [[pages[0], -1], [pages[1], pages[2]], [pages[3], -1]]
+    assert table.tolist() == want
+    assert used.tolist() == [min(at + 4, 2**31 - 1)]
+    for r, n in enumerate([1, 5, 3]):
+        assert pos[r].tolist() == [t if t < n else -1 for t in range(5)]
+        assert slots[r].tolist() == [want[r][t // 4] * 4 + t % 4 if t < n and want[r][t // 4] >= 0 else -1
+                                     for t in range(5)]
+
+
 @pytest.mark.parametrize("case", [(2, 3, 5, 64, 8, bf16), (1, 1, 1, 128, 16, f32), (3, 2, 70, 7, 4, bf16),
                                   (2, 2, 9, 5, 3, f32)], ids=str)
 def test_paged_cache_write(case):
