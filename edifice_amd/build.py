@@ -53,11 +53,15 @@ def sources():
 # kernel 84.6 -> 79.2 us, the others unchanged; identical results).  The row scans do the same
 # with theirs at every step of a chunk (without the flag 8x2048x8x128 bf16 608 -> 623 us, KDA
 # 4x1000x8x128 344 -> 350, 2x777x8x64 float32 gated 239 -> 267).
+# The windowed attention's backward kernels hold two accumulators and scale P and dP with VALU
+# work (backward without and with the flag: bf16 4x16(4)x2000x96 window 500 239 -> 204 us,
+# float32 8x16(4)x1500x64 window 256 729 -> 640, 2x8(4)x1000x64 103 -> 96).
 PER_FILE_FLAGS = {
     "flash_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "delta_rule_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "delta_rule_row.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "delta_rule_row_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "window_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 
