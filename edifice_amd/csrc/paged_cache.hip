@@ -127,7 +127,8 @@ __global__ __launch_bounds__(PX_NT) void paged_extend_kernel(int* __restrict__ t
       const int c = p / block, off = p - c * block;
       if (c < width) {
         const int page = page_of(c);
-        if (page >= 0) slot = page * block + off;
+        const long s = (long)page * block + off;
+        if (page >= 0 && s <= INT32_MAX) slot = (int)s;
         if (off == 0) table[(long)r * width + c] = page;  // the first token of a new page enters it
       }
     }
