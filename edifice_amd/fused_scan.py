@@ -1176,7 +1176,7 @@ class _WindowAttention(torch.autograd.Function):
         out = torch.empty_like(q)
         keep = ctx is not None  # None: no gradient is asked for
         lse = torch.empty((bsz, nh, seq), dtype=torch.float32, device=q.device) if keep else None
-        conf = (bsz, nh, nkv, seq, hd, window, sinks, dtype_flag(q))
+        conf = (bsz, nh, nkv, seq, hd, min(window, seq), min(sinks, seq), dtype_flag(q))  # more sees no more keys
         nat.call("edf_window_attention", stream, _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
         if keep:
             ctx.conf = conf
@@ -1293,6 +1293,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lengths = _i32("lengths", lengths, (bsz,))
     stream = _here(q, k_cache, v_cache, table, lengths)
     out = torch.empty_like(q)
+    window, sinks = (min(int(x), width * block) for x in (window, sinks))  # more sees no more keys
     wsb = nat.query("edf_paged_attention_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
     ws = _u8(wsb, q) if wsb else None
     nat.call("edf_paged_attention", stream, _p(q), _p(k_cache), _p(v_cache), _p(table), _p(lengths), _p(out), _p(ws),

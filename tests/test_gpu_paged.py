@@ -160,6 +160,18 @@ def test_paged_attention(case):
     assert torch.equal(fs.paged_attention(dev[0][:, :, None], *dev[1:], window=window, sinks=sinks)[:, :, 0], got)
 
 
+def test_a_window_without_end():
+    """A window and sinks past any int see every key, as no window does."""
+    from edifice_amd import fused_scan as fs
+    announce("paged_window_without_end")
+    kc, vc, table, n, g = _pool([70, 5], 2, 64, 16, f32)
+    dev = [t.cuda() for t in (torch.randn(2, 4, 64, generator=g), kc, vc, table, n)]
+    want = fs.paged_attention(*dev)
+    for window, sinks in ((2**63 - 1, 0), (2**32 + 3, 0), (1, 2**32 + 3)):
+        _check(fs.paged_attention(*dev, window=window, sinks=sinks), dev[0].cpu(), kc, vc, table, n, 0, 0, f32)
+    assert torch.equal(fs.paged_attention(*dev, window=0, sinks=2**32 + 3), want)
+
+
 def test_bad_pages_and_lengths():
     """Page numbers outside the cache hold no keys; a length past the table counts to the table's end, a negative
     one as none.  (The kernel checks each number against the cache before it forms an address.)"""

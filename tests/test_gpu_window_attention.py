@@ -138,6 +138,18 @@ def test_causal_window_matches_flash_attention():
     _within(got, want.cpu().double(), 2 * tol, "flash")
 
 
+def test_a_window_without_end():
+    """A window and sinks past any int are those of the whole length, not their low bits."""
+    from edifice_amd import fused_scan as fs
+    announce("window_without_end")
+    q, k, v, _ = _make((1, 4, 2, 77, 64, 77, 0, bf16))
+    q, k, v = q.cuda(), k.cuda(), v.cuda()
+    want = fs.window_attention(q, k, v, 77)
+    assert torch.equal(fs.window_attention(q, k, v, 2**63 - 1), want)
+    assert torch.equal(fs.window_attention(q, k, v, 2**32 + 3), want)
+    assert torch.equal(fs.window_attention(q, k, v, 77, 2**32 + 3), want)
+
+
 def test_many_heads():
     """More heads than a grid's second axis holds, and sinks whose gradients are divided."""
     from edifice_amd import fused_scan as fs
