@@ -453,8 +453,9 @@ class SequenceModel(nn.Module):
     def step(self, x, cache: PagedCache, counts=None):
         """The next tokens x [requests, T, embed] of a cache's places -> their hidden states [requests, T, hidden]:
         prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
-        time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text.  A step of one token does not wait
-        for the GPU and may be captured; one of several checks that their places are empty."""
+        time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text; a token that found no page
+        (``PagedCache.exhausted``) is not seen by those after it.  A step of one token does not wait for the GPU and
+        may be captured; one of several checks that their places are empty."""
         blocks = getattr(self, self._blocks_name)
         if x.shape[0] != cache.lengths.numel() or len(cache.k) != len(blocks):
             raise ValueError(f"x of {x.shape[0]} texts and {len(blocks)} layers, a cache of {cache.lengths.numel()} places "
@@ -462,6 +463,8 @@ class SequenceModel(nn.Module):
         if x.shape[1] > 1 and bool((cache.lengths * (1 if counts is None else counts)).any()):
             raise ValueError("several tokens at once go into empty places only")
         slots, positions = cache.extend(x.shape[1], counts)
+        if x.shape[1] > 1 and counts is not None:  # whatever the padding holds, its keys and values are finite
+            x = x.masked_fill((positions < 0)[..., None], 0.0)
         h = self.input_projection(x) if hasattr(self, "input_projection") else x
         for layer, blk in enumerate(blocks):
             h = blk.step(h, cache, layer, slots, positions)

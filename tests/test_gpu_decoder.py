@@ -1,5 +1,7 @@
 """The decoder's attention operators run together, as a model uses them: training through the block, and prompts and
 steps over a paged cache, against float64 and against the whole sequence at once."""
+import math
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -103,6 +105,25 @@ def test_prompts_and_steps_match_the_whole_sequence(dtype, opts):
             # two layers of bf16 products and norms, each side with its own roundings
             assert_close(host(torch.stack(got[r])), host(want), 1e-4 if dtype == torch.float32 else 3e-2, f"text {r}",
                          elementwise=False)
+
+
+def test_what_the_padding_holds_does_not_matter():
+    """Padding of NaN behind ragged prompts, and in a place that takes no tokens: the real tokens' states are finite
+    and those of zero padding."""
+    announce("gqa_padding")
+    m = _model(torch.float32, **OPTS)
+    x = torch.randn(3, 9, 48, generator=torch.Generator().manual_seed(4)).cuda()
+    counts = torch.tensor([4, 9, 0], dtype=torch.int32, device="cuda")
+    pad = (torch.arange(9, device="cuda") >= counts[:, None])[..., None]
+    a, b = (m.paged_cache(3, 16, block_size=4) for _ in range(2))
+    want = m.step(x.masked_fill(pad, 0.0), a, counts)
+    got = m.step(x.masked_fill(pad, math.nan), b, counts)
+    assert torch.isfinite(got[~pad[..., 0]]).all() and torch.equal(got[~pad[..., 0]], want[~pad[..., 0]])
+    assert torch.equal(a.k[1], b.k[1]) and torch.equal(a.v[0], b.v[0])
+    x1 = torch.full((3, 1, 48), math.nan, device="cuda")
+    x1[:2] = x[:2, :1]
+    one = torch.tensor([1, 1, 0], dtype=torch.int32, device="cuda")
+    assert torch.isfinite(m.step(x1, b, one)[:2]).all()
 
 
 def test_release_and_exhaustion():
