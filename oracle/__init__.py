@@ -13,6 +13,10 @@ Contents
   * ``blocks.py``     numpy restatement of the block-level callers (layer norm,
                       dense, MinGRU / DeltaNet / Mamba / GQA models) used to pin
                       the scans against the reference's safetensors fixtures.
+  * ``decoder.py``    float64 torch restatement of the decoder attention operators
+                      (head split with norms and rotary positions, windowed
+                      attention, the paged cache); no reference counterpart, pinned
+                      by ``tests/test_oracle_decoder.py``.
   * ``cref.c``        plain-C (OpenMP, float32) restatement of the same
                       recurrences, used as the timed CPU baseline.
 
