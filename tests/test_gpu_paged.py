@@ -172,6 +172,29 @@ def test_a_window_without_end():
     assert torch.equal(fs.paged_attention(*dev, window=0, sinks=2**32 + 3), want)
 
 
+@pytest.mark.parametrize("dtype", [bf16, f32], ids=str)
+def test_pages_one_element_off(dtype):
+    """Caches and queries whose rows are off 16 bytes: the write and the attention by elements."""
+    from edifice_amd import fused_scan as fs
+    announce("paged_off", dtype=dtype)
+
+    def off(t):
+        buf = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+    kc, vc, table, n, g = _pool([150, 33], 2, 64, 16, dtype)
+    q = torch.randn(2, 6, 64, generator=g).to(dtype)
+    k, v = (torch.randn(2, 2, 1, 64, generator=g).to(dtype) for _ in range(2))
+    kd, vd, qd = off(kc), off(vc), off(q)
+    slots = torch.stack([table[b, (n[b] - 1) // 16] * 16 + (n[b] - 1) % 16 for b in range(2)])[:, None]
+    fs.paged_cache_write(off(k), off(v), slots.to(torch.int32).cuda(), kd, vd)
+    for b in range(2):
+        s = int(slots[b])
+        kc[s // 16, :, s % 16], vc[s // 16, :, s % 16] = k[b, :, 0], v[b, :, 0]
+    assert torch.equal(kd.cpu(), kc) and torch.equal(vd.cpu(), vc)
+    _check(fs.paged_attention(qd, kd, vd, table.cuda(), n.cuda()), q, kc, vc, table, n, 0, 0, dtype)
+
+
 def test_bad_pages_and_lengths():
     """Page numbers outside the cache hold no keys; a length past the table counts to the table's end, a negative
     one as none.  (The kernel checks each number against the cache before it forms an address.)"""

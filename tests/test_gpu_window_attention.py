@@ -183,6 +183,27 @@ def test_strided_and_broadcast_inputs():
     _within(dk, exp["dK"][0].sum(1, keepdim=True), exp["dK"][1].sum(1, keepdim=True), "dK")
 
 
+@pytest.mark.parametrize("case", [(1, 4, 2, 300, 128, 90, 3, bf16), (1, 4, 1, 200, 64, 70, 2, bf16),
+                                  (2, 2, 1, 150, 96, 40, 0, bf16), (1, 2, 1, 170, 64, 50, 1, f32),
+                                  (1, 2, 2, 140, 128, 64, 2, f32), (10, 8, 2, 150, 128, 60, 2, bf16)], ids=str)
+def test_tensors_one_element_off(case):
+    """Contiguous tensors whose rows are off 16 bytes, in and for the gradient of the result."""
+    from edifice_amd import fused_scan as fs
+    announce("window_off", case=case)
+
+    def off(t):
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        buf[1:] = t.reshape(-1)
+        return buf[1:].view(t.shape)
+    q, k, v, do = _make(case)
+    leaves = [off(t).requires_grad_() for t in (q, k, v)]
+    out = fs.window_attention(*leaves, *case[5:7])
+    grads = torch.autograd.grad(out, leaves, off(do))
+    exp = _expected(case, q, k, v, do)
+    for name, got in zip(("O", "dQ", "dK", "dV"), (out, *grads)):
+        _within(got, *exp[name], name)
+
+
 def test_extreme_scores():
     """Scores far apart (one key takes all) and large equal ones: finite, and the softmax of the definition."""
     from edifice_amd import fused_scan as fs
