@@ -126,6 +126,24 @@ def test_far_queries_against_a_band():
             _within(out[0, h, i], p @ vj, (2.0 ** -7 + 256 * U) * (p @ vj.abs()) + 2.0 ** -8 * (p @ vj).abs(), f"row {i}")
 
 
+@pytest.mark.parametrize("T, d, dtype", [((1 << 22) - 1, 128, bf16), ((1 << 22) - 1, 128, f32), ((1 << 22) + 70, 128, f32),
+                                         ((1 << 22) + 70, 64, bf16)], ids=str)
+def test_the_end_of_a_very_long_sequence(T, d, dtype):
+    """Offsets up to and past 2^31 bytes of one head: without sinks the last tokens are a sequence of their own."""
+    from edifice_amd import fused_scan as fs
+    announce("window_very_long", T=T, d=d, dtype=dtype)
+    window, last = 50, 400
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v, do = (torch.randn(1, 1, T, d, device="cuda", generator=g, dtype=dtype) for _ in range(4))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = fs.window_attention(q, k, v, window)
+    grads = torch.autograd.grad(out, leaves, do)
+    exp = _expected((1, 1, 1, last, d, window, 0, dtype), *(t.detach()[:, :, -last:].cpu() for t in (q, k, v, do)))
+    for name, got in zip(("O", "dQ", "dK", "dV"), (out, *grads)):
+        # from here on every query's keys, and every key's queries', lie in the piece
+        _within(got[:, :, -(last - window):], *(t[:, :, window:] for t in exp[name]), name)
+
+
 def test_causal_window_matches_flash_attention():
     """window >= T, one key head per query head: the causal flash kernel's result to their roundings."""
     from edifice_amd import fused_scan as fs
