@@ -18,13 +18,16 @@ struct WindowArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
   float *lse, *dd;   // [B Hq T]: natural-log row sums; D = rowsum(dO o O) / unscaled
-  float* part;       // backward: float32 dK, dV partials of key blocks that several workgroups share
+  float *part, *far;  // backward: float32 dK, dV parts of key blocks, and of sinks from far queries
   int T, G, d, W, S;
   int nx;            // workgroups per head (the grid is one-dimensional: its other axes end at 65535)
-  int c_sink, c_win, len_sink, len_win, nsb;  // backward: chunks and tiles per chunk of sink / other key blocks
+  // dK, dV (KvPlan): chunks and tiles per chunk of sink / other key blocks; parts of a head; blocks, 32-key groups,
+  // chunks and tiles per chunk of the sinks whose far queries have a kernel of their own; queries of a near tile
+  int nsb, c_sink, len_sink, c_win, len_win, slots, fsb, ng, c_far, len_far, bq;
   float scale, scale_log2;
 };
 
+constexpr int WINDOW_KB = 128;  // keys of a dK, dV workgroup
 constexpr int WINDOW_VEC_T = (1 << 22) - 1;  // longest sequence of the buffer loads: a head of 512-byte rows below 2^31 bytes
 
 EDF_DEVICE bool window_sees(int q, int key, int W, int S) { return key <= q && (q - key < W || key < S); }
@@ -262,53 +265,68 @@ struct KeyTiles {
   }
 };
 
-// Query tiles of BQ that see a key of block [k0, k0 + KB): from qs on, n of them per query head.
-template <int KB, int BQ>
-EDF_DEVICE void query_tiles(int k0, int T, int W, int S, int& qs, int& n) {
-  qs = k0;
-  const int end = k0 < S ? T : min(T, k0 + KB - 1 + W);  // one past the last query
-  n = (end - qs + BQ - 1) / BQ;
+// Query tiles of BQ that see a key of block [k0, k0 + KB), n of them per query head, from query k0 on; far: the queries
+// past the block's windows, which see its sinks alone, are left out.
+template <int KB>
+__host__ __device__ inline int query_tiles(int k0, int BQ, int T, int W, int S, bool far) {
+  const int end = T - k0;
+  return ((k0 < S && !far || end < KB - 1 + W ? end : KB - 1 + W) + BQ - 1) / BQ;
 }
 
 // The key block of workgroup xb of a dK, dV kernel and its share [t0, t1) of the block's (query head, tile) pairs,
-// nt tiles a head from query qs on; per: workgroups that share the block.
+// nt tiles a head from query qs on; slot: where its sums go if they are only a part of the block's, else -1.
 template <int KB, int BQ>
 struct KeyChunk {
-  int key0, qs, nt, t0, t1, per;
-  EDF_DEVICE KeyChunk(const WindowArgs& a, int xb) {
+  int key0, qs, nt, t0, t1;
+  long slot;
+  EDF_DEVICE KeyChunk(const WindowArgs& a, int xb, long bh) {
     const bool sink = xb < a.nsb * a.c_sink;
     const int x = sink ? xb : xb - a.nsb * a.c_sink, len = sink ? a.len_sink : a.len_win;
-    per = sink ? a.c_sink : a.c_win;
-    const int blk = (sink ? 0 : a.nsb) + x / per;
+    const int per = sink ? a.c_sink : a.c_win, blk = (sink ? 0 : a.nsb) + x / per;
     key0 = blk * KB;
-    query_tiles<KB, BQ>(key0, a.T, a.W, a.S, qs, nt);
+    qs = key0;
+    nt = query_tiles<KB>(key0, BQ, a.T, a.W, a.S, a.ng > 0);
     t0 = x % per * len;
     t1 = min(t0 + len, nt * a.G);
+    slot = per > 1 || blk < a.fsb ? bh * a.slots + xb : -1;
   }
 };
 
-// dK, dV of the blocks that were divided: the chunks' sums added in order, four elements a thread.  A workgroup takes
-// one of the pieces of a block's [dK | dV][key][dim]; blocks of one chunk are already in place.
+// The far queries of the sinks of key block k0: from query qs on, n tiles of 32 a head.
+struct FarTiles {
+  int qs, n;
+  EDF_DEVICE FarTiles(int k0, int BQ, int T, int W) {
+    qs = k0 + query_tiles<WINDOW_KB>(k0, BQ, T, W, 0, true) * BQ;
+    n = max(0, (T - qs + 31) / 32);
+  }
+};
+
+// dK, dV of the blocks whose sums are in parts: the chunks of the near queries, then those of the far ones, added in
+// order, four elements a thread.  A workgroup takes one of the pieces of a block's [dK | dV][key][dim].
 template <typename T, int HD, int KB, int BQ>
 __global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int blocks) {
   constexpr int PIECES = 2 * KB * HD / 1024;
   const int piece = blockIdx.x % PIECES, kblk = blockIdx.x / PIECES % blocks;
   const long bh = blockIdx.x / PIECES / blocks;  // batch x key head
-  const int kb0 = kblk * KB, per = kblk < a.nsb ? a.c_sink : a.c_win;
-  if (per == 1) return;
-  int qs, nt;
-  query_tiles<KB, BQ>(kb0, a.T, a.W, a.S, qs, nt);
-  const int len = kblk < a.nsb ? a.len_sink : a.len_win;
-  const int n = min(per, (nt * a.G + len - 1) / len);  // chunks that hold a tile
+  const int kb0 = kblk * KB, per = kblk < a.nsb ? a.c_sink : a.c_win, len = kblk < a.nsb ? a.len_sink : a.len_win;
+  if (per == 1 && kblk >= a.fsb) return;  // in place already
   const int x0 = kblk < a.nsb ? kblk * a.c_sink : a.nsb * a.c_sink + (kblk - a.nsb) * a.c_win;
+  const int tiles = query_tiles<KB>(kb0, BQ, a.T, a.W, a.S, a.ng > 0) * a.G;
+  const int n = min(per, (tiles + len - 1) / len);  // chunks that hold a tile
   const int e = (piece * 256 + threadIdx.x) * 4;
   const bool is_v = e >= KB * HD;
   const int key = e / HD % KB, c = e % HD;
   if (kb0 + key >= a.T || c >= a.d) return;
-  const float* in = a.part + (bh * a.nx + x0) * (2L * KB * HD) + e;
+  const float* in = a.part + (bh * a.slots + x0) * (2L * KB * HD) + e;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
   for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * KB * HD));
+  if (const int grp = (kb0 + key) / 32; grp < a.ng) {
+    const int nf = (FarTiles(kb0, BQ, a.T, a.W).n * a.G + a.len_far - 1) / a.len_far;
+    const float* far = a.far + (bh * a.ng + grp) * a.c_far * (64L * HD) + (is_v ? 32 * HD : 0) + key % 32 * HD + c;
+#pragma unroll 8
+    for (int i = 0; i < nf; ++i) s += *(const f32x4*)(far + i * (64L * HD));
+  }
   if (!is_v) s *= a.scale;
   T* out = (T*)(is_v ? a.dv : a.dk) + (bh * a.T + kb0 + key) * a.d + c;
 #pragma unroll
@@ -317,35 +335,66 @@ __global__ __launch_bounds__(256) void window_sum_kernel(WindowArgs a, int block
 }
 
 struct KvPlan {
-  int nkb, nsb, c_sink, c_win, len_sink, len_win;
+  int nkb, nsb, c_sink, c_win, len_sink, len_win;  // key blocks; the chunks of those with sinks and of the others
+  int fsb, ng, c_far, len_far;                     // blocks, 32-key groups and chunks of sinks with a kernel of their own
+  double rounds, cost;                             // of the GPU's places; in tiles
   int gx() const { return nsb * c_sink + (nkb - nsb) * c_win; }
-  bool divided() const { return (nsb > 0 && c_sink > 1) || (nkb > nsb && c_win > 1); }
+  // a head's workgroups that may leave parts, and the blocks that may be in parts, from the first
+  int slots() const { return (nsb > 0 && c_sink > 1) || (nkb > nsb && c_win > 1) ? gx() : fsb; }
+  int blocks() const { return nkb > nsb && c_win > 1 ? nkb : nsb > 0 && c_sink > 1 ? nsb : fsb; }
+  size_t part(int KB, int hd) const { return (size_t)slots() * 2 * KB * hd; }
+  size_t far(int hd) const { return (size_t)ng * c_far * 64 * hd; }
 };
 // How many workgroups share the tiles of a block of KB keys.  The GPU runs `slots` workgroups at once, so a call takes
 // about ceil(workgroups / slots) rounds of the longest share, and every workgroup of a divided block costs `join`
 // tiles more for its float32 sums, written and read again: the division with the least of that is taken.  A sink
 // block's tiles are divided into shares no longer than another block's (with many sink keys into longer ones, so
 // that there are not more of them than four rounds).
-inline KvPlan kv_plan(int heads, int G, int T, int W, int S, int KB, int BQ, int slots, int join) {
+inline KvPlan kv_divide(int heads, int G, int T, int W, int S, int KB, int BQ, int slots, int join) {
   KvPlan best{};
-  double least = 0.0;
   const int nkb = (T + KB - 1) / KB, nsb = std::min(nkb, (S + KB - 1) / KB);
   const long n_sink = (long)G * ((T + BQ - 1) / BQ);
   const long n_win = std::min(n_sink, (long)G * ((KB - 1 + W + BQ - 1) / BQ));
   for (long c = 1; c <= 64 && c <= n_win; ++c) {
-    KvPlan p{nkb, nsb, 1, 1, 0, 0};
+    KvPlan p{nkb, nsb, 1, 1, 0, 0, 0, 0, 0, 0, 0.0, 0.0};
     p.len_win = (int)((n_win + c - 1) / c);
     p.c_win = (int)((n_win + p.len_win - 1) / p.len_win);
     p.len_sink = (int)std::max((long)p.len_win, (n_sink * nsb * heads + 4L * slots - 1) / (4L * slots));
     p.c_sink = (int)std::max(1L, (n_sink + p.len_sink - 1) / p.len_sink);
-    const double wgs = (double)heads * p.gx(), rounds = std::max(1.0, wgs / slots);
+    const double rounds = std::max(1.0, (double)heads * p.gx() / slots);
     // a last round that is not full counts by half of what it lacks: workgroups end at different times
     const double whole = (double)(long)(rounds + 0.999999);
-    const double cost = 0.5 * (rounds + whole) * (std::max(p.len_win, nsb > 0 ? p.len_sink : 0) + 2.0 +
-                                                  (p.c_win > 1 ? join : 0));
-    if (c == 1 || cost < least) best = p, least = cost;
+    p.rounds = rounds;
+    p.cost = 0.5 * (rounds + whole) * (std::max(p.len_win, nsb > 0 ? p.len_sink : 0) + 2.0 + (p.c_win > 1 ? join : 0));
+    if (c == 1 || p.cost < best.cost) best = p;
   }
   return best;
+}
+// The far queries of sinks take part in the dK, dV kernel, where 32 keys keep one wave of four busy, or have a kernel
+// whose waves divide them (window_far_kernel).  That one costs 12 us of launch and latencies, and reads the queries'
+// rows at about 3.6 TB/s.  In the dK, dV kernel their tiles take the time of any others (about 0.9 PFLOP/s in bf16, 0.14
+// in float32), and in a call of less than two rounds without them much of the round that they add.  dK and dV together with dQ, in the
+// kernel / apart: bf16 1x32(8)x8192x128 window 300 353 / 323 us, 1x16(2)x16384x64 window 2048 650 / 592,
+// 4x16(4)x2000x96 window 500 204 / 177, 4x32(8)x4096x128 window 1024 1037 / 1034, 2x16(4)x3000x64 window 700 125 / 143,
+// 8x16(4)x1500x64 window 256 129 / 144; float32 1x8(4)x4000x128 window 2000 1122 / 1034, 2x8(4)x1000x64 window 300 96 /
+// 107.  Their own kernel has about one workgroup a CU, of at least two tiles a wave (more have more sums to join:
+// 4x32(8)x4096x128 54 us, 65 with two a CU), and 64 a group at most, which the sums read one by one.
+inline KvPlan kv_plan(int heads, int G, int T, int W, int S, int hd, int KB, int BQ, int es, int slots, int join) {
+  const KvPlan with = kv_divide(heads, G, T, W, S, KB, BQ, slots, join);
+  const int near = query_tiles<WINDOW_KB>(0, BQ, T, W, 0, true) * BQ;
+  if (S == 0 || near >= T) return with;
+  KvPlan p = kv_divide(heads, G, T, W, 0, KB, BQ, slots, join);
+  const double tile = 8.0 * KB * BQ * hd / (es == 2 ? 0.9e9 : 0.14e9);  // us of the whole GPU
+  const double far = (double)heads * G * (T - near);                  // query rows
+  const int ng = (S + 31) / 32;
+  const double more = far / BQ * with.nsb * tile + (p.rounds < 2.0 ? 0.6 * (with.cost - p.cost) * tile * slots : 0.0);
+  if (more < 1.2 * (12.0 + far * ng * 2.0 * hd * es / 3.6e6)) return with;
+  p.fsb = with.nsb, p.ng = ng;
+  const long n = (long)G * ((T - near + 31) / 32);  // of the first block, which has the most
+  const long len = std::max({8L, (long)((double)n * ng * heads / 256.0), (n + 63) / 64});
+  p.len_far = (int)((len + 3) / 4 * 4);
+  p.c_far = (int)((n + p.len_far - 1) / p.len_far);
+  return p;
 }
 
 inline int window_pad(int d) { return (d + 31) / 32 * 32; }
@@ -362,18 +411,25 @@ int kv_join(int KB, int BQ) {
   return sizeof(T) == 4 ? 2 : 16 * 32 / BQ;
 }
 
-// a dK, dV kernel and the sums of the blocks that several of its workgroups share
-template <typename T, int HD, int KB, int BQ, typename F>
+// dK, dV sums of the sinks' far queries (window_narrow.hip)
+int window_far_run(hipStream_t s, const WindowArgs& a, int BHkv, int dtype, bool vec);
+
+// a dK, dV kernel, the sinks' far queries, and the sums of the blocks that are in parts
+template <typename T, int HD, int KB, int BQ, bool VEC, typename F>
 int launch_dkdv(hipStream_t s, WindowArgs a, int BHkv, F kernel) {
-  const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, KB, BQ, kv_slots<T>(HD), kv_join<T>(KB, BQ));
-  a.nsb = p.nsb, a.c_sink = p.c_sink, a.c_win = p.c_win, a.len_sink = p.len_sink, a.len_win = p.len_win;
+  const KvPlan p = kv_plan(BHkv, a.G, a.T, a.W, a.S, HD, KB, BQ, sizeof(T), kv_slots<T>(HD), kv_join<T>(KB, BQ));
+  a.nsb = p.nsb, a.c_sink = p.c_sink, a.len_sink = p.len_sink, a.c_win = p.c_win, a.len_win = p.len_win;
+  a.slots = p.slots(), a.fsb = p.fsb, a.ng = p.ng, a.c_far = p.c_far, a.len_far = p.len_far, a.bq = BQ;
+  a.far = a.part + p.part(KB, HD) * BHkv;
   a.nx = p.gx();
-  const int blocks = p.nkb > p.nsb && p.c_win > 1 ? p.nkb : p.nsb;  // the divided ones, from the first
-  const long wgs = (long)a.nx * BHkv, sums = 2L * KB * HD / 1024 * blocks * BHkv;
-  EDF_REQUIRE(wgs < (1L << 31) && sums < (1L << 31), EDF_ERR_UNSUPPORTED, "batch x heads x seq_len too large for one call");
+  const int blocks = p.blocks();
+  const long wgs = (long)a.nx * BHkv, sums = 2L * KB * HD / 1024 * blocks * BHkv, far = (long)p.ng * p.c_far * BHkv;
+  EDF_REQUIRE(wgs < (1L << 31) && sums < (1L << 31) && far < (1L << 31), EDF_ERR_UNSUPPORTED,
+              "batch x heads x seq_len too large for one call");
   kernel<<<(unsigned)wgs, 256, 0, s>>>(a);
-  const int rc = check_launch("window attention dK, dV");
-  if (rc || !p.divided()) return rc;
+  int rc = check_launch("window attention dK, dV");
+  if (!rc && far) rc = window_far_run(s, a, BHkv, sizeof(T) == 2 ? EDF_BF16 : EDF_F32, VEC);
+  if (rc || !blocks) return rc;
   window_sum_kernel<T, HD, KB, BQ><<<(unsigned)sums, 256, 0, s>>>(a, blocks);
   return check_launch("window attention dK, dV sums");
 }

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
   long bh;  // batch x key head
   window_block(a, xb, bh);
   const int T_ = a.T, d = a.d;
-  const KeyChunk<WB_M, BQ> kc_(a, xb);
+  const KeyChunk<WB_M, BQ> kc_(a, xb, bh);
   const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
 
   const T* K = (const T*)a.k + bh * T_ * d;
@@ -395,8 +395,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     }
     __syncthreads();
   }
-  if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
-    float* out = a.part + (bh * a.nx + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
+  if (kc_.slot >= 0) {  // these sums are a part: [dK | dV][key][dim] of the block
+    float* out = a.part + kc_.slot * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -457,7 +457,7 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
   long bh;  // batch x key head
   window_block(a, xb, bh);
   const int T = a.T;
-  const KeyChunk<WB_M, BQ> kc_(a, xb);
+  const KeyChunk<WB_M, BQ> kc_(a, xb, bh);
   const int kb0 = kc_.key0, kw = kb0 + 32 * w, mykey = kw + li, qs = kc_.qs, nt = kc_.nt, t0 = kc_.t0, t1 = kc_.t1;
 
   // keys past the end read zero rows of V: they only feed their own columns, never stored
@@ -575,8 +575,8 @@ __global__ __launch_bounds__(256, 2) void window_dkdv128_kernel(WindowArgs a) {
     step(b0, t);
     if (t + 1 < t1) step(b1, t + 1);
   }
-  if (kc_.per > 1) {  // this chunk's sums: [dK | dV][key][dim] of the block
-    float* out = a.part + (bh * a.nx + xb) * (2L * WB_M * HD) + (32 * w + li) * HD;
+  if (kc_.slot >= 0) {  // these sums are a part: [dK | dV][key][dim] of the block
+    float* out = a.part + kc_.slot * (2L * WB_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -627,9 +627,9 @@ int launch_bwd(hipStream_t s, WindowArgs a, int BH, int BHkv) {
   }
   if (rc) return rc;
   if constexpr (dma) {
-    if (fast) return launch_dkdv<bf16, 128, WB_M, BQ_32>(s, a, BHkv, window_dkdv128_kernel);
+    if (fast) return launch_dkdv<bf16, 128, WB_M, BQ_32, VEC>(s, a, BHkv, window_dkdv128_kernel);
   }
-  return launch_dkdv<T, HD, WB_M, BQ>(s, a, BHkv, window_dkdv_kernel<T, HD, BQ, VEC>);
+  return launch_dkdv<T, HD, WB_M, BQ, VEC>(s, a, BHkv, window_dkdv_kernel<T, HD, BQ, VEC>);
 }
 
 
@@ -660,9 +660,9 @@ size_t edf_window_attention_backward_workspace_bytes(int batch, int num_heads, i
   auto need = [&](int kb, int bq) {
     const int hd = window_pad(head_dim), G = num_heads / num_kv_heads;
     const KvPlan p = dtype == EDF_BF16
-                         ? kv_plan(heads, G, seq_len, W, S, kb, bq, kv_slots<bf16>(hd), kv_join<bf16>(kb, bq))
-                         : kv_plan(heads, G, seq_len, W, S, kb, bq, kv_slots<float>(hd), kv_join<float>(kb, bq));
-    if (p.divided()) sums = std::max(sums, (size_t)heads * p.gx() * 2 * kb * hd * sizeof(float));
+                         ? kv_plan(heads, G, seq_len, W, S, hd, kb, bq, 2, kv_slots<bf16>(hd), kv_join<bf16>(kb, bq))
+                         : kv_plan(heads, G, seq_len, W, S, hd, kb, bq, 4, kv_slots<float>(hd), kv_join<float>(kb, bq));
+    sums = std::max(sums, heads * (p.part(kb, hd) + p.far(hd)) * sizeof(float));
   };
   need(WB_M, BQ_32);
   if (dtype == EDF_BF16) need(WB_M, BQ_BF16);

@@ -2,7 +2,7 @@
 // a workgroup owns 32 queries and its four waves divide the key tiles among them, each with results of its own that
 // are joined in LDS at the end.  No tile is shared, so there is no barrier in the loops, and a call has four times
 // the workgroups of the wide form: it takes the calls whose wide grid would leave the GPU half empty
-// (window_narrow).  Rows of whole 16-byte pieces only.
+// (window_narrow).  Rows of whole 16-byte pieces only.  The far queries' kernel at the end is built the same way.
 //
 // Row operands (a lane's 8 elements of one row) come straight from memory, a tile ahead of their use.
 // Transposed operands come through a wave-private LDS copy of the tile; the forward in float32 past head_dim 64 reads
@@ -27,10 +27,11 @@ struct NTile {
   static constexpr int NKK = HD / 16, NDT = HD / 32;
   using Tile = WTile<T, HD, WN_R>;
   // rows past the end repeat the last one: their scores are masked
+  template <bool VEC = true>
   EDF_DEVICE static void rows(const T* x, int r0, int T_, int d, int l, WFrag<T>* f) {
     const T* row = x + (long)min(r0 + (l & 31), T_ - 1) * d;
 #pragma unroll
-    for (int kk = 0; kk < NKK; ++kk) f[kk] = window_row<T, HD, true>(row, kk * 16 + 8 * (l >> 5), d);
+    for (int kk = 0; kk < NKK; ++kk) f[kk] = window_row<T, HD, VEC>(row, kk * 16 + 8 * (l >> 5), d);
   }
   EDF_DEVICE static void keep(T* lds, int l, const WFrag<T>* f) {  // row fragments into the wave's LDS tile
 #pragma unroll
@@ -276,6 +277,119 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(4, 1))) void narrow_dq_
   if (w == 0 && myq < T_) store_rows_t<T, HD>((T*)a.dq + qrow * d, dq, a.scale, d, g);
 }
 
+// dK, dV parts of 32 sink keys from a chunk of their far queries: the waves divide the chunk's tiles of 32 queries, as
+// in the kernels above, with the roles of queries and keys exchanged.  In the dK, dV kernels, whose four waves take 32
+// keys of a block each, a few sinks leave three of them idle over all queries (kv_plan has the times of both).  Bound by
+// the rows of Q and dO, read a second time: 1x32(8)x8192x128 window 300 37 us, 3.4 TB/s.
+template <typename T, int HD, bool VEC>
+__global__ __launch_bounds__(256, 1) void window_far_kernel(WindowArgs a) {
+  constexpr int NKK = HD / 16, NDT = HD / 32;
+  using N = NTile<T, HD, true>;
+  constexpr int TILE = N::Tile::ELEMS * (int)sizeof(T), JOIN = 2 * NDT * 64 * 64;
+  __shared__ __attribute__((aligned(16))) char smem[2 * WN_WAVES * TILE > JOIN ? 2 * WN_WAVES * TILE : JOIN];
+  __shared__ __attribute__((aligned(16))) float sL[WN_WAVES][32], sD[WN_WAVES][32];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  int xb;
+  long bh;  // batch x key head
+  window_block(a, xb, bh);
+  const int T_ = a.T, d = a.d;
+  const int grp = xb / a.c_far, chunk = xb % a.c_far, key0 = 32 * grp;
+  const FarTiles ft(key0 / WINDOW_KB * WINDOW_KB, a.bq, T_, a.W);
+  const int t0 = chunk * a.len_far, t1 = min(t0 + a.len_far, ft.n * a.G);
+  T* sq = reinterpret_cast<T*>(smem + 2 * w * TILE);
+  T* so = reinterpret_cast<T*>(smem + (2 * w + 1) * TILE);
+
+  WFrag<T> kf[NKK], vf[NKK], qf[NKK], of[NKK];
+  N::template rows<VEC>((const T*)a.k + bh * T_ * d, key0, T_, d, l, kf);
+  N::template rows<VEC>((const T*)a.v + bh * T_ * d, key0, T_, d, l, vf);
+  f32x16 dk[NDT], dv[NDT];  // dK^T, dV^T: rows are dims, the column this lane's key
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    dk[dt] = zero16();
+    dv[dt] = zero16();
+  }
+  float rl = 0.0f, rd = 0.0f;
+  auto load = [&](int t) {
+    const int h = t / ft.n, q0 = ft.qs + (t - h * ft.n) * 32;
+    const long base = (bh * a.G + h) * T_;
+    N::template rows<VEC>((const T*)a.q + base * d, q0, T_, d, l, qf);
+    N::template rows<VEC>((const T*)a.go + base * d, q0, T_, d, l, of);
+    const long q = base + min(q0 + li, T_ - 1);
+    rl = q0 + li < T_ ? a.lse[q] * LOG2E : INFINITY;  // a query past the end gets P = 0
+    rd = a.dd[q];
+  };
+  if (t0 + w < t1) load(t0 + w);
+  for (int t = t0 + w; t < t1; t += WN_WAVES) {
+    N::keep(sq, l, qf);
+    N::keep(so, l, of);
+    if (g == 0) sL[w][li] = rl, sD[w][li] = rd;
+    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      s = WFrag<T>::mma(qf[kk], kf[kk], s);
+      dp = WFrag<T>::mma(of[kk], vf[kk], dp);
+    }
+    if (t + WN_WAVES < t1) load(t + WN_WAVES);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const f32x4 lv = *(const f32x4*)(&sL[w][8 * rb + 4 * g]);
+      const f32x4 dv4 = *(const f32x4*)(&sD[w][8 * rb + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 4 + e;
+        const float p = fast_exp2(fmaf(s[r], a.scale_log2, -lv[e]));
+        dp[r] = p * (dp[r] - dv4[e]);  // 1 / sqrt(d) is applied with the sums
+        s[r] = p;
+      }
+    }
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      WFrag<T> pf, df;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pf.set(e, s[8 * kc + e]);
+        df.set(e, dp[8 * kc + e]);
+      }
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        dv[dt] = WFrag<T>::mma(N::Tile::trans(so, 16 * kc, dt, l), pf, dv[dt]);
+        dk[dt] = WFrag<T>::mma(N::Tile::trans(sq, 16 * kc, dt, l), df, dk[dt]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  join_waves<NDT>(dk, (f32x16*)smem, w, l);
+  join_waves<NDT>(dv, (f32x16*)smem, w, l);
+  if (w != 0) return;
+  const bool sink = key0 + li < a.S;  // the group's other keys are not seen from here
+  float* out = a.far + ((bh * a.ng + grp) * a.c_far + chunk) * (64L * HD) + li * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      f32x4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = sink ? dk[dt][rb * 4 + e] : 0.0f;
+        y[e] = sink ? dv[dt][rb * 4 + e] : 0.0f;
+      }
+      *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) = x;
+      *(f32x4*)(out + 32 * HD + dt * 32 + 8 * rb + 4 * g) = y;
+    }
+}
+
+template <typename T, bool VEC>
+void run_far(hipStream_t s, const WindowArgs& a, unsigned grid) {
+  switch (window_pad(a.d)) {
+    case 32: window_far_kernel<T, 32, VEC><<<grid, 256, 0, s>>>(a); break;
+    case 64: window_far_kernel<T, 64, VEC><<<grid, 256, 0, s>>>(a); break;
+    case 96: window_far_kernel<T, 96, VEC><<<grid, 256, 0, s>>>(a); break;
+    default: window_far_kernel<T, 128, VEC><<<grid, 256, 0, s>>>(a);
+  }
+}
+
 template <typename T, int HD>
 void run(bool backward, hipStream_t s, WindowArgs a, int BH) {
   a.nx = (a.T + WN_R - 1) / WN_R;
@@ -299,6 +413,15 @@ int window_narrow_run(bool backward, hipStream_t s, const WindowArgs& a, int BH,
   if (dtype == EDF_BF16) run_d<bf16>(backward, s, a, BH);
   else run_d<float>(backward, s, a, BH);
   return check_launch(backward ? "window attention dQ" : "window attention");
+}
+
+int window_far_run(hipStream_t s, const WindowArgs& args, int BHkv, int dtype, bool vec) {
+  WindowArgs a = args;
+  a.nx = a.ng * a.c_far;
+  const unsigned grid = (unsigned)a.nx * (unsigned)BHkv;
+  if (dtype == EDF_BF16) vec ? run_far<bf16, true>(s, a, grid) : run_far<bf16, false>(s, a, grid);
+  else vec ? run_far<float, true>(s, a, grid) : run_far<float, false>(s, a, grid);
+  return check_launch("window attention dK, dV of far queries");
 }
 
 }  // namespace edf

@@ -126,6 +126,60 @@ def test_far_queries_against_a_band():
             _within(out[0, h, i], p @ vj, (2.0 ** -7 + 256 * U) * (p @ vj.abs()) + 2.0 ** -8 * (p @ vj).abs(), f"row {i}")
 
 
+def _banded(q, k, v, do, window, sinks, h):
+    """_expected for one query head [T, d] of a long sequence and a short window, from the keys that each query sees."""
+    T, d = q.shape
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    i = torch.arange(T, device=q.device)[:, None]
+    near, sink = i - torch.arange(window, device=q.device), torch.arange(sinks, device=q.device).expand(T, sinks)
+    idx = torch.cat([near.clamp(min=0), sink], 1)
+    seen = torch.cat([near >= 0, sink <= i - window], 1)
+    kj, vj, s = k[idx], v[idx], d ** -0.5
+    p = torch.softmax(((kj * q[:, None]).sum(-1) * s).masked_fill(~seen, -math.inf), 1)
+    o = (p[..., None] * vj).sum(1)
+    dp, dd = (vj * do[:, None]).sum(-1), (do * o).sum(-1, keepdim=True)
+    ds = p * (dp - dd)
+    size = p * ((vj.abs() * do.abs()[:, None]).sum(-1) + (do * o).abs().sum(-1, keepdim=True))
+    e = h * (p * (do * o).abs().sum(-1, keepdim=True) + ds.abs()) + 256 * U * size
+    # a sink's sums: fewer than 2048 additions, one after another, in a wave, between waves and between workgroups
+    n = 2048 * U
+    back = lambda w, x: torch.zeros_like(k).index_add_(0, idx.flatten(), (w[..., None] * x[:, None]).flatten(0, 1))  # noqa: E731
+    return ((s * back(ds, q), s * back(e + n * ds.abs(), q.abs())), (back(p, do), (h + n) * back(p, do.abs())),
+            (s * (ds[..., None] * kj).sum(1), s * (e[..., None] * kj.abs()).sum(1)))
+
+
+@pytest.mark.parametrize("case", [(1, 8, 1, 6000, 32, bf16, 0, 3), (1, 128, 8, 8192, 32, bf16, 0, 3), (1, 128, 8, 8192, 32, bf16, 1, 3),
+                                  (2, 32, 4, 6000, 64, bf16, 0, 3), (2, 32, 4, 6000, 64, bf16, 0, 40), (2, 32, 4, 6001, 64, bf16, 1, 3),
+                                  (1, 128, 8, 8192, 88, bf16, 0, 3), (1, 128, 8, 8180, 88, bf16, 1, 3),
+                                  (2, 32, 4, 6000, 128, bf16, 0, 3), (2, 32, 4, 6000, 128, bf16, 1, 3),
+                                  (2, 16, 2, 6000, 32, f32, 0, 3), (2, 16, 2, 6000, 32, f32, 1, 40), (1, 8, 1, 6001, 64, f32, 0, 40),
+                                  (1, 8, 1, 6000, 64, f32, 1, 3), (1, 8, 2, 6000, 84, f32, 0, 3), (1, 8, 2, 6000, 84, f32, 1, 3),
+                                  (1, 8, 1, 5999, 128, f32, 0, 140), (1, 8, 1, 3000, 126, f32, 0, 3)], ids=str)
+def test_sinks_of_a_long_sequence(case):
+    """dK and dV of sinks that thousands of queries see past their windows, in the calls that give these queries a
+    kernel of their own and those that do not; tensors whole 16 bytes or one element off them."""
+    from edifice_amd import fused_scan as fs
+    B, Hq, Hkv, T, d, dtype, off, sinks = case
+    announce("window_sinks", case=case)
+    window, g = 9, torch.Generator(device="cuda").manual_seed(sinks)
+
+    def make(H_):
+        buf = torch.randn(B * H_ * T * d + off, device="cuda", generator=g, dtype=torch.float32).to(dtype)
+        return buf[off:].view(B, H_, T, d)
+    q, k, v, do = (make(n) for n in (Hq, Hkv, Hkv, Hq))
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(fs.window_attention(q, k, v, window, sinks), leaves, do)
+    G, half = Hq // Hkv, max(H[dtype], U)
+    b, kh = B - 1, Hkv - 1
+    heads = [_banded(*(t.detach()[b, h] for t, h in ((q, h), (k, kh), (v, kh), (do, h))), window, sinks, H[dtype])
+             for h in range(kh * G, (kh + 1) * G)]
+    for x, got, name in ((0, dk, "dK"), (1, dv, "dV")):
+        want, tol = (sum(h[x][y] for h in heads) for y in (0, 1))
+        _within(got[b, kh], want.cpu(), (tol + half * want.abs()).cpu(), name)
+    want, tol = heads[-1][2]
+    _within(dq[b, -1], want.cpu(), (tol + half * want.abs()).cpu(), "dQ")
+
+
 @pytest.mark.parametrize("T, d, dtype", [((1 << 22) - 1, 128, bf16), ((1 << 22) - 1, 128, f32), ((1 << 22) + 70, 128, f32),
                                          ((1 << 22) + 70, 64, bf16)], ids=str)
 def test_the_end_of_a_very_long_sequence(T, d, dtype):
