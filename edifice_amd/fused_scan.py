@@ -1125,15 +1125,17 @@ class _SplitHeadsRotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk, dv):
         x, wq, wk, freq, positions = ctx.saved_tensors
-        g = [t.contiguous().to(x.dtype) for t in (dq, dk, dv)]
-        dx = torch.empty_like(x)
-        dwq, dwk = (None if w is None else torch.zeros_like(w) if not x.numel() else torch.empty_like(w)
-                    for w in (wq, wk))
-        if x.numel():
-            wsb = 0 if wq is None else nat.query("edf_heads_split_rotary_backward_workspace_bytes", ctx.conf[4])
+        dq, dk, dv = (t.contiguous() if t.dtype == x.dtype else t.contiguous().to(x.dtype) for t in (dq, dk, dv))
+        if not x.numel():
+            zero = None if wq is None else torch.zeros_like(wq)
+            return torch.empty_like(x), zero, zero, None, None, None, None, None, None, None
+        dx, dwq, dwk, ws, wsb = torch.empty_like(x), None, None, None, 0
+        if wq is not None:
+            dwq, dwk = torch.empty_like(wq), torch.empty_like(wk)
+            wsb = nat.query("edf_heads_split_rotary_backward_workspace_bytes", ctx.conf[4])
             ws = _u8(wsb, x)
-            nat.call("edf_heads_split_rotary_backward", _stream(), _p(x), _p(freq), _p(positions), _p(wq), _p(wk),
-                     *(_p(t) for t in g), _p(dx), _p(dwq), _p(dwk), _p(ws), wsb, *ctx.conf)
+        nat.call("edf_heads_split_rotary_backward", torch._C._cuda_getCurrentRawStream(x.get_device()), _p(x), _p(freq),
+                 _p(positions), _p(wq), _p(wk), _p(dq), _p(dk), _p(dv), _p(dx), _p(dwq), _p(dwk), _p(ws), wsb, *ctx.conf)
         return dx, dwq, dwk, None, None, None, None, None, None, None
 
 
