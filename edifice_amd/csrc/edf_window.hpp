@@ -28,7 +28,8 @@ struct WindowArgs {
 };
 
 constexpr int WINDOW_KB = 128;  // keys of a dK, dV workgroup
-constexpr int WINDOW_VEC_T = (1 << 22) - 1;  // longest sequence of the buffer loads: a head of 512-byte rows below 2^31 bytes
+// longest sequence of the buffer loads: a head of 512-byte rows below 2^31 bytes
+constexpr int WINDOW_VEC_T = (1 << 22) - 1;
 
 EDF_DEVICE bool window_sees(int q, int key, int W, int S) { return key <= q && (q - key < W || key < S); }
 // the same for key first + c of one query, c a constant after unrolling: three values stay in registers
@@ -373,9 +374,9 @@ inline KvPlan kv_divide(int heads, int G, int T, int W, int S, int KB, int BQ, i
 // The far queries of sinks take part in the dK, dV kernel, where 32 keys keep one wave of four busy, or have a kernel
 // whose waves divide them (window_far_kernel).  That one costs 12 us of launch and latencies, and reads the queries'
 // rows at about 3.6 TB/s.  In the dK, dV kernel their tiles take the time of any others (about 0.9 PFLOP/s in bf16, 0.14
-// in float32), and in a call of less than two rounds without them much of the round that they add.  dK and dV together with dQ, in the
-// kernel / apart: bf16 1x32(8)x8192x128 window 300 353 / 323 us, 1x16(2)x16384x64 window 2048 650 / 592,
-// 4x16(4)x2000x96 window 500 204 / 177, 4x32(8)x4096x128 window 1024 1037 / 1034, 2x16(4)x3000x64 window 700 125 / 143,
+// in float32), and in a call of less than two rounds without them much of the round that they add.  dK and dV together
+// with dQ, in the kernel / apart: bf16 1x32(8)x8192x128 window 300 353 / 313 us, 1x16(2)x16384x64 window 2048 650 / 592,
+// 4x16(4)x2000x96 window 500 204 / 175, 4x32(8)x4096x128 window 1024 1037 / 1034, 2x16(4)x3000x64 window 700 125 / 143,
 // 8x16(4)x1500x64 window 256 129 / 144; float32 1x8(4)x4000x128 window 2000 1122 / 1034, 2x8(4)x1000x64 window 300 96 /
 // 107.  Their own kernel has about one workgroup a CU, of at least two tiles a wave (more have more sums to join:
 // 4x32(8)x4096x128 54 us, 65 with two a CU), and 64 a group at most, which the sums read one by one.

@@ -189,7 +189,8 @@ int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, c
               "requests x table_width must be below 2^31");
   EDF_REQUIRE(table && old_lengths && new_lengths && (free_blocks || num_free == 0) && slots && positions && used,
               EDF_ERR_INVALID_ARG, "null tensor pointer");
-  EDF_REQUIRE(taken != used, EDF_ERR_INVALID_ARG, "taken and used must be two places: workgroups read one while the other is written");
+  EDF_REQUIRE(taken != used, EDF_ERR_INVALID_ARG,
+              "taken and used must be two places: workgroups read one while the other is written");
   const unsigned grid = (unsigned)(((long)requests * num_tokens + PX_ITEMS - 1) / PX_ITEMS);
   paged_extend_kernel<<<grid, PX_NT, 0, as_stream(stream)>>>(table, old_lengths, new_lengths, free_blocks, taken,
                                                              slots, positions, used, requests, table_width, num_free,

@@ -62,7 +62,8 @@ EDF_DEVICE void join_waves(f32x16* x, f32x16* lds, int w, int l) {
       for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          *((f32x4*)(lds) + (((w - half) * N + n) * 4 + r) * 64 + l) = f32x4{x[n][4 * r], x[n][4 * r + 1], x[n][4 * r + 2], x[n][4 * r + 3]};
+          *((f32x4*)(lds) + (((w - half) * N + n) * 4 + r) * 64 + l) =
+              f32x4{x[n][4 * r], x[n][4 * r + 1], x[n][4 * r + 2], x[n][4 * r + 3]};
     __syncthreads();
     if (w < half)
 #pragma unroll

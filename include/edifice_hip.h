@@ -670,7 +670,8 @@ int edf_heads_split_rotary_backward(void* stream, const void* x, const double* f
  *   scores / sqrt(d).
  * lse (may be NULL): float32 [batch, num_heads, seq_len] natural-log row sums, required by the backward.
  * head_dim <= 128, sinks <= 2^22.  Keys and values have to be finite: a value that is not may also reach queries that
- * do not see its key, where another key of its 64-key tile is seen.  The backward's workspace: edf_window_attention_backward_workspace_bytes().
+ * do not see its key, where another key of its 64-key tile is seen.
+ * The backward's workspace: edf_window_attention_backward_workspace_bytes().
  * ------------------------------------------------------------------------ */
 int edf_window_attention(void* stream, const void* q, const void* k, const void* v, void* out, float* lse, int batch,
                          int num_heads, int num_kv_heads, int seq_len, int head_dim, int window, int sinks, int dtype);
@@ -689,9 +690,10 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  * edf_paged_extend: request r grows from old_lengths[r] to new_lengths[r] tokens (negative ones count as 0;
  *   new <= old: nothing).  Its pages ceil(old / block_size) .. ceil(new / block_size) - 1 (within the table's
  *   width) are the next entries of free_blocks [num_free], request by request, after the first taken[0] (NULL: 0),
- *   and are written into table; past the list's end they are -1.  slots, positions [requests, num_tokens]: those of token old_lengths[r] + t, or
- *   -1 past new_lengths[r]; a token without a page has the position and slot -1.  used [1]: taken[0] plus the
- *   pages drawn (the next call's taken), which exceeds num_free when the list was too short; not taken itself.
+ *   and are written into table; past the list's end they are -1.  slots, positions [requests, num_tokens]: those of
+ *   token old_lengths[r] + t, or -1 past new_lengths[r]; a token without a page has the position and slot -1.
+ *   used [1]: taken[0] plus the pages drawn (the next call's taken), which exceeds num_free when the list was too
+ *   short; not taken itself.
  * edf_paged_cache_write: rows of k, v [batch, num_kv_heads, seq, d] into the pages by slots [batch, seq]; slots
  *   outside [0, num_blocks * block_size) are left out.  Slots have to differ from one another.
  * edf_paged_attention: one query per request, q, out [batch, num_heads, d], over the request's first lengths[b]

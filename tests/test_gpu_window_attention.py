@@ -309,11 +309,11 @@ def test_side_stream():
     assert torch.equal(got, want)
 
 
-def test_captured_forward_and_backward():
+@pytest.mark.parametrize("case", [(1, 4, 2, 300, 64, 100, 2, bf16), (1, 8, 1, 6001, 64, 9, 40, f32)], ids=str)
+def test_captured_forward_and_backward(case):
     """Forward and backward through the C entry points in one graph, replayed on new contents."""
     from edifice_amd import fused_scan as fs
-    announce("window_graph")
-    case = (1, 4, 2, 300, 64, 100, 2, bf16)
+    announce("window_graph", case=case)
     B, Hq, Hkv, T, d, window, sinks, dtype = case
     st = [t.cuda() for t in _make(case)]
 
