@@ -416,8 +416,9 @@ extern "C" {
 
 size_t edf_paged_attention_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width,
                                            int block_size, int window, int sinks) {
-  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || table_width <= 0 || block_size <= 0 ||
-      window < 0 || sinks < 0)
+  // a head count that the call refuses is no plan either (fewer query heads than key heads would divide by none)
+  if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || head_dim <= 0 ||
+      table_width <= 0 || block_size <= 0 || window < 0 || sinks < 0)
     return 0;
   int chunk, splits;
   edf::plan(batch, num_kv_heads, (num_heads / num_kv_heads + 15) / 16,
