@@ -302,9 +302,11 @@ class PagedCache:
         return fs.paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, window=window, sinks=sinks)
 
     def exhausted(self) -> bool:
-        """Whether some token found no page: the list of free ones ended, or a table row (waits for the GPU)."""
-        return int(self.taken) > self.available or bool(
-            (self.lengths > self.table.shape[1] * self.block_size).any())
+        """Whether some place holds a token that found no page: the list of free ones ended, or its table row (waits for
+        the GPU).  It does until that place is released: the rest of a missing page finds none either."""
+        width = self.table.shape[1]
+        held = torch.arange(width, device=self.table.device) * self.block_size < self.lengths[:, None]
+        return bool(((self.table < 0) & held).any() | (self.lengths > width * self.block_size).any())
 
     def release(self, place: int) -> None:
         """The place's pages back onto the list of free ones, its length 0 (waits for the GPU)."""

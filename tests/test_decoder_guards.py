@@ -5,8 +5,10 @@ import itertools
 import pytest
 import torch
 
+from edifice_amd import blocks
 from edifice_amd import fused_scan as fs
 from edifice_amd._native import EdificeHipError, lib
+from oracle import decoder as od
 
 INT_MAX = 2 ** 31 - 1
 
@@ -36,3 +38,36 @@ def test_paged_attention_refuses_head_counts(host_tensors, heads, kv_heads):
     q, cache = torch.zeros(1, heads, 64), torch.zeros(2, kv_heads, 8, 64)
     with pytest.raises(EdificeHipError, match="multiple"):
         fs.paged_attention(q, cache, cache.clone(), torch.zeros(1, 2).int(), torch.ones(1).int())
+
+
+def _listed(table, old, new, free, block, tokens, taken=None):
+    """paged_extend on the CPU, by the oracle."""
+    at = max(int(taken), 0) if taken is not None else 0
+    t, slots, positions, used = od.paged_extend(table.tolist(), old.tolist(), new.tolist(), free.tolist()[at:], block,
+                                                tokens)
+    table.copy_(torch.tensor(t))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return i32(slots), i32(positions), i32([at + used])
+
+
+def test_a_missing_page_is_reported_until_its_place_is_released(monkeypatch):
+    """Another place's release gives pages back and takes no report away: the place's later tokens of the missing page
+    find none, which the report says."""
+    monkeypatch.setattr(fs, "paged_extend", _listed)
+    c = blocks.PagedCache(1, 3, 8, 1, 32, block_size=4, num_blocks=1, device="cpu")
+    counts = lambda *n: torch.tensor(n, dtype=torch.int32)  # noqa: E731
+    c.extend(1, counts(1, 0, 0))
+    assert not c.exhausted()
+    c.extend(1, counts(0, 1, 0))
+    assert c.exhausted() and c.table.tolist() == [[0, -1], [-1, -1], [-1, -1]]
+    c.release(0)
+    slots, _ = c.extend(3, counts(0, 3, 0))
+    assert slots.tolist()[1] == [-1, -1, -1] and c.exhausted()
+    c.extend(1, counts(0, 1, 0))  # the next page is found
+    assert c.table.tolist()[1] == [-1, 0] and c.exhausted()
+    c.release(1)
+    assert not c.exhausted()
+    assert c.extend(4, counts(4, 0, 0))[0].tolist()[0] == [0, 1, 2, 3] and not c.exhausted()
+    c.release(0)
+    c.lengths[2] = 9  # past the table's row
+    assert c.exhausted()
