@@ -338,8 +338,28 @@ class GQAttention(nn.Module):
         self.window, self.sinks, self.rotary_dim, self.rotary_base = window, sinks, rotary_dim, rotary_base
         self.q_norm = nn.Parameter(torch.ones(hd)) if qk_norm else None
         self.k_norm = nn.Parameter(torch.ones(hd)) if qk_norm else None
-        self._frequencies = None  # float64 whatever the module is cast to, so not a buffer
         self.shared = bool(rotary_dim or qk_norm or window or sinks)
+        self._frequencies = None  # float64 whatever the module is cast to, so not a buffer
+        self._angles(self.q_proj.weight.device)
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        self._angles(self.q_proj.weight.device)  # on the new device before the first call, which may be captured
+        return self
+
+    def _angles(self, device):
+        """Angle per position of each rotated pair on that device (None: no rotation)."""
+        if not self.rotary_dim:
+            return None
+        of = self.rotary_dim, self.rotary_base
+        if self._frequencies is None or self._frequencies_of != of or self._frequencies.device != device:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("rotary_dim, rotary_base or the input's device has changed: the first call after that "
+                                   "copies the angles from the host and cannot be captured")
+            with torch.inference_mode(False):  # whichever call comes first, a later one may train
+                self._frequencies = fs.rotary_frequencies(*of, device=device)
+            self._frequencies_of = of
+        return self._frequencies
 
     def _stacked(self, x):
         """q | k | v as one product over the stacked weights: [B, T, (num_heads + 2 num_kv_heads) head_dim]."""
@@ -351,9 +371,7 @@ class GQAttention(nn.Module):
         return _LinearFn.apply(x, w, b)
 
     def _heads(self, x, positions=None):
-        if self.rotary_dim and (self._frequencies is None or self._frequencies.device != x.device):
-            self._frequencies = fs.rotary_frequencies(self.rotary_dim, self.rotary_base, device=x.device)
-        return fs.split_heads_rotary(self._stacked(x), self.num_heads, self.num_kv_heads, self._frequencies, positions,
+        return fs.split_heads_rotary(self._stacked(x), self.num_heads, self.num_kv_heads, self._angles(x.device), positions,
                                      self.q_norm, self.k_norm)
 
     def _seen(self, seq):

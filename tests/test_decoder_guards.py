@@ -71,3 +71,28 @@ def test_a_missing_page_is_reported_until_its_place_is_released(monkeypatch):
     c.release(0)
     c.lengths[2] = 9  # past the table's row
     assert c.exhausted()
+
+
+def test_rotary_angles_serve_inference_and_training(monkeypatch):
+    """The angles that a block keeps: float64 on its device from the start, fit for training whichever mode came first,
+    and those of its present options."""
+    seen = []
+    monkeypatch.setattr(fs, "split_heads_rotary", lambda x, hq, hkv, f, *rest: seen.append(f))
+    x = torch.zeros(1, 3, 32)
+    with torch.inference_mode():
+        a = blocks.GQAttention(32, 4, 2, rotary_dim=8, rotary_base=100.0)
+        b = blocks.GQAttention(32, 4, 2, rotary_dim=8, rotary_base=100.0)
+    for m in (a.bfloat16(), blocks.GQAttention(32, 4, 2, rotary_dim=8, rotary_base=100.0)):
+        with torch.inference_mode():
+            m._heads(x.to(m.q_proj.weight.dtype))
+        want = fs.rotary_frequencies(8, 100.0, device="cpu")
+        assert not seen[-1].is_inference() and torch.equal(seen[-1], want) and seen[-1].dtype == torch.float64
+    b.rotary_base, b.rotary_dim = 50.0, 4
+    b._heads(x)
+    assert torch.equal(seen[-1], fs.rotary_frequencies(4, 50.0, device="cpu"))
+    meta = blocks.GQAttention(32, 4, 2, rotary_dim=8).to("meta")
+    assert meta._frequencies.device.type == "meta"
+    assert torch.equal(meta.to_empty(device="cpu")._frequencies, fs.rotary_frequencies(8, device="cpu"))
+    b.rotary_dim = 0
+    b._heads(x)
+    assert seen[-1] is None
