@@ -18,6 +18,7 @@ import math
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from ._native import EdificeHipError
@@ -1140,7 +1141,12 @@ class _SplitHeadsRotary(torch.autograd.Function):
 
 
 def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    """Whether a derivative of the call is asked for: backward, or forward mode (whose tensors do not require grad; the
+    autograd node refuses them)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def split_heads_rotary(x: torch.Tensor, num_heads: int, num_kv_heads: int, frequencies: torch.Tensor = None,
@@ -1255,7 +1261,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     place: token (b, t) into slot slots[b, t] (int32 [B, T], as ``paged_extend`` gives them; -1, or any other slot
     outside the cache: left out).  Slots have to differ from one another.  Inference only."""
     if _wants_grad(k, v, k_cache, v_cache):
-        raise EdificeHipError("paged_cache_write has no backward: call it under torch.no_grad()")
+        raise EdificeHipError("paged_cache_write has no derivative: call it under torch.no_grad() and without tangents")
     k, v = k.contiguous(), v.contiguous()
     _rank("k", k, 4)
     bsz, nkv, seq, d = k.shape
@@ -1283,7 +1289,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     The launch depends on shapes alone (a table as wide as the longest request may get), so a captured call may be
     replayed after the lengths and the table have changed."""
     if _wants_grad(q, k_cache, v_cache):
-        raise EdificeHipError("paged_attention has no backward: call it under torch.no_grad()")
+        raise EdificeHipError("paged_attention has no derivative: call it under torch.no_grad() and without tangents")
     q = q.contiguous()
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
         raise EdificeHipError(f"q must be [B, H, d] or [B, H, 1, d], got shape {tuple(q.shape)}")

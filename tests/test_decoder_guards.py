@@ -4,6 +4,7 @@ import itertools
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from edifice_amd import blocks
 from edifice_amd import fused_scan as fs
@@ -96,3 +97,23 @@ def test_rotary_angles_serve_inference_and_training(monkeypatch):
     b.rotary_dim = 0
     b._heads(x)
     assert seen[-1] is None
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused(host_tensors, monkeypatch, grad_mode):
+    """A tangent on any input is refused, as by the other ops, and not dropped."""
+    monkeypatch.setattr(fs.nat, "call", lambda *a: None)
+    x, w = torch.zeros(1, 3, 4 * 32), torch.ones(32)
+    q, k = torch.zeros(1, 4, 8, 64), torch.zeros(1, 2, 8, 64)
+    cache, i32 = torch.zeros(2, 2, 8, 64), torch.zeros(1, 2).int()
+    calls = [(lambda x, w: fs.split_heads_rotary(x, 2, 1, None, None, w, w), (x, w)),
+             (lambda q, k, v: fs.window_attention(q, k, v, 4), (q, k, k)),
+             (lambda q, k, v: fs.paged_attention(q, k, v, i32, i32[0, :1]), (q[:, :, 0], cache, cache)),
+             (lambda k, v, kc, vc: fs.paged_cache_write(k, v, i32[:, :1], kc, vc), (k[:, :, :1], k[:, :, :1], cache, cache))]
+    with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+        for call, args in calls:
+            call(*args)  # tensors without a tangent pass
+            for i, t in enumerate(args):
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises((NotImplementedError, EdificeHipError)):
+                    call(*args[:i], dual, *args[i + 1:])
