@@ -281,17 +281,19 @@ class PagedCache:
         self.free = torch.arange(blocks, **i32)  # free pages, -1 behind them; the first ``taken`` are in use again
         self.taken = torch.zeros(1, **i32)
         self.available = blocks
-        self._old = torch.zeros(requests, **i32)
 
     def extend(self, num_tokens: int, counts: torch.Tensor = None):
         """Room for the next counts[r] tokens of each place (int [requests], taken as 0 .. num_tokens; None: num_tokens
-        each): their (slots, positions) [requests, num_tokens], -1 past counts[r].  lengths then holds them."""
-        if counts is not None and tuple(counts.shape) != tuple(self.lengths.shape):
-            raise ValueError(f"counts must be [{self.lengths.numel()}], got {tuple(counts.shape)}")
-        self._old.copy_(self.lengths)
-        self.lengths.add_(num_tokens if counts is None else counts.clamp(0, num_tokens))
-        slots, positions, used = fs.paged_extend(self.table, self._old, self.lengths, self.free, self.block_size,
-                                                 num_tokens, self.taken)
+        each): their (slots, positions) [requests, num_tokens], -1 past counts[r].  lengths then holds them; a call
+        that raises leaves everything as it was."""
+        if num_tokens <= 0:
+            raise ValueError(f"num_tokens must be positive, got {num_tokens}")
+        if counts is not None and (tuple(counts.shape) != tuple(self.lengths.shape) or counts.is_floating_point()):
+            raise ValueError(f"counts must be integers [{self.lengths.numel()}], got {counts.dtype} {tuple(counts.shape)}")
+        new = (self.lengths + (num_tokens if counts is None else counts.clamp(0, num_tokens))).to(torch.int32)
+        slots, positions, used = fs.paged_extend(self.table, self.lengths, new, self.free, self.block_size, num_tokens,
+                                                 self.taken)
+        self.lengths.copy_(new)
         self.taken.copy_(used)
         return slots, positions
 

@@ -117,3 +117,23 @@ def test_forward_mode_is_refused(host_tensors, monkeypatch, grad_mode):
                 dual = forward_ad.make_dual(t, torch.ones_like(t))
                 with pytest.raises((NotImplementedError, EdificeHipError)):
                     call(*args[:i], dual, *args[i + 1:])
+
+
+def _state(c):
+    return [t.clone() for t in (c.table, c.lengths, c.free, c.taken)]
+
+
+def _unmoved(c, before):
+    return all(torch.equal(a, b) for a, b in zip(_state(c), before))
+
+
+def test_an_extension_that_raises_moves_nothing():
+    """Refused arguments, and an op that raises (it takes no CPU tensors): lengths and pages stay."""
+    c = blocks.PagedCache(1, 2, 8, 1, 32, block_size=4, device="cpu")
+    c.lengths[0] = 3
+    before = _state(c)
+    for tokens, counts in ((0, None), (-1, None), (-2, torch.ones(2)), (1, torch.ones(3).int()), (1, torch.ones(2)),
+                           (1, torch.ones(2, dtype=torch.int32))):
+        with pytest.raises((ValueError, EdificeHipError)):
+            c.extend(tokens, counts)
+        assert _unmoved(c, before), (tokens, counts)
