@@ -482,7 +482,7 @@ class SequenceModel(nn.Module):
         if x.shape[0] != cache.lengths.numel() or len(cache.k) != len(blocks):
             raise ValueError(f"x of {x.shape[0]} texts and {len(blocks)} layers, a cache of {cache.lengths.numel()} places "
                              f"and {len(cache.k)} layers")
-        if x.shape[1] > 1 and bool((cache.lengths * (1 if counts is None else counts)).any()):
+        if x.shape[1] > 1 and bool(((cache.lengths > 0) & (True if counts is None else counts > 0)).any()):
             raise ValueError("several tokens at once go into empty places only")
         slots, positions = cache.extend(x.shape[1], counts)
         if x.shape[1] > 1 and counts is not None:  # whatever the padding holds, its keys and values are finite

@@ -137,3 +137,19 @@ def test_an_extension_that_raises_moves_nothing():
         with pytest.raises((ValueError, EdificeHipError)):
             c.extend(tokens, counts)
         assert _unmoved(c, before), (tokens, counts)
+
+
+def _gqa(num_heads=4, **opts):
+    return blocks.build("gqa", embed_size=32, num_heads=num_heads, num_kv_heads=2, window=4, **opts)
+
+
+def test_a_prompt_into_a_long_place_is_refused(monkeypatch):
+    """A place of 2^16 tokens and a prompt of as many: their product is zero in 32 bits."""
+    monkeypatch.setattr(fs, "paged_extend", _listed)
+    m = _gqa()
+    c = m.paged_cache(2, 8)
+    c.lengths[1] = 1 << 16
+    for counts in (None, torch.tensor([0, 1 << 16], dtype=torch.int32)):
+        with pytest.raises(ValueError, match="empty places"):
+            m.step(torch.zeros(2, 2, 32), c, counts)
+    assert c.lengths.tolist() == [0, 1 << 16]
