@@ -477,11 +477,26 @@ class SequenceModel(nn.Module):
         prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
         time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text; a token that found no page
         (``PagedCache.exhausted``) is not seen by those after it.  A step of one token does not wait for the GPU and
-        may be captured; one of several checks that their places are empty."""
+        may be captured; one of several checks that their places are empty.  What does not fit the model or the cache is
+        refused before anything moves."""
         blocks = getattr(self, self._blocks_name)
+        if not all(isinstance(b, GQABlock) for b in blocks):
+            raise ValueError("only models of attention blocks take a paged cache")
+        attn = blocks[0].attn
+        w, hd = attn.k_proj.weight, attn.k_proj.weight.shape[0] // attn.num_kv_heads
+        embed = (self.input_projection if hasattr(self, "input_projection") else attn.q_proj).weight.shape[1]
+        if x.dim() != 3 or x.shape[1] == 0 or x.shape[2] != embed or x.dtype != w.dtype or x.device != w.device:
+            raise ValueError(f"x must be [requests, T, {embed}] {w.dtype} on {w.device} with T > 0, got {tuple(x.shape)} "
+                             f"{x.dtype} on {x.device}")
         if x.shape[0] != cache.lengths.numel() or len(cache.k) != len(blocks):
             raise ValueError(f"x of {x.shape[0]} texts and {len(blocks)} layers, a cache of {cache.lengths.numel()} places "
                              f"and {len(cache.k)} layers")
+        k = cache.k[0]
+        if (k.shape[1], k.shape[3]) != (attn.num_kv_heads, hd) or k.dtype != w.dtype or k.device != w.device:
+            raise ValueError(f"the cache holds {k.shape[1]} heads of {k.shape[3]} ({k.dtype} on {k.device}), the model has "
+                             f"{attn.num_kv_heads} of {hd} ({w.dtype} on {w.device})")
+        if x.shape[1] > 1 and hd > 128:
+            raise ValueError(f"several tokens at once need head_dim <= 128, got {hd}")
         if x.shape[1] > 1 and bool(((cache.lengths > 0) & (True if counts is None else counts > 0)).any()):
             raise ValueError("several tokens at once go into empty places only")
         slots, positions = cache.extend(x.shape[1], counts)

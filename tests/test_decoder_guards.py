@@ -143,6 +143,36 @@ def _gqa(num_heads=4, **opts):
     return blocks.build("gqa", embed_size=32, num_heads=num_heads, num_kv_heads=2, window=4, **opts)
 
 
+_MAMBA = lambda: blocks.build("mamba", embed_size=32)  # noqa: E731
+_WIDE = lambda: blocks.build("gqa", embed_size=32, hidden_size=320, num_heads=2)  # noqa: E731
+
+
+@pytest.mark.parametrize("model, owner, x, cache", [
+    (_gqa, None, torch.zeros(2, 1, 31), {}),
+    (_gqa, None, torch.zeros(2, 0, 32), {}),
+    (_gqa, None, torch.zeros(2, 32), {}),
+    (_gqa, None, torch.zeros(3, 1, 32), {}),
+    (_gqa, None, torch.zeros(2, 1, 32, dtype=torch.bfloat16), {}),
+    (_gqa, None, torch.zeros(2, 1, 32, device="meta"), {}),
+    (_gqa, None, torch.zeros(2, 1, 32), dict(dtype=torch.bfloat16)),
+    (_gqa, lambda: _gqa(num_layers=1), torch.zeros(2, 1, 32), {}),
+    (_gqa, lambda: _gqa(num_heads=2), torch.zeros(2, 1, 32), {}),
+    (_MAMBA, _gqa, torch.zeros(2, 1, 32), {}),
+    (_WIDE, None, torch.zeros(2, 2, 32), {}),
+], ids=["embed", "no tokens", "rank", "texts", "type", "device", "cache type", "layers", "head_dim", "family",
+        "a prompt of wide heads"])
+def test_a_step_that_does_not_fit_moves_nothing(monkeypatch, model, owner, x, cache):
+    """A model, an input or a cache (here of the model ``owner``) that do not belong together: refused before the cache
+    makes room."""
+    monkeypatch.setattr(fs, "paged_extend", _listed)
+    m = model()
+    c = (owner() if owner else m).paged_cache(2, 8, **cache)
+    before = _state(c)
+    with pytest.raises(ValueError):
+        m.step(x, c)
+    assert _unmoved(c, before)
+
+
 def test_a_prompt_into_a_long_place_is_refused(monkeypatch):
     """A place of 2^16 tokens and a prompt of as many: their product is zero in 32 bits."""
     monkeypatch.setattr(fs, "paged_extend", _listed)
