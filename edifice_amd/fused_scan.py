@@ -1185,7 +1185,10 @@ class _WindowAttention(torch.autograd.Function):
         keep = ctx is not None  # None: no gradient is asked for
         lse = torch.empty((bsz, nh, seq), dtype=torch.float32, device=q.device) if keep else None
         conf = (bsz, nh, nkv, seq, hd, min(window, seq), min(sinks, seq), dtype_flag(q))  # more sees no more keys
-        nat.call("edf_window_attention", stream, _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
+        if q.numel():
+            nat.call("edf_window_attention", stream, _p(q), _p(k), _p(v), _p(out), _p(lse), *conf)
+        elif window <= 0 or sinks < 0:
+            raise EdificeHipError("window must be positive and sinks not negative")
         if keep:
             ctx.conf = conf
             ctx.save_for_backward(q, k, v, out, lse)
@@ -1194,6 +1197,8 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
+        if not q.numel():
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None
         dout = dout.contiguous().to(q.dtype)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         wsb = nat.query("edf_window_attention_backward_workspace_bytes", *ctx.conf)
@@ -1247,6 +1252,11 @@ def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: to
     if taken is not None:
         taken = _i32("taken", taken, (1,))
     stream = _here(table, old_lengths, new_lengths, free_blocks, taken)
+    if not reqs:
+        if num_tokens <= 0 or block_size <= 0:
+            raise EdificeHipError("block_size and num_tokens must be positive")
+        slots = table.new_empty((0, num_tokens))
+        return slots, torch.empty_like(slots), table.new_zeros((1,)) if taken is None else taken.clamp(min=0)
     slots = table.new_empty((reqs, num_tokens))
     positions = torch.empty_like(slots)
     used = table.new_empty((1,))
@@ -1301,6 +1311,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lengths = _i32("lengths", lengths, (bsz,))
     stream = _here(q, k_cache, v_cache, table, lengths)
     out = torch.empty_like(q)
+    if not q.numel():
+        if window < 0 or sinks < 0:
+            raise EdificeHipError("window and sinks must not be negative")
+        return out
     window, sinks = (min(int(x), width * block) for x in (window, sinks))  # more sees no more keys
     wsb = nat.query("edf_paged_attention_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
     ws = _u8(wsb, q) if wsb else None

@@ -183,3 +183,32 @@ def test_a_prompt_into_a_long_place_is_refused(monkeypatch):
         with pytest.raises(ValueError, match="empty places"):
             m.step(torch.zeros(2, 2, 32), c, counts)
     assert c.lengths.tolist() == [0, 1 << 16]
+
+
+def _uncalled(*a):
+    raise AssertionError("an entry point was called")
+
+
+def test_nothing_to_do(host_tensors, monkeypatch):
+    """Batches of no texts and texts of no tokens answer with empty results, as the head split and the write do; other
+    refusals stay."""
+    monkeypatch.setattr(fs.nat, "call", _uncalled)
+    z = lambda *s: torch.zeros(*s, requires_grad=True)  # noqa: E731
+    for B, T in ((0, 5), (2, 0)):
+        q, k, v = z(B, 4, T, 64), z(B, 2, T, 64), z(B, 2, T, 64)
+        out = fs.window_attention(q, k, v, 3, 1)
+        assert out.shape == q.shape
+        assert [g.shape for g in torch.autograd.grad(out.sum(), (q, k, v))] == [t.shape for t in (q, k, v)]
+        for window, sinks in ((0, 0), (2, -1)):
+            with pytest.raises(EdificeHipError):
+                fs.window_attention(q, k, v, window, sinks)
+    cache, i32 = torch.zeros(2, 2, 8, 64), lambda *s: torch.zeros(*s, dtype=torch.int32)
+    for shape in ((0, 4, 64), (0, 4, 1, 64)):
+        assert fs.paged_attention(torch.zeros(shape), cache, cache, i32(0, 2), i32(0)).shape == shape
+    with pytest.raises(EdificeHipError):
+        fs.paged_attention(torch.zeros(0, 4, 64), cache, cache, i32(0, 2), i32(0), window=-1)
+    for taken, used in ((None, 0), (torch.tensor([3], dtype=torch.int32), 3), (torch.tensor([-1], dtype=torch.int32), 0)):
+        slots, positions, got = fs.paged_extend(i32(0, 2), i32(0), i32(0), i32(3), 8, 5, taken)
+        assert slots.shape == positions.shape == (0, 5) and got.tolist() == [used] and got is not taken
+    with pytest.raises(EdificeHipError):
+        fs.paged_extend(i32(0, 2), i32(0), i32(0), i32(3), 8, 0)
