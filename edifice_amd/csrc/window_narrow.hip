@@ -168,25 +168,23 @@ __global__ __launch_bounds__(256, (waves_per_simd<T, HD>(3, 1))) void narrow_fwd
       m = mnew;
     }
     const float mns = m == -INFINITY ? 0.0f : m * a.scale_log2;
-    float rs = 0.0f;
+    float rs = 0.0f;  // of P as the product has it: the weights of a row add to one
+    WFrag<T> pf[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      s[r] = fast_exp2(fmaf(s[r], a.scale_log2, -mns));
-      rs += s[r];
-    }
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        rs = pf[kc].set2(e, fast_exp2(fmaf(s[8 * kc + e], a.scale_log2, -mns)),
+                         fast_exp2(fmaf(s[8 * kc + e + 1], a.scale_log2, -mns)), rs);
     lsum += rs + __shfl_xor(rs, 32);
     if constexpr (LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int kc = 0; kc < 2; ++kc) {
-      WFrag<T> pf;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pf.set(e, s[8 * kc + e]);
+    for (int kc = 0; kc < 2; ++kc)
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
-        if constexpr (LDS) o[dt] = WFrag<T>::mma(N::trans(V, sv, k0, T_, d, kc, dt, l), pf, o[dt]);
-        else o[dt] = WFrag<T>::mma(vt[kc * NDT + dt], pf, o[dt]);
+        if constexpr (LDS) o[dt] = WFrag<T>::mma(N::trans(V, sv, k0, T_, d, kc, dt, l), pf[kc], o[dt]);
+        else o[dt] = WFrag<T>::mma(vt[kc * NDT + dt], pf[kc], o[dt]);
       }
-    }
     if constexpr (LDS) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
   // the waves' maxima, then their sums and outputs in units of the common one

@@ -113,3 +113,18 @@ def test_scores_that_move_the_maximum(case, course):
     at = torch.linspace(0, 1, case[3], dtype=torch.float64)[:, None]
     size = {"growing": 1 + 11 * at, "falling": 12 - 11 * at, "a step": 3.0 + 0.6 * (at > 0.5)}[course]
     _compare(case, q, (k.double() * size).to(k.dtype), v, do)
+
+
+@pytest.mark.parametrize("B, Hq, d", [(1, 2, 64), (1, 2, 128), (20, 8, 64), (20, 8, 96), (20, 8, 128)])
+def test_the_weights_of_a_row_add_to_one(B, Hq, d):
+    """Values of one: the sum that divides is that of the probabilities as the product has them, in the kernels of
+    small and of large calls alike.  All but the first key's scores give 0.50176, which bf16 rounds to 0.5: divided by
+    the unrounded sum, a row of 32 keys would answer 0.9967, which rounds to 0.99609."""
+    from edifice_amd import fused_scan as fs
+    announce("window_weights", B=B, d=d)
+    T, score = 32, -0.689637 * d ** 0.5 / 8  # log of 0.50176
+    q, k = (torch.zeros(B, Hq, T, d, dtype=bf16, device="cuda") for _ in range(2))
+    q[..., :2] = 8.0
+    k[..., 1:, 0] = score
+    k[..., 1:, 1] = score - float(k[0, 0, 1, 0])
+    assert torch.equal(fs.window_attention(q, k, torch.ones_like(q), T), torch.ones_like(q))
