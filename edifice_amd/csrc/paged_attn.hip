@@ -3,7 +3,7 @@
 //   o[b, h] = sum_j softmax_j(q[b, h] . k_j / sqrt(d)) v_j,   key head h / G, G = Hq / Hkv query heads each,
 // over the keys j < len_b (window W > 0: j >= len_b - W or j < sinks), key j in page table[b][j / block].
 // Each key and value is read once for its G query heads: 2 Hkv len d elements a request, 4 G flops per
-// element pair, so the kernel is bound by memory up to about G = 60 in bf16.
+// element pair (6 G done in bf16), so the kernel is bound by memory up to about G = 40 in bf16.
 //
 // The visible keys are numbered through (sinks, then the window) and cut into chunks; a workgroup of four
 // waves takes one chunk of one key head, each wave tiles of 32 keys (16 where rows are longer than 256 bytes) with an
@@ -19,8 +19,9 @@
 // float32 and a second kernel joins the chunks.
 // float32 runs the same way on the float32 matrix instructions (eight 16x16x4 per 32 elements).
 //
-// Scores, softmax and O are float32; in bf16 P is rounded to bf16 for the matrix product (2^-8 of each
-// term, as the attention of the prompt does), its sum is that of the unrounded values.
+// Scores, softmax and O are float32; in bf16 P goes through the matrix product in two bf16 parts, off by 2^-16 of itself,
+// so the result's own rounding is the only one that shows.  One part, 2^-8 off: 64x32(8)x128 ragged to 4096 123.3 us, with
+// two 124.1; 3x16(2)x128 to 131000 37.6 and 38.2; 64x64(8)x64 to 4096, whose rows are shortest, 59.5 and 62.0.
 // Keys of a page outside [0, num_blocks) are left out, and a request without keys answers with zeros.
 #include <math.h>
 #include <stdint.h>
@@ -137,18 +138,25 @@ struct KVTile {
     if constexpr (sizeof(T) == 2) {
       const int row = 4 * g + (i >> 2), col = 16 * dt + 4 * (i & 3);
       if constexpr (NT == 2) {
-        Frag<T> v, pf;
+        Frag<T> v, hi, lo;
         v.v = cat4(lds_read_tr16(t + off(row, col)), lds_read_tr16(t + off(row + 16, col)));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) pf.set(e, p[e]);
-        return Frag<T>::mma(v, pf, o);
+        for (int e = 0; e < 8; ++e) {
+          hi.set(e, p[e]);
+          lo.set(e, p[e] - (float)hi.v[e]);
+        }
+        return Frag<T>::mma(v, hi, Frag<T>::mma(v, lo, o));
       } else {
         typedef __attribute__((ext_vector_type(4))) short s16x4;
-        bf16x4 pf;
+        const s16x4 v = __builtin_bit_cast(s16x4, lds_read_tr16(t + off(row, col)));
+        bf16x4 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) pf[e] = (bf16)p[e];
-        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, lds_read_tr16(t + off(row, col))),
-                                                         __builtin_bit_cast(s16x4, pf), o, 0, 0, 0);
+        for (int e = 0; e < 4; ++e) {
+          hi[e] = (bf16)p[e];
+          lo[e] = (bf16)(p[e] - (float)hi[e]);
+        }
+        o = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, __builtin_bit_cast(s16x4, lo), o, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v, __builtin_bit_cast(s16x4, hi), o, 0, 0, 0);
       }
     } else {
 #pragma unroll
