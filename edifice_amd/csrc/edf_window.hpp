@@ -271,7 +271,7 @@ struct KeyTiles {
 template <int KB>
 __host__ __device__ inline int query_tiles(int k0, int BQ, int T, int W, int S, bool far) {
   const int end = T - k0;
-  return ((k0 < S && !far || end < KB - 1 + W ? end : KB - 1 + W) + BQ - 1) / BQ;
+  return (((k0 < S && !far) || end < KB - 1 + W ? end : KB - 1 + W) + BQ - 1) / BQ;
 }
 
 // The key block of workgroup xb of a dK, dV kernel and its share [t0, t1) of the block's (query head, tile) pairs,

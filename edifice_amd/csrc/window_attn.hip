@@ -11,7 +11,8 @@
 // (one loop with the mask), the others after it (one loop without): the order of an online softmax is free.
 //
 // Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and its sum is
-// that of the rounded values.  float32 runs on the float32 matrix instructions.
+// that of the rounded values, here and in the narrow kernels, so the weights of a row add to one; the row sums that the
+// backward takes are the same (window_attn_bwd.hip has what that adds).  float32 runs on the float32 matrix instructions.
 #include <math.h>
 #include <stdint.h>
 

@@ -11,10 +11,13 @@
 //   with few keys and heads there are fewer workgroups than the GPU holds: such a block's tiles are then
 //   divided over several workgroups, each leaving float32 sums, added in order by a third kernel.  Where that
 //   is less, the queries past the windows meet the sinks in a kernel of their own (window_narrow.hip).
-// P and dS are rounded to bf16 as operands of the second products (2^-8 of each term), and D is formed from the rounded
-// O that the forward left; everything else is float32.  On random inputs (300 rows, window 100) the 2-norm of dQ is
-// 1.65e-3 off by its own rounding, as much by that of dS, and 0.8e-3 by D: 2.5e-3 together.  dS in two bf16 parts would
-// be two of the seven products again, D from an unrounded O a float32 O to keep until the backward.
+// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term), D is formed from the rounded O
+// that the forward left, and P from the forward's sum of rounded probabilities: a row's P is off as a whole by the mean
+// of their roundings, at most 2^-8 of itself, where one probability far above the others is not at the maximum that the
+// sums refer to.  Everything else is float32.  On random inputs (300 rows, window 100) the 2-norm of dQ is 1.65e-3 off by
+// its own rounding, as much by that of dS, 0.8e-3 by D and 0.3e-3 by the row sums: 2.5e-3 together.  dS in two bf16
+// parts would be two of the seven products again, D from an unrounded O a float32 O to keep until the backward, a second
+// sum of the unrounded P 32 additions a tile in the forward, whose vector instructions bound it.
 #include <math.h>
 #include <stdint.h>
 
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(256, 2) void window_dq128_kernel(WindowArgs a) {
     }
 }
 
-// bf16 widths to 96 keep to 256 registers, two workgroups a CU (at 96 with 30 of them spilled, and one load step less
+// bf16 widths to 96 keep to 256 registers, two workgroups a CU (at 96 with 24 of them spilled, and one load step less
 // ahead: 4x16(4)x1500x80 window 400 backward 157 -> 144 us).
 template <typename T, int HD, int BQ, bool VEC>
 __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) void window_dkdv_kernel(WindowArgs a) {

@@ -668,7 +668,8 @@ int edf_heads_split_rotary_backward(void* stream, const void* x, const double* f
  *   q, out [batch, num_heads, seq_len, d], k, v [batch, num_kv_heads, seq_len, d]; query head h reads key head
  *   h / (num_heads / num_kv_heads); query i sees key j when j <= i and (i - j < window or j < sinks);
  *   scores / sqrt(d).
- * lse (may be NULL): float32 [batch, num_heads, seq_len] natural-log row sums, required by the backward.
+ * lse (may be NULL): float32 [batch, num_heads, seq_len] natural-log row sums (in bf16 of the probabilities as the
+ * product has them, rounded), required by the backward.
  * head_dim <= 128, sinks <= 2^22.  Keys and values have to be finite: a value that is not may also reach queries that
  * do not see its key, where another key of its 64-key tile is seen.
  * The backward's workspace: edf_window_attention_backward_workspace_bytes().
@@ -699,8 +700,9 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  * edf_paged_attention: one query per request, q, out [batch, num_heads, d], over the request's first lengths[b]
  *   tokens (clamped to [0, table_width * block_size]), of which, with window > 0, the last `window` and the first
  *   `sinks` are seen.  Pages outside [0, num_blocks) hold no keys; a request that sees none answers with zeros.
- *   head_dim <= 256.  The grid and the workspace (edf_paged_attention_workspace_bytes()) depend on the shapes
- *   alone, not on lengths, so a captured call may be replayed after lengths and table have changed.
+ *   head_dim <= 256.  The grid and the workspace (edf_paged_attention_workspace_bytes(), 0 for sizes that the call
+ *   refuses) depend on the shapes alone, not on lengths, so a captured call may be replayed after lengths and table
+ *   have changed.
  * ------------------------------------------------------------------------ */
 int edf_paged_extend(void* stream, int32_t* table, const int32_t* old_lengths, const int32_t* new_lengths,
                      const int32_t* free_blocks, const int32_t* taken, int32_t* slots, int32_t* positions,
