@@ -79,6 +79,10 @@ SIGNATURES = {
     "edf_paged_cache_write": (I, [P, P, P, P, P, P, L, L, I, I, L, I, I]),
     "edf_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
     "edf_paged_attention": (I, [P, P, P, P, P, P, P, P, S, I, I, I, I, L, I, I, I, I, I]),
+    "edf_paged_cache_write8": (I, [P, P, P, P, P, P, P, P, L, L, I, I, L, I, I, I]),
+    "edf_paged_attention8_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),
+    "edf_paged_attention8": (I, [P, P, P, P, P, P, P, P, P, P, S, I, I, I, I, L, I, I, I, I, I, I]),
+    "edf_paged_cache_read": (I, [P, P, P, P, P, P, P, P, P, I, L, I, I, L, I, I, I, I]),
     "edf_embedding_backward_workspace_bytes": (S, [L, L]),
     "edf_embedding_backward": (I, [P, P, P, P, P, S, L, L, I, L, I]),
     "edf_softplus": (I, [P, P, P, L, I]),

@@ -1,0 +1,39 @@
+// 8-bit numbers of a paged cache: whole numbers -127 .. 127 (EDF_INT8) or e4m3 floats (EDF_E4M3), in units of a
+// float32 scale that the tokens of one page and key head share.
+#pragma once
+
+#include "edf_abi.hpp"
+#include "edf_common.hpp"
+#include "edf_mfma.hpp"
+
+namespace edf {
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
+
+// C: the code's kind.  unpack4: four codes as float32, exactly; pack4: four values to codes, ties to even, saturated.
+template <int C> struct Codes;
+template <> struct Codes<EDF_INT8> {
+  EDF_DEVICE static void unpack4(unsigned c, float* x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (float)(signed char)(c >> (8 * e));
+  }
+  EDF_DEVICE static unsigned pack4(const float* x) {
+    unsigned c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c |= ((unsigned)(int)clampf(rintf(x[e]), -127.0f, 127.0f) & 255u) << (8 * e);
+    return c;
+  }
+};
+template <> struct Codes<EDF_E4M3> {
+  EDF_DEVICE static void unpack4(unsigned c, float* x) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+    x[0] = lo[0], x[1] = lo[1], x[2] = hi[0], x[3] = hi[1];
+  }
+  EDF_DEVICE static unsigned pack4(const float* x) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+  }
+};
+
+}  // namespace edf

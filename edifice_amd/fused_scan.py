@@ -1220,16 +1220,33 @@ def window_attention(q, k, v, window: int, sinks: int = 0):
     return _WindowAttention.forward(None, *args)
 
 
-def _cache_dims(k_cache, v_cache, d, like):
+_CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_NO_CODE = -1
+
+
+def _cache_dims(k_cache, v_cache, d, like, k_scale=None, v_scale=None):
+    """(num_blocks, Hkv, block_size, code) of a cache for tensors of ``like``'s type and d elements a head: code -1 for a
+    cache of that type, else the kind of its 8-bit numbers."""
     _rank("k_cache", k_cache, 4)
     blocks, nkv, block, hd = k_cache.shape
     if v_cache.shape != k_cache.shape or hd != d:
         raise EdificeHipError(f"k_cache and v_cache must be [num_blocks, Hkv, block_size, {d}], got "
                               f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
-    _same(like, k_cache, v_cache)
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise EdificeHipError("edifice_amd ops need contiguous tensors")
-    return blocks, nkv, block
+    if k_cache.dtype not in _CODES:
+        if k_scale is not None or v_scale is not None:
+            raise EdificeHipError(f"scales belong to a cache of int8 or float8_e4m3fn, got {k_cache.dtype}")
+        if like is not None:
+            _same(like, k_cache)
+        _same(k_cache, v_cache)
+        return blocks, nkv, block, _NO_CODE
+    if v_cache.dtype != k_cache.dtype:
+        raise EdificeHipError(f"dtype mismatch: {v_cache.dtype} vs {k_cache.dtype}")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None or t.dtype != torch.float32 or t.shape != (blocks, nkv) or not t.is_contiguous():
+            raise EdificeHipError(f"a cache of {k_cache.dtype} needs {name}, contiguous float32 {(blocks, nkv)}")
+    return blocks, nkv, block, _CODES[k_cache.dtype]
 
 
 def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: torch.Tensor, free_blocks: torch.Tensor,
@@ -1266,11 +1283,18 @@ def paged_extend(table: torch.Tensor, old_lengths: torch.Tensor, new_lengths: to
 
 
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
-                      v_cache: torch.Tensor) -> None:
+                      v_cache: torch.Tensor, k_scale: torch.Tensor = None, v_scale: torch.Tensor = None) -> None:
     """Keys and values k, v [B, Hkv, T, d] into the pages k_cache, v_cache [num_blocks, Hkv, block_size, d], in
     place: token (b, t) into slot slots[b, t] (int32 [B, T], as ``paged_extend`` gives them; -1, or any other slot
-    outside the cache: left out).  Slots have to differ from one another.  Inference only."""
-    if _wants_grad(k, v, k_cache, v_cache):
+    outside the cache: left out).  Slots have to differ from one another.  Inference only.
+
+    The cache is of k's type, or of int8 or float8_e4m3fn with k_scale, v_scale float32 [num_blocks, Hkv]: an 8-bit number
+    stands for that many units of its page and head's scale.  The tokens of a page then share a scale that holds their
+    largest value (int8: a 127th of it; e4m3: a power of two); a page whose first slot is written starts anew, any other
+    keeps its scale, or doubles it until it holds the new tokens, its numbers halved and rounded.  The slots of one page
+    have to be those of consecutive tokens of one row, in ascending order.  A value that is not finite makes its page's head
+    NaN until that page starts anew.  Scales and numbers of pages that hold nothing may be anything finite (zeros)."""
+    if _wants_grad(k, v, k_cache, v_cache, k_scale, v_scale):
         raise EdificeHipError("paged_cache_write has no derivative: call it under torch.no_grad() and without tangents")
     k, v = k.contiguous(), v.contiguous()
     _rank("k", k, 4)
@@ -1278,48 +1302,93 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     if v.shape != k.shape:
         raise EdificeHipError(f"v must have shape {tuple(k.shape)}, got {tuple(v.shape)}")
     _same(k, v)
-    blocks, heads, block = _cache_dims(k_cache, v_cache, d, k)
+    blocks, heads, block, code = _cache_dims(k_cache, v_cache, d, k, k_scale, v_scale)
     if heads != nkv:
         raise EdificeHipError(f"k has {nkv} heads, the cache {heads}")
     slots = _i32("slots", slots, (bsz, seq))
-    stream = _here(k, v, slots, k_cache, v_cache)
-    if k.numel():
+    stream = _here(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+    if not k.numel():
+        return
+    if code == _NO_CODE:
         nat.call("edf_paged_cache_write", stream, _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), bsz, seq, nkv, d,
                  blocks, block, dtype_flag(k))
+    else:
+        nat.call("edf_paged_cache_write8", stream, _p(k), _p(v), _p(slots), _p(k_cache), _p(v_cache), _p(k_scale),
+                 _p(v_scale), bsz, seq, nkv, d, blocks, block, dtype_flag(k), code)
+
+
+def paged_cache_read(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, offsets: torch.Tensor, total: int,
+                     k_scale: torch.Tensor = None, v_scale: torch.Tensor = None, *, dtype: torch.dtype = None):
+    """Keys and values of a paged cache as texts laid end to end: k, v [Hkv, total, d], the first offsets[b + 1] -
+    offsets[b] tokens of request b as rows offsets[b] .. (offsets int32 [B + 1] on the GPU, ascending; table int32
+    [B, width]), as ``packed_attention`` takes them.  Rows outside the texts, and tokens of pages outside the cache, are
+    zeros.  A cache of int8 or float8_e4m3fn (``paged_cache_write``) takes its scales, and dtype says whether the result is
+    float32 or bfloat16 (the default); any other is copied as it is.  Inference only."""
+    if _wants_grad(k_cache, v_cache, k_scale, v_scale):
+        raise EdificeHipError("paged_cache_read has no derivative: call it under torch.no_grad() and without tangents")
+    _rank("k_cache", k_cache, 4)
+    d = k_cache.shape[3]
+    blocks, nkv, block, code = _cache_dims(k_cache, v_cache, d, None, k_scale, v_scale)
+    own = torch.bfloat16 if code != _NO_CODE else k_cache.dtype
+    dtype = own if dtype is None else dtype
+    if code == _NO_CODE and dtype != own:
+        raise EdificeHipError(f"a cache of {own} is read as it is, not as {dtype}")
+    _rank("table", table, 2)
+    reqs, width = table.shape
+    table = _i32("table", table, (reqs, width))
+    offsets = _i32("offsets", offsets, (reqs + 1,))
+    stream = _here(k_cache, v_cache, table, offsets, k_scale, v_scale)
+    if total < 0:
+        raise EdificeHipError(f"total must not be negative, got {total}")
+    k = torch.empty((nkv, total, d), dtype=dtype, device=k_cache.device)
+    flag = dtype_flag(k)
+    if not k.numel() or not reqs or not width or not blocks:  # no text, or none that has a page
+        return k.zero_(), torch.zeros_like(k)
+    v = torch.empty_like(k)
+    nat.call("edf_paged_cache_read", stream, _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), _p(table), _p(offsets),
+             _p(k), _p(v), reqs, total, nkv, d, blocks, block, width, flag, code)
+    return k, v
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
-                    lengths: torch.Tensor, *, window: int = 0, sinks: int = 0) -> torch.Tensor:
+                    lengths: torch.Tensor, *, window: int = 0, sinks: int = 0, k_scale: torch.Tensor = None,
+                    v_scale: torch.Tensor = None) -> torch.Tensor:
     """Attention of one new token per request over a paged cache: q [B, H, d] (or [B, H, 1, d]), k_cache, v_cache
     [num_blocks, Hkv, block_size, d], table int32 [B, width] (the request's pages in order), lengths int32 [B]
     (tokens in the cache, the new one among them).  window > 0: only the last ``window`` and the first ``sinks``
     tokens are seen.  Returns q's shape; a request of length 0 answers with zeros, and pages outside the cache hold
     no keys.  float32 or bfloat16, head_dim <= 256, scale 1/sqrt(d), H a multiple of Hkv.  Inference only.
+    The cache is of q's type, or of int8 or float8_e4m3fn with k_scale, v_scale (``paged_cache_write``).
 
     The launch depends on shapes alone (a table as wide as the longest request may get), so a captured call may be
     replayed after the lengths and the table have changed."""
-    if _wants_grad(q, k_cache, v_cache):
+    if _wants_grad(q, k_cache, v_cache, k_scale, v_scale):
         raise EdificeHipError("paged_attention has no derivative: call it under torch.no_grad() and without tangents")
     q = q.contiguous()
     if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
         raise EdificeHipError(f"q must be [B, H, d] or [B, H, 1, d], got shape {tuple(q.shape)}")
     bsz, nh, d = q.shape[0], q.shape[1], q.shape[-1]
-    blocks, nkv, block = _cache_dims(k_cache, v_cache, d, q)
+    blocks, nkv, block, code = _cache_dims(k_cache, v_cache, d, q, k_scale, v_scale)
     _rank("table", table, 2)
     width = table.shape[1]
     table = _i32("table", table, (bsz, width))
     lengths = _i32("lengths", lengths, (bsz,))
-    stream = _here(q, k_cache, v_cache, table, lengths)
+    stream = _here(q, k_cache, v_cache, table, lengths, k_scale, v_scale)
     out = torch.empty_like(q)
     if not q.numel():
         if window < 0 or sinks < 0:
             raise EdificeHipError("window and sinks must not be negative")
         return out
     window, sinks = (min(int(x), width * block) for x in (window, sinks))  # more sees no more keys
-    wsb = nat.query("edf_paged_attention_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
+    eight = "" if code == _NO_CODE else "8"
+    wsb = nat.query(f"edf_paged_attention{eight}_workspace_bytes", bsz, nh, nkv, d, width, block, window, sinks)
     ws = _u8(wsb, q) if wsb else None
-    nat.call("edf_paged_attention", stream, _p(q), _p(k_cache), _p(v_cache), _p(table), _p(lengths), _p(out), _p(ws),
-             wsb, bsz, nh, nkv, d, blocks, block, width, window, sinks, dtype_flag(q))
+    conf = (_p(table), _p(lengths), _p(out), _p(ws), wsb, bsz, nh, nkv, d, blocks, block, width, window, sinks,
+            dtype_flag(q))
+    if code == _NO_CODE:
+        nat.call("edf_paged_attention", stream, _p(q), _p(k_cache), _p(v_cache), *conf)
+    else:
+        nat.call("edf_paged_attention8", stream, _p(q), _p(k_cache), _p(v_cache), _p(k_scale), _p(v_scale), *conf, code)
     return out
 
 

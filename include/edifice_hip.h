@@ -49,6 +49,8 @@ enum {
 };
 
 enum { EDF_F32 = 0, EDF_BF16 = 1 };
+/* numbers of an 8-bit cache: whole ones, -127 .. 127, or e4m3 floats; EDF_NO_CODE: a cache of dtype */
+enum { EDF_NO_CODE = -1, EDF_INT8 = 0, EDF_E4M3 = 1 };
 
 /* selective-scan discretisation of B: per-channel dt (kernel semantics,
  * native/cuda/fused_selective_scan.cu:68-90) or mean over channels
@@ -716,6 +718,38 @@ int edf_paged_attention(void* stream, const void* q, const void* k_cache, const 
                         const int32_t* lengths, void* out, void* workspace, size_t workspace_bytes, int batch,
                         int num_heads, int num_kv_heads, int head_dim, long num_blocks, int block_size,
                         int table_width, int window, int sinks, int dtype);
+
+/* The same over a cache of 8-bit numbers, code EDF_INT8 or EDF_E4M3: k_cache, v_cache hold a byte a value, in units of
+ * k_scale, v_scale, float32 [num_blocks, num_kv_heads], one for the tokens of a page and head.
+ *
+ * edf_paged_cache_write8: rows of k, v in dtype.  The slots of one page have to be those of tokens that follow one another
+ *   in one row of k, in ascending order, as edf_paged_extend gives them.  The written tokens of a page and head need
+ *   a scale n = max |x| / 127 (int8: times the float32 nearest to 1 / 127) or the least power of two from max |x| / 448 on
+ *   (e4m3), at least 2^-100, or 0 where every x is 0.  A page whose first slot is written takes s = n; any other keeps its
+ *   scale, doubled until it is n at least, and its codes, halved as often and rounded (a scale of 0 or less: s = n, codes
+ *   0).  A value is held as x (1 / s), rounded to even; slots of the page that the call does not write keep what they stand
+ *   for, or, in a page that it begins, their codes.  A value that is not finite makes the scale NaN until the page is begun
+ *   anew, and with it all that the page's head stands for.  No value is read back for a page that the call begins.
+ * edf_paged_attention8: edf_paged_attention over such a cache; q and out in dtype.  The workspace is that of
+ *   edf_paged_attention8_workspace_bytes().
+ * edf_paged_cache_read: the first offsets[b + 1] - offsets[b] tokens of each request b as rows offsets[b] .. of k, v
+ *   [num_kv_heads, total, d] in dtype, float32 or bf16 (offsets int32 [requests + 1], ascending); from a cache of dtype with
+ *   code EDF_NO_CODE (the scales are not read).  Rows outside the texts, and tokens past the table's width or of pages
+ *   outside [0, num_blocks), are zeros. */
+int edf_paged_cache_write8(void* stream, const void* k, const void* v, const int32_t* slots, void* k_cache,
+                           void* v_cache, float* k_scale, float* v_scale, long batch, long seq, int num_kv_heads,
+                           int head_dim, long num_blocks, int block_size, int dtype, int code);
+size_t edf_paged_attention8_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width,
+                                            int block_size, int window, int sinks);
+int edf_paged_attention8(void* stream, const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                         const float* v_scale, const int32_t* table, const int32_t* lengths, void* out,
+                         void* workspace, size_t workspace_bytes, int batch, int num_heads, int num_kv_heads,
+                         int head_dim, long num_blocks, int block_size, int table_width, int window, int sinks,
+                         int dtype, int code);
+int edf_paged_cache_read(void* stream, const void* k_cache, const void* v_cache, const float* k_scale,
+                         const float* v_scale, const int32_t* table, const int32_t* offsets, void* k, void* v,
+                         int requests, long total, int num_kv_heads, int head_dim, long num_blocks, int block_size,
+                         int table_width, int dtype, int code);
 
 /* ------------------------------------------------------------------------
  * Token-embedding weight gradient (block callers: the language models' input embedding,

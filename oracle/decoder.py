@@ -91,3 +91,77 @@ def paged_extend(table, old, new, free, block, tokens):
         slots.append([table[r][p // block] * block + p % block
                       if p >= 0 and p // block < width and table[r][p // block] >= 0 else -1 for p in ps])
     return table, slots, positions, at
+
+
+def round_code(y, code):
+    """y to the nearest number of 8 bits, ties to even: "int8" (-127 .. 127) or "e4m3" (three bits behind the leading one,
+    a fixed step below 2^-6; |y| <= 448)."""
+    if code == "int8":
+        return torch.round(y).clamp(-127, 127)
+    _, e = torch.frexp(y)
+    step = torch.ldexp(torch.ones_like(y), (e - 1).clamp(min=-6) - 3)
+    return torch.round(y / step) * step
+
+
+def least_scale(amax, code):
+    """The scale (a float32 number) that values up to amax (float) need."""
+    if not math.isfinite(amax):
+        return math.nan
+    if amax == 0:
+        return 0.0
+    if code == "int8":
+        r = torch.tensor(amax, dtype=torch.float32) * torch.tensor(1 / 127, dtype=torch.float32)
+        return max(float(r), 2.0 ** -100)
+    e = -100
+    while 448 * 2.0 ** e < amax:
+        e += 1
+    return 2.0 ** e
+
+
+def paged_cache_write8(x, slots, cache, scale, code):
+    """x [B, Hkv, T, d], slots (list of lists), cache [num_blocks, Hkv, block, d] (the numbers as float64) and scale
+    [num_blocks, Hkv], the last two changed in place: one page at a time, from the definition.  A value is divided by its
+    scale as the operator's definition has it, x (1 / s) with the float32 quotient, before it is rounded."""
+    blocks, hkv, block, _ = cache.shape
+    pages = {}
+    for b, row in enumerate(slots):
+        for t, s in enumerate(row):
+            if 0 <= s < blocks * block:
+                pages.setdefault(s // block, []).append((s % block, b, t))
+    for page, tokens in pages.items():
+        offs = [o for o, _, _ in tokens]
+        others = [o for o in range(block) if o not in offs]
+        for h in range(hkv):
+            amax = max(float(x[b, h, t].abs().nan_to_num(math.inf, posinf=math.inf).max()) for _, b, t in tokens)
+            need, old = least_scale(amax, code), float(scale[page, h])
+            if 0 in offs:
+                new = need
+            elif old <= 0:
+                new = need
+                cache[page, h, others] = 0.0
+            elif math.isnan(old) or math.isnan(need):
+                new = math.nan
+            else:
+                new, halvings = old, 0
+                while new < need:
+                    new, halvings = 2 * new, halvings + 1
+                if halvings:
+                    cache[page, h, others] = round_code(cache[page, h, others] / 2.0 ** halvings, code)
+            for o, b, t in tokens:
+                if new > 0:
+                    inv = 1.0 / torch.tensor(new, dtype=torch.float32)
+                    cache[page, h, o] = round_code((x[b, h, t].float() * inv).double(), code)
+                else:
+                    cache[page, h, o] = 0.0
+            scale[page, h] = new
+
+
+def paged_cache_read(values, table, offsets, total):
+    """values [num_blocks, Hkv, block, d] -> [Hkv, total, d]."""
+    blocks, hkv, block, d = values.shape
+    out = torch.zeros(hkv, total, d, dtype=values.dtype)
+    for b in range(len(offsets) - 1):
+        for i, row in enumerate(range(offsets[b], offsets[b + 1])):
+            if 0 <= row < total and i < table.shape[1] * block and 0 <= int(table[b, i // block]) < blocks:
+                out[:, row] = values[int(table[b, i // block]), :, i % block]
+    return out
