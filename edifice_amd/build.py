@@ -62,6 +62,7 @@ PER_FILE_FLAGS = {
     "delta_rule_row.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "delta_rule_row_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "window_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "packed_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

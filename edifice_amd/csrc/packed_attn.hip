@@ -1,0 +1,337 @@
+// Causal attention over texts laid end to end, forward, with shared key heads and an optional window with sinks:
+//   O_i = sum_j P_ij V_j,  P_i = softmax over visible j of Q_i . K_j / sqrt(d),
+//   visible: j <= p and (p - j < W or j < S), p = i + m - n the position of query i of n among its text's m keys;
+// q, o [H, N, d], k, v [Hkv, M, d], query head h reads key head h / (H / Hkv).  Also writes the natural-log row sums
+// (float32 [H, N], infinity for a query that sees no key) for the backward.
+//
+// Work is 4 d flops per visible pair: bound by the matrix cores.  A workgroup of four waves owns 128 queries of one text,
+// 32 per wave with Q^T in registers, and walks the key tiles that one of them sees (window_attn.hip has the arrangement of
+// a tile's products: S^T = K Q^T, so that the softmax is local to a lane and P^T the next product's operand as it stands).
+// Tiles never cross texts: the keys behind a text's end are read as zeros.
+// Where queries are few against the GPU, the key tiles are cut into chunks, a workgroup each, which leave unnormalised
+// outputs with their maxima and sums to a second kernel.
+//
+// Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and its sum is that
+// of the rounded values, so the weights of a row add to one.  float32 runs on the float32 matrix instructions.
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "edf_packed.hpp"
+
+namespace edf {
+namespace {
+
+constexpr float LN2 = 0.6931471805599453f;
+
+// What a forward workgroup works on: its queries, its text's keys and its share [t0, t1) of their tiles.
+template <int BN>
+struct QueryTile {
+  int head, qrow, nq, krow, nk, first, chunk, t0, t1;  // first: the tile's first query within the text
+  bool none;
+  EDF_DEVICE int ahead() const { return nk - nq; }
+  EDF_DEVICE QueryTile(const PackArgs& a) {
+    int x;
+    packed_block(a, a.nx * a.chunks, x, head);
+    chunk = x % a.chunks;
+    const TextTile t = find_tile(a.qo, a.S, a.N, a.nx - 1 - x / a.chunks);
+    qrow = t.row0, nq = t.n, first = t.first;
+    none = first >= nq;
+    text_rows(a.ko, a.S, a.M, t.text, krow, nk);
+    t0 = t1 = 0;
+  }
+  EDF_DEVICE KeyTiles<PK_M, BN> tiles(const PackArgs& a) {
+    const KeyTiles<PK_M, BN> kt(first + ahead(), nk, a.W, a.sinks);
+    const int count = first + ahead() + PK_M > 0 ? max(kt.count, 0) : 0;
+    t0 = min(chunk * a.len, count);
+    t1 = min(t0 + a.len, count);
+    if (chunk > 0 && t0 >= count) none = true;  // the first chunk answers for a tile without keys
+    return kt;
+  }
+};
+
+template <typename T, int HD, int BN, bool VEC>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
+  constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
+  constexpr int AHEAD = sizeof(T) == 2 ? 4 : 1;
+  using Tile = WTile<T, HD, BN>;
+  __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
+  __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  QueryTile<BN> qt(a);
+  if (qt.none) return;
+  const KeyTiles<PK_M, BN> kt = qt.tiles(a);
+  if (qt.none) return;
+  const int d = a.d, pw = qt.first + 32 * w + qt.ahead(), myp = pw + li;  // positions
+  const int myq = qt.first + 32 * w + li;                                  // query within the text
+  const long row = (long)qt.head * a.N + qt.qrow + min(myq, qt.nq - 1);
+  const T* K = (const T*)a.k + ((long)(qt.head / a.G) * a.M + qt.krow) * d;
+  const T* V = (const T*)a.v + ((long)(qt.head / a.G) * a.M + qt.krow) * d;
+
+  WFrag<T> qf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) qf[kk] = window_row<T, HD, VEC>((const T*)a.q + row * d, kk * 16 + 8 * g, d);
+  f32x16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
+  float m = -INFINITY, lsum = 0.0f;
+
+  const TileLoader<T, HD, BN, VEC> ld(tid, d, qt.nk);
+  WFrag<T> rk[ld.N], rv[ld.N];
+  const int count = qt.t1 - qt.t0;
+  auto key0 = [&](int t) { return kt.key0(qt.t0 + t); };
+  auto gload = [&](int t) {
+    ld.load(K, key0(t), rk);
+    ld.load(V, key0(t), rv);
+  };
+  auto sstore = [&](int buf) {
+    ld.template store<Tile>(sK[buf], rk);
+    ld.template store<Tile>(sV[buf], rv);
+  };
+  auto tile = [&](int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const SeesKey sees(myp, key0(t) + 4 * g, a.W, a.sinks);
+    const T *sk = sK[t & 1], *sv = sV[t & 1];
+    f32x16 s[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) s[h] = zero16();
+    // consecutive products go to different halves' scores
+    edf::ahead<NH * NKK, AHEAD>([&](int i) { return Tile::row(sk, i % NH * 32 + li, i / NH * 16 + 8 * g); },
+                           [&](int i, const WFrag<T>& f) { s[i % NH] = WFrag<T>::mma(f, qf[i / NH], s[i % NH]); });
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if constexpr (MASK) s[h][r] = sees(h * 32 + d_row(r, 0)) ? s[h][r] : -INFINITY;
+        mx = fmaxf(mx, s[h][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    // O and the sum refer to a maximum that is moved only when a score exceeds it by a factor of 2^8: p <= 256 loses
+    // nothing in float32 or bf16
+    if (__any(mx * a.scale_log2 > m * a.scale_log2 + 8.0f)) {
+      const float mnew = fmaxf(m, mx);
+      const float alpha = fast_exp2(m * a.scale_log2 - (mnew == -INFINITY ? 0.0f : mnew * a.scale_log2));
+      lsum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m = mnew;
+    }
+    const float mns = m == -INFINITY ? 0.0f : m * a.scale_log2;
+    float rs = 0.0f;
+    WFrag<T> pf[2 * NH];
+#pragma unroll
+    for (int kc = 0; kc < 2 * NH; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const int r = 8 * (kc & 1) + e;
+        rs = pf[kc].set2(e, fast_exp2(fmaf(s[kc >> 1][r], a.scale_log2, -mns)),
+                         fast_exp2(fmaf(s[kc >> 1][r + 1], a.scale_log2, -mns)), rs);
+      }
+    lsum += rs + __shfl_xor(rs, 32);
+    edf::ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sv, 16 * (i / NDT), i % NDT, l); },
+                               [&](int i, const WFrag<T>& f) { o[i % NDT] = WFrag<T>::mma(f, pf[i / NDT], o[i % NDT]); });
+  };
+  auto advance = [&](int t) {  // the next tile into the other buffer, the one after it into registers
+    if (t + 1 < count) {
+      sstore((t + 1) & 1);
+      if (t + 2 < count) gload(t + 2);
+    }
+    __syncthreads();
+  };
+  if (count > 0) {
+    gload(0);
+    sstore(0);
+    if (count > 1) gload(1);
+  }
+  __syncthreads();
+  const int masked = min(count, max(kt.first_whole - qt.t0, 0));
+  int t = 0;
+  for (; t < masked; ++t) {
+    const int k0 = key0(t);
+    if ((k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks) tile(t, std::true_type{});  // some pair is visible
+    advance(t);
+  }
+  for (; t < count; ++t) {
+    tile(t, std::false_type{});
+    advance(t);
+  }
+
+  if (myq >= qt.nq) return;
+  if (a.chunks > 1) {
+    const long at = (long)qt.chunk * a.H * a.N + row;
+    float* out = a.part + at * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
+            f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
+    if (g == 0) {
+      a.ml[2 * at] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[2 * at + 1] = lsum;
+    }
+    return;
+  }
+  const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;  // a query that sees no key answers with zeros
+  T* O = (T*)a.out + row * d;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const int c = dt * 32 + 8 * rb + 4 * g;
+      if (VEC && c + 4 <= d) {
+        typedef __attribute__((ext_vector_type(4))) T vec4;
+        vec4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(o[dt][rb * 4 + e] * inv);
+        *(vec4*)(O + c) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < d) O[c + e] = from_f32<T>(o[dt][rb * 4 + e] * inv);
+      }
+    }
+  if (g == 0 && a.lse != nullptr)
+    a.lse[row] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
+}
+
+// The chunks of 32 rows joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, a row by eight lanes of four elements
+// at a time.
+template <typename T, int HD, int BN>
+__global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
+  int x, head;
+  packed_block(a, a.nx * 4, x, head);
+  const TextTile t = find_tile(a.qo, a.S, a.N, x >> 2);
+  const int q = t.first + 32 * (x & 3) + (threadIdx.x >> 3);
+  if (q >= t.n) return;
+  int krow, nk;
+  text_rows(a.ko, a.S, a.M, t.text, krow, nk);
+  const KeyTiles<PK_M, BN> kt(t.first + nk - t.n, nk, a.W, a.sinks);
+  const int count = t.first + nk - t.n + PK_M > 0 ? max(kt.count, 0) : 0;
+  const int n = min(a.chunks, max(1, (count + a.len - 1) / a.len));
+  const long row = (long)head * a.N + t.row0 + q, stride = (long)a.H * a.N;
+  float m = -INFINITY, sum = 0.0f;
+  for (int c = 0; c < n; ++c) m = fmaxf(m, a.ml[2 * (c * stride + row)]);
+  for (int c = 0; c < n; ++c) {
+    const float mc = a.ml[2 * (c * stride + row)];
+    sum = fmaf(mc == -INFINITY ? 0.0f : fast_exp2(mc - m), a.ml[2 * (c * stride + row) + 1], sum);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int e = 4 * (threadIdx.x & 7); e < a.d; e += 32) {
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < n; ++c) {
+      const float mc = a.ml[2 * (c * stride + row)];
+      const float f = mc == -INFINITY ? 0.0f : fast_exp2(mc - m);
+      acc += f * *(const f32x4*)(a.part + (c * stride + row) * HD + e);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e + i < a.d) st((T*)a.out, row * a.d + e + i, acc[i] * inv);
+  }
+  if ((threadIdx.x & 7) == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? INFINITY : (m + __log2f(sum)) * LN2;
+}
+
+// How the key tiles of a query tile are cut: into chunks of `len` tiles where the call's workgroups without it would not
+// fill the GPU's 512 places.  The longest text may have all keys, so the grid has a chunk for each part of those, most of
+// which find no tile.
+void packed_plan(PackArgs& a, int BN) {
+  a.nx = (int)packed_tiles(a.N, a.S);
+  a.chunks = 1, a.len = 1 << 30;
+  const long wgs = (long)a.H * a.nx;
+  if (wgs >= 512) return;
+  long keys = a.M;
+  if (a.W < PK_ALL) keys = std::min(keys, (long)a.W + PK_M + a.sinks + 2L * BN);
+  const long most = (keys + BN - 1) / BN + 1, want = std::min(32L, std::max(1L, 4096 / wgs));
+  const long len = std::max(4L, (most + want - 1) / want);
+  a.chunks = (int)((most + len - 1) / len);
+  if (a.chunks > 1) a.len = (int)len;
+}
+size_t packed_chunk_bytes(const PackArgs& a) {
+  return a.chunks == 1 ? 0 : (size_t)a.chunks * a.H * a.N * (window_pad(a.d) + 2) * sizeof(float);
+}
+
+template <typename T, int HD, int BN, bool VEC>
+int launch_fwd(hipStream_t s, PackArgs a) {
+  const long grid = (long)a.H * a.nx * a.chunks;
+  a.ml = a.part + (size_t)a.chunks * a.H * a.N * HD;
+  packed_fwd_kernel<T, HD, BN, VEC><<<(unsigned)grid, 256, 0, s>>>(a);
+  if (a.chunks > 1) packed_join_kernel<T, HD, BN><<<(unsigned)(a.H * a.nx * 4), 256, 0, s>>>(a);
+  return check_launch("packed attention");
+}
+template <typename T, int BN, bool VEC>
+int launch_fwd_d(hipStream_t s, const PackArgs& a) {
+  switch (window_pad(a.d)) {
+    case 32: return launch_fwd<T, 32, BN, VEC>(s, a);
+    case 64: return launch_fwd<T, 64, BN, VEC>(s, a);
+    case 96: return launch_fwd<T, 96, BN, VEC>(s, a);
+    default: return launch_fwd<T, 128, BN, VEC>(s, a);
+  }
+}
+
+constexpr int key_tile(int dtype) { return dtype == EDF_BF16 ? 64 : 32; }
+
+}  // namespace
+
+int packed_check(int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim, int window, int sinks,
+                 int dtype) {
+  EDF_REQUIRE(num_heads > 0 && num_kv_heads > 0 && rows > 0 && key_rows > 0 && head_dim > 0 && texts >= 0,
+              EDF_ERR_INVALID_ARG, "dimensions must be positive");
+  EDF_REQUIRE(valid_dtype(dtype), EDF_ERR_INVALID_ARG, "dtype must be 0 (f32) or 1 (bf16)");
+  EDF_REQUIRE(num_heads % num_kv_heads == 0, EDF_ERR_INVALID_ARG, "num_heads %d is no multiple of num_kv_heads %d",
+              num_heads, num_kv_heads);
+  EDF_REQUIRE(window >= 0 && sinks >= 0, EDF_ERR_INVALID_ARG, "window and sinks must not be negative");
+  EDF_REQUIRE(head_dim <= 128, EDF_ERR_UNSUPPORTED, "head_dim %d > 128 unsupported", head_dim);
+  EDF_REQUIRE(rows < (1L << 30) && key_rows < (1L << 30) && texts < (1 << 28) && sinks < (1 << 30), EDF_ERR_UNSUPPORTED,
+              "rows, keys, texts and sinks must be below 2^28");
+  EDF_REQUIRE((double)num_heads * packed_tiles(std::max(rows, key_rows), texts) * 4 < 2147483648.0, EDF_ERR_UNSUPPORTED,
+              "heads x rows too large for one call");
+  return EDF_OK;
+}
+
+}  // namespace edf
+
+extern "C" {
+
+size_t edf_packed_attention_workspace_bytes(int num_heads, int num_kv_heads, long rows, long key_rows, int texts,
+                                            int head_dim, int window, int sinks, int dtype) {
+  using namespace edf;
+  if (packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype)) return 0;
+  PackArgs a{};
+  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.d = head_dim;
+  a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
+  packed_plan(a, key_tile(dtype));
+  return packed_chunk_bytes(a);
+}
+
+int edf_packed_attention(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
+                         const int32_t* key_offsets, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                         int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim, int window,
+                         int sinks, int dtype) {
+  using namespace edf;
+  const int rc = packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype);
+  if (rc) return rc;
+  EDF_REQUIRE(q && k && v && offsets && key_offsets && out, EDF_ERR_INVALID_ARG, "null tensor pointer");
+  PackArgs a{};
+  a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.out = out, a.lse = lse;
+  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
+  a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
+  a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
+  packed_plan(a, key_tile(dtype));
+  const size_t need = packed_chunk_bytes(a);
+  EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
+              "workspace too small: need %zu bytes", need);
+  a.part = (float*)workspace;
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
+  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && key_rows <= WINDOW_VEC_T;
+  hipStream_t s = as_stream(stream);
+  if (dtype == EDF_BF16) return vec ? launch_fwd_d<bf16, 64, true>(s, a) : launch_fwd_d<bf16, 64, false>(s, a);
+  return vec ? launch_fwd_d<float, 32, true>(s, a) : launch_fwd_d<float, 32, false>(s, a);
+}
+
+}  // extern "C"

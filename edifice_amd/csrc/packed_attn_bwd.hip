@@ -1,0 +1,453 @@
+// Causal attention over texts laid end to end, backward (packed_attn.hip has the forward and its formulas):
+//   P from the forward's row sums; dV_j = sum_i P_ij dO_i, dP = dO V^T, D_i = dO_i . O_i,
+//   dS = P (dP - D) / sqrt(d), dQ = dS K, dK = dS^T Q; dK, dV summed over the query heads of a key head.
+// 10 d flops per visible pair (S and dP formed twice, once for each kernel): bound by the matrix cores.
+//
+//   dQ: a workgroup owns 128 queries of a text (32 per wave, Q^T and dO^T in registers) and walks the key tiles of the
+//   forward; it also forms D and leaves it for the second kernel.
+//   dK, dV: a workgroup owns 128 keys of a text (32 per wave, K^T and V^T in registers) of one key head and walks the
+//   query tiles that see one of them, query head by query head: the sum over shared heads needs no atomics.  Where key
+//   blocks are few against the GPU, each block's query tiles are shared out evenly among several workgroups, which leave
+//   float32 sums, added in order by a third kernel.
+// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term), D is formed from the rounded O that
+// the forward left, and P from the forward's sum of rounded probabilities; everything else is float32.
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "edf_packed.hpp"
+
+namespace edf {
+namespace {
+
+template <typename T, int HD, int BN, bool VEC>
+__global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
+  constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
+  constexpr int AHEAD = sizeof(T) == 2 ? 3 : 1;
+  using Tile = WTile<T, HD, BN>;
+  __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
+  __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  int x, head;
+  packed_block(a, a.nx, x, head);
+  const TextTile tt = find_tile(a.qo, a.S, a.N, a.nx - 1 - x);
+  if (tt.first >= tt.n) return;
+  int krow, nk;
+  text_rows(a.ko, a.S, a.M, tt.text, krow, nk);
+  const int d = a.d, p0 = tt.first + nk - tt.n, pw = p0 + 32 * w, myp = pw + li, myq = tt.first + 32 * w + li;
+  const long qrow = (long)head * a.N + tt.row0 + min(myq, tt.n - 1);
+  const T* K = (const T*)a.k + ((long)(head / a.G) * a.M + krow) * d;
+  const T* V = (const T*)a.v + ((long)(head / a.G) * a.M + krow) * d;
+
+  WFrag<T> qf[NKK], of[NKK];
+  float dd = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    const int col = kk * 16 + 8 * g;
+    qf[kk] = window_row<T, HD, VEC>((const T*)a.q + qrow * d, col, d);
+    of[kk] = window_row<T, HD, VEC>((const T*)a.go + qrow * d, col, d);
+    const WFrag<T> oo = window_row<T, HD, VEC>((const T*)a.o + qrow * d, col, d);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dd = fmaf(oo.get(e), of[kk].get(e), dd);
+  }
+  dd += __shfl_xor(dd, 32);
+  const float lse = a.lse[qrow] * LOG2E;
+  if (g == 0 && myq < tt.n) a.dd[qrow] = dd;
+  f32x16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
+
+  const KeyTiles<PK_M, BN> kt(p0, nk, a.W, a.sinks);
+  const int count = p0 + PK_M > 0 ? max(kt.count, 0) : 0;
+  const TileLoader<T, HD, BN, VEC> ld(tid, d, nk);
+  WFrag<T> rk[ld.N], rv[ld.N];
+  auto gload = [&](int t) {
+    const int k0 = kt.key0(t);
+    ld.load(K, k0, rk);
+    ld.load(V, k0, rv);
+  };
+  auto sstore = [&](int buf) {
+    ld.template store<Tile>(sK[buf], rk);
+    ld.template store<Tile>(sV[buf], rv);
+  };
+  auto tile = [&](int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const SeesKey sees(myp, kt.key0(t) + 4 * g, a.W, a.sinks);
+    const T *sk = sK[t & 1], *sv = sV[t & 1];
+    f32x16 s[NH], dp[NH];
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
+      s[h] = zero16();
+      dp[h] = zero16();
+    }
+    ahead<NH * NKK, AHEAD>(
+        [&](int i) {
+          const int row = i / NKK * 32 + li, col = i % NKK * 16 + 8 * g;
+          return Pair<T>{Tile::row(sk, row, col), Tile::row(sv, row, col)};
+        },
+        [&](int i, const Pair<T>& f) {
+          s[i / NKK] = WFrag<T>::mma(f.x, qf[i % NKK], s[i / NKK]);
+          dp[i / NKK] = WFrag<T>::mma(f.y, of[i % NKK], dp[i / NKK]);
+        });
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = fast_exp2(fmaf(s[h][r], a.scale_log2, -lse)) * (dp[h][r] - dd);  // 1 / sqrt(d) at the end
+        if constexpr (MASK) x = sees(h * 32 + d_row(r, 0)) ? x : 0.0f;
+        s[h][r] = x;
+      }
+    WFrag<T> df[2 * NH];
+#pragma unroll
+    for (int kc = 0; kc < 2 * NH; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) df[kc].set(e, s[kc >> 1][8 * (kc & 1) + e]);
+    ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sk, 16 * (i / NDT), i % NDT, l); },
+                               [&](int i, const WFrag<T>& f) { dq[i % NDT] = WFrag<T>::mma(f, df[i / NDT], dq[i % NDT]); });
+  };
+  auto advance = [&](int t) {
+    if (t + 1 < count) {
+      sstore((t + 1) & 1);
+      if (t + 2 < count) gload(t + 2);
+    }
+    __syncthreads();
+  };
+  if (count > 0) {
+    gload(0);
+    sstore(0);
+    if (count > 1) gload(1);
+  }
+  __syncthreads();
+  const int masked = min(count, kt.first_whole);
+  int t = 0;
+  for (; t < masked; ++t) {
+    const int k0 = kt.key0(t);
+    if ((k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks) tile(t, std::true_type{});
+    advance(t);
+  }
+  for (; t < count; ++t) {
+    tile(t, std::false_type{});
+    advance(t);
+  }
+  if (myq >= tt.n) return;
+  T* out = (T*)a.dq + qrow * d;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const int c = dt * 32 + 8 * rb + 4 * g;
+      if (VEC && c + 4 <= d) {
+        typedef __attribute__((ext_vector_type(4))) T vec4;
+        vec4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(dq[dt][rb * 4 + e] * a.scale);
+        *(vec4*)(out + c) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < d) out[c + e] = from_f32<T>(dq[dt][rb * 4 + e] * a.scale);
+      }
+    }
+}
+
+// The key block of a dK, dV workgroup and its share [t0, t1) of the block's (query head, tile of BQ queries) pairs: nt
+// tiles a head, from query qs of the text on.
+template <int BQ>
+struct KeyBlock {
+  int head, share, krow, nk, first, qrow, nq, qs, nt, t0, t1;  // first: the block's first key within the text
+  bool none;
+  EDF_DEVICE int ahead() const { return nk - nq; }
+  EDF_DEVICE KeyBlock(const PackArgs& a, int id_x, int id_head, int share_) : head(id_head), share(share_) {
+    const TextTile t = find_tile(a.ko, a.S, a.M, id_x);
+    krow = t.row0, nk = t.n, first = t.first;
+    none = first >= nk;
+    text_rows(a.qo, a.S, a.N, t.text, qrow, nq);
+    qs = max(0, first - ahead());  // the first query that sees the block's first key
+    int end = nq;
+    if (first >= a.sinks) end = (int)min((long)nq, (long)first + PK_M - 1 + a.W - ahead());  // past the last key's window
+    nt = max(0, (end - qs + BQ - 1) / BQ);
+    const long all = (long)nt * a.G;
+    t0 = (int)(all * share / a.chunks);
+    t1 = (int)(all * (share + 1) / a.chunks);
+  }
+};
+
+template <typename T, int HD, int BQ, bool VEC>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) void packed_dkdv_kernel(PackArgs a) {
+  constexpr int NKK = HD / 16, NDT = HD / 32;
+  constexpr int AHEAD = sizeof(T) == 4 ? 1 : HD == 96 ? 2 : 3;
+  using Tile = WTile<T, HD, BQ>;
+  __shared__ __attribute__((aligned(16))) T sQ[2][Tile::ELEMS];
+  __shared__ __attribute__((aligned(16))) T sO[2][Tile::ELEMS];
+  __shared__ __attribute__((aligned(16))) float sL[2][BQ], sD[2][BQ];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  int x, head;  // of the key heads
+  packed_block(a, a.nx * a.chunks, x, head);
+  const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
+  if (kb.none) return;
+  const int d = a.d, kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
+  const long krow = (long)head * a.M + kb.krow + min(mykey, kb.nk - 1);
+  WFrag<T> kf[NKK], vf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    kf[kk] = window_row<T, HD, VEC>((const T*)a.k + krow * d, kk * 16 + 8 * g, d);
+    vf[kk] = window_row<T, HD, VEC>((const T*)a.v + krow * d, kk * 16 + 8 * g, d);
+  }
+  f32x16 dk[NDT], dv[NDT];  // dK^T, dV^T: rows are dims, the column this lane's key
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    dk[dt] = zero16();
+    dv[dt] = zero16();
+  }
+  const TileLoader<T, HD, BQ, VEC> ld(tid, d, kb.nq);
+  WFrag<T> rq[ld.N], ro[ld.N];
+  float rl = 0.0f, rd = 0.0f;
+  auto gload = [&](int t) {
+    const int h = t / nt, q0 = kb.qs + (t - h * nt) * BQ;
+    const long base = (long)(head * a.G + h) * a.N + kb.qrow;
+    ld.load((const T*)a.q + base * d, q0, rq);
+    ld.load((const T*)a.go + base * d, q0, ro);
+    if (tid < BQ) {
+      const long q = base + min(q0 + tid, kb.nq - 1);
+      rl = q0 + tid < kb.nq ? a.lse[q] * LOG2E : INFINITY;  // a query past the end gets P = 0
+      rd = a.dd[q];
+    }
+  };
+  auto sstore = [&](int buf) {
+    ld.template store<Tile>(sQ[buf], rq);
+    ld.template store<Tile>(sO[buf], ro);
+    if (tid < BQ) {
+      sL[buf][tid] = rl;
+      sD[buf][tid] = rd;
+    }
+  };
+  if (t0 < t1) {
+    gload(t0);
+    sstore(0);
+    if (t0 + 1 < t1) gload(t0 + 1);
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    const int p0 = kb.qs + t % nt * BQ + kb.ahead();  // position of the tile's first query
+#pragma unroll
+    for (int sub = 0; sub < BQ / 32; ++sub) {
+      const int pb = p0 + 32 * sub;
+      // no query of the sub-tile sees a key of this wave
+      if (pb + 31 < kw || (pb > kw + 30 + a.W && kw >= a.sinks)) continue;
+      auto subtile = [&](auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        f32x16 s = zero16(), dp = zero16();
+        ahead<NKK, AHEAD>(
+            [&](int i) {
+              const int row = 32 * sub + li, col = i * 16 + 8 * g;
+              return Pair<T>{Tile::row(sQ[buf], row, col), Tile::row(sO[buf], row, col)};
+            },
+            [&](int i, const Pair<T>& f) {
+              s = WFrag<T>::mma(f.x, kf[i], s);
+              dp = WFrag<T>::mma(f.y, vf[i], dp);
+            });
+#pragma unroll
+        for (int rb = 0; rb < 4; ++rb) {
+          const f32x4 lv = *(const f32x4*)(&sL[buf][32 * sub + 8 * rb + 4 * g]);
+          const f32x4 dv4 = *(const f32x4*)(&sD[buf][32 * sub + 8 * rb + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = rb * 4 + e;
+            float p = fast_exp2(fmaf(s[r], a.scale_log2, -lv[e]));
+            float x = p * (dp[r] - dv4[e]);  // 1 / sqrt(d) is applied to dK at the end
+            if constexpr (MASK) {
+              const bool see = window_sees(pb + 8 * rb + 4 * g + e, mykey, a.W, a.sinks);
+              p = see ? p : 0.0f;
+              x = see ? x : 0.0f;
+            }
+            s[r] = p;
+            dp[r] = x;
+          }
+        }
+        WFrag<T> pf[2], df[2];
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            pf[kc].set(e, s[8 * kc + e]);
+            df[kc].set(e, dp[8 * kc + e]);
+          }
+        ahead<2 * NDT, AHEAD>(
+            [&](int i) {
+              const int r0 = 32 * sub + 16 * (i / NDT);
+              return Pair<T>{Tile::trans(sO[buf], r0, i % NDT, l), Tile::trans(sQ[buf], r0, i % NDT, l)};
+            },
+            [&](int i, const Pair<T>& f) {
+              dv[i % NDT] = WFrag<T>::mma(f.x, pf[i / NDT], dv[i % NDT]);
+              dk[i % NDT] = WFrag<T>::mma(f.y, df[i / NDT], dk[i % NDT]);
+            });
+      };
+      // every pair visible: the queries lie past the wave's keys and within the window of its first
+      if (pb >= kw + 31 && pb + 31 - kw < a.W) subtile(std::false_type{});
+      else subtile(std::true_type{});
+    }
+    if (t + 1 < t1) {
+      sstore(buf ^ 1);
+      if (t + 2 < t1) gload(t + 2);
+    }
+    __syncthreads();
+  }
+  if (a.chunks > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
+    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.chunks) * (2L * PK_M * HD) + (32 * w + li) * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) {
+        f32x4 u, v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u[e] = dk[dt][rb * 4 + e];
+          v[e] = dv[dt][rb * 4 + e];
+        }
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) = u;
+        *(f32x4*)(out + PK_M * HD + dt * 32 + 8 * rb + 4 * g) = v;
+      }
+    return;
+  }
+  if (mykey >= kb.nk) return;
+  T *kout = (T*)a.dk + krow * d, *vout = (T*)a.dv + krow * d;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const int c = dt * 32 + 8 * rb + 4 * g;
+      if (VEC && c + 4 <= d) {
+        typedef __attribute__((ext_vector_type(4))) T vec4;
+        vec4 u, v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u[e] = from_f32<T>(dk[dt][rb * 4 + e] * a.scale);
+          v[e] = from_f32<T>(dv[dt][rb * 4 + e]);
+        }
+        *(vec4*)(kout + c) = u;
+        *(vec4*)(vout + c) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < d) {
+            kout[c + e] = from_f32<T>(dk[dt][rb * 4 + e] * a.scale);
+            vout[c + e] = from_f32<T>(dv[dt][rb * 4 + e]);
+          }
+      }
+    }
+}
+
+// dK, dV of blocks whose sums are in shares, added in order, four elements a thread.  A workgroup takes one of the pieces
+// of a block's [dK | dV][key][dim].
+template <typename T, int HD>
+__global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
+  constexpr int PIECES = 2 * PK_M * HD / 1024;
+  const int piece = blockIdx.x % PIECES, x = blockIdx.x / PIECES % a.nx, head = blockIdx.x / PIECES / a.nx;
+  const TextTile t = find_tile(a.ko, a.S, a.M, x);
+  const int e = (piece * 256 + threadIdx.x) * 4;
+  const bool is_v = e >= PK_M * HD;
+  const int key = t.first + e / HD % PK_M, c = e % HD;
+  if (key >= t.n || c >= a.d) return;
+  const int hkv = a.H / a.G;
+  const float* in = a.part + ((long)head * a.nx + x) * (2L * PK_M * HD) + e;
+  const long stride = (long)hkv * a.nx * (2L * PK_M * HD);
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int i = 0; i < a.chunks; ++i) s += *(const f32x4*)(in + i * stride);
+  if (!is_v) s *= a.scale;
+  T* out = (T*)(is_v ? a.dv : a.dk) + ((long)head * a.M + t.row0 + key) * a.d + c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (c + i < a.d) out[i] = from_f32<T>(s[i]);
+}
+
+constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
+
+// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places.
+void backward_plan(PackArgs& a) {
+  a.nx = (int)packed_tiles(a.M, a.S);
+  const long wgs = (long)(a.H / a.G) * a.nx;
+  a.chunks = (int)std::max(1L, std::min(16L, 512 / wgs));
+}
+size_t share_bytes(const PackArgs& a) {
+  return a.chunks == 1 ? 0
+                       : (size_t)a.chunks * (a.H / a.G) * a.nx * (2 * PK_M) * window_pad(a.d) * sizeof(float);
+}
+size_t row_bytes(long heads, long rows) { return ((size_t)heads * rows * sizeof(float) + 255) & ~(size_t)255; }
+
+template <typename T, int HD, int BN, int BQ, bool VEC>
+int launch_bwd(hipStream_t s, PackArgs a) {
+  PackArgs q = a;
+  q.nx = (int)packed_tiles(a.N, a.S);
+  packed_dq_kernel<T, HD, BN, VEC><<<(unsigned)((long)a.H * q.nx), 256, 0, s>>>(q);
+  int rc = check_launch("packed attention dQ");
+  if (rc) return rc;
+  const int hkv = a.H / a.G;
+  packed_dkdv_kernel<T, HD, BQ, VEC><<<(unsigned)((long)hkv * a.nx * a.chunks), 256, 0, s>>>(a);
+  rc = check_launch("packed attention dK, dV");
+  if (rc || a.chunks == 1) return rc;
+  packed_sum_kernel<T, HD><<<(unsigned)(2L * PK_M * HD / 1024 * a.nx * hkv), 256, 0, s>>>(a);
+  return check_launch("packed attention dK, dV sums");
+}
+template <typename T, int BN, int BQ, bool VEC>
+int launch_bwd_d(hipStream_t s, const PackArgs& a) {
+  switch (window_pad(a.d)) {
+    case 32: return launch_bwd<T, 32, BN, BQ, VEC>(s, a);
+    case 64: return launch_bwd<T, 64, BN, BQ, VEC>(s, a);
+    case 96: return launch_bwd<T, 96, BN, BQ, VEC>(s, a);
+    default: return launch_bwd<T, 128, BN, BQ, VEC>(s, a);
+  }
+}
+
+}  // namespace
+}  // namespace edf
+
+extern "C" {
+
+size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_heads, long rows, long key_rows, int texts,
+                                                     int head_dim, int window, int sinks, int dtype) {
+  using namespace edf;
+  if (packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype)) return 0;
+  PackArgs a{};
+  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
+  backward_plan(a);
+  return row_bytes(num_heads, rows) + share_bytes(a);
+}
+
+int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
+                                  const int32_t* key_offsets, const void* out, const void* grad_out, const float* lse,
+                                  void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                                  int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim,
+                                  int window, int sinks, int dtype) {
+  using namespace edf;
+  const int rc = packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype);
+  if (rc) return rc;
+  EDF_REQUIRE(q && k && v && offsets && key_offsets && out && grad_out && lse && grad_q && grad_k && grad_v,
+              EDF_ERR_INVALID_ARG, "null tensor pointer (the forward's lse is required)");
+  PackArgs a{};
+  a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.o = out, a.go = grad_out;
+  a.lse = const_cast<float*>(lse), a.dq = grad_q, a.dk = grad_k, a.dv = grad_v;
+  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
+  a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
+  a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
+  backward_plan(a);
+  const size_t need = row_bytes(num_heads, rows) + share_bytes(a);
+  EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
+  a.dd = (float*)workspace;
+  a.part = (float*)((char*)workspace + row_bytes(num_heads, rows));
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)grad_out |
+                         (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
+  const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) &&
+                   std::max(rows, key_rows) <= WINDOW_VEC_T;
+  hipStream_t s = as_stream(stream);
+  if (dtype == EDF_BF16)
+    return vec ? launch_bwd_d<bf16, 64, BQ_BF16, true>(s, a) : launch_bwd_d<bf16, 64, BQ_BF16, false>(s, a);
+  return vec ? launch_bwd_d<float, 32, BQ_32, true>(s, a) : launch_bwd_d<float, 32, BQ_32, false>(s, a);
+}
+
+}  // extern "C"

@@ -1220,6 +1220,74 @@ def window_attention(q, k, v, window: int, sinks: int = 0):
     return _WindowAttention.forward(None, *args)
 
 
+class _PackedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, key_offsets, window, sinks):
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        _same(q, k, v)
+        if q.dim() not in (3, 4) or k.dim() != q.dim() or (q.dim() == 4 and (q.shape[0] != 1 or k.shape[0] != 1)):
+            raise EdificeHipError(f"q, k, v must be [H, rows, d] or [1, H, rows, d], got {tuple(q.shape)} and {tuple(k.shape)}")
+        nh, rows, hd = q.shape[-3:]
+        nkv, keys = k.shape[-3:-1]
+        if v.shape != k.shape or k.shape[-1] != hd or nkv == 0 or nh % nkv or (key_offsets is None and keys != rows):
+            raise EdificeHipError("packed_attention needs q [H, N, d] and k, v [Hkv, M, d] with H a multiple of Hkv (and "
+                                  f"M = N without key_offsets), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+        _rank("offsets", offsets, 1)
+        offsets = _i32("offsets", offsets, offsets.shape)
+        texts = offsets.numel() - 1
+        if texts < 0:
+            raise EdificeHipError("offsets must have a value for each text and one more")
+        key_offsets = offsets if key_offsets is None else _i32("key_offsets", key_offsets, offsets.shape)
+        stream = _here(q, k, v, offsets, key_offsets)
+        if window < 0 or sinks < 0:
+            raise EdificeHipError("window and sinks must not be negative")
+        keep = ctx is not None  # None: no gradient is asked for
+        lse = torch.empty((nh, rows), dtype=torch.float32, device=q.device) if keep else None
+        # more sees no more keys
+        conf = (nh, nkv, rows, keys, texts, hd, min(window, max(keys, 1)), min(sinks, keys), dtype_flag(q))
+        if q.numel() and keys:
+            out = torch.empty_like(q)
+            wsb = nat.query("edf_packed_attention_workspace_bytes", *conf)
+            ws = _u8(wsb, q) if wsb else None
+            nat.call("edf_packed_attention", stream, _p(q), _p(k), _p(v), _p(offsets), _p(key_offsets), _p(out), _p(lse),
+                     _p(ws), wsb, *conf)
+        else:
+            out = torch.zeros_like(q)
+        if keep:
+            ctx.conf = conf
+            ctx.save_for_backward(q, k, v, offsets, key_offsets, out, lse)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        q, k, v, offsets, key_offsets, out, lse = ctx.saved_tensors
+        if not q.numel() or not k.numel():
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None, None
+        dout = dout.contiguous().to(q.dtype)
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        wsb = nat.query("edf_packed_attention_backward_workspace_bytes", *ctx.conf)
+        ws = _u8(wsb, q)
+        nat.call("edf_packed_attention_backward", _stream(), _p(q), _p(k), _p(v), _p(offsets), _p(key_offsets), _p(out),
+                 _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(ws), wsb, *ctx.conf)
+        return dq, dk, dv, None, None, None, None
+
+
+def packed_attention(q, k, v, offsets, key_offsets=None, *, window: int = 0, sinks: int = 0):
+    """Causal attention over texts of different lengths laid end to end, with shared key heads: q [H, N, d] (or [1, H, N,
+    d]), k, v [Hkv, M, d], query head h reads key head h // (H // Hkv).  offsets, key_offsets: int32 [texts + 1] on the
+    GPU, ascending from 0; text s has queries offsets[s] .. offsets[s + 1] - 1 and keys key_offsets[s] .. (None: the
+    same rows).  The queries of a text are the last of its keys: query i of n stands at position p = i + m - n of m keys
+    and sees key j when j <= p and (window == 0 or p - j < window or j < sinks); scale 1/sqrt(d).  A query that sees no
+    key, and rows behind the last text, answer with zeros.  float32 or bfloat16, head_dim <= 128; differentiable (fused HIP
+    backward, the gradients of shared heads summed in a fixed order).  Keys and values have to be finite.
+
+    The launch depends on shapes alone, so a captured call may be replayed after the offsets have changed."""
+    args = (q, k, v, offsets, key_offsets, int(window), int(sinks))
+    if _wants_grad(q, k, v):
+        return _PackedAttention.apply(*args)
+    return _PackedAttention.forward(None, *args)
+
+
 _CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
 _NO_CODE = -1
 

@@ -165,3 +165,26 @@ def paged_cache_read(values, table, offsets, total):
             if 0 <= row < total and i < table.shape[1] * block and 0 <= int(table[b, i // block]) < blocks:
                 out[:, row] = values[int(table[b, i // block]), :, i % block]
     return out
+
+
+def packed_attention(q, k, v, offsets, key_offsets, window=0, sinks=0):
+    """q [H, N, d], k, v [Hkv, M, d], lists of offsets: one text after the other; differentiable."""
+    G = q.shape[0] // k.shape[0]
+    rows = []
+    for s in range(len(offsets) - 1):
+        a, b, c, e = offsets[s], offsets[s + 1], key_offsets[s], key_offsets[s + 1]
+        rows.append(text_probabilities(q[:, a:b], k[:, c:e], window, sinks) @ v[:, c:e].repeat_interleave(G, 0))
+    rows.append(torch.zeros_like(q[:, offsets[-1]:]))
+    return torch.cat(rows, 1)
+
+
+def text_probabilities(q, k, window, sinks):
+    """q [H, n, d] at the end of k [Hkv, m, d]: the probabilities [H, n, m], zeros where a query sees no key."""
+    n, m = q.shape[1], k.shape[1]
+    p, j = torch.arange(n)[:, None] + m - n, torch.arange(m)[None, :]
+    see = j <= p
+    if window:
+        see = see & ((p - j < window) | (j < sinks))
+    a = q @ k.repeat_interleave(q.shape[0] // k.shape[0], 0).transpose(-1, -2) / math.sqrt(q.shape[2])
+    some = see.any(1, keepdim=True)
+    return torch.softmax(a.masked_fill(~see & some, -math.inf), -1) * some if m else a
