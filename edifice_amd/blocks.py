@@ -20,7 +20,8 @@ forward and backward through a block runs the HIP kernels for the recurrence and
                      swish output gate)
   GQABlock           causal grouped-query attention routed to flash attention
                      (lib/edifice/blocks/sdpa.ex:74-91) + GELU feed-forward; with rotary positions,
-                     query / key norms, a window or sinks, and a step over a paged cache
+                     query / key norms, a window or sinks, over texts laid end to end, and a step over a
+                     paged cache of the model's type or of 8-bit numbers
 
 ``build(name, **opts)`` mirrors ``Edifice.build(name, opts)`` for these families and returns
 a model mapping [batch, seq, embed] to the last timestep's hidden state, as the reference's
@@ -265,7 +266,9 @@ class PagedCache:
 
     k[layer], v[layer] [num_blocks, num_kv_heads, block_size, head_dim]; table [requests, width] and lengths
     [requests] live on the GPU, and so does the list of free pages: ``extend`` makes room for new tokens without a
-    host synchronisation, and may be captured with the step that follows it."""
+    host synchronisation, and may be captured with the step that follows it.  dtype int8 or float8_e4m3fn: 8-bit numbers
+    in units of a scale that the tokens of a page and head share, k_scale[layer], v_scale[layer] float32 [num_blocks,
+    num_kv_heads] (``fused_scan.paged_cache_write``)."""
 
     def __init__(self, layers: int, requests: int, max_length: int, num_kv_heads: int, head_dim: int, *,
                  block_size: int = 16, num_blocks: int | None = None, dtype=torch.bfloat16, device="cuda"):
@@ -275,6 +278,9 @@ class PagedCache:
         shape = (blocks, num_kv_heads, block_size, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
+        scaled = dtype in (torch.int8, torch.float8_e4m3fn)
+        self.k_scale, self.v_scale = ([torch.zeros(shape[:2], device=device) if scaled else None for _ in range(layers)]
+                                      for _ in range(2))
         i32 = dict(dtype=torch.int32, device=device)
         self.table = torch.full((requests, width), -1, **i32)
         self.lengths = torch.zeros(requests, **i32)
@@ -298,10 +304,17 @@ class PagedCache:
         return slots, positions
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
-        fs.paged_cache_write(k, v, slots, self.k[layer], self.v[layer])
+        fs.paged_cache_write(k, v, slots, self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer])
 
     def attend(self, layer: int, q: torch.Tensor, window: int = 0, sinks: int = 0) -> torch.Tensor:
-        return fs.paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, window=window, sinks=sinks)
+        return fs.paged_attention(q, self.k[layer], self.v[layer], self.table, self.lengths, window=window, sinks=sinks,
+                                  k_scale=self.k_scale[layer], v_scale=self.v_scale[layer])
+
+    def read(self, layer: int, offsets: torch.Tensor, total: int, dtype: torch.dtype):
+        """Keys and values [num_kv_heads, total, head_dim] of the places' first offsets[r + 1] - offsets[r] tokens, laid end
+        to end (``fused_scan.paged_cache_read``)."""
+        return fs.paged_cache_read(self.k[layer], self.v[layer], self.table, offsets, total, self.k_scale[layer],
+                                   self.v_scale[layer], dtype=dtype)
 
     def exhausted(self) -> bool:
         """Whether some place holds a token that found no page: the list of free ones ended, or its table row (waits for
@@ -309,6 +322,16 @@ class PagedCache:
         width = self.table.shape[1]
         held = torch.arange(width, device=self.table.device) * self.block_size < self.lengths[:, None]
         return bool(((self.table < 0) & held).any() | (self.lengths > width * self.block_size).any())
+
+    def has_room(self, num_tokens: int, counts: torch.Tensor = None) -> bool:
+        """Whether ``extend`` with these arguments finds a page for every token and no place misses one already (waits for
+        the GPU)."""
+        if self.exhausted():
+            return False
+        new = self.lengths + (num_tokens if counts is None else counts.clamp(0, num_tokens))
+        pages = lambda n: (n + self.block_size - 1) // self.block_size  # noqa: E731
+        drawn = int((pages(new) - pages(self.lengths)).sum())
+        return int(new.max()) <= self.table.shape[1] * self.block_size and int(self.taken) + drawn <= self.available
 
     def release(self, place: int) -> None:
         """The place's pages back onto the list of free ones, its length 0 (waits for the GPU)."""
@@ -399,6 +422,20 @@ class GQAttention(nn.Module):
         o = fs.flash_attention(q, k, v, causal=True)
         return self.out_proj(fs.merge_heads(o))
 
+    def packed(self, x, offsets, positions):
+        """x [1, N, hidden], texts laid end to end at ``offsets``, positions int32 [1, N] within each."""
+        q, k, v = self._heads(x, positions)
+        return self.out_proj(fs.merge_heads(fs.packed_attention(q, k, v, offsets, window=self.window, sinks=self.sinks)))
+
+    def go_on(self, x, cache: PagedCache, layer: int, slots, positions, offsets, key_offsets, total):
+        """x [1, N, hidden], the tokens that cache.extend just made room for laid end to end at ``offsets``: each text's
+        attend to what its place holds, themselves among it, read back to ``total`` rows at ``key_offsets``."""
+        q, k, v = self._heads(x, positions)
+        cache.write(layer, k, v, slots)
+        k, v = cache.read(layer, key_offsets, total, q.dtype)
+        o = fs.packed_attention(q, k[None], v[None], offsets, key_offsets, window=self.window, sinks=self.sinks)
+        return self.out_proj(fs.merge_heads(o))
+
     def step(self, x, cache: PagedCache, layer: int, slots, positions):
         """x [places, T, hidden], the tokens that cache.extend just made room for: T = 1 attends over the cache;
         T > 1 is a prompt into empty places and attends to itself.  Inference (call under torch.no_grad())."""
@@ -432,6 +469,14 @@ class GQABlock(nn.Module):
         x = x + self.attn.step(self.attn_norm(x), cache, layer, slots, positions)
         return x + self.ffn(self.ffn_norm(x))
 
+    def packed(self, x, offsets, positions):
+        x = x + self.attn.packed(self.attn_norm(x), offsets, positions)
+        return x + self.ffn(self.ffn_norm(x))
+
+    def go_on(self, x, *args):
+        x = x + self.attn.go_on(self.attn_norm(x), *args)
+        return x + self.ffn(self.ffn_norm(x))
+
     def ffn(self, n):
         return self.ffn_down(F.gelu(self.ffn_up(n)))
 
@@ -461,27 +506,40 @@ class SequenceModel(nn.Module):
     def forward(self, x):
         return self.sequence(x)[:, -1]
 
-    def paged_cache(self, requests: int, max_length: int, **opts) -> PagedCache:
-        """An empty cache for ``step`` (the "gqa" family): options as ``PagedCache``."""
+    def _attention_blocks(self):
         blocks = getattr(self, self._blocks_name)
         if not all(isinstance(b, GQABlock) for b in blocks):
-            raise ValueError("only models of attention blocks take a paged cache")
+            raise ValueError("only models of attention blocks take a paged cache or packed texts")
+        return blocks
+
+    def packed(self, x, offsets):
+        """Hidden states [N, hidden] of texts of different lengths laid end to end (the "gqa" family): x [N, embed], text s
+        the rows offsets[s] .. offsets[s + 1] - 1 (int32 [texts + 1] on the GPU, ascending from 0; rows behind the last
+        text hold no text and should be finite).  Each text's are those of ``sequence`` over it alone; differentiable."""
+        blocks = self._attention_blocks()
+        if x.dim() != 2:
+            raise ValueError(f"x must be [rows, embed], got {tuple(x.shape)}")
+        rows = torch.arange(x.shape[0], dtype=torch.int32, device=x.device)
+        text = torch.bucketize(rows, offsets[1:], right=True)
+        positions = (rows - offsets[text])[None]
+        h = x[None]
+        h = self.input_projection(h) if hasattr(self, "input_projection") else h
+        for blk in blocks:
+            h = blk.packed(h, offsets, positions)
+        return (self.final_norm(h) if hasattr(self, "final_norm") else h)[0]
+
+    def paged_cache(self, requests: int, max_length: int, **opts) -> PagedCache:
+        """An empty cache for ``step`` (the "gqa" family): options as ``PagedCache``, the model's type unless dtype says
+        int8 or float8_e4m3fn."""
+        blocks = self._attention_blocks()
         w = blocks[0].attn.k_proj.weight
         nkv = blocks[0].attn.num_kv_heads
         return PagedCache(len(blocks), requests, max_length, nkv, w.shape[0] // nkv,
                           **{"dtype": w.dtype, "device": w.device, **opts})
 
-    @torch.no_grad()
-    def step(self, x, cache: PagedCache, counts=None):
-        """The next tokens x [requests, T, embed] of a cache's places -> their hidden states [requests, T, hidden]:
-        prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
-        time (T = 1, counts[r] 0 or 1).  Equal to ``sequence`` over the whole text; a token that found no page
-        (``PagedCache.exhausted``) is not seen by those after it.  A step of one token does not wait for the GPU and
-        may be captured; one of several checks that their places are empty.  What does not fit the model or the cache is
-        refused before anything moves."""
-        blocks = getattr(self, self._blocks_name)
-        if not all(isinstance(b, GQABlock) for b in blocks):
-            raise ValueError("only models of attention blocks take a paged cache")
+    def _check_step(self, x, cache):
+        """The model's blocks, if it, the input and the cache belong together."""
+        blocks = self._attention_blocks()
         attn = blocks[0].attn
         w, hd = attn.k_proj.weight, attn.k_proj.weight.shape[0] // attn.num_kv_heads
         embed = (self.input_projection if hasattr(self, "input_projection") else attn.q_proj).weight.shape[1]
@@ -492,13 +550,26 @@ class SequenceModel(nn.Module):
             raise ValueError(f"x of {x.shape[0]} texts and {len(blocks)} layers, a cache of {cache.lengths.numel()} places "
                              f"and {len(cache.k)} layers")
         k = cache.k[0]
-        if (k.shape[1], k.shape[3]) != (attn.num_kv_heads, hd) or k.dtype != w.dtype or k.device != w.device:
+        fits = k.dtype == w.dtype or cache.k_scale[0] is not None
+        if (k.shape[1], k.shape[3]) != (attn.num_kv_heads, hd) or not fits or k.device != w.device:
             raise ValueError(f"the cache holds {k.shape[1]} heads of {k.shape[3]} ({k.dtype} on {k.device}), the model has "
                              f"{attn.num_kv_heads} of {hd} ({w.dtype} on {w.device})")
         if x.shape[1] > 1 and hd > 128:
             raise ValueError(f"several tokens at once need head_dim <= 128, got {hd}")
+        return blocks
+
+    @torch.no_grad()
+    def step(self, x, cache: PagedCache, counts=None):
+        """The next tokens x [requests, T, embed] of a cache's places -> their hidden states [requests, T, hidden]:
+        prompts into empty places (T > 1, counts[r] <= T of them real, the rest padding behind), then one token at a
+        time (T = 1, counts[r] 0 or 1); ``go_on`` takes several tokens onto what places hold.  Equal to ``sequence`` over the
+        whole text, but for the rounding of a cache of 8-bit numbers; a token that found no page
+        (``PagedCache.exhausted``) is not seen by those after it.  A step of one token does not wait for the GPU and
+        may be captured; one of several checks that their places are empty.  What does not fit the model or the cache is
+        refused before anything moves."""
+        blocks = self._check_step(x, cache)
         if x.shape[1] > 1 and bool(((cache.lengths > 0) & (True if counts is None else counts > 0)).any()):
-            raise ValueError("several tokens at once go into empty places only")
+            raise ValueError("several tokens at once go into empty places only (go_on takes them onto filled ones)")
         slots, positions = cache.extend(x.shape[1], counts)
         if x.shape[1] > 1 and counts is not None:  # whatever the padding holds, its keys and values are finite
             x = x.masked_fill((positions < 0)[..., None], 0.0)
@@ -506,6 +577,35 @@ class SequenceModel(nn.Module):
         for layer, blk in enumerate(blocks):
             h = blk.step(h, cache, layer, slots, positions)
         return self.final_norm(h) if hasattr(self, "final_norm") else h
+
+    @torch.no_grad()
+    def go_on(self, x, cache: PagedCache, counts=None):
+        """``step`` for any number of tokens a place, whatever it holds already: a prompt that follows on a conversation.
+        x [requests, T, embed], counts[r] <= T of them real (None: T) -> hidden states [requests, T, hidden], zeros for
+        the padding.  The real tokens run as texts laid end to end, whose queries are the last of their place's keys, read
+        back from the cache.  All of them have to find pages (refused before anything moves).  Waits for the GPU."""
+        blocks = self._check_step(x, cache)
+        if cache.k[0].shape[3] > 128:
+            raise ValueError(f"go_on needs head_dim <= 128, got {cache.k[0].shape[3]}")
+        if not cache.has_room(x.shape[1], counts):
+            raise ValueError("tokens onto filled places need pages for all of them")
+        slots, positions = cache.extend(x.shape[1], counts)
+        real = torch.nonzero(positions.flatten() >= 0)[:, 0]
+        out = x.new_zeros(x.shape[0] * x.shape[1], blocks[0].attn.out_proj.weight.shape[0])
+        if not real.numel():
+            return out.view(x.shape[0], x.shape[1], -1)
+        n = (positions >= 0).sum(1)
+        ends = torch.stack([n, torch.where(n > 0, cache.lengths, 0)]).cumsum(1).to(torch.int32)
+        offsets, key_offsets = F.pad(ends, (1, 0)).unbind(0)
+        total = int(key_offsets[-1])
+        h = x.flatten(0, 1)[real][None]
+        slots, positions = (t.flatten()[real][None] for t in (slots, positions))
+        h = self.input_projection(h) if hasattr(self, "input_projection") else h
+        for layer, blk in enumerate(blocks):
+            h = blk.go_on(h, cache, layer, slots, positions, offsets, key_offsets, total)
+        h = self.final_norm(h) if hasattr(self, "final_norm") else h
+        out[real] = h[0]
+        return out.view(x.shape[0], x.shape[1], -1)
 
     def load_reference_weights(self, weights: dict):
         """Load a reference weight file's ``weight.<layer>.<param>`` tensors (PyTorch layout)."""

@@ -98,4 +98,58 @@ def test_oracle_gradients_against_differences():
     q = torch.randn(2, 5, 4, generator=g, dtype=torch.float64, requires_grad=True)
     k, v = (torch.randn(1, 7, 4, generator=g, dtype=torch.float64, requires_grad=True) for _ in range(2))
     assert torch.autograd.gradcheck(lambda *x: od.packed_attention(*x, [0, 2, 5], [0, 1, 7], 3, 1), (q, k, v))
-    assert math.isfinite(float(q.sum()))
+    assert math.isfinite(float(q.detach().sum()))
+
+
+def _cache(**opts):
+    from edifice_amd import blocks
+    m = blocks.build("gqa", embed_size=32, num_heads=4, num_kv_heads=2)
+    return m, m.paged_cache(2, 12, block_size=4, **opts)
+
+
+@pytest.mark.parametrize("lengths, taken, counts, room", [
+    ([0, 0], 0, None, True),
+    ([5, 0], 2, [7, 3], True),        # 12 tokens of three pages, and one page
+    ([5, 0], 2, [8, 0], False),       # past the table's width
+    ([5, 0], 5, [3, 0], True),        # within the page that is held
+    ([5, 0], 5, [4, 4], False),       # two pages, one left
+    ([5, 0], 2, [-9, 100], True),     # taken as 0 .. the tokens asked for
+])
+def test_room_for_several_tokens(lengths, taken, counts, room):
+    _, c = _cache()
+    c.lengths[:] = torch.tensor(lengths, dtype=torch.int32)
+    for r, n in enumerate(lengths):
+        c.table[r, :-(-n // 4)] = torch.arange(-(-n // 4), dtype=torch.int32)
+    c.taken[0] = taken
+    counts = None if counts is None else torch.tensor(counts, dtype=torch.int32)
+    assert c.has_room(12 if lengths == [0, 0] else 8, counts) == room
+    c.lengths[1], c.table[1, 0] = 1, -1  # a token that found no page
+    assert not c.has_room(1, None)
+
+
+def test_go_on_refuses_before_anything_moves(monkeypatch):
+    from edifice_amd import blocks
+    monkeypatch.setattr(fs, "paged_extend", lambda *a: (_ for _ in ()).throw(AssertionError("made room")))
+    m, c = _cache()
+    with pytest.raises(ValueError, match="pages for all"):
+        m.go_on(torch.zeros(2, 13, 32), c)
+    with pytest.raises(ValueError, match="x must be"):
+        m.go_on(torch.zeros(2, 3, 31), c)
+    wide = blocks.build("gqa", embed_size=32, hidden_size=320, num_heads=2)
+    for tokens in (1, 2):
+        with pytest.raises(ValueError, match="head_dim"):
+            wide.go_on(torch.zeros(2, tokens, 32), wide.paged_cache(2, 8))
+    with pytest.raises(ValueError, match="rows, embed"):
+        m.packed(torch.zeros(1, 4, 32), OFF)
+    with pytest.raises(ValueError, match="attention blocks"):
+        blocks.build("mamba", embed_size=32).packed(torch.zeros(4, 32), OFF)
+
+
+def test_eight_bit_cache_of_a_model():
+    m, c = _cache(dtype=torch.int8)
+    assert c.k[0].dtype == torch.int8 and c.k_scale[0].shape == (6, 2) and c.k_scale[0].dtype == torch.float32
+    assert _cache()[1].k_scale[0] is None
+    with pytest.raises(EdificeHipError, match="GPU tensors"):
+        m.step(torch.zeros(2, 1, 32), c)  # the cache fits the model; the ops take no CPU tensors
+    with pytest.raises(ValueError, match="the cache holds"):
+        m.step(torch.zeros(2, 1, 32), _cache(dtype=torch.bfloat16)[1])
