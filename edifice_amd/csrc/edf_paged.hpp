@@ -82,34 +82,7 @@ struct KVTile {
     f.load(t + off(r, col));
     return f;
   }
-  // o += V^T P^T for dims 16 dt + i; p: N bf16 parts, largest first, of the lane's 4 NT probabilities
-  template <int N>
-  EDF_DEVICE static f32x4 pv_parts(const bf16* t, int dt, int g, int i, const bf16 (*p)[4 * NT], f32x4 o) {
-    typedef __attribute__((ext_vector_type(4))) short s16x4;
-    const int row = 4 * g + (i >> 2), col = 16 * dt + 4 * (i & 3);
-    const bf16x4 v0 = lds_read_tr16(t + off(row, col));
-    if constexpr (NT == 2) {
-      const bf16x8 v = cat4(v0, lds_read_tr16(t + off(row + 16, col)));
-#pragma unroll
-      for (int n = N - 1; n >= 0; --n) {
-        bf16x8 x;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = p[n][e];
-        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, x, o, 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int n = N - 1; n >= 0; --n) {
-        bf16x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = p[n][e];
-        o = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, v0), __builtin_bit_cast(s16x4, x), o, 0, 0,
-                                                      0);
-      }
-    }
-    return o;
-  }
-  // the same; p: the probabilities, in bf16 taken in two parts
+  // o += V^T P^T for dims 16 dt + i; p: the lane's 4 NT probabilities
   EDF_DEVICE static f32x4 pv(const T* t, int dt, int g, int i, const float* p, f32x4 o) {
     if constexpr (sizeof(T) == 2) {
       const int row = 4 * g + (i >> 2), col = 16 * dt + 4 * (i & 3);

@@ -3,11 +3,14 @@
 // model's type:
 //   s_j = (q . c_j) ks / sqrt(d),  o = sum_j softmax_j(s) vs c'_j,   codes c, c', scales ks, vs of key j's page.
 //
-// Half the bytes of a bf16 cache, and bound by them.  The codes are exact in bf16, so the matrix products run on bf16
-// operands and the scales multiply scores and probabilities, one of each a key: the codes go to bf16 on their way into the
-// wave's LDS tiles (half an instruction an element for e4m3, two for whole numbers) and no dequantised value is formed.
-// float32 queries and probabilities go through the same products in three bf16 parts each (off by 2^-24), bf16 queries in
-// one and probabilities in two (2^-16), so the results' own rounding is the one that shows.
+// Half the bytes of a bf16 cache, and bound by them.  The codes are exact in float16, so the matrix products run on float16
+// operands and the scales multiply scores and probabilities, one of each a key; no dequantised value is formed.
+//   Keys go from memory to the matrix operand: a lane's 16 codes of each 64 of a row are 16 columns of the contraction,
+//   and the query has the same order.  A tile's rows are read whole by four lanes each.
+//   Values become float16 on their way into the wave's LDS tile, from where transposed reads take them.
+// Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, P vs by 2^15 over the largest vs so far (a power
+// of two that the running maximum's rescaling takes along), so that float16's range holds them to 2^-39 of the largest.
+// bf16 queries are exact in it; float32 ones, and P vs, go through the products in two parts, off by 2^-23 of themselves.
 // Tiles, chunks and joins are paged_attn.hip's.
 #include <math.h>
 #include <stdint.h>
@@ -20,12 +23,18 @@
 namespace edf {
 namespace {
 
-// 16 codes of a row from column col on, zeros past d.  VEC: d a multiple of 16 and the cache aligned to 16.
-template <int HD, bool VEC>
+// How rows are read: element by element, in pieces of 16 codes (d a multiple of 16, the cache aligned to 16), or in pieces
+// with d = HD (no code past d).
+enum { BY_ELEMENT, BY_PIECE, WHOLE };
+
+// 16 codes of a row from column col on, zeros past d
+template <int HD, int MODE>
 EDF_DEVICE u32x4 code_piece(const unsigned char* row, int col, int d) {
-  if constexpr (VEC) {
+  if constexpr (MODE == WHOLE) {
+    return *(const u32x4*)(row + col);
+  } else if constexpr (MODE == BY_PIECE) {
     u32x4 c = *(const u32x4*)(row + min(col, d - 16));
-    if (d < HD && col >= d) c = u32x4{0, 0, 0, 0};
+    if (col >= d) c = u32x4{0, 0, 0, 0};
     return c;
   } else {
     u32x4 c = {0, 0, 0, 0};
@@ -35,35 +44,35 @@ EDF_DEVICE u32x4 code_piece(const unsigned char* row, int col, int d) {
   }
 }
 
-// 8 codes as bf16, exactly
-template <int C>
-EDF_DEVICE bf16x8 codes_bf16(unsigned lo, unsigned hi) {
-  float f[8];
-  Codes<C>::unpack4(lo, f);
-  Codes<C>::unpack4(hi, f + 4);
-  const u32x4 p = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
-  return __builtin_bit_cast(bf16x8, p);
-}
-
-// x as the sum of N bf16 numbers, largest first
+// x as the sum of N float16 numbers, largest first
 template <int N, typename F>
-EDF_DEVICE void bf16_parts(float x, F put) {
+EDF_DEVICE void half_parts(float x, F put) {
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    const bf16 y = (bf16)x;
+    const _Float16 y = (_Float16)x;
     put(p, y);
     x -= (float)y;
   }
 }
+EDF_DEVICE f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-template <typename T, int C, int HD, bool VEC>
-__global__ __launch_bounds__(256, 2) void paged_attn8_kernel(PagedArgs a) {
+// A wave's values in LDS, float16: a block for each 16 columns, of rows of 48 bytes (16 columns and padding), so that a
+// lane's addresses are one base and constants.  16 lanes write 16 bytes each to 16 places of the 64 banks: they hold 64 / HD
+// of a row's pieces of each of HD / 64 .. 4 rows, and the blocks' distances are chosen by that.
+template <int HD, int KEYS>
+struct ValueTile {
+  static constexpr int ROW = 24, BLOCK = KEYS * ROW + (HD <= 64 ? 32 : HD <= 128 ? 48 : 8), ELEMS = HD / 16 * BLOCK;
+};
+
+template <typename T, int C, int HD, int MODE>
+__global__ __launch_bounds__(256, (sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 2) : 2)) void paged_attn8_kernel(PagedArgs a) {
   constexpr int NT = HD > 128 ? 1 : 2, KEYS = 16 * NT, STEP = PA_WAVES * KEYS;
   constexpr int NKK = HD / 32, NDT = HD / 16;
   constexpr int CPR = HD / 16, NV = KEYS * CPR / 64;  // pieces of 16 codes per row, and per lane of a tile
-  constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;  // bf16 parts of a query and of P
-  using Tile = KVTile<bf16, HD, NT>;
-  constexpr int TILE_BYTES = 2 * Tile::ELEMS * 2, OUT_BYTES = 16 * (HD + 4) * 4;
+  constexpr int NK = HD / 64;                         // pieces of a key that a lane reads
+  constexpr int QP = sizeof(T) == 2 ? 1 : 2, PP = 2;  // float16 parts of a query and of P vs
+  using Tile = ValueTile<HD, KEYS>;
+  constexpr int TILE_BYTES = Tile::ELEMS * 2, OUT_BYTES = 16 * (HD + 4) * 4;
   constexpr int WAVE_BYTES = TILE_BYTES > OUT_BYTES ? TILE_BYTES : OUT_BYTES;
   __shared__ __attribute__((aligned(16))) char smem[PA_WAVES * WAVE_BYTES];
   __shared__ __attribute__((aligned(16))) float sS[PA_WAVES][2][KEYS];
@@ -82,77 +91,119 @@ __global__ __launch_bounds__(256, 2) void paged_attn8_kernel(PagedArgs a) {
   const int skip = lo - ns;
   const int n1 = min((split + 1) * a.chunk, nvis);  // this workgroup's keys: split * chunk .. n1 - 1
 
-  Frag<bf16> qf[QP][NKK];
-#pragma unroll
-  for (int kk = 0; kk < NKK; ++kk) {
+  // The contraction takes a key's columns in the order in which a lane reads them: its group's 16 of each 64.
+  f16x8 qf[QP][NKK];
+  float qscale;  // what a score is multiplied by for the query's power of two
+  {
     const T* q = (const T*)a.q + ((long)b * a.Hq + hq0 + min(i, nq - 1)) * a.d;
+    float x[NKK][8], top = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int col = 32 * kk + 8 * g + e;
-      const float x = to_f32(q[min(col, a.d - 1)]);
-      bf16_parts<QP>(i < nq && col < a.d ? x : 0.0f, [&](int p, bf16 y) { qf[p][kk].v[e] = y; });
+    for (int kk = 0; kk < NKK; ++kk) {
+      const int col = 64 * (kk >> 1) + 16 * g + 8 * (kk & 1);
+      if constexpr (MODE == WHOLE) {
+        typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T piece;
+#pragma unroll
+        for (int n = 0; n < (int)sizeof(T) / 2; ++n) {
+          const piece p = *(const piece*)(q + col + 4 * n);
+#pragma unroll
+          for (int e = 0; e < 16 / (int)sizeof(T); ++e) x[kk][4 * n + e] = to_f32(p[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = to_f32(q[min(col + e, a.d - 1)]);
+          x[kk][e] = col + e < a.d ? y : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[kk][e]));
     }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    int e0;
+    frexpf(top, &e0);
+    const int up = top > 0.0f && top < INFINITY ? 15 - e0 : 0;
+    qscale = ldexpf(1.0f, -up);
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        half_parts<QP>(i < nq ? ldexpf(x[kk][e], up) : 0.0f, [&](int p, _Float16 y) { qf[p][kk][e] = y; });
   }
   f32x4 o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, lsum = 0.0f;
+  int ve = -100;  // o is in units of 2^(ve - 15), 2^ve the least power of two above every vs so far
 
-  // Page and head [num_blocks Hkv] of visible key n, or -1, and its row within the page; one key a lane, repeated every
-  // KEYS lanes.
+  // Page and head [num_blocks Hkv] of visible key n, or -1, and its row of the cache; one key a lane, repeated every KEYS
+  // lanes.
   const int* tb = a.table + (long)b * a.width;
   struct Place {
-    int at, off;
+    int at, row;
   };
   auto place_of = [&](int nbase) {
     const int n = nbase + (l & (KEYS - 1));
     const int key = a.window > 0 ? n + (n >= ns ? skip : 0) : n;
     const int c = key / a.block;
     const int page = tb[min(c, a.width - 1)];
-    return Place{n < n1 && page >= 0 && page < a.num_blocks ? page * a.Hkv + h : -1, key - c * a.block};
+    const bool there = n < n1 && page >= 0 && page < a.num_blocks;
+    const int at = there ? page * a.Hkv + h : -1;
+    return Place{at, there ? at * a.block + (key - c * a.block) : 0};
   };
   const unsigned char *K = (const unsigned char*)a.kc, *V = (const unsigned char*)a.vc;
-  u32x4 kr[NV], vr[NV];
+  u32x4 kr[NT][NK], vr[NV];
   float ksr = 0.0f, vsr = 0.0f;
-  auto load_tile = [&](Place p) {  // an absent key reads row 0: it is masked and its value zeroed
-    const int rows = p.at < 0 ? 0 : p.at * a.block + p.off;
+  // an absent key reads row 0: it is masked and its value zeroed
+  auto load_k = [&](Place p) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const long r = __shfl(p.row, 16 * t + i);
+#pragma unroll
+      for (int n = 0; n < NK; ++n) kr[t][n] = code_piece<HD, MODE>(K + r * a.d, 64 * n + 16 * g, a.d);
+    }
+    ksr = a.ks[max(p.at, 0)];
+  };
+  auto load_v = [&](Place p) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       const int c = l + 64 * n;
-      const long r = __shfl(rows, c / CPR);
-      kr[n] = code_piece<HD, VEC>(K + r * a.d, c % CPR * 16, a.d);
-      vr[n] = code_piece<HD, VEC>(V + r * a.d, c % CPR * 16, a.d);
+      const long r = __shfl(p.row, c / CPR);
+      vr[n] = code_piece<HD, MODE>(V + r * a.d, c % CPR * 16, a.d);
     }
-    ksr = a.ks[max(p.at, 0)];
     vsr = a.vs[max(p.at, 0)];
   };
-  bf16* sk = reinterpret_cast<bf16*>(smem + w * WAVE_BYTES);
-  bf16* sv = sk + Tile::ELEMS;
+  _Float16* sv = reinterpret_cast<_Float16*>(smem + w * WAVE_BYTES);
+  _Float16* sput = sv + l % CPR * Tile::BLOCK + l / CPR * Tile::ROW;  // this lane's first piece
+  const bf16* sget = (const bf16*)sv + (4 * g + (i >> 2)) * Tile::ROW + 4 * (i & 3);
   int nb = split * a.chunk + KEYS * w;
   Place here = place_of(nb);
-  if (nb < n1) load_tile(here);
+  if (nb < n1) {
+    load_k(here);
+    load_v(here);
+  }
   Place next = place_of(nb + STEP);
   for (; nb < n1; nb += STEP) {
     const unsigned long long live = __ballot(here.at >= 0);  // bit k (repeated): key k of the tile
-    // absent keys' values and scales as zeros, since a masked P of 0 would keep a NaN
+    const bool more = nb + STEP < n1;
+    if (live != ~0ull) {  // absent keys' values and scales as zeros, since a masked P of 0 would keep a NaN
+#pragma unroll
+      for (int n = 0; n < NV; ++n)
+        if (!((live >> ((l + 64 * n) / CPR)) & 1)) vr[n] = u32x4{0, 0, 0, 0};
+      if (here.at < 0) ksr = vsr = 0.0f;
+    }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      const int c = l + 64 * n, row = c / CPR, col = c % CPR * 16;
-      if (live != ~0ull && !((live >> row) & 1)) vr[n] = u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        *(bf16x8*)(sk + Tile::off(row, col + 8 * e)) = codes_bf16<C>(kr[n][2 * e], kr[n][2 * e + 1]);
-        *(bf16x8*)(sv + Tile::off(row, col + 8 * e)) = codes_bf16<C>(vr[n][2 * e], vr[n][2 * e + 1]);
-      }
+      _Float16* to = sput + 64 / CPR * n * Tile::ROW;
+      *(f16x8*)to = Codes<C>::half8(vr[n][0], vr[n][1]);
+      *(f16x8*)(to + 8) = Codes<C>::half8(vr[n][2], vr[n][3]);
     }
     if (l < KEYS) {
-      sS[w][0][l] = here.at >= 0 ? ksr * a.scale_log2 : 0.0f;
-      sS[w][1][l] = here.at >= 0 ? vsr : 0.0f;
+      sS[w][0][l] = ksr * a.scale_log2;
+      sS[w][1][l] = vsr;
     }
-    here = next;
-    if (nb + STEP < n1) load_tile(here);
-    next = place_of(nb + 2 * STEP);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (more) load_v(next);
+    __builtin_amdgcn_sched_barrier(0);
     f32x4 s[NT], vs[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -160,55 +211,85 @@ __global__ __launch_bounds__(256, 2) void paged_attn8_kernel(PagedArgs a) {
     for (int kk = 0; kk < NKK; ++kk)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const Frag<bf16> kf = Tile::row(sk, 16 * t + i, 32 * kk + 8 * g);
+        const f16x8 kf = Codes<C>::half8(kr[t][kk >> 1][2 * (kk & 1)], kr[t][kk >> 1][2 * (kk & 1) + 1]);
 #pragma unroll
-        for (int p = QP - 1; p >= 0; --p) s[t] = Frag<bf16>::mma(kf, qf[p][kk], s[t]);
+        for (int p = QP - 1; p >= 0; --p) s[t] = mfma16(kf, qf[p][kk], s[t]);
       }
-    float mx = -INFINITY;
+    if (more) load_k(next);
+    here = next;
+    next = place_of(nb + 2 * STEP);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    float mx = -INFINITY, vx = 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      s[t] *= *(const f32x4*)(&sS[w][0][16 * t + 4 * g]);
+      s[t] *= *(const f32x4*)(&sS[w][0][16 * t + 4 * g]) * qscale;
       vs[t] = *(const f32x4*)(&sS[w][1][16 * t + 4 * g]);
+      if (live != ~0ull) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[t][r] = (live >> (16 * t + 4 * g + r)) & 1 ? s[t][r] : -INFINITY;
+      }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if (live != ~0ull) s[t][r] = (live >> (16 * t + 4 * g + r)) & 1 ? s[t][r] : -INFINITY;
         mx = fmaxf(mx, s[t][r]);
+        vx = fmaxf(vx, vs[t][r]);
       }
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
+    vx = fmaxf(vx, __shfl_xor(vx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
+    vx = fmaxf(vx, __shfl_xor(vx, 32));
     const float mnew = fmaxf(m, mx);
     const float mns = mnew == -INFINITY ? 0.0f : mnew;
-    if (__any(mnew > m)) {
-      const float alpha = fast_exp2(m - mns);
+    const int venew = max(ve, __builtin_amdgcn_frexp_expf(vx));  // that of 0 is 0, of a wave without keys, or of zeros alone
+    if (__any(mnew > m || venew > ve)) {
+      const float alpha = fast_exp2(m - mns), beta = ldexpf(alpha, ve - venew);
       lsum *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
+        for (int r = 0; r < 4; ++r) o[dt][r] *= beta;
     }
     m = mnew;
+    ve = venew;
     float rs = 0.0f;
-    bf16 pf[PP][4 * NT];
+    f16x4 pf[PP][NT];
 #pragma unroll
     for (int e = 0; e < 4 * NT; ++e) {
       const float p = fast_exp2(s[e >> 2][e & 3] - mns);
       rs += p;
-      bf16_parts<PP>(p * vs[e >> 2][e & 3], [&](int n, bf16 y) { pf[n][e] = y; });
+      half_parts<PP>(p * ldexpf(vs[e >> 2][e & 3], 15 - ve), [&](int n, _Float16 y) { pf[n][e >> 2][e & 3] = y; });
     }
     rs += __shfl_xor(rs, 16);
     lsum += rs + __shfl_xor(rs, 32);
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) o[dt] = Tile::template pv_parts<PP>(sv, dt, g, i, pf, o[dt]);
+    for (int dt = 0; dt < NDT; ++dt) {
+      const f16x4 v0 = __builtin_bit_cast(f16x4, lds_read_tr16(sget + dt * Tile::BLOCK));
+      if constexpr (NT == 2) {
+        const f16x4 v1 = __builtin_bit_cast(f16x4, lds_read_tr16(sget + dt * Tile::BLOCK + 16 * Tile::ROW));
+        const f16x8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int n = PP - 1; n >= 0; --n)
+          o[dt] = mfma16(v, __builtin_shufflevector(pf[n][0], pf[n][1], 0, 1, 2, 3, 4, 5, 6, 7), o[dt]);
+      } else {
+#pragma unroll
+        for (int n = PP - 1; n >= 0; --n) o[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(v0, pf[n][0], o[dt], 0, 0, 0);
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[dt][r] = ldexpf(o[dt][r], ve - 15);
   join_waves<T, HD, WAVE_BYTES>(a, smem, sML, o, m, lsum, b, hq0, nq, split);
 }
 
 template <typename T, int C, int HD>
 void launch_paged8(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
-  if (vec) paged_attn8_kernel<T, C, HD, true><<<grid, 256, 0, s>>>(a);
-  else paged_attn8_kernel<T, C, HD, false><<<grid, 256, 0, s>>>(a);
+  if (vec && a.d == HD && !((uintptr_t)a.q & 15)) paged_attn8_kernel<T, C, HD, WHOLE><<<grid, 256, 0, s>>>(a);
+  else if (vec) paged_attn8_kernel<T, C, HD, BY_PIECE><<<grid, 256, 0, s>>>(a);
+  else paged_attn8_kernel<T, C, HD, BY_ELEMENT><<<grid, 256, 0, s>>>(a);
 }
 template <typename T, int C>
 void launch_paged8_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
