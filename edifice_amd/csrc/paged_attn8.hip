@@ -184,12 +184,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <=
   }
   Place next = place_of(nb + STEP);
   for (; nb < n1; nb += STEP) {
-    const unsigned long long live = __ballot(here.at >= 0);  // bit k (repeated): key k of the tile
+    const unsigned live = (unsigned)__ballot(here.at >= 0);  // bit k (repeated): key k of the tile
     const bool more = nb + STEP < n1;
-    if (live != ~0ull) {  // absent keys' values and scales as zeros, since a masked P of 0 would keep a NaN
+    if (live != ~0u) {  // absent keys' values and scales as zeros, since a masked P of 0 would keep a NaN
+      const unsigned mine = live >> (l / CPR);  // from this lane's first row on
 #pragma unroll
       for (int n = 0; n < NV; ++n)
-        if (!((live >> ((l + 64 * n) / CPR)) & 1)) vr[n] = u32x4{0, 0, 0, 0};
+        if (!(mine & (1u << 64 / CPR * n))) vr[n] = u32x4{0, 0, 0, 0};
       if (here.at < 0) ksr = vsr = 0.0f;
     }
 #pragma unroll
@@ -225,9 +226,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <=
     for (int t = 0; t < NT; ++t) {
       s[t] *= *(const f32x4*)(&sS[w][0][16 * t + 4 * g]) * qscale;
       vs[t] = *(const f32x4*)(&sS[w][1][16 * t + 4 * g]);
-      if (live != ~0ull) {
+      if (live != ~0u) {
+        const unsigned mine = live >> (4 * g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[t][r] = (live >> (16 * t + 4 * g + r)) & 1 ? s[t][r] : -INFINITY;
+        for (int r = 0; r < 4; ++r) s[t][r] = mine & (1u << (16 * t + r)) ? s[t][r] : -INFINITY;
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
