@@ -201,6 +201,229 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
     a.lse[row] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
 }
 
+// bf16 at head_dim 128: the same decomposition with tiles moved by 16-byte DMA loads into half-row-block LDS
+// tiles (stage_hb: no staging registers, fragment addresses are bases plus immediates), two workgroups per CU,
+// and K one tile ahead of V: the matrix products of the next tile's scores run between the exponentials of the
+// current one wherever both are whole.
+__global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
+  constexpr int HD = 128, BN = 64, NKK = HD / 16, NDT = HD / 32;
+  // X0 = {K buffer 0, V buffer 1}, X1 = {K buffer 1, V buffer 0}: iteration t (parity B) writes only X_B
+  __shared__ __attribute__((aligned(16))) bf16 sX0[2 * BN * HD];
+  __shared__ __attribute__((aligned(16))) bf16 sX1[2 * BN * HD];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  QueryTile<BN> qt(a);
+  if (qt.none) return;
+  const KeyTiles<PK_M, BN> kt = qt.tiles(a);
+  if (qt.none) return;
+  const int pw = qt.first + 32 * w + qt.ahead(), myp = pw + li;  // positions
+  const int qw = qt.first + 32 * w, myq = qw + li;                // queries within the text
+  const long row0 = (long)qt.head * a.N + qt.qrow;
+  const bf16* Qrow = (const bf16*)a.q + (row0 + min(myq, qt.nq - 1)) * HD;
+  const long kvbase = ((long)(qt.head / a.G) * a.M + qt.krow) * HD;
+  // buffer resources over the text's keys: rows past its end read as zeros (their scores are masked)
+  const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)qt.nk * HD * 2);
+  const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)qt.nk * HD * 2);
+
+  bf16x8 qf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) qf[kk] = *(const bf16x8*)(Qrow + kk * 16 + 8 * g);
+  f32x16 o[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
+  float m = -INFINITY, lsum = 0.0f;
+
+  const int grp = l >> 4, i16 = l & 15;
+  const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
+  const int krow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
+  const int vtr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
+  const int nkt = qt.t1 - qt.t0, whole = in_vector_register(max(kt.first_whole - qt.t0, 0));
+  auto key0 = [&](int t) __attribute__((always_inline)) { return kt.key0(qt.t0 + t); };
+  auto visible = [&](int t) __attribute__((always_inline)) {
+    const int k0 = key0(t);
+    return (k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks;
+  };
+  auto issue_k = [&](auto bt, int t) __attribute__((always_inline)) {
+    stage_hb<BN>(rK, decltype(bt)::value ? sX1 : sX0, key0(t), wu, l);
+  };
+  auto issue_v = [&](auto bt, int t) __attribute__((always_inline)) {
+    stage_hb<BN>(rV, (decltype(bt)::value ? sX0 : sX1) + BN * HD, key0(t), wu, l);
+  };
+  auto scores = [&](auto bt, f32x16* s) __attribute__((always_inline)) {
+    const bf16* sk = decltype(bt)::value ? sX1 : sX0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = zero16();
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk)
+        s[h] = mfma32(*(const bf16x8*)(&sk[krow[kk & 1] + hb_row_off<BN>(kk, 32 * h)]), qf[kk], s[h]);
+    }
+  };
+  f32x16 sc[2], sn[2];  // scores of the current and the next tile
+  // first half of the softmax: mask, row maximum, rescale; the maximum in scaled log2 units
+  auto softmax_max = [&](f32x16* s, int t, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(masked)::value;
+    const SeesKey sees(myp, key0(t) + 4 * g, a.W, a.sinks);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        if constexpr (MASK) s[h][r] = sees(h * 32 + d_row(r, 0)) ? s[h][r] : -INFINITY;
+        mx = fmaxf(mx, s[h][r]);
+      }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    // O and the sum refer to a maximum that is moved only when a score exceeds it by a factor of 2^8: p <= 256
+    // loses nothing in float32 or bf16
+    if (__any(mx * a.scale_log2 > m * a.scale_log2 + 8.0f)) {
+      const float mnew = fmaxf(m, mx);
+      const float alpha = fast_exp2(m * a.scale_log2 - (mnew == -INFINITY ? 0.0f : mnew * a.scale_log2));
+      lsum *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+      m = mnew;
+    }
+    return m == -INFINITY ? 0.0f : m * a.scale_log2;
+  };
+  // second half for elements 2 j, 2 j + 1: p into the row sum and the P^T fragments.  pin: an empty volatile asm
+  // keeps this arithmetic in the scheduling step that issued it.
+  auto softmax_pair = [&](f32x16* s, int j, float mns, float& rs, bf16x8* pf, auto pin) __attribute__((always_inline)) {
+    const int h = j >> 3, r = (2 * j) & 15;
+    const float p0 = fast_exp2(fmaf(s[h][r], a.scale_log2, -mns)), p1 = fast_exp2(fmaf(s[h][r + 1], a.scale_log2, -mns));
+    unsigned pk = pack_bf16x2(p0, p1);
+    // the row sum of the bf16 P that the product consumes, one dot2 per pair
+    rs = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), bf16x2{(bf16)1.0f, (bf16)1.0f}, rs, false);
+    if constexpr (decltype(pin)::value) asm volatile("" : "+v"(pk), "+v"(rs));
+    const int kc = 2 * h + (r >> 3), it = r & 7;
+    const bf16x2 pp = __builtin_bit_cast(bf16x2, pk);
+    pf[kc][it] = pp[0];
+    pf[kc][it + 1] = pp[1];
+  };
+  // O^T += V^T P^T: consecutive products go to different accumulators, V^T is read three steps ahead
+  auto pv_mma = [&](auto bt, const bf16x8* pf) __attribute__((always_inline)) {
+    const bf16* sv = (decltype(bt)::value ? sX0 : sX1) + BN * HD;
+    auto vfrag = [&](int j) __attribute__((always_inline)) {
+      const int o16 = hb_tr_off<BN>(j & 3, j >> 2, 0);
+      return cat4(lds_read_tr16(&sv[vtr[0] + o16]), lds_read_tr16(&sv[vtr[1] + o16]));
+    };
+    bf16x8 v[3] = {vfrag(0), vfrag(1), vfrag(2)};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      o[j & 3] = mfma32(v[j % 3], pf[j >> 2], o[j & 3]);
+      if (j + 3 < 16) v[j % 3] = vfrag(j + 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto consume = [&](auto bt, f32x16* s, int t, auto masked) __attribute__((always_inline)) {
+    const float mns = softmax_max(s, t, masked);
+    float rs = 0.0f;
+    bf16x8 pf[4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) softmax_pair(s, j, mns, rs, pf, std::false_type{});
+    lsum += rs + __shfl_xor(rs, 32);
+    pv_mma(bt, pf);
+  };
+  // whole tile t with a successor: the 16 products of S(t + 1) alternate with the exponentials of S(t)
+  auto fused = [&](auto bt, int t) __attribute__((always_inline)) {
+    const bf16* sk = decltype(bt)::value ? sX0 : sX1;
+    const float mns = softmax_max(sc, t, std::false_type{});
+    auto kfrag = [&](int i) __attribute__((always_inline)) {
+      const int kk = i >> 1;
+      return *(const bf16x8*)(&sk[krow[kk & 1] + hb_row_off<BN>(kk, 32 * (i & 1))]);
+    };
+    bf16x8 fr[4] = {kfrag(0), kfrag(1), kfrag(2), kfrag(3)};
+    sn[0] = zero16();
+    sn[1] = zero16();
+    float rs = 0.0f;
+    bf16x8 pf[4];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      sn[i & 1] = mfma32(fr[i & 3], qf[i >> 1], sn[i & 1]);
+      if (i + 4 < 16) fr[i & 3] = kfrag(i + 4);
+      softmax_pair(sc, i, mns, rs, pf, std::true_type{});
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    lsum += rs + __shfl_xor(rs, 32);
+    pv_mma(bt, pf);
+  };
+  const std::integral_constant<int, 0> b0{};
+  const std::integral_constant<int, 1> b1{};
+  if (nkt > 0) {
+    issue_k(b0, 0);
+    issue_v(b0, 0);
+  }
+  wait_vm();
+  if (nkt > 1) issue_k(b1, 1);
+  __syncthreads();  // K(0), V(0) visible
+  if (nkt > 0 && visible(0)) scores(b0, sc);
+  wait_vm();
+  __syncthreads();  // K(1) visible, K buffer 0 free
+  // iteration t (buffer parity B = t % 2): K(t + 2) into K buffer B, V(t + 1) into V buffer 1 - B
+  auto step = [&](auto bt, int t) __attribute__((always_inline)) {
+    const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
+    if (t + 2 < nkt) issue_k(bt, t + 2);
+    if (t + 1 < nkt) issue_v(ot, t + 1);
+    const bool next = t + 1 < nkt;
+    if (t >= whole && next) {
+      fused(bt, t);
+    } else {
+      if (next && visible(t + 1)) scores(ot, sn);
+      if (t >= whole) consume(bt, sc, t, std::false_type{});
+      else if (visible(t)) consume(bt, sc, t, std::true_type{});
+    }
+    wait_vm();
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) sc[h] = sn[h];
+  };
+  for (int t = 0; t < nkt; t += 2) {
+    step(b0, t);
+    if (t + 1 < nkt) step(b1, t + 1);
+  }
+
+  if (a.chunks > 1) {
+    if (myq >= qt.nq) return;
+    const long at = (long)qt.chunk * a.H * a.N + row0 + myq;
+    float* out = a.part + at * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
+            f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
+    if (g == 0) {
+      a.ml[2 * at] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[2 * at + 1] = lsum;
+    }
+    return;
+  }
+  // O through the free array X0 (each wave its 32 rows), written as whole rows
+  bf16* so = sX0 + w * 32 * HD;
+  const float inv = myq >= qt.nq || lsum == 0.0f ? 0.0f : 1.0f / lsum;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (bf16)(o[dt][rb * 4 + e] * inv);
+      *(bf16x4*)(so + lds_off<HD>(li, dt * 32 + 8 * rb + 4 * g)) = v;
+    }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int e = l + 64 * i, row = e / 16, ch = e % 16;
+    if (qw + row < qt.nq)
+      *(bf16x8*)((bf16*)a.out + (row0 + qw + row) * HD + 8 * ch) = *(const bf16x8*)(so + lds_off<HD>(row, 8 * ch));
+  }
+  if (myq < qt.nq && g == 0 && a.lse != nullptr)
+    a.lse[row0 + myq] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
+}
+
 // The chunks of 32 rows joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, a row by eight lanes of four elements
 // at a time.
 template <typename T, int HD, int BN>
@@ -260,7 +483,14 @@ template <typename T, int HD, int BN, bool VEC>
 int launch_fwd(hipStream_t s, PackArgs a) {
   const long grid = (long)a.H * a.nx * a.chunks;
   a.ml = a.part + (size_t)a.chunks * a.H * a.N * HD;
-  packed_fwd_kernel<T, HD, BN, VEC><<<(unsigned)grid, 256, 0, s>>>(a);
+  bool done = false;
+  if constexpr (sizeof(T) == 2 && HD == 128 && VEC) {
+    if (a.d == 128) {
+      packed_fwd128_kernel<<<(unsigned)grid, 256, 0, s>>>(a);
+      done = true;
+    }
+  }
+  if (!done) packed_fwd_kernel<T, HD, BN, VEC><<<(unsigned)grid, 256, 0, s>>>(a);
   if (a.chunks > 1) packed_join_kernel<T, HD, BN><<<(unsigned)(a.H * a.nx * 4), 256, 0, s>>>(a);
   return check_launch("packed attention");
 }

@@ -153,6 +153,125 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     }
 }
 
+// dQ, bf16 at head_dim 128: tiles by DMA loads, each as two 32-key halves so that one half's S and dP are live;
+// two workgroups per CU, so one wave's exponentials and waits overlap another's products.
+__global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
+  constexpr int HD = 128, BN = 64, NKK = HD / 16, NDT = HD / 32;
+  __shared__ __attribute__((aligned(16))) bf16 sR0[2 * BN * HD];  // ring slot: K then V
+  __shared__ __attribute__((aligned(16))) bf16 sR1[2 * BN * HD];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  int x, head;
+  packed_block(a, a.nx, x, head);
+  const TextTile tt = find_tile(a.qo, a.S, a.N, a.nx - 1 - x);
+  if (tt.first >= tt.n) return;
+  int kbegin, nk;
+  text_rows(a.ko, a.S, a.M, tt.text, kbegin, nk);
+  const int p0 = tt.first + nk - tt.n, pw = p0 + 32 * w, myp = pw + li, myq = tt.first + 32 * w + li;
+  const long qrow = (long)head * a.N + tt.row0 + min(myq, tt.n - 1);
+  const long kvbase = ((long)(head / a.G) * a.M + kbegin) * HD;
+  const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)nk * HD * 2);
+  const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)nk * HD * 2);
+
+  bf16x8 qf[NKK], of[NKK];
+  float dd = 0.0f;
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk) {
+    const long at = qrow * HD + kk * 16 + 8 * g;
+    qf[kk] = *(const bf16x8*)((const bf16*)a.q + at);
+    of[kk] = *(const bf16x8*)((const bf16*)a.go + at);
+    const bf16x8 ov = *(const bf16x8*)((const bf16*)a.o + at);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)ov[e], dd);
+  }
+  dd += __shfl_xor(dd, 32);
+  const float lse = a.lse[qrow] * LOG2E;
+  if (g == 0 && myq < tt.n) a.dd[qrow] = dd;
+  f32x16 dq[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
+
+  const int grp = l >> 4, i16 = l & 15;
+  const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
+  const int krow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
+  const int ktr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
+  const KeyTiles<PK_M, BN> kt(p0, nk, a.W, a.sinks);
+  const int count = p0 + PK_M > 0 ? max(kt.count, 0) : 0;
+  const int whole = in_vector_register(kt.first_whole);
+  auto issue = [&](auto bt, int t) {
+    constexpr int B = decltype(bt)::value;
+    const int k0 = kt.key0(t);
+    stage_hb<BN>(rK, B ? sR1 : sR0, k0, wu, l);
+    stage_hb<BN>(rV, (B ? sR1 : sR0) + BN * HD, k0, wu, l);
+  };
+  auto tile = [&](auto bt, int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const bf16* sK = decltype(bt)::value ? sR1 : sR0;
+    const bf16* sV = sK + BN * HD;
+    const int k0 = kt.key0(t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int kb = k0 + 32 * h;
+      if (MASK && !((kb <= pw + 31 && kb + 32 + a.W > pw + 1) || kb < a.sinks)) continue;  // no visible pair
+      const SeesKey sees(myp, kb + 4 * g, a.W, a.sinks);
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int kk = 0; kk < NKK; ++kk) {
+        const int off = krow[kk & 1] + hb_row_off<BN>(kk, 32 * h);
+        s = mfma32(*(const bf16x8*)(&sK[off]), qf[kk], s);
+        dp = mfma32(*(const bf16x8*)(&sV[off]), of[kk], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float x = fast_exp2(fmaf(s[r], a.scale_log2, -lse)) * (dp[r] - dd);
+        if constexpr (MASK) x = sees(d_row(r, 0)) ? x : 0.0f;
+        s[r] = x;
+      }
+      bf16x8 df[2];
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) df[kc][e] = (bf16)s[8 * kc + e];
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int kc = 0; kc < 2; ++kc) {
+          const int o = hb_tr_off<BN>(dt, kc, 32 * h);
+          dq[dt] = mfma32(cat4(lds_read_tr16(&sK[ktr[0] + o]), lds_read_tr16(&sK[ktr[1] + o])), df[kc], dq[dt]);
+        }
+    }
+  };
+  auto step = [&](auto bt, int t) {
+    const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
+    if (t + 1 < count) issue(ot, t + 1);
+    if (t >= whole) tile(bt, t, std::false_type{});
+    else tile(bt, t, std::true_type{});
+    wait_vm();
+    __syncthreads();
+  };
+  const std::integral_constant<int, 0> b0{};
+  const std::integral_constant<int, 1> b1{};
+  if (count > 0) issue(b0, 0);
+  wait_vm();
+  __syncthreads();
+  for (int t = 0; t < count; t += 2) {
+    step(b0, t);
+    if (t + 1 < count) step(b1, t + 1);
+  }
+  if (myq >= tt.n) return;
+  bf16* out = (bf16*)a.dq + qrow * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      bf16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = (bf16)(dq[dt][rb * 4 + e] * a.scale);
+      *(bf16x4*)(out + dt * 32 + 8 * rb + 4 * g) = v;
+    }
+}
+
 // The key block of a dK, dV workgroup and its share [t0, t1) of the block's (query head, tile of BQ queries) pairs: nt
 // tiles a head, from query qs of the text on.
 template <int BQ>
@@ -342,6 +461,174 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     }
 }
 
+// dK, dV, bf16 at head_dim 128: V is read from an LDS copy of the workgroup's 128 keys (its fragments would not
+// fit 256 registers beside the two accumulators), Q and dO come in 32-query tiles by DMA loads, two workgroups per
+// CU.
+__global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
+  constexpr int HD = 128, BQ = 32, NKK = HD / 16, NDT = HD / 32;
+  __shared__ __attribute__((aligned(16))) bf16 sV[PK_M * HD];
+  __shared__ __attribute__((aligned(16))) bf16 sR0[2 * BQ * HD];  // ring slot: Q then dO
+  __shared__ __attribute__((aligned(16))) bf16 sR1[2 * BQ * HD];
+  __shared__ __attribute__((aligned(16))) float sL0[BQ], sL1[BQ], sD0[BQ], sD1[BQ];
+
+  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
+  const int wu = __builtin_amdgcn_readfirstlane(w);
+  int x, head;  // of the key heads
+  packed_block(a, a.nx * a.chunks, x, head);
+  const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
+  if (kb.none) return;
+  const int kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
+  const long kbase = (long)head * a.M + kb.krow, krow = kbase + min(mykey, kb.nk - 1);
+
+  // keys past the text's end read zero rows of V: they only feed their own columns, never stored
+  stage_hb<PK_M>(make_rsrc((const bf16*)a.v + kbase * HD, (unsigned)kb.nk * HD * 2), sV, kb.first, wu, l);
+  bf16x8 kf[NKK];
+#pragma unroll
+  for (int kk = 0; kk < NKK; ++kk)
+    kf[kk] = *(const bf16x8*)((const bf16*)a.k + krow * HD + kk * 16 + 8 * g);
+  f32x16 dk[NDT], dv[NDT];
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt) {
+    dk[dt] = zero16();
+    dv[dt] = zero16();
+  }
+  float rl = 0.0f, rd = 0.0f;
+  // Tile t into ring slot B: Q and dO by DMA, row sums and D into registers of the first wave, which publish()
+  // writes to LDS once the tile's loads have landed.
+  auto issue = [&](auto bt, int t) {
+    constexpr int B = decltype(bt)::value;
+    const int h = t / nt, q0 = kb.qs + (t - h * nt) * BQ;
+    const long row = (long)(head * a.G + h) * a.N + kb.qrow;
+    stage_hb<BQ>(make_rsrc((const bf16*)a.q + row * HD, (unsigned)kb.nq * HD * 2), B ? sR1 : sR0, q0, wu, l);
+    stage_hb<BQ>(make_rsrc((const bf16*)a.go + row * HD, (unsigned)kb.nq * HD * 2), (B ? sR1 : sR0) + BQ * HD, q0, wu, l);
+    if (tid < BQ) {
+      const long q = row + min(q0 + tid, kb.nq - 1);
+      rl = q0 + tid < kb.nq ? a.lse[q] : INFINITY;  // a query past the end gets P = 0
+      rd = a.dd[q];
+    }
+  };
+  auto publish = [&](auto bt) {
+    constexpr int B = decltype(bt)::value;
+    wait_vm();
+    if (tid < BQ) {
+      (B ? sL1 : sL0)[tid] = rl * LOG2E;
+      (B ? sD1 : sD0)[tid] = rd;
+    }
+  };
+  const int grp = l >> 4, i16 = l & 15;
+  const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
+  const int qrow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
+  const int vrow[2] = {hb_row_base(li, g, 0) + hb_row_off<PK_M>(0, 32 * w),
+                       hb_row_base(li, g, 1) + hb_row_off<PK_M>(0, 32 * w)};
+  const int qtr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
+  auto subtile = [&](auto bt, int pb, auto masked) {
+    constexpr int B = decltype(bt)::value;
+    constexpr bool MASK = decltype(masked)::value;
+    const bf16* sQ = B ? sR1 : sR0;
+    const bf16* sO = sQ + BQ * HD;
+    // distinct barriers keep the two bodies' equal LDS reads from being hoisted above their branch
+    __builtin_amdgcn_sched_barrier(MASK ? 1 : 2);
+    f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const int off = qrow[kk & 1] + hb_row_off<BQ>(kk, 0);
+      const bf16x8 vf = *(const bf16x8*)(&sV[vrow[kk & 1] + hb_row_off<PK_M>(kk, 0)]);
+      s = mfma32(*(const bf16x8*)(&sQ[off]), kf[kk], s);
+      dp = mfma32(*(const bf16x8*)(&sO[off]), vf, dp);
+    }
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      const f32x4 lv = *(const f32x4*)(&(B ? sL1 : sL0)[8 * rb + 4 * g]);
+      const f32x4 dv4 = *(const f32x4*)(&(B ? sD1 : sD0)[8 * rb + 4 * g]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = rb * 4 + e;
+        float p = fast_exp2(fmaf(s[r], a.scale_log2, -lv[e]));
+        float x = p * (dp[r] - dv4[e]);
+        if constexpr (MASK) {
+          const bool see = window_sees(pb + 8 * rb + 4 * g + e, mykey, a.W, a.sinks);
+          p = see ? p : 0.0f;
+          x = see ? x : 0.0f;
+        }
+        s[r] = p;
+        dp[r] = x;
+      }
+    }
+    bf16x8 pf[2], df[2];
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        pf[kc][e] = (bf16)s[8 * kc + e];
+        df[kc][e] = (bf16)dp[8 * kc + e];
+      }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        const int o = hb_tr_off<BQ>(dt, kc, 0);
+        dv[dt] = mfma32(cat4(lds_read_tr16(&sO[qtr[0] + o]), lds_read_tr16(&sO[qtr[1] + o])), pf[kc], dv[dt]);
+        dk[dt] = mfma32(cat4(lds_read_tr16(&sQ[qtr[0] + o]), lds_read_tr16(&sQ[qtr[1] + o])), df[kc], dk[dt]);
+      }
+  };
+  auto step = [&](auto bt, int t) {
+    const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
+    if (t + 1 < t1) issue(ot, t + 1);
+    const int pb = kb.qs + t % nt * BQ + kb.ahead();  // position of the tile's first query
+    if (!(pb + 31 < kw || (pb > kw + 30 + a.W && kw >= a.sinks))) {  // some query sees a key of this wave
+      if (pb >= kw + 31 && pb + 31 - kw < a.W) subtile(bt, pb, std::false_type{});
+      else subtile(bt, pb, std::true_type{});
+    }
+    if (t + 1 < t1) publish(ot);
+    __syncthreads();
+  };
+  const std::integral_constant<int, 0> b0{};
+  const std::integral_constant<int, 1> b1{};
+  if (t0 < t1) {
+    issue(b0, t0);
+    publish(b0);
+  } else {
+    wait_vm();
+  }
+  __syncthreads();
+  for (int t = t0; t < t1; t += 2) {
+    step(b0, t);
+    if (t + 1 < t1) step(b1, t + 1);
+  }
+  if (a.chunks > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
+    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.chunks) * (2L * PK_M * HD) + (32 * w + li) * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) {
+        f32x4 u, v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u[e] = dk[dt][rb * 4 + e];
+          v[e] = dv[dt][rb * 4 + e];
+        }
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) = u;
+        *(f32x4*)(out + PK_M * HD + dt * 32 + 8 * rb + 4 * g) = v;
+      }
+    return;
+  }
+  if (mykey >= kb.nk) return;
+  const long row = krow * HD;
+#pragma unroll
+  for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+    for (int rb = 0; rb < 4; ++rb) {
+      bf16x4 x, y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = (bf16)(dk[dt][rb * 4 + e] * a.scale);
+        y[e] = (bf16)dv[dt][rb * 4 + e];
+      }
+      *(bf16x4*)((bf16*)a.dk + row + dt * 32 + 8 * rb + 4 * g) = x;
+      *(bf16x4*)((bf16*)a.dv + row + dt * 32 + 8 * rb + 4 * g) = y;
+    }
+}
+
 // dK, dV of blocks whose sums are in shares, added in order, four elements a thread.  A workgroup takes one of the pieces
 // of a block's [dK | dV][key][dim].
 template <typename T, int HD>
@@ -382,13 +669,19 @@ size_t row_bytes(long heads, long rows) { return ((size_t)heads * rows * sizeof(
 
 template <typename T, int HD, int BN, int BQ, bool VEC>
 int launch_bwd(hipStream_t s, PackArgs a) {
+  constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
+  const bool fast = dma && a.d == 128;
   PackArgs q = a;
   q.nx = (int)packed_tiles(a.N, a.S);
-  packed_dq_kernel<T, HD, BN, VEC><<<(unsigned)((long)a.H * q.nx), 256, 0, s>>>(q);
+  const unsigned qgrid = (unsigned)((long)a.H * q.nx);
+  const int hkv = a.H / a.G;
+  const unsigned kgrid = (unsigned)((long)hkv * a.nx * a.chunks);
+  if (fast) packed_dq128_kernel<<<qgrid, 256, 0, s>>>(q);
+  else packed_dq_kernel<T, HD, BN, VEC><<<qgrid, 256, 0, s>>>(q);
   int rc = check_launch("packed attention dQ");
   if (rc) return rc;
-  const int hkv = a.H / a.G;
-  packed_dkdv_kernel<T, HD, BQ, VEC><<<(unsigned)((long)hkv * a.nx * a.chunks), 256, 0, s>>>(a);
+  if (fast) packed_dkdv128_kernel<<<kgrid, 256, 0, s>>>(a);
+  else packed_dkdv_kernel<T, HD, BQ, VEC><<<kgrid, 256, 0, s>>>(a);
   rc = check_launch("packed attention dK, dV");
   if (rc || a.chunks == 1) return rc;
   packed_sum_kernel<T, HD><<<(unsigned)(2L * PK_M * HD / 1024 * a.nx * hkv), 256, 0, s>>>(a);
