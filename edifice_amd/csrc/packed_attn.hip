@@ -26,50 +26,20 @@ namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
 
-// What a forward workgroup works on: its queries, its text's keys and its share [t0, t1) of their tiles.
-template <int BN>
-struct QueryTile {
-  int head, qrow, nq, krow, nk, first, chunk, t0, t1;  // first: the tile's first query within the text
-  bool none;
-  EDF_DEVICE int ahead() const { return nk - nq; }
-  EDF_DEVICE QueryTile(const PackArgs& a) {
-    int x;
-    packed_block(a, a.nx * a.chunks, x, head);
-    chunk = x % a.chunks;
-    const TextTile t = find_tile(a.qo, a.S, a.N, a.nx - 1 - x / a.chunks);
-    qrow = t.row0, nq = t.n, first = t.first;
-    none = first >= nq;
-    text_rows(a.ko, a.S, a.M, t.text, krow, nk);
-    t0 = t1 = 0;
-  }
-  EDF_DEVICE KeyTiles<PK_M, BN> tiles(const PackArgs& a) {
-    const KeyTiles<PK_M, BN> kt(first + ahead(), nk, a.W, a.sinks);
-    const int count = first + ahead() + PK_M > 0 ? max(kt.count, 0) : 0;
-    t0 = min(chunk * a.len, count);
-    t1 = min(t0 + a.len, count);
-    if (chunk > 0 && t0 >= count) none = true;  // the first chunk answers for a tile without keys
-    return kt;
-  }
-};
-
 template <typename T, int HD, int BN, bool VEC>
-__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
+__global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(PackArgs a) {
   constexpr int NKK = HD / 16, NDT = HD / 32, NH = BN / 32;
   constexpr int AHEAD = sizeof(T) == 2 ? 4 : 1;
   using Tile = WTile<T, HD, BN>;
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
 
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
-  QueryTile<BN> qt(a);
+  const int tid = threadIdx.x, l = tid & 63, g = l >> 5, li = l & 31;
+  const QueryTile<BN> qt(a);
   if (qt.none) return;
-  const KeyTiles<PK_M, BN> kt = qt.tiles(a);
-  if (qt.none) return;
-  const int d = a.d, pw = qt.first + 32 * w + qt.ahead(), myp = pw + li;  // positions
-  const int myq = qt.first + 32 * w + li;                                  // query within the text
-  const long row = (long)qt.head * a.N + qt.qrow + min(myq, qt.nq - 1);
-  const T* K = (const T*)a.k + ((long)(qt.head / a.G) * a.M + qt.krow) * d;
-  const T* V = (const T*)a.v + ((long)(qt.head / a.G) * a.M + qt.krow) * d;
+  const int d = a.d, myq = qt.myq, myp = qt.pw + li;
+  const long row = qt.row0 + min(myq, qt.nq - 1);
+  const T *K = (const T*)a.k + qt.krow * d, *V = (const T*)a.v + qt.krow * d;
 
   WFrag<T> qf[NKK];
 #pragma unroll
@@ -82,10 +52,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
   const TileLoader<T, HD, BN, VEC> ld(tid, d, qt.nk);
   WFrag<T> rk[ld.N], rv[ld.N];
   const int count = qt.t1 - qt.t0;
-  auto key0 = [&](int t) { return kt.key0(qt.t0 + t); };
   auto gload = [&](int t) {
-    ld.load(K, key0(t), rk);
-    ld.load(V, key0(t), rv);
+    ld.load(K, qt.key0(t), rk);
+    ld.load(V, qt.key0(t), rv);
   };
   auto sstore = [&](int buf) {
     ld.template store<Tile>(sK[buf], rk);
@@ -93,7 +62,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
   };
   auto tile = [&](int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
-    const SeesKey sees(myp, key0(t) + 4 * g, a.W, a.sinks);
+    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
     const T *sk = sK[t & 1], *sv = sV[t & 1];
     f32x16 s[NH];
 #pragma unroll
@@ -150,11 +119,10 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(PackArgs a) {
     if (count > 1) gload(1);
   }
   __syncthreads();
-  const int masked = min(count, max(kt.first_whole - qt.t0, 0));
+  const int masked = min(count, max(qt.kt.first_whole - qt.t0, 0));
   int t = 0;
   for (; t < masked; ++t) {
-    const int k0 = key0(t);
-    if ((k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks) tile(t, std::true_type{});  // some pair is visible
+    if (qt.visible(a, qt.key0(t), BN)) tile(t, std::true_type{});
     advance(t);
   }
   for (; t < count; ++t) {
@@ -213,18 +181,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
-  QueryTile<BN> qt(a);
+  const QueryTile<BN> qt(a);
   if (qt.none) return;
-  const KeyTiles<PK_M, BN> kt = qt.tiles(a);
-  if (qt.none) return;
-  const int pw = qt.first + 32 * w + qt.ahead(), myp = pw + li;  // positions
-  const int qw = qt.first + 32 * w, myq = qw + li;                // queries within the text
-  const long row0 = (long)qt.head * a.N + qt.qrow;
-  const bf16* Qrow = (const bf16*)a.q + (row0 + min(myq, qt.nq - 1)) * HD;
-  const long kvbase = ((long)(qt.head / a.G) * a.M + qt.krow) * HD;
+  const int myp = qt.pw + li, myq = qt.myq;
+  const bf16* Qrow = (const bf16*)a.q + (qt.row0 + min(myq, qt.nq - 1)) * HD;
   // buffer resources over the text's keys: rows past its end read as zeros (their scores are masked)
-  const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)qt.nk * HD * 2);
-  const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)qt.nk * HD * 2);
+  const rsrc_t rK = make_rsrc((const bf16*)a.k + qt.krow * HD, (unsigned)qt.nk * HD * 2);
+  const rsrc_t rV = make_rsrc((const bf16*)a.v + qt.krow * HD, (unsigned)qt.nk * HD * 2);
 
   bf16x8 qf[NKK];
 #pragma unroll
@@ -238,17 +201,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
   const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
   const int krow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
   const int vtr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
-  const int nkt = qt.t1 - qt.t0, whole = in_vector_register(max(kt.first_whole - qt.t0, 0));
-  auto key0 = [&](int t) __attribute__((always_inline)) { return kt.key0(qt.t0 + t); };
-  auto visible = [&](int t) __attribute__((always_inline)) {
-    const int k0 = key0(t);
-    return (k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks;
-  };
+  const int nkt = qt.t1 - qt.t0, whole = in_vector_register(max(qt.kt.first_whole - qt.t0, 0));
+  auto visible = [&](int t) __attribute__((always_inline)) { return qt.visible(a, qt.key0(t), BN); };
   auto issue_k = [&](auto bt, int t) __attribute__((always_inline)) {
-    stage_hb<BN>(rK, decltype(bt)::value ? sX1 : sX0, key0(t), wu, l);
+    stage_hb<BN>(rK, decltype(bt)::value ? sX1 : sX0, qt.key0(t), wu, l);
   };
   auto issue_v = [&](auto bt, int t) __attribute__((always_inline)) {
-    stage_hb<BN>(rV, (decltype(bt)::value ? sX0 : sX1) + BN * HD, key0(t), wu, l);
+    stage_hb<BN>(rV, (decltype(bt)::value ? sX0 : sX1) + BN * HD, qt.key0(t), wu, l);
   };
   auto scores = [&](auto bt, f32x16* s) __attribute__((always_inline)) {
     const bf16* sk = decltype(bt)::value ? sX1 : sX0;
@@ -264,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
   // first half of the softmax: mask, row maximum, rescale; the maximum in scaled log2 units
   auto softmax_max = [&](f32x16* s, int t, auto masked) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(masked)::value;
-    const SeesKey sees(myp, key0(t) + 4 * g, a.W, a.sinks);
+    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
     float mx = -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -387,7 +346,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
 
   if (a.chunks > 1) {
     if (myq >= qt.nq) return;
-    const long at = (long)qt.chunk * a.H * a.N + row0 + myq;
+    const long at = (long)qt.chunk * a.H * a.N + qt.row0 + myq;
     float* out = a.part + at * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
@@ -417,27 +376,27 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int e = l + 64 * i, row = e / 16, ch = e % 16;
-    if (qw + row < qt.nq)
-      *(bf16x8*)((bf16*)a.out + (row0 + qw + row) * HD + 8 * ch) = *(const bf16x8*)(so + lds_off<HD>(row, 8 * ch));
+    if (myq - li + row < qt.nq)
+      *(bf16x8*)((bf16*)a.out + (qt.row0 + myq - li + row) * HD + 8 * ch) = *(const bf16x8*)(so + lds_off<HD>(row, 8 * ch));
   }
   if (myq < qt.nq && g == 0 && a.lse != nullptr)
-    a.lse[row0 + myq] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
+    a.lse[qt.row0 + myq] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
 }
 
 // The chunks of 32 rows joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, a row by eight lanes of four elements
 // at a time.
 template <typename T, int HD, int BN>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
+  const int ms = 7 - a.hs, per = (1 << ms) / 32;
   int x, head;
-  packed_block(a, a.nx * 4, x, head);
-  const TextTile t = find_tile(a.qo, a.S, a.N, x >> 2);
-  const int q = t.first + 32 * (x & 3) + (threadIdx.x >> 3);
+  if (!packed_block(a.H, a.nx * per, x, head)) return;
+  const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / per);
+  const int q = t.first + 32 * (x % per) + (threadIdx.x >> 3);
   if (q >= t.n) return;
   int krow, nk;
   text_rows(a.ko, a.S, a.M, t.text, krow, nk);
-  const KeyTiles<PK_M, BN> kt(t.first + nk - t.n, nk, a.W, a.sinks);
-  const int count = t.first + nk - t.n + PK_M > 0 ? max(kt.count, 0) : 0;
-  const int n = min(a.chunks, max(1, (count + a.len - 1) / a.len));
+  const BlockTiles<BN> kt(t.first + nk - t.n, 1 << ms, nk, a.W, a.sinks);
+  const int n = min(a.chunks, max(1, (kt.count + a.len - 1) / a.len));
   const long row = (long)head * a.N + t.row0 + q, stride = (long)a.H * a.N;
   float m = -INFINITY, sum = 0.0f;
   for (int c = 0; c < n; ++c) m = fmaxf(m, a.ml[2 * (c * stride + row)]);
@@ -460,28 +419,9 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
   if ((threadIdx.x & 7) == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? INFINITY : (m + __log2f(sum)) * LN2;
 }
 
-// How the key tiles of a query tile are cut: into chunks of `len` tiles where the call's workgroups without it would not
-// fill the GPU's 512 places.  The longest text may have all keys, so the grid has a chunk for each part of those, most of
-// which find no tile.
-void packed_plan(PackArgs& a, int BN) {
-  a.nx = (int)packed_tiles(a.N, a.S);
-  a.chunks = 1, a.len = 1 << 30;
-  const long wgs = (long)a.H * a.nx;
-  if (wgs >= 512) return;
-  long keys = a.M;
-  if (a.W < PK_ALL) keys = std::min(keys, (long)a.W + PK_M + a.sinks + 2L * BN);
-  const long most = (keys + BN - 1) / BN + 1, want = std::min(32L, std::max(1L, 4096 / wgs));
-  const long len = std::max(4L, (most + want - 1) / want);
-  a.chunks = (int)((most + len - 1) / len);
-  if (a.chunks > 1) a.len = (int)len;
-}
-size_t packed_chunk_bytes(const PackArgs& a) {
-  return a.chunks == 1 ? 0 : (size_t)a.chunks * a.H * a.N * (window_pad(a.d) + 2) * sizeof(float);
-}
-
 template <typename T, int HD, int BN, bool VEC>
 int launch_fwd(hipStream_t s, PackArgs a) {
-  const long grid = (long)a.H * a.nx * a.chunks;
+  const long grid = packed_grid(a.H >> a.hs, (long)a.nx * a.chunks);
   a.ml = a.part + (size_t)a.chunks * a.H * a.N * HD;
   bool done = false;
   if constexpr (sizeof(T) == 2 && HD == 128 && VEC) {
@@ -491,7 +431,7 @@ int launch_fwd(hipStream_t s, PackArgs a) {
     }
   }
   if (!done) packed_fwd_kernel<T, HD, BN, VEC><<<(unsigned)grid, 256, 0, s>>>(a);
-  if (a.chunks > 1) packed_join_kernel<T, HD, BN><<<(unsigned)(a.H * a.nx * 4), 256, 0, s>>>(a);
+  if (a.chunks > 1) packed_join_kernel<T, HD, BN><<<(unsigned)packed_grid(a.H, (long)a.nx * (PK_M >> a.hs) / 32), 256, 0, s>>>(a);
   return check_launch("packed attention");
 }
 template <typename T, int BN, bool VEC>
@@ -503,8 +443,6 @@ int launch_fwd_d(hipStream_t s, const PackArgs& a) {
     default: return launch_fwd<T, 128, BN, VEC>(s, a);
   }
 }
-
-constexpr int key_tile(int dtype) { return dtype == EDF_BF16 ? 64 : 32; }
 
 }  // namespace
 
@@ -519,7 +457,7 @@ int packed_check(int num_heads, int num_kv_heads, long rows, long key_rows, int 
   EDF_REQUIRE(head_dim <= 128, EDF_ERR_UNSUPPORTED, "head_dim %d > 128 unsupported", head_dim);
   EDF_REQUIRE(rows < (1L << 30) && key_rows < (1L << 30) && texts < (1 << 28) && sinks < (1 << 30), EDF_ERR_UNSUPPORTED,
               "rows, keys, texts and sinks must be below 2^28");
-  EDF_REQUIRE((double)num_heads * packed_tiles(std::max(rows, key_rows), texts) * 4 < 2147483648.0, EDF_ERR_UNSUPPORTED,
+  EDF_REQUIRE((double)num_heads * packed_tiles(std::max(rows, key_rows), texts, 32) * 4 < 2147483648.0, EDF_ERR_UNSUPPORTED,
               "heads x rows too large for one call");
   return EDF_OK;
 }
@@ -533,10 +471,10 @@ size_t edf_packed_attention_workspace_bytes(int num_heads, int num_kv_heads, lon
   using namespace edf;
   if (packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype)) return 0;
   PackArgs a{};
-  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.d = head_dim;
+  a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
-  packed_plan(a, key_tile(dtype));
-  return packed_chunk_bytes(a);
+  query_plan(a, key_tile(dtype));
+  return chunk_bytes(a, 2);
 }
 
 int edf_packed_attention(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
@@ -552,8 +490,8 @@ int edf_packed_attention(void* stream, const void* q, const void* k, const void*
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
-  packed_plan(a, key_tile(dtype));
-  const size_t need = packed_chunk_bytes(a);
+  query_plan(a, key_tile(dtype));
+  const size_t need = chunk_bytes(a, 2);
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
   a.part = (float*)workspace;

@@ -30,17 +30,12 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   __shared__ __attribute__((aligned(16))) T sK[2][Tile::ELEMS];
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
 
-  const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
-  int x, head;
-  packed_block(a, a.nx, x, head);
-  const TextTile tt = find_tile(a.qo, a.S, a.N, a.nx - 1 - x);
-  if (tt.first >= tt.n) return;
-  int krow, nk;
-  text_rows(a.ko, a.S, a.M, tt.text, krow, nk);
-  const int d = a.d, p0 = tt.first + nk - tt.n, pw = p0 + 32 * w, myp = pw + li, myq = tt.first + 32 * w + li;
-  const long qrow = (long)head * a.N + tt.row0 + min(myq, tt.n - 1);
-  const T* K = (const T*)a.k + ((long)(head / a.G) * a.M + krow) * d;
-  const T* V = (const T*)a.v + ((long)(head / a.G) * a.M + krow) * d;
+  const int tid = threadIdx.x, l = tid & 63, g = l >> 5, li = l & 31;
+  const QueryTile<BN> qt(a);
+  if (qt.none) return;
+  const int d = a.d, myq = qt.myq, myp = qt.pw + li;
+  const long qrow = qt.row0 + min(myq, qt.nq - 1);
+  const T *K = (const T*)a.k + qt.krow * d, *V = (const T*)a.v + qt.krow * d;
 
   WFrag<T> qf[NKK], of[NKK];
   float dd = 0.0f;
@@ -55,17 +50,16 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < tt.n) a.dd[qrow] = dd;
+  if (g == 0 && myq < qt.nq && qt.chunk == 0) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
 
-  const KeyTiles<PK_M, BN> kt(p0, nk, a.W, a.sinks);
-  const int count = p0 + PK_M > 0 ? max(kt.count, 0) : 0;
-  const TileLoader<T, HD, BN, VEC> ld(tid, d, nk);
+  const int count = qt.t1 - qt.t0;
+  const TileLoader<T, HD, BN, VEC> ld(tid, d, qt.nk);
   WFrag<T> rk[ld.N], rv[ld.N];
   auto gload = [&](int t) {
-    const int k0 = kt.key0(t);
+    const int k0 = qt.key0(t);
     ld.load(K, k0, rk);
     ld.load(V, k0, rv);
   };
@@ -75,7 +69,7 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   };
   auto tile = [&](int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
-    const SeesKey sees(myp, kt.key0(t) + 4 * g, a.W, a.sinks);
+    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
     const T *sk = sK[t & 1], *sv = sV[t & 1];
     f32x16 s[NH], dp[NH];
 #pragma unroll
@@ -121,18 +115,27 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     if (count > 1) gload(1);
   }
   __syncthreads();
-  const int masked = min(count, kt.first_whole);
+  const int masked = min(count, max(qt.kt.first_whole - qt.t0, 0));
   int t = 0;
   for (; t < masked; ++t) {
-    const int k0 = kt.key0(t);
-    if ((k0 <= pw + 31 && k0 + BN + a.W > pw + 1) || k0 < a.sinks) tile(t, std::true_type{});
+    if (qt.visible(a, qt.key0(t), BN)) tile(t, std::true_type{});
     advance(t);
   }
   for (; t < count; ++t) {
     tile(t, std::false_type{});
     advance(t);
   }
-  if (myq >= tt.n) return;
+  if (myq >= qt.nq) return;
+  if (a.chunks > 1) {
+    float* out = a.part + ((long)qt.chunk * a.H * a.N + qrow) * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
+            f32x4{dq[dt][rb * 4], dq[dt][rb * 4 + 1], dq[dt][rb * 4 + 2], dq[dt][rb * 4 + 3]};
+    return;
+  }
   T* out = (T*)a.dq + qrow * d;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
@@ -162,17 +165,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
-  int x, head;
-  packed_block(a, a.nx, x, head);
-  const TextTile tt = find_tile(a.qo, a.S, a.N, a.nx - 1 - x);
-  if (tt.first >= tt.n) return;
-  int kbegin, nk;
-  text_rows(a.ko, a.S, a.M, tt.text, kbegin, nk);
-  const int p0 = tt.first + nk - tt.n, pw = p0 + 32 * w, myp = pw + li, myq = tt.first + 32 * w + li;
-  const long qrow = (long)head * a.N + tt.row0 + min(myq, tt.n - 1);
-  const long kvbase = ((long)(head / a.G) * a.M + kbegin) * HD;
-  const rsrc_t rK = make_rsrc((const bf16*)a.k + kvbase, (unsigned)nk * HD * 2);
-  const rsrc_t rV = make_rsrc((const bf16*)a.v + kvbase, (unsigned)nk * HD * 2);
+  const QueryTile<BN> qt(a);
+  if (qt.none) return;
+  const int pw = qt.pw, myp = pw + li, myq = qt.myq;
+  const long qrow = qt.row0 + min(myq, qt.nq - 1);
+  const rsrc_t rK = make_rsrc((const bf16*)a.k + qt.krow * HD, (unsigned)qt.nk * HD * 2);
+  const rsrc_t rV = make_rsrc((const bf16*)a.v + qt.krow * HD, (unsigned)qt.nk * HD * 2);
 
   bf16x8 qf[NKK], of[NKK];
   float dd = 0.0f;
@@ -187,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < tt.n) a.dd[qrow] = dd;
+  if (g == 0 && myq < qt.nq && qt.chunk == 0) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
@@ -196,12 +194,10 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
   const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
   const int krow[2] = {hb_row_base(li, g, 0), hb_row_base(li, g, 1)};
   const int ktr[2] = {hb_tr_base(kr, d0, 0), hb_tr_base(kr, d0, 1)};
-  const KeyTiles<PK_M, BN> kt(p0, nk, a.W, a.sinks);
-  const int count = p0 + PK_M > 0 ? max(kt.count, 0) : 0;
-  const int whole = in_vector_register(kt.first_whole);
+  const int count = qt.t1 - qt.t0, whole = in_vector_register(max(qt.kt.first_whole - qt.t0, 0));
   auto issue = [&](auto bt, int t) {
     constexpr int B = decltype(bt)::value;
-    const int k0 = kt.key0(t);
+    const int k0 = qt.key0(t);
     stage_hb<BN>(rK, B ? sR1 : sR0, k0, wu, l);
     stage_hb<BN>(rV, (B ? sR1 : sR0) + BN * HD, k0, wu, l);
   };
@@ -209,11 +205,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     constexpr bool MASK = decltype(masked)::value;
     const bf16* sK = decltype(bt)::value ? sR1 : sR0;
     const bf16* sV = sK + BN * HD;
-    const int k0 = kt.key0(t);
+    const int k0 = qt.key0(t);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int kb = k0 + 32 * h;
-      if (MASK && !((kb <= pw + 31 && kb + 32 + a.W > pw + 1) || kb < a.sinks)) continue;  // no visible pair
+      if (MASK && !qt.visible(a, kb, 32)) continue;  // no visible pair
       const SeesKey sees(myp, kb + 4 * g, a.W, a.sinks);
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -259,7 +255,17 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     step(b0, t);
     if (t + 1 < count) step(b1, t + 1);
   }
-  if (myq >= tt.n) return;
+  if (myq >= qt.nq) return;
+  if (a.chunks > 1) {
+    float* out = a.part + ((long)qt.chunk * a.H * a.N + qrow) * HD;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb)
+        *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
+            f32x4{dq[dt][rb * 4], dq[dt][rb * 4 + 1], dq[dt][rb * 4 + 2], dq[dt][rb * 4 + 3]};
+    return;
+  }
   bf16* out = (bf16*)a.dq + qrow * HD;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
@@ -280,7 +286,7 @@ struct KeyBlock {
   bool none;
   EDF_DEVICE int ahead() const { return nk - nq; }
   EDF_DEVICE KeyBlock(const PackArgs& a, int id_x, int id_head, int share_) : head(id_head), share(share_) {
-    const TextTile t = find_tile(a.ko, a.S, a.M, id_x);
+    const TextTile t = a.by_work ? find_tile_by_work(a.ko, a.S, a.M, 7, id_x, false) : find_tile(a.ko, a.S, a.M, 7, id_x);
     krow = t.row0, nk = t.n, first = t.first;
     none = first >= nk;
     text_rows(a.qo, a.S, a.N, t.text, qrow, nq);
@@ -305,7 +311,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int x, head;  // of the key heads
-  packed_block(a, a.nx * a.chunks, x, head);
+  if (!packed_block(a.H / a.G, a.nx * a.chunks, x, head)) return;
   const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
   if (kb.none) return;
   const int d = a.d, kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
@@ -474,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
   int x, head;  // of the key heads
-  packed_block(a, a.nx * a.chunks, x, head);
+  if (!packed_block(a.H / a.G, a.nx * a.chunks, x, head)) return;
   const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
   if (kb.none) return;
   const int kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
@@ -635,7 +641,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
   constexpr int PIECES = 2 * PK_M * HD / 1024;
   const int piece = blockIdx.x % PIECES, x = blockIdx.x / PIECES % a.nx, head = blockIdx.x / PIECES / a.nx;
-  const TextTile t = find_tile(a.ko, a.S, a.M, x);
+  const TextTile t = find_tile(a.ko, a.S, a.M, 7, x);
   const int e = (piece * 256 + threadIdx.x) * 4;
   const bool is_v = e >= PK_M * HD;
   const int key = t.first + e / HD % PK_M, c = e % HD;
@@ -653,17 +659,49 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
     if (c + i < a.d) out[i] = from_f32<T>(s[i]);
 }
 
+// dQ of 32 rows whose key tiles are in chunks, added in order, a row by eight lanes of four elements at a time.
+template <typename T, int HD, int BN>
+__global__ __launch_bounds__(256) void packed_dq_sum_kernel(PackArgs a) {
+  const int ms = 7 - a.hs, per = (1 << ms) / 32;
+  int x, head;
+  if (!packed_block(a.H, a.nx * per, x, head)) return;
+  const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / per);
+  const int q = t.first + 32 * (x % per) + (threadIdx.x >> 3);
+  if (q >= t.n) return;
+  int krow, nk;
+  text_rows(a.ko, a.S, a.M, t.text, krow, nk);
+  const BlockTiles<BN> kt(t.first + nk - t.n, 1 << ms, nk, a.W, a.sinks);
+  const int n = min(a.chunks, max(1, (kt.count + a.len - 1) / a.len));
+  const long row = (long)head * a.N + t.row0 + q, stride = (long)a.H * a.N;
+  for (int e = 4 * (threadIdx.x & 7); e < a.d; e += 32) {
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) s += *(const f32x4*)(a.part + (c * stride + row) * HD + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (e + i < a.d) st((T*)a.dq, row * a.d + e + i, s[i] * a.scale);
+  }
+}
+
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
 
 // Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places.
 void backward_plan(PackArgs& a) {
-  a.nx = (int)packed_tiles(a.M, a.S);
+  a.nx = (int)packed_tiles(a.M, a.S, PK_M);
   const long wgs = (long)(a.H / a.G) * a.nx;
   a.chunks = (int)std::max(1L, std::min(16L, 512 / wgs));
+  a.by_work = order_by_work(a, wgs);
 }
 size_t share_bytes(const PackArgs& a) {
   return a.chunks == 1 ? 0
                        : (size_t)a.chunks * (a.H / a.G) * a.nx * (2 * PK_M) * window_pad(a.d) * sizeof(float);
+}
+// the larger of what the two kernels leave, one after the other
+size_t part_bytes(PackArgs a, int dtype) {
+  query_plan(a, key_tile(dtype));
+  const size_t queries = chunk_bytes(a, 0);
+  backward_plan(a);
+  return std::max(queries, share_bytes(a));
 }
 size_t row_bytes(long heads, long rows) { return ((size_t)heads * rows * sizeof(float) + 255) & ~(size_t)255; }
 
@@ -672,14 +710,19 @@ int launch_bwd(hipStream_t s, PackArgs a) {
   constexpr bool dma = sizeof(T) == 2 && HD == 128 && VEC;
   const bool fast = dma && a.d == 128;
   PackArgs q = a;
-  q.nx = (int)packed_tiles(a.N, a.S);
-  const unsigned qgrid = (unsigned)((long)a.H * q.nx);
+  query_plan(q, BN);
+  const unsigned qgrid = (unsigned)packed_grid(a.H >> q.hs, (long)q.nx * q.chunks);
   const int hkv = a.H / a.G;
-  const unsigned kgrid = (unsigned)((long)hkv * a.nx * a.chunks);
+  const unsigned kgrid = (unsigned)packed_grid(hkv, (long)a.nx * a.chunks);
   if (fast) packed_dq128_kernel<<<qgrid, 256, 0, s>>>(q);
   else packed_dq_kernel<T, HD, BN, VEC><<<qgrid, 256, 0, s>>>(q);
   int rc = check_launch("packed attention dQ");
   if (rc) return rc;
+  if (q.chunks > 1) {
+    packed_dq_sum_kernel<T, HD, BN><<<(unsigned)packed_grid(a.H, (long)q.nx * (PK_M >> q.hs) / 32), 256, 0, s>>>(q);
+    rc = check_launch("packed attention dQ sums");
+    if (rc) return rc;
+  }
   if (fast) packed_dkdv128_kernel<<<kgrid, 256, 0, s>>>(a);
   else packed_dkdv_kernel<T, HD, BQ, VEC><<<kgrid, 256, 0, s>>>(a);
   rc = check_launch("packed attention dK, dV");
@@ -708,8 +751,8 @@ size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_h
   if (packed_check(num_heads, num_kv_heads, rows, key_rows, texts, head_dim, window, sinks, dtype)) return 0;
   PackArgs a{};
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
-  backward_plan(a);
-  return row_bytes(num_heads, rows) + share_bytes(a);
+  a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
+  return row_bytes(num_heads, rows) + part_bytes(a, dtype);
 }
 
 int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
@@ -729,7 +772,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
   backward_plan(a);
-  const size_t need = row_bytes(num_heads, rows) + share_bytes(a);
+  const size_t need = row_bytes(num_heads, rows) + part_bytes(a, dtype);
   EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   a.dd = (float*)workspace;
   a.part = (float*)((char*)workspace + row_bytes(num_heads, rows));
