@@ -14,14 +14,16 @@ struct PackArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
   float *lse, *dd;       // [H N]
-  float *part, *ml;      // forward: [chunk][H N] unnormalised outputs of chunks of keys, their maxima and sums;
-                         // backward: part [chunk][Hkv M / 128 ...] dK and dV of chunks of queries
+  float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks of keys, maxima and sums;
+                         // keys: part [share][Hkv][block] dK and dV of shares of queries
+  int* plan;             // queries: [head group][tile] first item and number of chunks
   const int *qo, *ko;
   int N, M, S, H, G, d, W, sinks;
   int hs;                // the four waves of a query workgroup take 2^hs heads of one key head, 128 >> hs queries of each
   int nx;                // tiles a head (an upper bound: which of them exist is known on the GPU)
   int by_work;           // tiles in order of their work, the longest first, rather than of the texts
-  int chunks, len;       // queries: chunks of len key tiles; keys: shares of a key block's query tiles
+  int items;             // queries: chunks of key tiles a head group (an upper bound), 0: tiles are not cut
+  int shares;            // keys: of a key block's query tiles
   float scale, scale_log2;
 };
 
@@ -167,45 +169,168 @@ struct BlockTiles {
   }
 };
 
+// Where queries are few against the GPU their key tiles are cut into chunks, an item of work each.  All workgroups of a call
+// come to the same plan from the offsets alone: chunks of len key tiles, so that there are about PK_ITEMS of them, numbered
+// from tile to tile.  Item `item` of a head group's; threads look at two tiles each, of which there are fewer than 512.
+constexpr int PK_ITEMS = 768, PK_PLAN = 512;
+struct Item {
+  TextTile tile;
+  int x, nk, krow, chunk, chunks, len;  // the tile's number, its text's keys, which of its chunks, how many, key tiles of one
+  bool none;
+};
+template <int BN>
+EDF_DEVICE Item find_item(const PackArgs& a, int groups, int item, int* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, ms = 7 - a.hs;
+  int *so = lds, *sk = lds + PK_PLAN + 2, *sum = sk + PK_PLAN + 2, *found = sum + 8;
+  for (int s = tid; s <= a.S; s += 256) {
+    so[s] = text_begin(a.qo, s, a.N);
+    sk[s] = text_begin(a.ko, s, a.M);
+  }
+  if (tid == 0) {
+    so[a.S + 1] = a.N;
+    found[0] = -1;
+  }
+  __syncthreads();
+  int count[2], text[2], chunks[2];
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int x = 2 * tid + i;
+    count[i] = -1, text[i] = 0;
+    if (x >= a.nx) continue;
+    int lo = 0, hi = a.S + 1;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((so[mid] >> ms) + mid <= x) lo = mid;
+      else hi = mid;
+    }
+    text[i] = lo;
+    const int n = max(so[lo + 1] - so[lo], 0), first = (x - (so[lo] >> ms) - lo) << ms;
+    if (first >= n) continue;
+    const int nk = lo < a.S ? max(sk[lo + 1] - sk[lo], 0) : 0;
+    count[i] = BlockTiles<BN>(first + nk - n, 1 << ms, nk, a.W, a.sinks).count;
+    mine += count[i];
+  }
+  const int ws = wave_sum_i(mine);
+  if (lane == 0) sum[tid >> 6] = ws;
+  __syncthreads();
+  const long all = (long)sum[0] + sum[1] + sum[2] + sum[3];
+  const int len = (int)max(4L, (all * groups + PK_ITEMS - 1) / PK_ITEMS);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) chunks[i] = count[i] < 0 ? 0 : max(1, (count[i] + len - 1) / len);
+  int incl = chunks[0] + chunks[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(incl, o);
+    incl += lane >= o ? up : 0;
+  }
+  if (lane == 63) sum[4 + (tid >> 6)] = incl;
+  __syncthreads();
+  int at = incl - chunks[0] - chunks[1];  // items before this thread's tiles
+  for (int w = 0; w < (tid >> 6); ++w) at += sum[4 + w];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if (item >= at && item < at + chunks[i]) {
+      found[0] = 2 * tid + i;
+      found[1] = text[i];
+      found[2] = item - at;
+      found[3] = chunks[i];
+    }
+    at += chunks[i];
+  }
+  __syncthreads();
+  Item t;
+  t.x = __builtin_amdgcn_readfirstlane(found[0]);
+  t.none = t.x < 0;
+  const int s = __builtin_amdgcn_readfirstlane(found[1]);
+  if (t.none) return t;
+  t.tile.text = s;
+  t.tile.row0 = __builtin_amdgcn_readfirstlane(so[s]);
+  t.tile.n = __builtin_amdgcn_readfirstlane(max(so[s + 1] - so[s], 0));
+  t.tile.first = (t.x - (t.tile.row0 >> ms) - s) << ms;
+  t.krow = s < a.S ? __builtin_amdgcn_readfirstlane(sk[s]) : 0;
+  t.nk = s < a.S ? __builtin_amdgcn_readfirstlane(max(sk[s + 1] - sk[s], 0)) : 0;
+  t.chunk = __builtin_amdgcn_readfirstlane(found[2]);
+  t.chunks = __builtin_amdgcn_readfirstlane(found[3]);
+  t.len = __builtin_amdgcn_readfirstlane(len);
+  __syncthreads();  // the caller's tiles go into the same memory
+  return t;
+}
+
 // What a workgroup of queries works on: four waves, each 32 queries of one head at positions pw .. pw + 31 of the text's nk
 // keys, and the workgroup's chunk [t0, t1) of their key tiles.
 template <int BN>
 struct QueryTile {
-  int head, kvhead, myq, nq, pw, nk, chunk, t0, t1;  // head, myq (query within the text), pw: of the wave or lane
-  long row0, krow;                                   // rows of the text's first query (of the wave's head) and key
-  bool none;
+  int head, kvhead, myq, nq, pw, nk, t0, t1;  // head, myq (query within the text), pw: of the wave or lane
+  long row0, krow;                            // rows of the text's first query (of the wave's head) and key
+  long slot;                                  // of one of several chunks: this lane's row of part and ml, or -1
+  bool none, first;                           // first: the tile's first chunk
   BlockTiles<BN> kt;
-  EDF_DEVICE static TextTile tile(const PackArgs& a, int x) {
-    const int ms = 7 - a.hs;
-    return a.by_work ? find_tile_by_work(a.qo, a.S, a.N, ms, x, true) : find_tile(a.qo, a.S, a.N, ms, a.nx - 1 - x);
-  }
-  EDF_DEVICE QueryTile(const PackArgs& a) : kt(0, 0, 0, 1, 0) {
+  // lds: 4 KB and some that the kernel uses later
+  EDF_DEVICE QueryTile(const PackArgs& a, void* lds) : kt(0, 0, 0, 1, 0) {
     const int w = threadIdx.x >> 6, li = threadIdx.x & 31, wu = __builtin_amdgcn_readfirstlane(w);
-    int x, grp;
-    none = !packed_block(a.H >> a.hs, a.nx * a.chunks, x, grp);
+    const int groups = a.H >> a.hs, ms = 7 - a.hs;
+    int x, grp, key0, chunk = 0, len = 0;
+    none = !packed_block(groups, a.items > 0 ? a.items : a.nx, x, grp);
     if (none) return;
-    chunk = x % a.chunks;
-    const TextTile t = tile(a, x / a.chunks);
+    TextTile t;
+    slot = -1;
+    if (a.items > 0) {
+      const Item it = find_item<BN>(a, groups, x, (int*)lds);
+      none = it.none;
+      if (none) return;
+      t = it.tile, key0 = it.krow, nk = it.nk, chunk = it.chunk, len = it.len;
+      if (it.chunks > 1) slot = ((long)grp * a.items + x) * PK_M + 32 * w + li;
+      if (chunk == 0 && threadIdx.x == 0) {
+        int* p = a.plan + 2 * ((long)grp * a.nx + it.x);
+        p[0] = x;
+        p[1] = it.chunks;
+      }
+    } else {
+      t = a.by_work ? find_tile_by_work(a.qo, a.S, a.N, ms, x, true) : find_tile(a.qo, a.S, a.N, ms, a.nx - 1 - x);
+      none = t.first >= t.n;
+      if (none) return;
+      text_rows(a.ko, a.S, a.M, t.text, key0, nk);
+    }
     head = (grp << a.hs) + (wu & ((1 << a.hs) - 1));
     kvhead = (grp << a.hs) / a.G;
     nq = t.n;
-    none = t.first >= nq;
-    int key0;
-    text_rows(a.ko, a.S, a.M, t.text, key0, nk);
     const int wq = t.first + 32 * (w >> a.hs);  // the wave's first query
     myq = wq + li;
     pw = wq + nk - nq;
     row0 = (long)head * a.N + t.row0;
     krow = (long)kvhead * a.M + key0;
     kt = BlockTiles<BN>(t.first + nk - nq, PK_M >> a.hs, nk, a.W, a.sinks);
-    t0 = min(chunk * a.len, kt.count);
-    t1 = min(t0 + a.len, kt.count);
-    if (chunk > 0 && t0 >= kt.count) none = true;  // the first chunk answers for a tile without keys
+    first = chunk == 0;
+    t0 = chunk * len;
+    t1 = a.items > 0 ? min(t0 + len, kt.count) : kt.count;
   }
   EDF_DEVICE int key0(int t) const { return kt.key0(t0 + t); }
   // some query of the wave sees a key of the bn keys from k0 on
   EDF_DEVICE bool visible(const PackArgs& a, int k0, int bn) const {
     return (k0 <= pw + 31 && k0 + bn + a.W > pw + 1) || k0 < a.sinks;
+  }
+};
+
+// One row of a query tile in chunks, for the kernels that join them: LANES lanes a row, 256 / LANES rows a workgroup.
+template <int LANES>
+struct ChunkRow {
+  static constexpr int PIECES = PK_M * LANES / 256;  // workgroups a tile
+  int chunks;      // 0: nothing to do
+  long row, slot;  // of the outputs; of part and ml, the first chunk's
+  EDF_DEVICE ChunkRow(const PackArgs& a) : chunks(0) {
+    int x, grp;
+    if (!packed_block(a.H >> a.hs, a.nx * PIECES, x, grp)) return;
+    const int ms = 7 - a.hs, r = x % PIECES * (256 / LANES) + threadIdx.x / LANES;
+    const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / PIECES);
+    const int q = t.first + 32 * (r >> 5 >> a.hs) + (r & 31);
+    if (t.first >= t.n || q >= t.n) return;
+    const int* p = a.plan + 2 * ((long)grp * a.nx + x / PIECES);
+    const int item = p[0], n = p[1];
+    if (n <= 1 || item < 0 || n > a.items - item) return;  // one chunk, or no plan (offsets that do not ascend)
+    chunks = n;
+    row = (long)((grp << a.hs) + ((r >> 5) & ((1 << a.hs) - 1))) * a.N + t.row0 + q;
+    slot = ((long)grp * a.items + item) * PK_M + r;
   }
 };
 
@@ -217,26 +342,25 @@ inline bool order_by_work(const PackArgs& a, long wgs) {
 
 // heads of a query workgroup: as many of a key head's as the four waves take
 inline int head_shift(int G) { return G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0; }
-// How the key tiles (of BN) of a query workgroup are cut: into chunks of `len` tiles where the call's workgroups without it
-// would not fill the GPU's 512 places.  The longest text may have all keys, so the grid has a chunk for each part of those,
-// most of which find no tile.
+// Tiles are cut where the call's workgroups would not fill the GPU's 512 places.  A tile has a chunk for each len of its key
+// tiles and one for the rest, so there are at most PK_ITEMS over all groups and one a tile.
 inline void query_plan(PackArgs& a, int BN) {
   a.hs = head_shift(a.G);
-  const int m = PK_M >> a.hs;
-  a.nx = (int)packed_tiles(a.N, a.S, m);
-  a.chunks = 1, a.len = 1 << 30;
-  const long wgs = (long)(a.H >> a.hs) * a.nx;
+  a.nx = (int)packed_tiles(a.N, a.S, PK_M >> a.hs);
+  const long groups = a.H >> a.hs, wgs = groups * a.nx;
   a.by_work = order_by_work(a, wgs);
-  if (wgs >= 512) return;
-  long keys = a.M;
-  if (a.W < PK_ALL) keys = std::min(keys, (long)a.W + m + a.sinks + 2L * BN);
-  const long most = (keys + BN - 1) / BN + 1, want = std::min(32L, std::max(1L, 4096 / wgs));
-  const long len = std::max(4L, (most + want - 1) / want);
-  a.chunks = (int)((most + len - 1) / len);
-  if (a.chunks > 1) a.len = (int)len;
+  // (the plan's sum of key tiles is an int: 2^24 keys of 512 tiles)
+  a.items = wgs < PK_PLAN && a.M > 4 * BN && a.M < (1 << 24) ? (int)((PK_ITEMS + groups - 1) / groups) + a.nx : 0;
 }
 inline size_t chunk_bytes(const PackArgs& a, int extra) {  // extra: floats a row beside the padded head
-  return a.chunks == 1 ? 0 : (size_t)a.chunks * a.H * a.N * (window_pad(a.d) + extra) * sizeof(float);
+  const size_t groups = a.H >> a.hs;
+  return a.items == 0 ? 0
+                      : groups * a.items * PK_M * (window_pad(a.d) + extra) * sizeof(float) + groups * a.nx * 2 * sizeof(int);
+}
+inline void chunk_memory(PackArgs& a, float* part, int extra) {
+  const size_t rows = (size_t)(a.H >> a.hs) * a.items * PK_M;
+  a.part = part, a.ml = part + rows * window_pad(a.d);
+  a.plan = (int*)(a.ml + rows * extra);
 }
 constexpr int key_tile(int dtype) { return dtype == EDF_BF16 ? 64 : 32; }
 

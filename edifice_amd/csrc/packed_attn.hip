@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
 
   const int tid = threadIdx.x, l = tid & 63, g = l >> 5, li = l & 31;
-  const QueryTile<BN> qt(a);
+  const QueryTile<BN> qt(a, sK);
   if (qt.none) return;
   const int d = a.d, myq = qt.myq, myp = qt.pw + li;
   const long row = qt.row0 + min(myq, qt.nq - 1);
@@ -131,9 +131,8 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
   }
 
   if (myq >= qt.nq) return;
-  if (a.chunks > 1) {
-    const long at = (long)qt.chunk * a.H * a.N + row;
-    float* out = a.part + at * HD;
+  if (qt.slot >= 0) {
+    float* out = a.part + qt.slot * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -141,8 +140,8 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
         *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
             f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
     if (g == 0) {
-      a.ml[2 * at] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
-      a.ml[2 * at + 1] = lsum;
+      a.ml[2 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[2 * qt.slot + 1] = lsum;
     }
     return;
   }
@@ -181,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
-  const QueryTile<BN> qt(a);
+  const QueryTile<BN> qt(a, sX0);
   if (qt.none) return;
   const int myp = qt.pw + li, myq = qt.myq;
   const bf16* Qrow = (const bf16*)a.q + (qt.row0 + min(myq, qt.nq - 1)) * HD;
@@ -344,10 +343,9 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
     if (t + 1 < nkt) step(b1, t + 1);
   }
 
-  if (a.chunks > 1) {
+  if (qt.slot >= 0) {
     if (myq >= qt.nq) return;
-    const long at = (long)qt.chunk * a.H * a.N + qt.row0 + myq;
-    float* out = a.part + at * HD;
+    float* out = a.part + qt.slot * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -355,8 +353,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
         *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
             f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
     if (g == 0) {
-      a.ml[2 * at] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
-      a.ml[2 * at + 1] = lsum;
+      a.ml[2 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[2 * qt.slot + 1] = lsum;
     }
     return;
   }
@@ -383,46 +381,36 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
     a.lse[qt.row0 + myq] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
 }
 
-// The chunks of 32 rows joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, a row by eight lanes of four elements
-// at a time.
-template <typename T, int HD, int BN>
+// The chunks of a row joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, four elements a lane.
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
-  const int ms = 7 - a.hs, per = (1 << ms) / 32;
-  int x, head;
-  if (!packed_block(a.H, a.nx * per, x, head)) return;
-  const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / per);
-  const int q = t.first + 32 * (x % per) + (threadIdx.x >> 3);
-  if (q >= t.n) return;
-  int krow, nk;
-  text_rows(a.ko, a.S, a.M, t.text, krow, nk);
-  const BlockTiles<BN> kt(t.first + nk - t.n, 1 << ms, nk, a.W, a.sinks);
-  const int n = min(a.chunks, max(1, (kt.count + a.len - 1) / a.len));
-  const long row = (long)head * a.N + t.row0 + q, stride = (long)a.H * a.N;
+  constexpr int LANES = HD <= 32 ? 8 : HD <= 64 ? 16 : 32;
+  const ChunkRow<LANES> r(a);
+  if (r.chunks == 0) return;
+  const int j = threadIdx.x % LANES, e = 4 * j;
+  const float* ml = a.ml + 2 * r.slot;
   float m = -INFINITY, sum = 0.0f;
-  for (int c = 0; c < n; ++c) m = fmaxf(m, a.ml[2 * (c * stride + row)]);
-  for (int c = 0; c < n; ++c) {
-    const float mc = a.ml[2 * (c * stride + row)];
-    sum = fmaf(mc == -INFINITY ? 0.0f : fast_exp2(mc - m), a.ml[2 * (c * stride + row) + 1], sum);
+  for (int c = j; c < r.chunks; c += LANES) m = fmaxf(m, ml[2L * PK_M * c]);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* in = a.part + r.slot * HD + min(e, HD - 4);
+#pragma unroll 4
+  for (int c = 0; c < r.chunks; ++c) {
+    const float mc = ml[2L * PK_M * c], f = mc == -INFINITY ? 0.0f : fast_exp2(mc - m);
+    sum = fmaf(f, ml[2L * PK_M * c + 1], sum);
+    acc += f * *(const f32x4*)(in + (long)PK_M * HD * c);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int e = 4 * (threadIdx.x & 7); e < a.d; e += 32) {
-    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = 0; c < n; ++c) {
-      const float mc = a.ml[2 * (c * stride + row)];
-      const float f = mc == -INFINITY ? 0.0f : fast_exp2(mc - m);
-      acc += f * *(const f32x4*)(a.part + (c * stride + row) * HD + e);
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (e + i < a.d) st((T*)a.out, row * a.d + e + i, acc[i] * inv);
-  }
-  if ((threadIdx.x & 7) == 0 && a.lse != nullptr) a.lse[row] = sum == 0.0f ? INFINITY : (m + __log2f(sum)) * LN2;
+  for (int i = 0; i < 4; ++i)
+    if (e + i < a.d) st((T*)a.out, r.row * a.d + e + i, acc[i] * inv);
+  if (j == 0 && a.lse != nullptr) a.lse[r.row] = sum == 0.0f ? INFINITY : (m + __log2f(sum)) * LN2;
 }
 
 template <typename T, int HD, int BN, bool VEC>
 int launch_fwd(hipStream_t s, PackArgs a) {
-  const long grid = packed_grid(a.H >> a.hs, (long)a.nx * a.chunks);
-  a.ml = a.part + (size_t)a.chunks * a.H * a.N * HD;
+  const long groups = a.H >> a.hs, grid = packed_grid(groups, a.items > 0 ? a.items : a.nx);
   bool done = false;
   if constexpr (sizeof(T) == 2 && HD == 128 && VEC) {
     if (a.d == 128) {
@@ -431,7 +419,8 @@ int launch_fwd(hipStream_t s, PackArgs a) {
     }
   }
   if (!done) packed_fwd_kernel<T, HD, BN, VEC><<<(unsigned)grid, 256, 0, s>>>(a);
-  if (a.chunks > 1) packed_join_kernel<T, HD, BN><<<(unsigned)packed_grid(a.H, (long)a.nx * (PK_M >> a.hs) / 32), 256, 0, s>>>(a);
+  if (a.items > 0)
+    packed_join_kernel<T, HD><<<(unsigned)packed_grid(groups, (long)a.nx * (HD <= 32 ? 4 : HD <= 64 ? 8 : 16)), 256, 0, s>>>(a);
   return check_launch("packed attention");
 }
 template <typename T, int BN, bool VEC>
@@ -494,7 +483,7 @@ int edf_packed_attention(void* stream, const void* q, const void* k, const void*
   const size_t need = chunk_bytes(a, 2);
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
-  a.part = (float*)workspace;
+  chunk_memory(a, (float*)workspace, 2);
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && key_rows <= WINDOW_VEC_T;
   hipStream_t s = as_stream(stream);

@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   __shared__ __attribute__((aligned(16))) T sV[2][Tile::ELEMS];
 
   const int tid = threadIdx.x, l = tid & 63, g = l >> 5, li = l & 31;
-  const QueryTile<BN> qt(a);
+  const QueryTile<BN> qt(a, sK);
   if (qt.none) return;
   const int d = a.d, myq = qt.myq, myp = qt.pw + li;
   const long qrow = qt.row0 + min(myq, qt.nq - 1);
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < qt.nq && qt.chunk == 0) a.dd[qrow] = dd;
+  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
@@ -126,8 +126,8 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     advance(t);
   }
   if (myq >= qt.nq) return;
-  if (a.chunks > 1) {
-    float* out = a.part + ((long)qt.chunk * a.H * a.N + qrow) * HD;
+  if (qt.slot >= 0) {
+    float* out = a.part + qt.slot * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
-  const QueryTile<BN> qt(a);
+  const QueryTile<BN> qt(a, sR0);
   if (qt.none) return;
   const int pw = qt.pw, myp = pw + li, myq = qt.myq;
   const long qrow = qt.row0 + min(myq, qt.nq - 1);
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < qt.nq && qt.chunk == 0) a.dd[qrow] = dd;
+  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
@@ -256,8 +256,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     if (t + 1 < count) step(b1, t + 1);
   }
   if (myq >= qt.nq) return;
-  if (a.chunks > 1) {
-    float* out = a.part + ((long)qt.chunk * a.H * a.N + qrow) * HD;
+  if (qt.slot >= 0) {
+    float* out = a.part + qt.slot * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -295,8 +295,8 @@ struct KeyBlock {
     if (first >= a.sinks) end = (int)min((long)nq, (long)first + PK_M - 1 + a.W - ahead());  // past the last key's window
     nt = max(0, (end - qs + BQ - 1) / BQ);
     const long all = (long)nt * a.G;
-    t0 = (int)(all * share / a.chunks);
-    t1 = (int)(all * (share + 1) / a.chunks);
+    t0 = (int)(all * share / a.shares);
+    t1 = (int)(all * (share + 1) / a.shares);
   }
 };
 
@@ -311,8 +311,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   int x, head;  // of the key heads
-  if (!packed_block(a.H / a.G, a.nx * a.chunks, x, head)) return;
-  const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
+  if (!packed_block(a.H / a.G, a.nx * a.shares, x, head)) return;
+  const KeyBlock<BQ> kb(a, x / a.shares, head, x % a.shares);
   if (kb.none) return;
   const int d = a.d, kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
   const long krow = (long)head * a.M + kb.krow + min(mykey, kb.nk - 1);
@@ -422,8 +422,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     }
     __syncthreads();
   }
-  if (a.chunks > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
-    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.chunks) * (2L * PK_M * HD) + (32 * w + li) * HD;
+  if (a.shares > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
+    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.shares) * (2L * PK_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -480,8 +480,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
   int x, head;  // of the key heads
-  if (!packed_block(a.H / a.G, a.nx * a.chunks, x, head)) return;
-  const KeyBlock<BQ> kb(a, x / a.chunks, head, x % a.chunks);
+  if (!packed_block(a.H / a.G, a.nx * a.shares, x, head)) return;
+  const KeyBlock<BQ> kb(a, x / a.shares, head, x % a.shares);
   if (kb.none) return;
   const int kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
   const long kbase = (long)head * a.M + kb.krow, krow = kbase + min(mykey, kb.nk - 1);
@@ -601,8 +601,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
     step(b0, t);
     if (t + 1 < t1) step(b1, t + 1);
   }
-  if (a.chunks > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
-    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.chunks) * (2L * PK_M * HD) + (32 * w + li) * HD;
+  if (a.shares > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
+    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.shares) * (2L * PK_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -651,7 +651,7 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
   const long stride = (long)hkv * a.nx * (2L * PK_M * HD);
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int i = 0; i < a.chunks; ++i) s += *(const f32x4*)(in + i * stride);
+  for (int i = 0; i < a.shares; ++i) s += *(const f32x4*)(in + i * stride);
   if (!is_v) s *= a.scale;
   T* out = (T*)(is_v ? a.dv : a.dk) + ((long)head * a.M + t.row0 + key) * a.d + c;
 #pragma unroll
@@ -659,28 +659,20 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
     if (c + i < a.d) out[i] = from_f32<T>(s[i]);
 }
 
-// dQ of 32 rows whose key tiles are in chunks, added in order, a row by eight lanes of four elements at a time.
-template <typename T, int HD, int BN>
+// dQ of rows whose key tiles are in chunks, added in order, four elements a lane.
+template <typename T, int HD>
 __global__ __launch_bounds__(256) void packed_dq_sum_kernel(PackArgs a) {
-  const int ms = 7 - a.hs, per = (1 << ms) / 32;
-  int x, head;
-  if (!packed_block(a.H, a.nx * per, x, head)) return;
-  const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / per);
-  const int q = t.first + 32 * (x % per) + (threadIdx.x >> 3);
-  if (q >= t.n) return;
-  int krow, nk;
-  text_rows(a.ko, a.S, a.M, t.text, krow, nk);
-  const BlockTiles<BN> kt(t.first + nk - t.n, 1 << ms, nk, a.W, a.sinks);
-  const int n = min(a.chunks, max(1, (kt.count + a.len - 1) / a.len));
-  const long row = (long)head * a.N + t.row0 + q, stride = (long)a.H * a.N;
-  for (int e = 4 * (threadIdx.x & 7); e < a.d; e += 32) {
-    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int LANES = HD <= 32 ? 8 : HD <= 64 ? 16 : 32;
+  const ChunkRow<LANES> r(a);
+  const int e = 4 * (threadIdx.x % LANES);
+  if (r.chunks == 0 || e >= a.d) return;
+  const float* in = a.part + r.slot * HD + e;
+  f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int c = 0; c < n; ++c) s += *(const f32x4*)(a.part + (c * stride + row) * HD + e);
+  for (int c = 0; c < r.chunks; ++c) s += *(const f32x4*)(in + (long)PK_M * HD * c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (e + i < a.d) st((T*)a.dq, row * a.d + e + i, s[i] * a.scale);
-  }
+  for (int i = 0; i < 4; ++i)
+    if (e + i < a.d) st((T*)a.dq, r.row * a.d + e + i, s[i] * a.scale);
 }
 
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
@@ -689,12 +681,12 @@ constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and flo
 void backward_plan(PackArgs& a) {
   a.nx = (int)packed_tiles(a.M, a.S, PK_M);
   const long wgs = (long)(a.H / a.G) * a.nx;
-  a.chunks = (int)std::max(1L, std::min(16L, 512 / wgs));
+  a.shares = (int)std::max(1L, std::min(16L, 512 / wgs));
   a.by_work = order_by_work(a, wgs);
 }
 size_t share_bytes(const PackArgs& a) {
-  return a.chunks == 1 ? 0
-                       : (size_t)a.chunks * (a.H / a.G) * a.nx * (2 * PK_M) * window_pad(a.d) * sizeof(float);
+  return a.shares == 1 ? 0
+                       : (size_t)a.shares * (a.H / a.G) * a.nx * (2 * PK_M) * window_pad(a.d) * sizeof(float);
 }
 // the larger of what the two kernels leave, one after the other
 size_t part_bytes(PackArgs a, int dtype) {
@@ -711,22 +703,25 @@ int launch_bwd(hipStream_t s, PackArgs a) {
   const bool fast = dma && a.d == 128;
   PackArgs q = a;
   query_plan(q, BN);
-  const unsigned qgrid = (unsigned)packed_grid(a.H >> q.hs, (long)q.nx * q.chunks);
+  chunk_memory(q, a.part, 0);
+  const long groups = a.H >> q.hs;
+  const unsigned qgrid = (unsigned)packed_grid(groups, q.items > 0 ? q.items : q.nx);
   const int hkv = a.H / a.G;
-  const unsigned kgrid = (unsigned)packed_grid(hkv, (long)a.nx * a.chunks);
+  const unsigned kgrid = (unsigned)packed_grid(hkv, (long)a.nx * a.shares);
   if (fast) packed_dq128_kernel<<<qgrid, 256, 0, s>>>(q);
   else packed_dq_kernel<T, HD, BN, VEC><<<qgrid, 256, 0, s>>>(q);
   int rc = check_launch("packed attention dQ");
   if (rc) return rc;
-  if (q.chunks > 1) {
-    packed_dq_sum_kernel<T, HD, BN><<<(unsigned)packed_grid(a.H, (long)q.nx * (PK_M >> q.hs) / 32), 256, 0, s>>>(q);
+  if (q.items > 0) {
+    packed_dq_sum_kernel<T, HD>
+        <<<(unsigned)packed_grid(groups, (long)q.nx * (HD <= 32 ? 4 : HD <= 64 ? 8 : 16)), 256, 0, s>>>(q);
     rc = check_launch("packed attention dQ sums");
     if (rc) return rc;
   }
   if (fast) packed_dkdv128_kernel<<<kgrid, 256, 0, s>>>(a);
   else packed_dkdv_kernel<T, HD, BQ, VEC><<<kgrid, 256, 0, s>>>(a);
   rc = check_launch("packed attention dK, dV");
-  if (rc || a.chunks == 1) return rc;
+  if (rc || a.shares == 1) return rc;
   packed_sum_kernel<T, HD><<<(unsigned)(2L * PK_M * HD / 1024 * a.nx * hkv), 256, 0, s>>>(a);
   return check_launch("packed attention dK, dV sums");
 }
