@@ -13,8 +13,9 @@ namespace edf {
 struct PackArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
+  bf16* rest;            // [H N d]: what rounding took from a bf16 output, for D; or null
   float *lse, *dd;       // [H N]
-  float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks of keys, maxima and sums;
+  float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks of keys; ml: maxima, two sums;
                          // keys: part [share][Hkv][block] dK and dV of shares of queries
   int* plan;             // queries: [head group][tile] first item and number of chunks
   const int *qo, *ko;
@@ -172,7 +173,7 @@ struct BlockTiles {
 // Where queries are few against the GPU their key tiles are cut into chunks, an item of work each.  All workgroups of a call
 // come to the same plan from the offsets alone: chunks of len key tiles, so that there are about PK_ITEMS of them, numbered
 // from tile to tile.  Item `item` of a head group's; threads look at two tiles each, of which there are fewer than 512.
-constexpr int PK_ITEMS = 768, PK_PLAN = 512;
+constexpr int PK_ITEMS = 512, PK_PLAN = 512;
 struct Item {
   TextTile tile;
   int x, nk, krow, chunk, chunks, len;  // the tile's number, its text's keys, which of its chunks, how many, key tiles of one

@@ -11,8 +11,10 @@
 // Where queries are few against the GPU, the key tiles are cut into chunks, a workgroup each, which leave unnormalised
 // outputs with their maxima and sums to a second kernel.
 //
-// Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and its sum is that
-// of the rounded values, so the weights of a row add to one.  float32 runs on the float32 matrix instructions.
+// Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and O's sum is that
+// of the rounded values, so the weights of a row add to one.  For the backward, the row sums of partly hidden tiles, the
+// only ones of a row of few keys, are those of P as it was (the others' roundings even out), and what O's own rounding took
+// is kept in bf16 beside it.  float32 runs on the float32 matrix instructions.
 #include <math.h>
 #include <stdint.h>
 
@@ -25,6 +27,9 @@ namespace edf {
 namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
+
+// what rounding x to bf16 takes from it
+EDF_DEVICE bf16 rounded_off(float x) { return (bf16)(x - (float)(bf16)x); }
 
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(PackArgs a) {
@@ -47,7 +52,7 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
   f32x16 o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
-  float m = -INFINITY, lsum = 0.0f;
+  float m = -INFINITY, lsum = 0.0f, lex = 0.0f;
 
   const TileLoader<T, HD, BN, VEC> ld(tid, d, qt.nk);
   WFrag<T> rk[ld.N], rv[ld.N];
@@ -85,6 +90,7 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
       const float mnew = fmaxf(m, mx);
       const float alpha = fast_exp2(m * a.scale_log2 - (mnew == -INFINITY ? 0.0f : mnew * a.scale_log2));
       lsum *= alpha;
+      lex *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -92,17 +98,21 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
       m = mnew;
     }
     const float mns = m == -INFINITY ? 0.0f : m * a.scale_log2;
-    float rs = 0.0f;
+    float rs = 0.0f, re = 0.0f;
     WFrag<T> pf[2 * NH];
 #pragma unroll
     for (int kc = 0; kc < 2 * NH; ++kc)
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const int r = 8 * (kc & 1) + e;
-        rs = pf[kc].set2(e, fast_exp2(fmaf(s[kc >> 1][r], a.scale_log2, -mns)),
-                         fast_exp2(fmaf(s[kc >> 1][r + 1], a.scale_log2, -mns)), rs);
+        const float p0 = fast_exp2(fmaf(s[kc >> 1][r], a.scale_log2, -mns));
+        const float p1 = fast_exp2(fmaf(s[kc >> 1][r + 1], a.scale_log2, -mns));
+        rs = pf[kc].set2(e, p0, p1, rs);
+        if constexpr (MASK && sizeof(T) == 2) re += p0 + p1;
       }
-    lsum += rs + __shfl_xor(rs, 32);
+    rs += __shfl_xor(rs, 32);
+    lsum += rs;
+    lex += MASK && sizeof(T) == 2 ? re + __shfl_xor(re, 32) : rs;
     edf::ahead<2 * NH * NDT, AHEAD>([&](int i) { return Tile::trans(sv, 16 * (i / NDT), i % NDT, l); },
                                [&](int i, const WFrag<T>& f) { o[i % NDT] = WFrag<T>::mma(f, pf[i / NDT], o[i % NDT]); });
   };
@@ -140,8 +150,9 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
         *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
             f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
     if (g == 0) {
-      a.ml[2 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
-      a.ml[2 * qt.slot + 1] = lsum;
+      a.ml[3 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[3 * qt.slot + 1] = lsum;
+      a.ml[3 * qt.slot + 2] = lex;
     }
     return;
   }
@@ -164,8 +175,27 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
           if (c + e < d) O[c + e] = from_f32<T>(o[dt][rb * 4 + e] * inv);
       }
     }
+  if (sizeof(T) == 2 && a.rest != nullptr) {
+    bf16* R = a.rest + row * d;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int rb = 0; rb < 4; ++rb) {
+        const int c = dt * 32 + 8 * rb + 4 * g;
+        bf16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = rounded_off(o[dt][rb * 4 + e] * inv);
+        if (VEC && c + 4 <= d) {
+          *(bf16x4*)(R + c) = v;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c + e < d) R[c + e] = v[e];
+        }
+      }
+  }
   if (g == 0 && a.lse != nullptr)
-    a.lse[row] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
+    a.lse[row] = lex == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lex)) * LN2;
 }
 
 // bf16 at head_dim 128: the same decomposition with tiles moved by 16-byte DMA loads into half-row-block LDS
@@ -194,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
   f32x16 o[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = zero16();
-  float m = -INFINITY, lsum = 0.0f;
+  float m = -INFINITY, lsum = 0.0f, lex = 0.0f;
 
   const int grp = l >> 4, i16 = l & 15;
   const int d0 = 16 * (grp & 1) + 4 * (i16 & 3), kr = 4 * (grp >> 1) + (i16 >> 2);
@@ -238,6 +268,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
       const float mnew = fmaxf(m, mx);
       const float alpha = fast_exp2(m * a.scale_log2 - (mnew == -INFINITY ? 0.0f : mnew * a.scale_log2));
       lsum *= alpha;
+      lex *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -248,13 +279,14 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
   };
   // second half for elements 2 j, 2 j + 1: p into the row sum and the P^T fragments.  pin: an empty volatile asm
   // keeps this arithmetic in the scheduling step that issued it.
-  auto softmax_pair = [&](f32x16* s, int j, float mns, float& rs, bf16x8* pf, auto pin) __attribute__((always_inline)) {
+  auto softmax_pair = [&](f32x16* s, int j, float mns, float& rs, float& re, bf16x8* pf, auto pin) __attribute__((always_inline)) {
     const int h = j >> 3, r = (2 * j) & 15;
     const float p0 = fast_exp2(fmaf(s[h][r], a.scale_log2, -mns)), p1 = fast_exp2(fmaf(s[h][r + 1], a.scale_log2, -mns));
     unsigned pk = pack_bf16x2(p0, p1);
     // the row sum of the bf16 P that the product consumes, one dot2 per pair
     rs = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pk), bf16x2{(bf16)1.0f, (bf16)1.0f}, rs, false);
     if constexpr (decltype(pin)::value) asm volatile("" : "+v"(pk), "+v"(rs));
+    else re += p0 + p1;
     const int kc = 2 * h + (r >> 3), it = r & 7;
     const bf16x2 pp = __builtin_bit_cast(bf16x2, pk);
     pf[kc][it] = pp[0];
@@ -277,11 +309,12 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
   };
   auto consume = [&](auto bt, f32x16* s, int t, auto masked) __attribute__((always_inline)) {
     const float mns = softmax_max(s, t, masked);
-    float rs = 0.0f;
+    float rs = 0.0f, re = 0.0f;
     bf16x8 pf[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) softmax_pair(s, j, mns, rs, pf, std::false_type{});
+    for (int j = 0; j < 16; ++j) softmax_pair(s, j, mns, rs, re, pf, std::false_type{});
     lsum += rs + __shfl_xor(rs, 32);
+    lex += re + __shfl_xor(re, 32);
     pv_mma(bt, pf);
   };
   // whole tile t with a successor: the 16 products of S(t + 1) alternate with the exponentials of S(t)
@@ -302,10 +335,12 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
     for (int i = 0; i < 16; ++i) {
       sn[i & 1] = mfma32(fr[i & 3], qf[i >> 1], sn[i & 1]);
       if (i + 4 < 16) fr[i & 3] = kfrag(i + 4);
-      softmax_pair(sc, i, mns, rs, pf, std::true_type{});
+      softmax_pair(sc, i, mns, rs, rs, pf, std::true_type{});
       __builtin_amdgcn_sched_barrier(0);
     }
-    lsum += rs + __shfl_xor(rs, 32);
+    rs += __shfl_xor(rs, 32);
+    lsum += rs;
+    lex += rs;
     pv_mma(bt, pf);
   };
   const std::integral_constant<int, 0> b0{};
@@ -353,32 +388,42 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
         *(f32x4*)(out + dt * 32 + 8 * rb + 4 * g) =
             f32x4{o[dt][rb * 4], o[dt][rb * 4 + 1], o[dt][rb * 4 + 2], o[dt][rb * 4 + 3]};
     if (g == 0) {
-      a.ml[2 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
-      a.ml[2 * qt.slot + 1] = lsum;
+      a.ml[3 * qt.slot] = m == -INFINITY ? -INFINITY : m * a.scale_log2;
+      a.ml[3 * qt.slot + 1] = lsum;
+      a.ml[3 * qt.slot + 2] = lex;
     }
     return;
   }
-  // O through the free array X0 (each wave its 32 rows), written as whole rows
-  bf16* so = sX0 + w * 32 * HD;
+  // O through the free array X0 (each wave its 32 rows), written as whole rows, and what its rounding took through X1
   const float inv = myq >= qt.nq || lsum == 0.0f ? 0.0f : 1.0f / lsum;
+  const bool rest = a.rest != nullptr;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int rb = 0; rb < 4; ++rb) {
-      bf16x4 v;
+      const int at = w * 32 * HD + lds_off<HD>(li, dt * 32 + 8 * rb + 4 * g);
+      bf16x4 v, r;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (bf16)(o[dt][rb * 4 + e] * inv);
-      *(bf16x4*)(so + lds_off<HD>(li, dt * 32 + 8 * rb + 4 * g)) = v;
+      *(bf16x4*)(sX0 + at) = v;
+      if (rest) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = rounded_off(o[dt][rb * 4 + e] * inv);
+        *(bf16x4*)(sX1 + at) = r;
+      }
     }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int e = l + 64 * i, row = e / 16, ch = e % 16;
-    if (myq - li + row < qt.nq)
-      *(bf16x8*)((bf16*)a.out + (qt.row0 + myq - li + row) * HD + 8 * ch) = *(const bf16x8*)(so + lds_off<HD>(row, 8 * ch));
+    const int e = l + 64 * i, row = e / 16, ch = e % 16, at = w * 32 * HD + lds_off<HD>(row, 8 * ch);
+    if (myq - li + row < qt.nq) {
+      const long to = (qt.row0 + myq - li + row) * HD + 8 * ch;
+      *(bf16x8*)((bf16*)a.out + to) = *(const bf16x8*)(sX0 + at);
+      if (rest) *(bf16x8*)(a.rest + to) = *(const bf16x8*)(sX1 + at);
+    }
   }
   if (myq < qt.nq && g == 0 && a.lse != nullptr)
-    a.lse[qt.row0 + myq] = lsum == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lsum)) * LN2;
+    a.lse[qt.row0 + myq] = lex == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lex)) * LN2;
 }
 
 // The chunks of a row joined: out = sum_c 2^(m_c - m) O_c / sum_c 2^(m_c - m) l_c, four elements a lane.
@@ -388,24 +433,28 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
   const ChunkRow<LANES> r(a);
   if (r.chunks == 0) return;
   const int j = threadIdx.x % LANES, e = 4 * j;
-  const float* ml = a.ml + 2 * r.slot;
-  float m = -INFINITY, sum = 0.0f;
-  for (int c = j; c < r.chunks; c += LANES) m = fmaxf(m, ml[2L * PK_M * c]);
+  const float* ml = a.ml + 3 * r.slot;
+  float m = -INFINITY, sum = 0.0f, exact = 0.0f;
+  for (int c = j; c < r.chunks; c += LANES) m = fmaxf(m, ml[3L * PK_M * c]);
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* in = a.part + r.slot * HD + min(e, HD - 4);
 #pragma unroll 4
   for (int c = 0; c < r.chunks; ++c) {
-    const float mc = ml[2L * PK_M * c], f = mc == -INFINITY ? 0.0f : fast_exp2(mc - m);
-    sum = fmaf(f, ml[2L * PK_M * c + 1], sum);
+    const float mc = ml[3L * PK_M * c], f = mc == -INFINITY ? 0.0f : fast_exp2(mc - m);
+    sum = fmaf(f, ml[3L * PK_M * c + 1], sum);
+    exact = fmaf(f, ml[3L * PK_M * c + 2], exact);
     acc += f * *(const f32x4*)(in + (long)PK_M * HD * c);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (e + i < a.d) st((T*)a.out, r.row * a.d + e + i, acc[i] * inv);
-  if (j == 0 && a.lse != nullptr) a.lse[r.row] = sum == 0.0f ? INFINITY : (m + __log2f(sum)) * LN2;
+    if (e + i < a.d) {
+      st((T*)a.out, r.row * a.d + e + i, acc[i] * inv);
+      if (sizeof(T) == 2 && a.rest != nullptr) a.rest[r.row * a.d + e + i] = rounded_off(acc[i] * inv);
+    }
+  if (j == 0 && a.lse != nullptr) a.lse[r.row] = exact == 0.0f ? INFINITY : (m + __log2f(exact)) * LN2;
 }
 
 template <typename T, int HD, int BN, bool VEC>
@@ -463,11 +512,11 @@ size_t edf_packed_attention_workspace_bytes(int num_heads, int num_kv_heads, lon
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   query_plan(a, key_tile(dtype));
-  return chunk_bytes(a, 2);
+  return chunk_bytes(a, 3);
 }
 
 int edf_packed_attention(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                         const int32_t* key_offsets, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                         const int32_t* key_offsets, void* out, float* lse, void* rest, void* workspace, size_t workspace_bytes,
                          int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim, int window,
                          int sinks, int dtype) {
   using namespace edf;
@@ -476,15 +525,16 @@ int edf_packed_attention(void* stream, const void* q, const void* k, const void*
   EDF_REQUIRE(q && k && v && offsets && key_offsets && out, EDF_ERR_INVALID_ARG, "null tensor pointer");
   PackArgs a{};
   a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.out = out, a.lse = lse;
+  a.rest = dtype == EDF_BF16 ? (bf16*)rest : nullptr;
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
   query_plan(a, key_tile(dtype));
-  const size_t need = chunk_bytes(a, 2);
+  const size_t need = chunk_bytes(a, 3);
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
-  chunk_memory(a, (float*)workspace, 2);
-  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
+  chunk_memory(a, (float*)workspace, 3);
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)a.rest;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && key_rows <= WINDOW_VEC_T;
   hipStream_t s = as_stream(stream);
   if (dtype == EDF_BF16) return vec ? launch_fwd_d<bf16, 64, true>(s, a) : launch_fwd_d<bf16, 64, false>(s, a);

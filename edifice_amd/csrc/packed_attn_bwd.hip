@@ -9,8 +9,8 @@
 //   query tiles that see one of them, query head by query head: the sum over shared heads needs no atomics.  Where key
 //   blocks are few against the GPU, each block's query tiles are shared out evenly among several workgroups, which leave
 //   float32 sums, added in order by a third kernel.
-// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term), D is formed from the rounded O that
-// the forward left, and P from the forward's sum of rounded probabilities; everything else is float32.
+// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term); D is formed from O and what its
+// rounding took (off by 2^-17 of each term), and everything else is float32.
 #include <math.h>
 #include <stdint.h>
 
@@ -47,6 +47,13 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     const WFrag<T> oo = window_row<T, HD, VEC>((const T*)a.o + qrow * d, col, d);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dd = fmaf(oo.get(e), of[kk].get(e), dd);
+    if constexpr (sizeof(T) == 2) {
+      if (a.rest != nullptr) {
+        const WFrag<T> rr = window_row<T, HD, VEC>(a.rest + qrow * d, col, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dd = fmaf(rr.get(e), of[kk].get(e), dd);
+      }
+    }
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
@@ -182,6 +189,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     const bf16x8 ov = *(const bf16x8*)((const bf16*)a.o + at);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)ov[e], dd);
+    if (a.rest != nullptr) {
+      const bf16x8 rv = *(const bf16x8*)(a.rest + at);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)rv[e], dd);
+    }
   }
   dd += __shfl_xor(dd, 32);
   const float lse = a.lse[qrow] * LOG2E;
@@ -751,7 +763,8 @@ size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_h
 }
 
 int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                                  const int32_t* key_offsets, const void* out, const void* grad_out, const float* lse,
+                                  const int32_t* key_offsets, const void* out, const void* rest, const void* grad_out,
+                                  const float* lse,
                                   void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
                                   int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim,
                                   int window, int sinks, int dtype) {
@@ -762,6 +775,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
               EDF_ERR_INVALID_ARG, "null tensor pointer (the forward's lse is required)");
   PackArgs a{};
   a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.o = out, a.go = grad_out;
+  a.rest = dtype == EDF_BF16 ? (bf16*)const_cast<void*>(rest) : nullptr;
   a.lse = const_cast<float*>(lse), a.dq = grad_q, a.dk = grad_k, a.dv = grad_v;
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
@@ -771,7 +785,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
   EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   a.dd = (float*)workspace;
   a.part = (float*)((char*)workspace + row_bytes(num_heads, rows));
-  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)grad_out |
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)a.rest | (uintptr_t)grad_out |
                          (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) &&
                    std::max(rows, key_rows) <= WINDOW_VEC_T;
