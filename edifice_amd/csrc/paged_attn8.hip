@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <=
     vx = fmaxf(vx, __shfl_xor(vx, 32));
     const float mnew = fmaxf(m, mx);
     const float mns = mnew == -INFINITY ? 0.0f : mnew;
-    const int venew = max(ve, __builtin_amdgcn_frexp_expf(vx));  // that of 0 is 0, of a wave without keys, or of zeros alone
+    const int venew = vx > 0.0f ? max(ve, __builtin_amdgcn_frexp_expf(vx)) : ve;
     if (__any(mnew > m || venew > ve)) {
       const float alpha = fast_exp2(m - mns), beta = ldexpf(alpha, ve - venew);
       lsum *= alpha;

@@ -316,6 +316,23 @@ def test_attention_scales_far_apart():
             0, f32)
 
 
+def test_pages_of_zeros_before_tiny_ones():
+    """Pages whose scale is 0 (all zeros) do not set what later, tiny ones are held against."""
+    from edifice_amd import fused_scan as fs
+    announce("paged_attention8, zeros before tiny values")
+    for code, dtype in (("int8", f32), ("e4m3", bf16)):
+        g = torch.Generator().manual_seed(10)
+        caches, table, n = _pool((300,), 1, 16, 64, code, g)
+        (kc, ks), (vc, vs) = caches
+        vs *= 2.0 ** -80
+        vs[table[0, :8].long()] = 0.0
+        q = torch.randn(1, 2, 64, generator=g).to(dtype)
+        (kd, ksd), (vd, vsd) = (_to_gpu(*c, code) for c in caches)
+        got = fs.paged_attention(q.cuda(), kd, vd, table.cuda(), n.cuda(), k_scale=ksd, v_scale=vsd)
+        assert bool(got.any())
+        _expect(got, q, caches, table, n, 0, 0, dtype)
+
+
 def test_page_that_is_not_finite_reaches_who_sees_it():
     from edifice_amd import fused_scan as fs
     announce("paged_attention8, a page of NaN")
