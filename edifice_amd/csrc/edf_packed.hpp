@@ -38,25 +38,45 @@ inline long packed_tiles(long rows, long texts, int m) { return rows / m + texts
 
 struct TextTile {
   int text, row0, n, first;  // the text, its first row and its rows; the tile's first row within the text (>= n: no tile)
+  int other0, m;             // its first row and rows in the other tensor (none behind the last text)
 };
 EDF_DEVICE int text_begin(const int* off, int s, int rows) { return s == 0 ? 0 : min(max(off[s], 0), rows); }
 EDF_DEVICE int text_end(const int* off, int S, int s, int rows, int begin) {
   return s >= S ? rows : max(text_begin(off, s + 1, rows), begin);
 }
+// the rows of text s in the other tensor
+EDF_DEVICE void other_rows(const int* off, int S, int rows, TextTile& t) {
+  t.other0 = t.m = 0;
+  if (t.text == S) return;
+  t.other0 = __builtin_amdgcn_readfirstlane(text_begin(off, t.text, rows));
+  t.m = max(__builtin_amdgcn_readfirstlane(text_begin(off, t.text + 1, rows)) - t.other0, 0);
+}
 // tile x of 2^ms rows; all 64 lanes of a wave take part; the result is uniform
-EDF_DEVICE TextTile find_tile(const int* off, int S, int rows, int ms, int x) {
+EDF_DEVICE TextTile find_tile(const int* off, int rows, const int* off2, int rows2, int S, int ms, int x) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, hi = S + 1;  // the text's number is in [lo, hi)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-    const bool at = s < hi && (text_begin(off, min(s, S), rows) >> ms) + s <= x;
-    lo += (max((int)__popcll(__ballot(at)), 1) - 1) * step;
-    hi = min(hi, lo + step);
-  }
   TextTile t;
-  t.text = __builtin_amdgcn_readfirstlane(lo);
-  t.row0 = __builtin_amdgcn_readfirstlane(text_begin(off, t.text, rows));
-  t.n = __builtin_amdgcn_readfirstlane(text_end(off, S, t.text, rows, t.row0)) - t.row0;
+  if (S < 64) {  // a lane a text: all offsets in one load
+    const int s = min(lane, S), b = text_begin(off, s, rows), e = text_end(off, S, s, rows, b);
+    const int b2 = s == S ? 0 : text_begin(off2, s, rows2), e2 = s == S ? 0 : max(text_begin(off2, s + 1, rows2), b2);
+    const int from = max((int)__popcll(__ballot(lane <= S && (b >> ms) + lane <= x)), 1) - 1;
+    t.text = from;
+    t.row0 = __builtin_amdgcn_readlane(b, from);
+    t.n = __builtin_amdgcn_readlane(e, from) - t.row0;
+    t.other0 = __builtin_amdgcn_readlane(b2, from);
+    t.m = __builtin_amdgcn_readlane(e2, from) - t.other0;
+  } else {
+    int lo = 0, hi = S + 1;  // the text's number is in [lo, hi)
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 63) / 64, s = lo + lane * step;
+      const bool at = s < hi && (text_begin(off, min(s, S), rows) >> ms) + s <= x;
+      lo += (max((int)__popcll(__ballot(at)), 1) - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    t.text = __builtin_amdgcn_readfirstlane(lo);
+    t.row0 = __builtin_amdgcn_readfirstlane(text_begin(off, t.text, rows));
+    t.n = __builtin_amdgcn_readfirstlane(text_end(off, S, t.text, rows, t.row0)) - t.row0;
+    other_rows(off2, S, rows2, t);
+  }
   t.first = (x - (t.row0 >> ms) - t.text) << ms;
   return t;
 }
@@ -69,7 +89,8 @@ EDF_DEVICE int wave_sum_i(int v) {
 // from the start) of their text come before those that are (r - 1)-th.  A tile of queries sees the keys before it, a tile of
 // keys is seen by the queries behind it, so that the longest work comes first, whichever text it is in.
 // f(r) = sum over texts of max(0, tiles - r) tiles come before the r-th ones, of which a text with r tiles or more has one.
-EDF_DEVICE TextTile find_tile_by_work(const int* off, int S, int rows, int ms, int x, bool last_first) {
+EDF_DEVICE TextTile find_tile_by_work(const int* off, int rows, const int* off2, int rows2, int S, int ms, int x,
+                                      bool last_first) {
   constexpr int C = PK_SORT / 64;
   const int lane = threadIdx.x & 63;
   int nb[C], begin[C], size[C];
@@ -86,7 +107,7 @@ EDF_DEVICE TextTile find_tile_by_work(const int* off, int S, int rows, int ms, i
     for (int c = 0; c < C; ++c) v += max(nb[c] - r, 0);
     return __builtin_amdgcn_readfirstlane(wave_sum_i(v));
   };
-  TextTile t{0, 0, 0, 0};
+  TextTile t{0, 0, 0, 0, 0, 0};
   if (x >= before(0)) return t;  // past the last tile
   int lo = 0, hi = ((rows - 1) >> ms) + 1;  // before(lo) > x >= before(hi): no text has more than hi tiles
   while (hi - lo > 1) {
@@ -110,16 +131,9 @@ EDF_DEVICE TextTile find_tile_by_work(const int* off, int S, int rows, int ms, i
     }
     rank -= count;
   }
+  other_rows(off2, S, rows2, t);
   return t;
 }
-// the rows of text s among `rows` (none behind the last text)
-EDF_DEVICE void text_rows(const int* off, int S, int rows, int s, int& row0, int& n) {
-  row0 = n = 0;
-  if (s == S) return;
-  row0 = __builtin_amdgcn_readfirstlane(text_begin(off, s, rows));
-  n = __builtin_amdgcn_readfirstlane(text_end(off, S, s, rows, row0)) - row0;
-}
-
 // Workgroups of `groups` heads (or groups of heads) with `per` tiles each go round the eight XCDs.  A head's tiles, which
 // share its keys, stay on as few of them as give every XCD the same share of each part of the tiles' order, in which work
 // falls: one where there are a multiple of eight heads, 8 / groups of them for 1, 2 or 4 heads, all for any other number.
@@ -176,7 +190,7 @@ struct BlockTiles {
 constexpr int PK_ITEMS = 512, PK_PLAN = 512;
 struct Item {
   TextTile tile;
-  int x, nk, krow, chunk, chunks, len;  // the tile's number, its text's keys, which of its chunks, how many, key tiles of one
+  int x, chunk, chunks, len;  // the tile's number, which of its chunks, how many, key tiles of one
   bool none;
 };
 template <int BN>
@@ -249,8 +263,8 @@ EDF_DEVICE Item find_item(const PackArgs& a, int groups, int item, int* lds) {
   t.tile.row0 = __builtin_amdgcn_readfirstlane(so[s]);
   t.tile.n = __builtin_amdgcn_readfirstlane(max(so[s + 1] - so[s], 0));
   t.tile.first = (t.x - (t.tile.row0 >> ms) - s) << ms;
-  t.krow = s < a.S ? __builtin_amdgcn_readfirstlane(sk[s]) : 0;
-  t.nk = s < a.S ? __builtin_amdgcn_readfirstlane(max(sk[s + 1] - sk[s], 0)) : 0;
+  t.tile.other0 = s < a.S ? __builtin_amdgcn_readfirstlane(sk[s]) : 0;
+  t.tile.m = s < a.S ? __builtin_amdgcn_readfirstlane(max(sk[s + 1] - sk[s], 0)) : 0;
   t.chunk = __builtin_amdgcn_readfirstlane(found[2]);
   t.chunks = __builtin_amdgcn_readfirstlane(found[3]);
   t.len = __builtin_amdgcn_readfirstlane(len);
@@ -271,7 +285,7 @@ struct QueryTile {
   EDF_DEVICE QueryTile(const PackArgs& a, void* lds) : kt(0, 0, 0, 1, 0) {
     const int w = threadIdx.x >> 6, li = threadIdx.x & 31, wu = __builtin_amdgcn_readfirstlane(w);
     const int groups = a.H >> a.hs, ms = 7 - a.hs;
-    int x, grp, key0, chunk = 0, len = 0;
+    int x, grp, chunk = 0, len = 0;
     none = !packed_block(groups, a.items > 0 ? a.items : a.nx, x, grp);
     if (none) return;
     TextTile t;
@@ -280,7 +294,7 @@ struct QueryTile {
       const Item it = find_item<BN>(a, groups, x, (int*)lds);
       none = it.none;
       if (none) return;
-      t = it.tile, key0 = it.krow, nk = it.nk, chunk = it.chunk, len = it.len;
+      t = it.tile, chunk = it.chunk, len = it.len;
       if (it.chunks > 1) slot = ((long)grp * a.items + x) * PK_M + 32 * w + li;
       if (chunk == 0 && threadIdx.x == 0) {
         int* p = a.plan + 2 * ((long)grp * a.nx + it.x);
@@ -288,19 +302,19 @@ struct QueryTile {
         p[1] = it.chunks;
       }
     } else {
-      t = a.by_work ? find_tile_by_work(a.qo, a.S, a.N, ms, x, true) : find_tile(a.qo, a.S, a.N, ms, a.nx - 1 - x);
+      t = a.by_work ? find_tile_by_work(a.qo, a.N, a.ko, a.M, a.S, ms, x, true)
+                    : find_tile(a.qo, a.N, a.ko, a.M, a.S, ms, a.nx - 1 - x);
       none = t.first >= t.n;
       if (none) return;
-      text_rows(a.ko, a.S, a.M, t.text, key0, nk);
     }
     head = (grp << a.hs) + (wu & ((1 << a.hs) - 1));
     kvhead = (grp << a.hs) / a.G;
-    nq = t.n;
+    nq = t.n, nk = t.m;
     const int wq = t.first + 32 * (w >> a.hs);  // the wave's first query
     myq = wq + li;
     pw = wq + nk - nq;
     row0 = (long)head * a.N + t.row0;
-    krow = (long)kvhead * a.M + key0;
+    krow = (long)kvhead * a.M + t.other0;
     kt = BlockTiles<BN>(t.first + nk - nq, PK_M >> a.hs, nk, a.W, a.sinks);
     first = chunk == 0;
     t0 = chunk * len;
@@ -323,7 +337,7 @@ struct ChunkRow {
     int x, grp;
     if (!packed_block(a.H >> a.hs, a.nx * PIECES, x, grp)) return;
     const int ms = 7 - a.hs, r = x % PIECES * (256 / LANES) + threadIdx.x / LANES;
-    const TextTile t = find_tile(a.qo, a.S, a.N, ms, x / PIECES);
+    const TextTile t = find_tile(a.qo, a.N, a.ko, a.M, a.S, ms, x / PIECES);
     const int q = t.first + 32 * (r >> 5 >> a.hs) + (r & 31);
     if (t.first >= t.n || q >= t.n) return;
     const int* p = a.plan + 2 * ((long)grp * a.nx + x / PIECES);

@@ -298,10 +298,11 @@ struct KeyBlock {
   bool none;
   EDF_DEVICE int ahead() const { return nk - nq; }
   EDF_DEVICE KeyBlock(const PackArgs& a, int id_x, int id_head, int share_) : head(id_head), share(share_) {
-    const TextTile t = a.by_work ? find_tile_by_work(a.ko, a.S, a.M, 7, id_x, false) : find_tile(a.ko, a.S, a.M, 7, id_x);
+    const TextTile t = a.by_work ? find_tile_by_work(a.ko, a.M, a.qo, a.N, a.S, 7, id_x, false)
+                                 : find_tile(a.ko, a.M, a.qo, a.N, a.S, 7, id_x);
     krow = t.row0, nk = t.n, first = t.first;
     none = first >= nk;
-    text_rows(a.qo, a.S, a.N, t.text, qrow, nq);
+    qrow = t.other0, nq = t.m;
     qs = max(0, first - ahead());  // the first query that sees the block's first key
     int end = nq;
     if (first >= a.sinks) end = (int)min((long)nq, (long)first + PK_M - 1 + a.W - ahead());  // past the last key's window
@@ -653,7 +654,7 @@ template <typename T, int HD>
 __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
   constexpr int PIECES = 2 * PK_M * HD / 1024;
   const int piece = blockIdx.x % PIECES, x = blockIdx.x / PIECES % a.nx, head = blockIdx.x / PIECES / a.nx;
-  const TextTile t = find_tile(a.ko, a.S, a.M, 7, x);
+  const TextTile t = find_tile(a.ko, a.M, a.qo, a.N, a.S, 7, x);
   const int e = (piece * 256 + threadIdx.x) * 4;
   const bool is_v = e >= PK_M * HD;
   const int key = t.first + e / HD % PK_M, c = e % HD;
