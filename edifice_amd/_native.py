@@ -76,10 +76,10 @@ SIGNATURES = {
     "edf_window_attention_backward": (
         I, [P, P, P, P, P, P, P, P, P, P, P, S, I, I, I, I, I, I, I, I]),
     "edf_packed_attention_workspace_bytes": (S, [I, I, L, L, I, I, I, I, I]),
-    "edf_packed_attention": (I, [P, P, P, P, P, P, P, P, P, P, S, I, I, L, L, I, I, I, I, I]),
+    "edf_packed_attention": (I, [P, P, P, P, P, P, P, P, P, S, I, I, L, L, I, I, I, I, I]),
     "edf_packed_attention_backward_workspace_bytes": (S, [I, I, L, L, I, I, I, I, I]),
     "edf_packed_attention_backward": (
-        I, [P, P, P, P, P, P, P, P, P, P, P, P, P, P, S, I, I, L, L, I, I, I, I, I]),
+        I, [P, P, P, P, P, P, P, P, P, P, P, P, P, S, I, I, L, L, I, I, I, I, I]),
     "edf_paged_extend": (I, [P, P, P, P, P, P, P, P, P, I, I, I, I, I]),
     "edf_paged_cache_write": (I, [P, P, P, P, P, P, L, L, I, I, L, I, I]),
     "edf_paged_attention_workspace_bytes": (S, [I, I, I, I, I, I, I, I]),

@@ -13,7 +13,6 @@ namespace edf {
 struct PackArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
-  bf16* rest;            // [H N d]: what rounding took from a bf16 output, for D; or null
   float *lse, *dd;       // [H N]
   float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks of keys; ml: maxima, two sums;
                          // keys: part [share][Hkv][block] dK and dV of shares of queries

@@ -13,8 +13,8 @@
 //
 // Scores, softmax and O are float32.  In bf16 P is rounded to bf16 for the product (2^-8 of each term), and O's sum is that
 // of the rounded values, so the weights of a row add to one.  For the backward, the row sums of partly hidden tiles, the
-// only ones of a row of few keys, are those of P as it was (the others' roundings even out), and what O's own rounding took
-// is kept in bf16 beside it.  float32 runs on the float32 matrix instructions.
+// only ones of a row of few keys, are those of P as it was (the others' roundings even out).  float32 runs on the float32
+// matrix instructions.
 #include <math.h>
 #include <stdint.h>
 
@@ -27,9 +27,6 @@ namespace edf {
 namespace {
 
 constexpr float LN2 = 0.6931471805599453f;
-
-// what rounding x to bf16 takes from it
-EDF_DEVICE bf16 rounded_off(float x) { return (bf16)(x - (float)(bf16)x); }
 
 template <typename T, int HD, int BN, bool VEC>
 __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(PackArgs a) {
@@ -175,25 +172,6 @@ __global__ __launch_bounds__(256, (HD <= 64 ? 3 : 2)) void packed_fwd_kernel(Pac
           if (c + e < d) O[c + e] = from_f32<T>(o[dt][rb * 4 + e] * inv);
       }
     }
-  if (sizeof(T) == 2 && a.rest != nullptr) {
-    bf16* R = a.rest + row * d;
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-      for (int rb = 0; rb < 4; ++rb) {
-        const int c = dt * 32 + 8 * rb + 4 * g;
-        bf16x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = rounded_off(o[dt][rb * 4 + e] * inv);
-        if (VEC && c + 4 <= d) {
-          *(bf16x4*)(R + c) = v;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (c + e < d) R[c + e] = v[e];
-        }
-      }
-  }
   if (g == 0 && a.lse != nullptr)
     a.lse[row] = lex == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lex)) * LN2;
 }
@@ -394,33 +372,24 @@ __global__ __launch_bounds__(256, 2) void packed_fwd128_kernel(PackArgs a) {
     }
     return;
   }
-  // O through the free array X0 (each wave its 32 rows), written as whole rows, and what its rounding took through X1
+  // O through the free array X0 (each wave its 32 rows), written as whole rows
+  bf16* so = sX0 + w * 32 * HD;
   const float inv = myq >= qt.nq || lsum == 0.0f ? 0.0f : 1.0f / lsum;
-  const bool rest = a.rest != nullptr;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int rb = 0; rb < 4; ++rb) {
-      const int at = w * 32 * HD + lds_off<HD>(li, dt * 32 + 8 * rb + 4 * g);
-      bf16x4 v, r;
+      bf16x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = (bf16)(o[dt][rb * 4 + e] * inv);
-      *(bf16x4*)(sX0 + at) = v;
-      if (rest) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = rounded_off(o[dt][rb * 4 + e] * inv);
-        *(bf16x4*)(sX1 + at) = r;
-      }
+      *(bf16x4*)(so + lds_off<HD>(li, dt * 32 + 8 * rb + 4 * g)) = v;
     }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int e = l + 64 * i, row = e / 16, ch = e % 16, at = w * 32 * HD + lds_off<HD>(row, 8 * ch);
-    if (myq - li + row < qt.nq) {
-      const long to = (qt.row0 + myq - li + row) * HD + 8 * ch;
-      *(bf16x8*)((bf16*)a.out + to) = *(const bf16x8*)(sX0 + at);
-      if (rest) *(bf16x8*)(a.rest + to) = *(const bf16x8*)(sX1 + at);
-    }
+    const int e = l + 64 * i, row = e / 16, ch = e % 16;
+    if (myq - li + row < qt.nq)
+      *(bf16x8*)((bf16*)a.out + (qt.row0 + myq - li + row) * HD + 8 * ch) = *(const bf16x8*)(so + lds_off<HD>(row, 8 * ch));
   }
   if (myq < qt.nq && g == 0 && a.lse != nullptr)
     a.lse[qt.row0 + myq] = lex == 0.0f ? INFINITY : (m * a.scale_log2 + __log2f(lex)) * LN2;
@@ -450,10 +419,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(PackArgs a) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (e + i < a.d) {
-      st((T*)a.out, r.row * a.d + e + i, acc[i] * inv);
-      if (sizeof(T) == 2 && a.rest != nullptr) a.rest[r.row * a.d + e + i] = rounded_off(acc[i] * inv);
-    }
+    if (e + i < a.d) st((T*)a.out, r.row * a.d + e + i, acc[i] * inv);
   if (j == 0 && a.lse != nullptr) a.lse[r.row] = exact == 0.0f ? INFINITY : (m + __log2f(exact)) * LN2;
 }
 
@@ -516,7 +482,7 @@ size_t edf_packed_attention_workspace_bytes(int num_heads, int num_kv_heads, lon
 }
 
 int edf_packed_attention(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                         const int32_t* key_offsets, void* out, float* lse, void* rest, void* workspace, size_t workspace_bytes,
+                         const int32_t* key_offsets, void* out, float* lse, void* workspace, size_t workspace_bytes,
                          int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim, int window,
                          int sinks, int dtype) {
   using namespace edf;
@@ -525,7 +491,6 @@ int edf_packed_attention(void* stream, const void* q, const void* k, const void*
   EDF_REQUIRE(q && k && v && offsets && key_offsets && out, EDF_ERR_INVALID_ARG, "null tensor pointer");
   PackArgs a{};
   a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.out = out, a.lse = lse;
-  a.rest = dtype == EDF_BF16 ? (bf16*)rest : nullptr;
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
@@ -534,7 +499,7 @@ int edf_packed_attention(void* stream, const void* q, const void* k, const void*
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
   chunk_memory(a, (float*)workspace, 3);
-  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)a.rest;
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) && key_rows <= WINDOW_VEC_T;
   hipStream_t s = as_stream(stream);
   if (dtype == EDF_BF16) return vec ? launch_fwd_d<bf16, 64, true>(s, a) : launch_fwd_d<bf16, 64, false>(s, a);

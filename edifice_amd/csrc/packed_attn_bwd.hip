@@ -3,14 +3,16 @@
 //   dS = P (dP - D) / sqrt(d), dQ = dS K, dK = dS^T Q; dK, dV summed over the query heads of a key head.
 // 10 d flops per visible pair (S and dP formed twice, once for each kernel): bound by the matrix cores.
 //
-//   dQ: a workgroup owns 128 queries of a text (32 per wave, Q^T and dO^T in registers) and walks the key tiles of the
-//   forward; it also forms D and leaves it for the second kernel.
+//   dQ: a workgroup's four waves own 32 queries each (Q^T and dO^T in registers) and walk the key tiles of the forward; it
+//   also forms D and leaves it for the second kernel.
 //   dK, dV: a workgroup owns 128 keys of a text (32 per wave, K^T and V^T in registers) of one key head and walks the
 //   query tiles that see one of them, query head by query head: the sum over shared heads needs no atomics.  Where key
 //   blocks are few against the GPU, each block's query tiles are shared out evenly among several workgroups, which leave
 //   float32 sums, added in order by a third kernel.
-// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term); D is formed from O and what its
-// rounding took (off by 2^-17 of each term), and everything else is float32.
+// In bf16 P and dS are rounded as operands of the second products (2^-8 of each term); D is formed from the rounded O that
+// the forward left, or where keys are few, and O with its rounding as large as V, as sum P dP; everything else is float32.
+// (O's rounding kept in bf16 beside it does the same for twice the bytes of O: forward and backward of 200 texts of 150
+// tokens on average, 16(4)x64, 296 us, and 260 so; of 60 texts of 300, 16(4)x128, 392 and 334.)
 #include <math.h>
 #include <stdint.h>
 
@@ -37,6 +39,9 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
   const long qrow = qt.row0 + min(myq, qt.nq - 1);
   const T *K = (const T*)a.k + qt.krow * d, *V = (const T*)a.v + qt.krow * d;
 
+  // With few keys O is as large as V, and its rounding shows in D = dO . O: D = sum P dP there, from the tiles themselves
+  // (all of them: a chunk has four tiles at least).
+  const bool few = sizeof(T) == 2 && qt.kt.count <= 2;
   WFrag<T> qf[NKK], of[NKK];
   float dd = 0.0f;
 #pragma unroll
@@ -44,20 +49,17 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     const int col = kk * 16 + 8 * g;
     qf[kk] = window_row<T, HD, VEC>((const T*)a.q + qrow * d, col, d);
     of[kk] = window_row<T, HD, VEC>((const T*)a.go + qrow * d, col, d);
-    const WFrag<T> oo = window_row<T, HD, VEC>((const T*)a.o + qrow * d, col, d);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dd = fmaf(oo.get(e), of[kk].get(e), dd);
-    if constexpr (sizeof(T) == 2) {
-      if (a.rest != nullptr) {
-        const WFrag<T> rr = window_row<T, HD, VEC>(a.rest + qrow * d, col, d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dd = fmaf(rr.get(e), of[kk].get(e), dd);
-      }
-    }
   }
-  dd += __shfl_xor(dd, 32);
+  if (!few) {
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const WFrag<T> oo = window_row<T, HD, VEC>((const T*)a.o + qrow * d, kk * 16 + 8 * g, d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dd = fmaf(oo.get(e), of[kk].get(e), dd);
+    }
+    dd += __shfl_xor(dd, 32);
+  }
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
@@ -74,11 +76,8 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     ld.template store<Tile>(sK[buf], rk);
     ld.template store<Tile>(sV[buf], rv);
   };
-  auto tile = [&](int t, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
-    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
+  auto scores = [&](int t, f32x16* s, f32x16* dp) {
     const T *sk = sK[t & 1], *sv = sV[t & 1];
-    f32x16 s[NH], dp[NH];
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
       s[h] = zero16();
@@ -93,6 +92,27 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
           s[i / NKK] = WFrag<T>::mma(f.x, qf[i % NKK], s[i / NKK]);
           dp[i / NKK] = WFrag<T>::mma(f.y, of[i % NKK], dp[i / NKK]);
         });
+  };
+  auto row_sum = [&](int t) {  // this lane's share of sum P dP
+    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
+    f32x16 s[NH], dp[NH];
+    scores(t, s, dp);
+    float x = 0.0f;
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float y = fast_exp2(fmaf(s[h][r], a.scale_log2, -lse)) * dp[h][r];
+        x += sees(h * 32 + d_row(r, 0)) ? y : 0.0f;
+      }
+    return x;
+  };
+  auto tile = [&](int t, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    const SeesKey sees(myp, qt.key0(t) + 4 * g, a.W, a.sinks);
+    const T* sk = sK[t & 1];
+    f32x16 s[NH], dp[NH];
+    scores(t, s, dp);
 #pragma unroll
     for (int h = 0; h < NH; ++h)
 #pragma unroll
@@ -121,17 +141,28 @@ __global__ __launch_bounds__(256, 1) void packed_dq_kernel(PackArgs a) {
     sstore(0);
     if (count > 1) gload(1);
   }
-  __syncthreads();
-  const int masked = min(count, max(qt.kt.first_whole - qt.t0, 0));
-  int t = 0;
-  for (; t < masked; ++t) {
-    if (qt.visible(a, qt.key0(t), BN)) tile(t, std::true_type{});
-    advance(t);
+  if (few) {  // both tiles at once, gone through twice
+    if (count > 1) sstore(1);
+    __syncthreads();
+    for (int t = 0; t < count; ++t)
+      if (qt.visible(a, qt.key0(t), BN)) dd += row_sum(t);
+    dd += __shfl_xor(dd, 32);
+    for (int t = 0; t < count; ++t)
+      if (qt.visible(a, qt.key0(t), BN)) tile(t, std::true_type{});
+  } else {
+    __syncthreads();
+    const int masked = min(count, max(qt.kt.first_whole - qt.t0, 0));
+    int t = 0;
+    for (; t < masked; ++t) {
+      if (qt.visible(a, qt.key0(t), BN)) tile(t, std::true_type{});
+      advance(t);
+    }
+    for (; t < count; ++t) {
+      tile(t, std::false_type{});
+      advance(t);
+    }
   }
-  for (; t < count; ++t) {
-    tile(t, std::false_type{});
-    advance(t);
-  }
+  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   if (myq >= qt.nq) return;
   if (qt.slot >= 0) {
     float* out = a.part + qt.slot * HD;
@@ -179,6 +210,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
   const rsrc_t rK = make_rsrc((const bf16*)a.k + qt.krow * HD, (unsigned)qt.nk * HD * 2);
   const rsrc_t rV = make_rsrc((const bf16*)a.v + qt.krow * HD, (unsigned)qt.nk * HD * 2);
 
+  const bool few = qt.kt.count <= 2;  // as above
   bf16x8 qf[NKK], of[NKK];
   float dd = 0.0f;
 #pragma unroll
@@ -186,18 +218,17 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     const long at = qrow * HD + kk * 16 + 8 * g;
     qf[kk] = *(const bf16x8*)((const bf16*)a.q + at);
     of[kk] = *(const bf16x8*)((const bf16*)a.go + at);
-    const bf16x8 ov = *(const bf16x8*)((const bf16*)a.o + at);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)ov[e], dd);
-    if (a.rest != nullptr) {
-      const bf16x8 rv = *(const bf16x8*)(a.rest + at);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)rv[e], dd);
-    }
   }
-  dd += __shfl_xor(dd, 32);
+  if (!few) {
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const bf16x8 ov = *(const bf16x8*)((const bf16*)a.o + qrow * HD + kk * 16 + 8 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dd = fmaf((float)of[kk][e], (float)ov[e], dd);
+    }
+    dd += __shfl_xor(dd, 32);
+  }
   const float lse = a.lse[qrow] * LOG2E;
-  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   f32x16 dq[NDT];
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) dq[dt] = zero16();
@@ -213,23 +244,48 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     stage_hb<BN>(rK, B ? sR1 : sR0, k0, wu, l);
     stage_hb<BN>(rV, (B ? sR1 : sR0) + BN * HD, k0, wu, l);
   };
+  // S and dP of the 32 keys of half h (a constant) of a tile
+  auto scores = [&](const bf16* sK, int h, f32x16& s, f32x16& dp) __attribute__((always_inline)) {
+    const bf16* sV = sK + BN * HD;
+    s = zero16();
+    dp = zero16();
+#pragma unroll
+    for (int kk = 0; kk < NKK; ++kk) {
+      const int off = krow[kk & 1] + hb_row_off<BN>(kk, 32 * h);
+      s = mfma32(*(const bf16x8*)(&sK[off]), qf[kk], s);
+      dp = mfma32(*(const bf16x8*)(&sV[off]), of[kk], dp);
+    }
+  };
+  auto row_sum = [&](auto bt, int t) {  // this lane's share of sum P dP
+    const bf16* sK = decltype(bt)::value ? sR1 : sR0;
+    const int k0 = qt.key0(t);
+    float x = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int kb = k0 + 32 * h;
+      if (!qt.visible(a, kb, 32)) continue;
+      const SeesKey sees(myp, kb + 4 * g, a.W, a.sinks);
+      f32x16 s, dp;
+      scores(sK, h, s, dp);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float y = fast_exp2(fmaf(s[r], a.scale_log2, -lse)) * dp[r];
+        x += sees(d_row(r, 0)) ? y : 0.0f;
+      }
+    }
+    return x;
+  };
   auto tile = [&](auto bt, int t, auto masked) {
     constexpr bool MASK = decltype(masked)::value;
     const bf16* sK = decltype(bt)::value ? sR1 : sR0;
-    const bf16* sV = sK + BN * HD;
     const int k0 = qt.key0(t);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int kb = k0 + 32 * h;
       if (MASK && !qt.visible(a, kb, 32)) continue;  // no visible pair
       const SeesKey sees(myp, kb + 4 * g, a.W, a.sinks);
-      f32x16 s = zero16(), dp = zero16();
-#pragma unroll
-      for (int kk = 0; kk < NKK; ++kk) {
-        const int off = krow[kk & 1] + hb_row_off<BN>(kk, 32 * h);
-        s = mfma32(*(const bf16x8*)(&sK[off]), qf[kk], s);
-        dp = mfma32(*(const bf16x8*)(&sV[off]), of[kk], dp);
-      }
+      f32x16 s, dp;
+      scores(sK, h, s, dp);
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float x = fast_exp2(fmaf(s[r], a.scale_log2, -lse)) * (dp[r] - dd);
@@ -261,12 +317,22 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
   const std::integral_constant<int, 0> b0{};
   const std::integral_constant<int, 1> b1{};
   if (count > 0) issue(b0, 0);
+  if (few && count > 1) issue(b1, 1);
   wait_vm();
   __syncthreads();
-  for (int t = 0; t < count; t += 2) {
-    step(b0, t);
-    if (t + 1 < count) step(b1, t + 1);
+  if (few) {  // both tiles at once, gone through twice
+    if (count > 0) dd = row_sum(b0, 0);
+    if (count > 1) dd += row_sum(b1, 1);
+    dd += __shfl_xor(dd, 32);
+    if (count > 0) tile(b0, 0, std::true_type{});
+    if (count > 1) tile(b1, 1, std::true_type{});
+  } else {
+    for (int t = 0; t < count; t += 2) {
+      step(b0, t);
+      if (t + 1 < count) step(b1, t + 1);
+    }
   }
+  if (g == 0 && myq < qt.nq && qt.first) a.dd[qrow] = dd;
   if (myq >= qt.nq) return;
   if (qt.slot >= 0) {
     float* out = a.part + qt.slot * HD;
@@ -764,8 +830,8 @@ size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_h
 }
 
 int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                                  const int32_t* key_offsets, const void* out, const void* rest, const void* grad_out,
-                                  const float* lse,
+                                  const int32_t* key_offsets, const void* out, const void* grad_out, const float* lse,
+                                 
                                   void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
                                   int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim,
                                   int window, int sinks, int dtype) {
@@ -776,7 +842,6 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
               EDF_ERR_INVALID_ARG, "null tensor pointer (the forward's lse is required)");
   PackArgs a{};
   a.q = q, a.k = k, a.v = v, a.qo = offsets, a.ko = key_offsets, a.o = out, a.go = grad_out;
-  a.rest = dtype == EDF_BF16 ? (bf16*)const_cast<void*>(rest) : nullptr;
   a.lse = const_cast<float*>(lse), a.dq = grad_q, a.dk = grad_k, a.dv = grad_v;
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
@@ -786,7 +851,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
   EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   a.dd = (float*)workspace;
   a.part = (float*)((char*)workspace + row_bytes(num_heads, rows));
-  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)a.rest | (uintptr_t)grad_out |
+  const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)grad_out |
                          (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) &&
                    std::max(rows, key_rows) <= WINDOW_VEC_T;

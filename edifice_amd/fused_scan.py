@@ -1243,27 +1243,24 @@ class _PackedAttention(torch.autograd.Function):
             raise EdificeHipError("window and sinks must not be negative")
         keep = ctx is not None  # None: no gradient is asked for
         lse = torch.empty((nh, rows), dtype=torch.float32, device=q.device) if keep else None
-        rest = None  # what rounding takes from a bfloat16 output, for the backward
         # more sees no more keys
         conf = (nh, nkv, rows, keys, texts, hd, min(window, max(keys, 1)), min(sinks, keys), dtype_flag(q))
         if q.numel() and keys:
             out = torch.empty_like(q)
-            if keep and q.dtype == torch.bfloat16:
-                rest = torch.empty_like(q)
             wsb = nat.query("edf_packed_attention_workspace_bytes", *conf)
             ws = _u8(wsb, q) if wsb else None
             nat.call("edf_packed_attention", stream, _p(q), _p(k), _p(v), _p(offsets), _p(key_offsets), _p(out), _p(lse),
-                     _p(rest), _p(ws), wsb, *conf)
+                     _p(ws), wsb, *conf)
         else:
             out = torch.zeros_like(q)
         if keep:
             ctx.conf = conf
-            ctx.save_for_backward(q, k, v, offsets, key_offsets, out, lse, rest)
+            ctx.save_for_backward(q, k, v, offsets, key_offsets, out, lse)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        q, k, v, offsets, key_offsets, out, lse, rest = ctx.saved_tensors
+        q, k, v, offsets, key_offsets, out, lse = ctx.saved_tensors
         if not q.numel() or not k.numel():
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None, None
         dout = dout.contiguous().to(q.dtype)
@@ -1271,7 +1268,7 @@ class _PackedAttention(torch.autograd.Function):
         wsb = nat.query("edf_packed_attention_backward_workspace_bytes", *ctx.conf)
         ws = _u8(wsb, q)
         nat.call("edf_packed_attention_backward", _stream(), _p(q), _p(k), _p(v), _p(offsets), _p(key_offsets), _p(out),
-                 _p(rest), _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(ws), wsb, *ctx.conf)
+                 _p(dout), _p(lse), _p(dq), _p(dk), _p(dv), _p(ws), wsb, *ctx.conf)
         return dq, dk, dv, None, None, None, None
 
 

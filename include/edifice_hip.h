@@ -692,8 +692,7 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  *   Its n queries are the last of its m keys: query i stands at p = i + m - n and sees key j when j <= p and (window == 0
  *   or p - j < window or j < sinks).  A query that sees no key, and rows behind the last text, answer with zeros.
  * lse (may be NULL): float32 [num_heads, rows] natural-log row sums, infinity for a query that sees no key; required by the
- * backward, which writes every row of the gradients.  rest (may be NULL; bf16 alone): [num_heads, rows, d], what rounding
- * took from out; the backward given it is that much nearer (D = dO . O has O unrounded).  head_dim <= 128; rows, key_rows < 2^30.  Keys and values have to be finite, as
+ * backward, which writes every row of the gradients.  head_dim <= 128; rows, key_rows < 2^30.  Keys and values have to be finite, as
  * above, within each text; no value of one text reaches another.
  * The grids and workspaces (edf_packed_attention{,_backward}_workspace_bytes(), which may be 0) depend on the sizes alone,
  * not on the offsets, so a captured call may be replayed after those have changed.
@@ -701,15 +700,14 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
 size_t edf_packed_attention_workspace_bytes(int num_heads, int num_kv_heads, long rows, long key_rows, int texts,
                                             int head_dim, int window, int sinks, int dtype);
 int edf_packed_attention(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                         const int32_t* key_offsets, void* out, float* lse, void* rest, void* workspace,
-                         size_t workspace_bytes,
+                         const int32_t* key_offsets, void* out, float* lse, void* workspace, size_t workspace_bytes,
                          int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim, int window,
                          int sinks, int dtype);
 size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_heads, long rows, long key_rows, int texts,
                                                      int head_dim, int window, int sinks, int dtype);
 int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
-                                  const int32_t* key_offsets, const void* out, const void* rest, const void* grad_out,
-                                  const float* lse, void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
+                                  const int32_t* key_offsets, const void* out, const void* grad_out, const float* lse,
+                                  void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
                                   int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim,
                                   int window, int sinks, int dtype);
 

@@ -12,11 +12,11 @@ P = 16  # a non-null address that no refused call reads
 
 
 def _fwd(L, H=2, hkv=1, N=4, M=4, S=1, d=64, window=0, sinks=0, q=P, off=P, ws=None, wsb=0, dtype=1):
-    return L.edf_packed_attention(None, q, P, P, off, P, P, None, None, ws, wsb, H, hkv, N, M, S, d, window, sinks, dtype)
+    return L.edf_packed_attention(None, q, P, P, off, P, P, None, ws, wsb, H, hkv, N, M, S, d, window, sinks, dtype)
 
 
 def _bwd(L, H=2, hkv=1, N=4, M=4, S=1, d=64, lse=P, ws=P, wsb=1 << 40, window=0):
-    return L.edf_packed_attention_backward(None, P, P, P, P, P, P, None, P, lse, P, P, P, ws, wsb, H, hkv, N, M, S, d, window, 0, 1)
+    return L.edf_packed_attention_backward(None, P, P, P, P, P, P, P, lse, P, P, P, ws, wsb, H, hkv, N, M, S, d, window, 0, 1)
 
 
 @pytest.mark.parametrize("call, code, message", [
