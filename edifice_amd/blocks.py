@@ -328,6 +328,8 @@ class PagedCache:
         the GPU)."""
         if self.exhausted():
             return False
+        if not self.lengths.numel():
+            return True
         new = self.lengths + (num_tokens if counts is None else counts.clamp(0, num_tokens))
         pages = lambda n: (n + self.block_size - 1) // self.block_size  # noqa: E731
         drawn = int((pages(new) - pages(self.lengths)).sum())
@@ -519,6 +521,11 @@ class SequenceModel(nn.Module):
         blocks = self._attention_blocks()
         if x.dim() != 2:
             raise ValueError(f"x must be [rows, embed], got {tuple(x.shape)}")
+        if offsets.dim() != 1 or not offsets.numel() or offsets.dtype != torch.int32 or offsets.device != x.device:
+            raise ValueError(f"offsets must be int32 [texts + 1] on {x.device}, got {offsets.dtype} {tuple(offsets.shape)} on "
+                             f"{offsets.device}")
+        if not x.shape[0]:
+            return x.new_zeros(0, blocks[0].attn.out_proj.weight.shape[0])
         rows = torch.arange(x.shape[0], dtype=torch.int32, device=x.device)
         text = torch.bucketize(rows, offsets[1:], right=True)
         positions = (rows - offsets[text])[None]

@@ -459,8 +459,9 @@ int packed_check(int num_heads, int num_kv_heads, long rows, long key_rows, int 
               num_heads, num_kv_heads);
   EDF_REQUIRE(window >= 0 && sinks >= 0, EDF_ERR_INVALID_ARG, "window and sinks must not be negative");
   EDF_REQUIRE(head_dim <= 128, EDF_ERR_UNSUPPORTED, "head_dim %d > 128 unsupported", head_dim);
-  EDF_REQUIRE(rows < (1L << 30) && key_rows < (1L << 30) && texts < (1 << 28) && sinks < (1 << 30), EDF_ERR_UNSUPPORTED,
-              "rows, keys, texts and sinks must be below 2^28");
+  // a key, a window of 2^30 and a tile past it together stay an int
+  EDF_REQUIRE(rows < (1L << 29) && key_rows < (1L << 29) && texts < (1 << 28) && sinks < (1 << 29), EDF_ERR_UNSUPPORTED,
+              "rows, keys and sinks must be below 2^29, texts below 2^28");
   EDF_REQUIRE((double)num_heads * packed_tiles(std::max(rows, key_rows), texts, 32) * 4 < 2147483648.0, EDF_ERR_UNSUPPORTED,
               "heads x rows too large for one call");
   return EDF_OK;

@@ -692,8 +692,8 @@ int edf_window_attention_backward(void* stream, const void* q, const void* k, co
  *   Its n queries are the last of its m keys: query i stands at p = i + m - n and sees key j when j <= p and (window == 0
  *   or p - j < window or j < sinks).  A query that sees no key, and rows behind the last text, answer with zeros.
  * lse (may be NULL): float32 [num_heads, rows] natural-log row sums, infinity for a query that sees no key; required by the
- * backward, which writes every row of the gradients.  head_dim <= 128; rows, key_rows < 2^30.  Keys and values have to be finite, as
- * above, within each text; no value of one text reaches another.
+ * backward, which writes every row of the gradients.  head_dim <= 128; rows, key_rows, sinks < 2^29, texts < 2^28.  Keys and
+ * values have to be finite, as above, within each text; no value of one text reaches another.
  * The grids and workspaces (edf_packed_attention{,_backward}_workspace_bytes(), which may be 0) depend on the sizes alone,
  * not on the offsets, so a captured call may be replayed after those have changed.
  * ------------------------------------------------------------------------ */

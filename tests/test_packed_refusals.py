@@ -153,3 +153,23 @@ def test_eight_bit_cache_of_a_model():
         m.step(torch.zeros(2, 1, 32), c)  # the cache fits the model; the ops take no CPU tensors
     with pytest.raises(ValueError, match="the cache holds"):
         m.step(torch.zeros(2, 1, 32), _cache(dtype=torch.bfloat16)[1])
+
+
+@pytest.mark.parametrize("off", [OFF.long(), OFF[:0], OFF[None], OFF.to("meta")], ids=["int64", "empty", "2-d", "elsewhere"])
+def test_packed_model_refuses_offsets(off):
+    """Before they are looked up: an index past them would end the process on the GPU."""
+    m, _ = _cache()
+    with pytest.raises(ValueError, match="offsets must be"):
+        m.packed(torch.zeros(4, 32), off)
+
+
+def test_no_rows_and_no_places():
+    m, _ = _cache()
+    assert m.packed(torch.zeros(0, 32), OFF[:1]).shape == (0, m.final_norm.weight.numel())
+    assert m.paged_cache(0, 12).has_room(3)
+
+
+@pytest.mark.parametrize("sizes", [dict(N=1 << 29), dict(M=1 << 29), dict(sinks=1 << 29), dict(S=1 << 28)], ids=str)
+def test_sizes_whose_sums_pass_an_int(sizes):
+    L = lib()
+    assert _fwd(L, **sizes) == 2 and b"below 2^29" in L.edf_last_error()
