@@ -50,14 +50,14 @@ EDF_DEVICE void other_rows(const int* off, int S, int rows, TextTile& t) {
   t.other0 = __builtin_amdgcn_readfirstlane(text_begin(off, t.text, rows));
   t.m = max(__builtin_amdgcn_readfirstlane(text_begin(off, t.text + 1, rows)) - t.other0, 0);
 }
-// tile x of 2^ms rows; all 64 lanes of a wave take part; the result is uniform
+// tile x of 2^ms rows, of the last text that can have it; all 64 lanes of a wave take part; the result is uniform
 EDF_DEVICE TextTile find_tile(const int* off, int rows, const int* off2, int rows2, int S, int ms, int x) {
   const int lane = threadIdx.x & 63;
   TextTile t;
   if (S < 64) {  // a lane a text: all offsets in one load
     const int s = min(lane, S), b = text_begin(off, s, rows), e = text_end(off, S, s, rows, b);
     const int b2 = s == S ? 0 : text_begin(off2, s, rows2), e2 = s == S ? 0 : max(text_begin(off2, s + 1, rows2), b2);
-    const int from = max((int)__popcll(__ballot(lane <= S && (b >> ms) + lane <= x)), 1) - 1;
+    const int from = 63 - __builtin_clzll(__ballot(lane <= S && (b >> ms) + lane <= x));  // text 0 begins at 0
     t.text = from;
     t.row0 = __builtin_amdgcn_readlane(b, from);
     t.n = __builtin_amdgcn_readlane(e, from) - t.row0;
@@ -67,8 +67,8 @@ EDF_DEVICE TextTile find_tile(const int* off, int rows, const int* off2, int row
     int lo = 0, hi = S + 1;  // the text's number is in [lo, hi)
     while (hi - lo > 1) {
       const int step = (hi - lo + 63) / 64, s = lo + lane * step;
-      const bool at = s < hi && (text_begin(off, min(s, S), rows) >> ms) + s <= x;
-      lo += (max((int)__popcll(__ballot(at)), 1) - 1) * step;
+      const bool at = s < hi && (text_begin(off, min(s, S), rows) >> ms) + s <= x;  // so for lo
+      lo += (63 - __builtin_clzll(__ballot(at))) * step;
       hi = min(hi, lo + step);
     }
     t.text = __builtin_amdgcn_readfirstlane(lo);

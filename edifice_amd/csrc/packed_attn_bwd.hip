@@ -831,7 +831,6 @@ size_t edf_packed_attention_backward_workspace_bytes(int num_heads, int num_kv_h
 
 int edf_packed_attention_backward(void* stream, const void* q, const void* k, const void* v, const int32_t* offsets,
                                   const int32_t* key_offsets, const void* out, const void* grad_out, const float* lse,
-                                 
                                   void* grad_q, void* grad_k, void* grad_v, void* workspace, size_t workspace_bytes,
                                   int num_heads, int num_kv_heads, long rows, long key_rows, int texts, int head_dim,
                                   int window, int sinks, int dtype) {

@@ -286,3 +286,39 @@ def test_a_long_text():
         kj, vj = k[h // 2, js].double(), v[h // 2, js].double()
         p = torch.softmax(kj @ q[h, i].double() / math.sqrt(d), 0)
         _within(out[h, i], (p @ vj).cpu(), ((2.0 ** -7 + 256 * U) * (p @ vj.abs()) + 2.0 ** -8 * (p @ vj).abs()).cpu(), f"{h} {i}")
+
+
+@pytest.mark.parametrize("M, d", [((1 << 22) - 1, 128), (4300001, 64)], ids=["rows in pieces", "rows by element"])
+def test_keys_past_two_to_the_31_bytes(M, d):
+    """A text of a few queries on so many keys that its heads pass 2^31 bytes, and one behind it, forward and backward."""
+    from edifice_amd import fused_scan as fs
+    announce("packed, long keys", M=M, d=d)
+    first, n = M - 300, 20
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, do = (torch.randn(4, n + 5, d, generator=g, device="cuda", dtype=bf16) for _ in range(2))
+    k, v = (torch.randn(4, M, d, generator=g, device="cuda", dtype=bf16) for _ in range(2))  # 4.3 and 2.2 GB
+    # query 3 of the first text finds a key near its end, so far above the rest that P is 1 there
+    at = first - n - 100
+    q[:, 3] = torch.randn(d, generator=g, device="cuda").sign()
+    k[:, at] = 8 * q[:, 3]
+    qo, ko = _dev([0, n, n + 5]), _dev([0, first, M])
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = fs.packed_attention(*leaves, qo, ko)
+    dq, dk, dv = torch.autograd.grad(out, leaves, do)
+    # scores of query 3: 8 sqrt(d) >= 64 against |q . k| / sqrt(d) <= 6.5 or so of M random ones: exp(-57) M is nothing
+    assert torch.equal(out[:, 3], v[:, at])
+    # dV there: dO of query 3, and P of the others.  Their scores at that key are sums of d float32 terms of 8 |q| / sqrt(d), 72
+    # together: off by d U 72 < 2^-10.8 here and in the kernel, twice over with the row sums: 2^-8
+    with torch.no_grad():
+        p = torch.zeros(4, n, dtype=torch.float64, device="cuda")
+        for h in range(4):
+            s = torch.cat([c.float() @ q[h, :n].float().T for c in k[h, :first].split(1 << 20)]).double() / math.sqrt(d)
+            s.masked_fill_(torch.arange(first, device="cuda")[:, None] > torch.arange(first - n, first, device="cuda"), -math.inf)
+            p[h] = torch.softmax(s, 0)[at]
+        want = (p[..., None] * do[:, :n].double()).sum(1)
+        size = (p[..., None] * do[:, :n].double().abs()).sum(1)
+    _within(dv[:, at], want.cpu(), ((2.0 ** -7 + 256 * U + 2.0 ** -8) * size + 2.0 ** -8 * want.abs()).cpu(), "dV")
+    case = ((5,), (300,), 0, 4, 4, d, 0, 0, bf16)
+    exp = _expected(case, *(t.detach().cpu() for t in (q[:, n:], k[:, first:], v[:, first:], do[:, n:])))
+    for name, got in (("O", out[:, n:]), ("dQ", dq[:, n:]), ("dK", dk[:, first:]), ("dV", dv[:, first:])):
+        _within(got, *exp[name], name)
