@@ -756,11 +756,13 @@ __global__ __launch_bounds__(256) void packed_dq_sum_kernel(PackArgs a) {
 
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
 
-// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places.
-void backward_plan(PackArgs& a) {
+// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places, or as
+// the rows have tiles.
+void backward_plan(PackArgs& a, int dtype) {
   a.nx = (int)packed_tiles(a.M, a.S, PK_M);
-  const long wgs = (long)(a.H / a.G) * a.nx;
-  a.shares = (int)std::max(1L, std::min(16L, 512 / wgs));
+  const int bq = dtype == EDF_BF16 ? BQ_BF16 : BQ_32;
+  const long wgs = (long)(a.H / a.G) * a.nx, tiles = (long)a.G * ((a.N + bq - 1) / bq);
+  a.shares = (int)std::max(1L, std::min(std::min(16L, tiles), 512 / wgs));
   a.by_work = order_by_work(a, wgs);
 }
 size_t share_bytes(const PackArgs& a) {
@@ -771,7 +773,7 @@ size_t share_bytes(const PackArgs& a) {
 size_t part_bytes(PackArgs a, int dtype) {
   query_plan(a, key_tile(dtype));
   const size_t queries = chunk_bytes(a, 0);
-  backward_plan(a);
+  backward_plan(a, dtype);
   return std::max(queries, share_bytes(a));
 }
 size_t row_bytes(long heads, long rows) { return ((size_t)heads * rows * sizeof(float) + 255) & ~(size_t)255; }
@@ -845,7 +847,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
   a.N = (int)rows, a.M = (int)key_rows, a.S = texts, a.H = num_heads, a.G = num_heads / num_kv_heads, a.d = head_dim;
   a.W = window > 0 ? std::min(window, PK_ALL) : PK_ALL, a.sinks = sinks;
   a.scale = 1.0f / sqrtf((float)head_dim), a.scale_log2 = a.scale * LOG2E;
-  backward_plan(a);
+  backward_plan(a, dtype);
   const size_t need = row_bytes(num_heads, rows) + part_bytes(a, dtype);
   EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   a.dd = (float*)workspace;
