@@ -186,6 +186,8 @@ struct BlockTiles {
 // Where queries are few against the GPU their key tiles are cut into chunks, an item of work each.  All workgroups of a call
 // come to the same plan from the offsets alone: chunks of len key tiles, so that there are about PK_ITEMS of them, numbered
 // from tile to tile.  Item `item` of a head group's; threads look at two tiles each, of which there are fewer than 512.
+// Uncut, and cut: 8 texts of up to 64 queries on 28563 keys, 32(8)x128, 80 and 45 us; 500 queries on 30000 keys 224 and 157.
+// 320 to 1536 items were tried: 512 are the fastest at both.
 constexpr int PK_ITEMS = 512, PK_PLAN = 512;
 struct Item {
   TextTile tile;
@@ -349,12 +351,16 @@ struct ChunkRow {
 };
 
 // Tiles in order of their work where they are some rounds of the GPU's 512 places, so that the last ones to start count, and
-// texts are long enough (128 keys on average) that a workgroup's search for its tile does not.
+// texts are long enough (128 keys on average) that a workgroup's search for its tile does not.  In the texts' order, and in
+// that of work: dK and dV of 12 texts to 4096, 32(8)x128, 1451 and 1209 us; forward of 3 texts to 10000, 16(2)x64, 302 and
+// 286; of 8 texts to 4096, 8x128, 173 and 153.  Past 4096 workgroups the two are even.
 inline bool order_by_work(const PackArgs& a, long wgs) {
   return wgs > 512 && wgs <= 4096 && a.S < PK_SORT && a.M >= 128L * a.S;
 }
 
-// heads of a query workgroup: as many of a key head's as the four waves take
+// Heads of a query workgroup: as many of a key head's as the four waves take, since they read its keys once and few queries
+// of a text fill the waves all the same.  One head a workgroup, and four: 8 texts of up to 64 queries on 28563 keys, 32(8)x128,
+// 152 and 80 us (before chunks); 200 texts of 150 tokens, 16(4)x64, forward and backward 302 and 253.
 inline int head_shift(int G) { return G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0; }
 // Tiles are cut where the call's workgroups would not fill the GPU's 512 places.  A tile has a chunk for each len of its key
 // tiles and one for the rest, so there are at most PK_ITEMS over all groups and one a tile.
