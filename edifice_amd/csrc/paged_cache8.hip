@@ -78,7 +78,8 @@ EDF_DEVICE float least_scale(float amax) {
 }
 
 // G threads a run (64: the waves of a workgroup take a run each), which keep REG pieces of 8 values each between the maximum
-// and the codes and read what is more again; VEC: d a multiple of 8 and everything aligned to 16
+// and the codes and read what is more again; VEC: d a multiple of 8 and everything aligned to 16.  Four workgroups a CU: six
+// are no faster, and eight spill (float32 in eight pieces spills 3 registers at four).
 template <typename T, int C, int G, int REG, bool VEC>
 __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
   __shared__ float smax[4];
