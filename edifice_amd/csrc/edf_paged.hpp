@@ -118,9 +118,9 @@ struct KVTile {
   }
 };
 
-// The four waves' results joined: O^T as [query][dim] rows of HD + 4 floats in the wave's part of smem, then each thread
+// The NW waves' results joined: O^T as [query][dim] rows of HD + 4 floats in the wave's part of smem, then each thread
 // sums its elements.  m: the running maximum in log2 units; a workgroup that is one of several chunks leaves its sums.
-template <typename T, int HD, int WAVE_BYTES>
+template <typename T, int HD, int WAVE_BYTES, int NW = PA_WAVES>
 EDF_DEVICE void join_waves(const PagedArgs& a, char* smem, float (*sML)[16][2], const f32x4* o, float m, float lsum, int b,
                            int hq0, int nq, int split) {
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4, i = l & 15;
@@ -132,14 +132,14 @@ EDF_DEVICE void join_waves(const PagedArgs& a, char* smem, float (*sML)[16][2], 
     sML[w][i][1] = lsum;
   }
   __syncthreads();
-  for (int e = tid; e < nq * a.d; e += 256) {
+  for (int e = tid; e < nq * a.d; e += 64 * NW) {
     const int q = e / a.d, c = e - q * a.d;
     float mm = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < PA_WAVES; ++x) mm = fmaxf(mm, sML[x][q][0]);
+    for (int x = 0; x < NW; ++x) mm = fmaxf(mm, sML[x][q][0]);
     float acc = 0.0f, sum = 0.0f;
 #pragma unroll
-    for (int x = 0; x < PA_WAVES; ++x) {
+    for (int x = 0; x < NW; ++x) {
       const float f = mm == -INFINITY ? 0.0f : fast_exp2(sML[x][q][0] - mm);
       sum = fmaf(f, sML[x][q][1], sum);
       acc = fmaf(f, reinterpret_cast<const float*>(smem + x * WAVE_BYTES)[q * (HD + 4) + c], acc);
@@ -245,8 +245,8 @@ size_t paged_workspace(int batch, int num_heads, int num_kv_heads, int head_dim,
   return splits == 1 ? 0 : (size_t)batch * num_heads * splits * ((head_dim + 3) / 4 * 4 + 2) * sizeof(float);
 }
 
-// The call's checks, and what the kernels take beside the tensors
-int paged_setup(PagedArgs& a, bool pointers, void* workspace, size_t workspace_bytes, int batch, int num_heads,
+// The call's checks, and what the kernels take beside the tensors; whole: requests are not cut, whatever their length
+int paged_setup(PagedArgs& a, bool whole, bool pointers, void* workspace, size_t workspace_bytes, int batch, int num_heads,
                 int num_kv_heads, int head_dim, long num_blocks, int block_size, int table_width, int window, int sinks,
                 int dtype) {
   EDF_REQUIRE(batch > 0 && num_heads > 0 && num_kv_heads > 0 && head_dim > 0 && num_blocks > 0 && block_size > 0 &&
@@ -267,10 +267,12 @@ int paged_setup(PagedArgs& a, bool pointers, void* workspace, size_t workspace_b
   a.num_blocks = num_blocks;
   a.scale_log2 = LOG2E / sqrtf((float)head_dim);
   plan(batch, num_kv_heads, a.qt, visible_keys(table_width, block_size, window, sinks), a.chunk, a.splits);
+  if (whole) a.chunk = 1 << 30, a.splits = 1;
   const double wgs = (double)batch * num_kv_heads * a.qt * a.splits;
   EDF_REQUIRE(wgs < 2147483648.0 && (double)batch * num_heads < 2147483648.0, EDF_ERR_UNSUPPORTED,
               "batch x heads too large for one call");
-  const size_t need = paged_workspace(batch, num_heads, num_kv_heads, head_dim, table_width, block_size, window, sinks);
+  const size_t need =
+      whole ? 0 : paged_workspace(batch, num_heads, num_kv_heads, head_dim, table_width, block_size, window, sinks);
   EDF_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), EDF_ERR_WORKSPACE,
               "workspace too small: need %zu bytes", need);
   a.part = (float*)workspace;

@@ -222,7 +222,7 @@ int edf_paged_attention(void* stream, const void* q, const void* k_cache, const 
   using namespace edf;
   PagedArgs a{};
   a.q = q, a.kc = k_cache, a.vc = v_cache, a.table = table, a.len = lengths, a.out = out;
-  const int rc = paged_setup(a, q && k_cache && v_cache && table && lengths && out, workspace, workspace_bytes, batch,
+  const int rc = paged_setup(a, false, q && k_cache && v_cache && table && lengths && out, workspace, workspace_bytes, batch,
                              num_heads, num_kv_heads, head_dim, num_blocks, block_size, table_width, window, sinks, dtype);
   if (rc) return rc;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 &&

@@ -14,7 +14,7 @@
 // Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, P vs by 2^15 over the largest vs so far (a power
 // of two that the running maximum's rescaling takes along), so that float16's range holds them to 2^-39 of the largest.
 // bf16 queries are exact in it; float32 ones, and P vs, go through the products in two parts, off by 2^-23 of themselves.
-// Tiles, chunks and joins are paged_attn.hip's.
+// Tiles, chunks and joins are paged_attn.hip's, but that fewer requests are cut (whole_requests).
 #include <math.h>
 #include <stdint.h>
 
@@ -68,10 +68,11 @@ struct ValueTile {
 };
 
 // As many workgroups a CU as registers allow: at 128 elements in bf16 a fourth one spills (106 us where three take 70).
-template <typename T, int C, int HD, int MODE>
-__global__ __launch_bounds__(256, (sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 2) : 2))
+template <typename T, int C, int HD, int MODE, int NW>
+__global__ __launch_bounds__(
+    64 * NW, (NW > PA_WAVES ? 1 : sizeof(T) == 2 && MODE != BY_ELEMENT ? (HD <= 64 ? 4 : HD <= 128 ? 3 : 2) : 2))
 void paged_attn8_kernel(PagedArgs a) {
-  constexpr int NT = HD > 128 ? 1 : 2, KEYS = 16 * NT, STEP = PA_WAVES * KEYS;
+  constexpr int NT = HD > 128 ? 1 : 2, KEYS = 16 * NT, STEP = NW * KEYS;
   constexpr int NKK = HD / 32, NDT = HD / 16;
   constexpr int CPR = HD / 16, NV = KEYS * CPR / 64;  // pieces of 16 codes per row, and per lane of a tile
   constexpr int NK = HD / 64;                         // pieces of a key that a lane reads
@@ -79,9 +80,9 @@ void paged_attn8_kernel(PagedArgs a) {
   using Tile = ValueTile<HD, KEYS>;
   constexpr int TILE_BYTES = Tile::ELEMS * 2, OUT_BYTES = 16 * (HD + 4) * 4;
   constexpr int WAVE_BYTES = TILE_BYTES > OUT_BYTES ? TILE_BYTES : OUT_BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[PA_WAVES * WAVE_BYTES];
-  __shared__ __attribute__((aligned(16))) float sS[PA_WAVES][2][KEYS];
-  __shared__ float sML[PA_WAVES][16][2];
+  __shared__ __attribute__((aligned(16))) char smem[NW * WAVE_BYTES];
+  __shared__ __attribute__((aligned(16))) float sS[NW][2][KEYS];
+  __shared__ float sML[NW][16][2];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 4, i = l & 15;
   const int split = blockIdx.x % a.splits;
@@ -289,20 +290,39 @@ void paged_attn8_kernel(PagedArgs a) {
   for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) o[dt][r] = ldexpf(o[dt][r], ve - 15);
-  join_waves<T, HD, WAVE_BYTES>(a, smem, sML, o, m, lsum, b, hq0, nq, split);
+  join_waves<T, HD, WAVE_BYTES, NW>(a, smem, sML, o, m, lsum, b, hq0, nq, split);
 }
 
-template <typename T, int C, int HD>
+// Requests that are not cut: short ones, where the join's launch costs more than chunks save, and longer ones where there
+// is a workgroup for each CU without cutting.  A workgroup of eight waves where each has a CU to itself.  In chunks, and
+// whole (us a pass, replayed from a graph / one call after the other):
+//   1x8(4)x64 of 600 float32 7.9 / 14.4, 7.3 / 10.6;  1x32(8)x128 of 600 8.9 / 14.2, 8.9 / 10.2, of 1270 9.2 / 14.3, 13.3 /
+//   12.9;  32x32(8)x128 to 750 15.4, 10.8, to 2040 25.0, 20.6;  64x32(8)x128 to 600 21.5, 14.9 (eight waves 18.0), to 2040
+//   35.7, 32.6, to 4096 52.0, 58.1;  256x16(4)x64 to 2040 37.9, 34.8;  40x32(8)x128 to 3100 34.6, 39.7.
+constexpr int WHOLE_WAVES = 8, ONE_PER_CU = 256;
+bool whole_requests(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width, int block_size, int window,
+                    int sinks) {
+  if (num_kv_heads <= 0 || num_heads < num_kv_heads || head_dim > 128) return false;
+  const long wgs = (long)batch * num_kv_heads * ((num_heads / num_kv_heads + 15) / 16);
+  return visible_keys(table_width, block_size, window, sinks) <= (wgs < ONE_PER_CU ? 768 : 2048);
+}
+
+template <typename T, int C, int HD, int NW>
 void launch_paged8(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
-  if (vec && a.d == HD && !((uintptr_t)a.q & 15)) paged_attn8_kernel<T, C, HD, WHOLE><<<grid, 256, 0, s>>>(a);
-  else if (vec) paged_attn8_kernel<T, C, HD, BY_PIECE><<<grid, 256, 0, s>>>(a);
-  else paged_attn8_kernel<T, C, HD, BY_ELEMENT><<<grid, 256, 0, s>>>(a);
+  if (vec && a.d == HD && !((uintptr_t)a.q & 15)) paged_attn8_kernel<T, C, HD, WHOLE, NW><<<grid, 64 * NW, 0, s>>>(a);
+  else if (vec) paged_attn8_kernel<T, C, HD, BY_PIECE, NW><<<grid, 64 * NW, 0, s>>>(a);
+  else paged_attn8_kernel<T, C, HD, BY_ELEMENT, NW><<<grid, 64 * NW, 0, s>>>(a);
 }
 template <typename T, int C>
-void launch_paged8_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec) {
-  if (a.d <= 64) launch_paged8<T, C, 64>(s, a, grid, vec);
-  else if (a.d <= 128) launch_paged8<T, C, 128>(s, a, grid, vec);
-  else launch_paged8<T, C, 256>(s, a, grid, vec);
+void launch_paged8_t(hipStream_t s, const PagedArgs& a, unsigned grid, bool vec, bool whole) {
+  if (whole && grid <= ONE_PER_CU) {
+    if (a.d <= 64) launch_paged8<T, C, 64, WHOLE_WAVES>(s, a, grid, vec);
+    else launch_paged8<T, C, 128, WHOLE_WAVES>(s, a, grid, vec);
+    return;
+  }
+  if (a.d <= 64) launch_paged8<T, C, 64, PA_WAVES>(s, a, grid, vec);
+  else if (a.d <= 128) launch_paged8<T, C, 128, PA_WAVES>(s, a, grid, vec);
+  else launch_paged8<T, C, 256, PA_WAVES>(s, a, grid, vec);
   if (a.splits > 1)
     paged_join_kernel<T><<<dim3((unsigned)(a.B * a.Hq), (unsigned)((a.d + 127) / 128)), 32 * PJ_G, 0, s>>>(a);
 }
@@ -314,6 +334,7 @@ extern "C" {
 
 size_t edf_paged_attention8_workspace_bytes(int batch, int num_heads, int num_kv_heads, int head_dim, int table_width,
                                             int block_size, int window, int sinks) {
+  if (edf::whole_requests(batch, num_heads, num_kv_heads, head_dim, table_width, block_size, window, sinks)) return 0;
   return edf_paged_attention_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, table_width, block_size, window,
                                              sinks);
 }
@@ -327,7 +348,8 @@ int edf_paged_attention8(void* stream, const void* q, const void* k_cache, const
   EDF_REQUIRE(code == EDF_INT8 || code == EDF_E4M3, EDF_ERR_INVALID_ARG, "code must be 0 (int8) or 1 (e4m3)");
   PagedArgs a{};
   a.q = q, a.kc = k_cache, a.vc = v_cache, a.ks = k_scale, a.vs = v_scale, a.table = table, a.len = lengths, a.out = out;
-  const int rc = paged_setup(a, q && k_cache && v_cache && k_scale && v_scale && table && lengths && out, workspace,
+  const bool whole = whole_requests(batch, num_heads, num_kv_heads, head_dim, table_width, block_size, window, sinks);
+  const int rc = paged_setup(a, whole, q && k_cache && v_cache && k_scale && v_scale && table && lengths && out, workspace,
                              workspace_bytes, batch, num_heads, num_kv_heads, head_dim, num_blocks, block_size,
                              table_width, window, sinks, dtype);
   if (rc) return rc;
@@ -335,9 +357,11 @@ int edf_paged_attention8(void* stream, const void* q, const void* k_cache, const
   const unsigned grid = (unsigned)((long)batch * num_kv_heads * a.qt * a.splits);
   hipStream_t s = as_stream(stream);
   if (dtype == EDF_BF16)
-    code == EDF_INT8 ? launch_paged8_t<bf16, EDF_INT8>(s, a, grid, vec) : launch_paged8_t<bf16, EDF_E4M3>(s, a, grid, vec);
+    code == EDF_INT8 ? launch_paged8_t<bf16, EDF_INT8>(s, a, grid, vec, whole)
+                     : launch_paged8_t<bf16, EDF_E4M3>(s, a, grid, vec, whole);
   else
-    code == EDF_INT8 ? launch_paged8_t<float, EDF_INT8>(s, a, grid, vec) : launch_paged8_t<float, EDF_E4M3>(s, a, grid, vec);
+    code == EDF_INT8 ? launch_paged8_t<float, EDF_INT8>(s, a, grid, vec, whole)
+                     : launch_paged8_t<float, EDF_E4M3>(s, a, grid, vec, whole);
   return check_launch("paged attention, 8 bits");
 }
 

@@ -288,6 +288,25 @@ def test_attention(case, code):
                                v_scale=vs), q, caches, table, n, window, sinks, dtype)
 
 
+def _ragged(n, top):
+    return tuple((i * 7919 + 13) % (top + 1) for i in range(n - 1)) + (top,)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("case", [
+    (_ragged(3, 766), 8, 4, 64, 16, 0, 0, f32),      # whole requests, a few and many of them
+    (_ragged(270, 120), 1, 1, 64, 16, 0, 0, bf16),
+    (_ragged(130, 1500), 4, 2, 128, 16, 0, 0, bf16),
+    (_ragged(100, 900), 3, 3, 48, 8, 200, 3, bf16),
+    (_ragged(90, 700), 3, 3, 33, 5, 0, 0, f32),
+    (_ragged(6, 1100), 4, 2, 128, 16, 0, 0, f32),    # cut, few and many
+    (_ragged(90, 2300), 3, 3, 64, 64, 0, 0, bf16),
+    (_ragged(3, 769), 2, 1, 256, 16, 700, 60, bf16),
+], ids=lambda c: f"{len(c[0])}to{max(c[0])}-" + "-".join(str(x) for x in c[1:]))
+def test_attention_of_whole_and_cut_requests(case, code):
+    test_attention(case, code)
+
+
 def test_attention_without_some_pages():
     from edifice_amd import fused_scan as fs
     announce("paged_attention8, pages missing")
