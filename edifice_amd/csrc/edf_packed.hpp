@@ -362,15 +362,18 @@ inline bool order_by_work(const PackArgs& a, long wgs) {
 // of a text fill the waves all the same.  One head a workgroup, and four: 8 texts of up to 64 queries on 28563 keys, 32(8)x128,
 // 152 and 80 us (before chunks); 200 texts of 150 tokens, 16(4)x64, forward and backward 302 and 253.
 inline int head_shift(int G) { return G % 4 == 0 ? 2 : G % 2 == 0 ? 1 : 0; }
-// Tiles are cut where the call's workgroups would not fill the GPU's 512 places.  A tile has a chunk for each len of its key
-// tiles and one for the rest, so there are at most PK_ITEMS over all groups and one a tile.
+// Tiles are cut where the call's workgroups would not fill the GPU's 512 places, and keys are enough that chunks are worth the
+// kernel that joins them: one text, 8(4)x64, cut and uncut, bf16 of 300 keys 14.3 and 9.7 us, 500 14.7 and 13.1, 1000 15.9 and
+// 18.8; float32 of 150 keys 20.2 and 16.1, 250 20.3 and 23.9.  A tile has a chunk for each len of its key tiles and one for
+// the rest, so there are at most PK_ITEMS over all groups and one a tile.
 inline void query_plan(PackArgs& a, int BN) {
   a.hs = head_shift(a.G);
   a.nx = (int)packed_tiles(a.N, a.S, PK_M >> a.hs);
   const long groups = a.H >> a.hs, wgs = groups * a.nx;
   a.by_work = order_by_work(a, wgs);
   // (the plan's sum of key tiles is an int: 2^24 keys of 512 tiles)
-  a.items = wgs < PK_PLAN && a.M > 4 * BN && a.M < (1 << 24) ? (int)((PK_ITEMS + groups - 1) / groups) + a.nx : 0;
+  const bool cut = wgs < PK_PLAN && a.M > (BN == 64 ? 512 : 192) && a.M < (1 << 24);
+  a.items = cut ? (int)((PK_ITEMS + groups - 1) / groups) + a.nx : 0;
 }
 inline size_t chunk_bytes(const PackArgs& a, int extra) {  // extra: floats a row beside the padded head
   const size_t groups = a.H >> a.hs;

@@ -760,11 +760,13 @@ __global__ __launch_bounds__(256) void packed_dq_sum_kernel(PackArgs a) {
 
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
 
-// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places, or as
-// the rows have tiles.
+// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places, but no
+// more than leave each two tiles (float32, whose tiles take four times as long: one) of one text of all rows.  bf16, forward
+// and backward, with one tile a share, and two: 4 texts to 300, 8x64, 52.5 and 46.9 us; 8 to 100, 8(4)x64, 33.8 and 29.5; one
+// of 100 27.2 and 29.0.  float32: one text of 100, 8x64, 49.1 and 53.5.
 void backward_plan(PackArgs& a, int dtype) {
   a.nx = (int)packed_tiles(a.M, a.S, PK_M);
-  const int bq = dtype == EDF_BF16 ? BQ_BF16 : BQ_32;
+  const int bq = dtype == EDF_BF16 ? 2 * BQ_BF16 : BQ_32;
   const long wgs = (long)(a.H / a.G) * a.nx, tiles = (long)a.G * ((a.N + bq - 1) / bq);
   a.shares = (int)std::max(1L, std::min(std::min(16L, tiles), 512 / wgs));
   a.by_work = order_by_work(a, wgs);

@@ -135,6 +135,26 @@ def test_packed_attention_fwd_bwd(case):
         assert torch.equal(fs.packed_attention(tq, tk, tv, qo, ko, window=window, sinks=sinks), out)
 
 
+@pytest.mark.parametrize("case", [
+    # few queries' key tiles in chunks, of each width and type
+    ((400, 303), None, 5, 2, 1, 32, 0, 0, bf16),
+    ((520, 1, 90), None, 0, 3, 3, 96, 70, 100, bf16),
+    ((30, 2), (900, 300), 0, 4, 2, 80, 0, 0, bf16),
+    ((600, 33), None, 3, 2, 1, 20, 0, 2, bf16),
+    ((40, 300), (600, 300), 0, 4, 1, 112, 0, 0, bf16),
+    ((250, 9), None, 1, 1, 1, 7, 0, 0, f32),
+    ((210, 60), None, 0, 2, 2, 100, 0, 0, f32),
+    ((5, 200), (500, 210), 2, 8, 2, 30, 150, 1, f32),
+    # and as many keys as are not cut
+    ((300, 212), None, 0, 2, 1, 64, 0, 0, bf16),
+    ((300, 213), None, 0, 2, 1, 128, 0, 0, bf16),
+    ((150, 42), None, 0, 2, 2, 64, 0, 0, f32),
+    ((150, 43), None, 0, 2, 2, 128, 0, 0, f32),
+], ids=_name)
+def test_chunks_of_each_width(case):
+    test_packed_attention_fwd_bwd(case)
+
+
 def test_texts_do_not_reach_one_another():
     """Values of one text that are not finite leave the others as they were, forward and backward."""
     from edifice_amd import fused_scan as fs
