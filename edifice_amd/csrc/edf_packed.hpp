@@ -14,16 +14,15 @@ struct PackArgs {
   const void *q, *k, *v, *o, *go;
   void *out, *dq, *dk, *dv;
   float *lse, *dd;       // [H N]
-  float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks of keys; ml: maxima, two sums;
-                         // keys: part [share][Hkv][block] dK and dV of shares of queries
-  int* plan;             // queries: [head group][tile] first item and number of chunks
+  float *part, *ml;      // queries: [head group][item][128] unnormalised outputs (or dQ) of chunks; ml: maxima, two sums;
+                         // keys: part [Hkv][item] dK and dV of chunks
+  int* plan;             // [head group][tile] first item and number of chunks
   const int *qo, *ko;
   int N, M, S, H, G, d, W, sinks;
   int hs;                // the four waves of a query workgroup take 2^hs heads of one key head, 128 >> hs queries of each
   int nx;                // tiles a head (an upper bound: which of them exist is known on the GPU)
   int by_work;           // tiles in order of their work, the longest first, rather than of the texts
-  int items;             // queries: chunks of key tiles a head group (an upper bound), 0: tiles are not cut
-  int shares;            // keys: of a key block's query tiles
+  int items;             // chunks a head group (an upper bound), 0: the other tensor's tiles are not cut
   float scale, scale_log2;
 };
 
@@ -183,38 +182,44 @@ struct BlockTiles {
   }
 };
 
-// Where queries are few against the GPU their key tiles are cut into chunks, an item of work each.  All workgroups of a call
-// come to the same plan from the offsets alone: chunks of len key tiles, so that there are about PK_ITEMS of them, numbered
-// from tile to tile.  Item `item` of a head group's; threads look at two tiles each, of which there are fewer than 512.
-// Uncut, and cut: 8 texts of up to 64 queries on 28563 keys, 32(8)x128, 80 and 45 us; 500 queries on 30000 keys 224 and 157.
-// 320 to 1536 items were tried: 512 are the fastest at both.
+// Where queries (or keys) are few against the GPU the key (or query) tiles that each of their tiles walks are cut into chunks,
+// an item of work each.  All workgroups of a call come to the same plan from the offsets alone: chunks of len tiles, so that
+// they and the tiles' last, shorter ones are as many as the GPU's places (a chunk more than those waits for a whole one to
+// end), numbered from tile to tile.  Item `item` of a head group's; threads look at two tiles of 2^ms rows each, of which
+// there are fewer than 512; count(first, n, m): the tiles that the one from row `first` on walks.
+// Queries uncut, and cut: 8 texts of up to 64 queries on 28563 keys, 32(8)x128, 80 and 46 us; 500 queries on 30000 keys 224
+// and 163.  Keys (forward and backward) with an equal number of shares of each block's query tiles, and with such chunks: 8
+// texts to 2000, 8(4)x128, 244 and 175 us, one of 4000, 16(4)x128, 548 and 420, 4 to 1500, 32(8)x128, 262 and 191, 12 to 4096,
+// 8(1)x128, 1189 and 700; float32 8 to 2000, 8(4)x64, 636 and 450.  As many chunks as 576 to 1536 places are slower at most of
+// these, and a search for the shortest len costs 1 to 4 us more than it saves.
 constexpr int PK_ITEMS = 512, PK_PLAN = 512;
 struct Item {
   TextTile tile;
-  int x, chunk, chunks, len;  // the tile's number, which of its chunks, how many, key tiles of one
+  int x, chunk, chunks, len;  // the tile's number, which of its chunks, how many, tiles of one
   bool none;
 };
-template <int BN>
-EDF_DEVICE Item find_item(const PackArgs& a, int groups, int item, int* lds) {
-  const int tid = threadIdx.x, lane = tid & 63, ms = 7 - a.hs;
+template <typename Count>
+EDF_DEVICE Item find_item(const int* off, int rows, const int* off2, int rows2, int S, int ms, int groups, int least,
+                          int item, int* lds, Count tiles) {
+  const int tid = threadIdx.x, lane = tid & 63;
   int *so = lds, *sk = lds + PK_PLAN + 2, *sum = sk + PK_PLAN + 2, *found = sum + 8;
-  for (int s = tid; s <= a.S; s += 256) {
-    so[s] = text_begin(a.qo, s, a.N);
-    sk[s] = text_begin(a.ko, s, a.M);
+  for (int s = tid; s <= S; s += 256) {
+    so[s] = text_begin(off, s, rows);
+    sk[s] = text_begin(off2, s, rows2);
   }
   if (tid == 0) {
-    so[a.S + 1] = a.N;
+    so[S + 1] = rows;
     found[0] = -1;
   }
   __syncthreads();
   int count[2], text[2], chunks[2];
-  int mine = 0;
+  int mine = 0, there = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int x = 2 * tid + i;
     count[i] = -1, text[i] = 0;
-    if (x >= a.nx) continue;
-    int lo = 0, hi = a.S + 1;
+    if (x >= (rows >> ms) + S + 1) continue;
+    int lo = 0, hi = S + 1;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if ((so[mid] >> ms) + mid <= x) lo = mid;
@@ -223,15 +228,21 @@ EDF_DEVICE Item find_item(const PackArgs& a, int groups, int item, int* lds) {
     text[i] = lo;
     const int n = max(so[lo + 1] - so[lo], 0), first = (x - (so[lo] >> ms) - lo) << ms;
     if (first >= n) continue;
-    const int nk = lo < a.S ? max(sk[lo + 1] - sk[lo], 0) : 0;
-    count[i] = BlockTiles<BN>(first + nk - n, 1 << ms, nk, a.W, a.sinks).count;
+    count[i] = tiles(first, n, lo < S ? max(sk[lo + 1] - sk[lo], 0) : 0);
     mine += count[i];
+    ++there;
   }
-  const int ws = wave_sum_i(mine);
-  if (lane == 0) sum[tid >> 6] = ws;
+  const int ws = wave_sum_i(mine), wt = wave_sum_i(there);
+  if (lane == 0) {
+    sum[tid >> 6] = ws;
+    sum[4 + (tid >> 6)] = wt;
+  }
   __syncthreads();
   const long all = (long)sum[0] + sum[1] + sum[2] + sum[3];
-  const int len = (int)max(4L, (all * groups + PK_ITEMS - 1) / PK_ITEMS);
+  // a tile's last chunk is half a chunk on average
+  const int parts = max(PK_ITEMS - (sum[4] + sum[5] + sum[6] + sum[7]) * groups / 2, PK_ITEMS / 2);
+  const int len = (int)max((long)least, (all * groups + parts - 1) / parts);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) chunks[i] = count[i] < 0 ? 0 : max(1, (count[i] + len - 1) / len);
   int incl = chunks[0] + chunks[1];
@@ -264,8 +275,8 @@ EDF_DEVICE Item find_item(const PackArgs& a, int groups, int item, int* lds) {
   t.tile.row0 = __builtin_amdgcn_readfirstlane(so[s]);
   t.tile.n = __builtin_amdgcn_readfirstlane(max(so[s + 1] - so[s], 0));
   t.tile.first = (t.x - (t.tile.row0 >> ms) - s) << ms;
-  t.tile.other0 = s < a.S ? __builtin_amdgcn_readfirstlane(sk[s]) : 0;
-  t.tile.m = s < a.S ? __builtin_amdgcn_readfirstlane(max(sk[s + 1] - sk[s], 0)) : 0;
+  t.tile.other0 = s < S ? __builtin_amdgcn_readfirstlane(sk[s]) : 0;
+  t.tile.m = s < S ? __builtin_amdgcn_readfirstlane(max(sk[s + 1] - sk[s], 0)) : 0;
   t.chunk = __builtin_amdgcn_readfirstlane(found[2]);
   t.chunks = __builtin_amdgcn_readfirstlane(found[3]);
   t.len = __builtin_amdgcn_readfirstlane(len);
@@ -292,7 +303,9 @@ struct QueryTile {
     TextTile t;
     slot = -1;
     if (a.items > 0) {
-      const Item it = find_item<BN>(a, groups, x, (int*)lds);
+      const Item it = find_item(a.qo, a.N, a.ko, a.M, a.S, ms, groups, 4, x, (int*)lds, [&](int first, int n, int m) {
+        return BlockTiles<BN>(first + m - n, 1 << ms, m, a.W, a.sinks).count;
+      });
       none = it.none;
       if (none) return;
       t = it.tile, chunk = it.chunk, len = it.len;

@@ -7,10 +7,10 @@
 //   also forms D and leaves it for the second kernel.
 //   dK, dV: a workgroup owns 128 keys of a text (32 per wave, K^T and V^T in registers) of one key head and walks the
 //   query tiles that see one of them, query head by query head: the sum over shared heads needs no atomics.  Where key
-//   blocks are few against the GPU, each block's query tiles are shared out evenly among several workgroups, which leave
-//   float32 sums, added in order by a third kernel.
+//   blocks are few against the GPU, their query tiles are cut into chunks, as those of the queries are, which leave float32
+//   sums, added in order by a third kernel.
 // 12 texts to 4096, 32(8)x128, bf16: dQ 853 us (947 TFLOP/s of the 6 d that it does), dK and dV 1210 (890 of 8 d), profiled.
-// 5 texts to 700, 8(4)x64, float32: 25 + 40 us, and 5 + 6 for the sums of chunks and shares.
+// 5 texts to 700, 8(4)x64, float32: 25 + 31 us, and 4 + 6 for the sums of chunks.
 // In bf16 P and dS are rounded as operands of the second products (2^-8 of each term); D is formed from the rounded O that
 // the forward left, or where keys are few, and O with its rounding as large as V, as sum P dP; everything else is float32.
 // (O's rounding kept in bf16 beside it does the same for twice the bytes of O: forward and backward of 200 texts of 150
@@ -358,26 +358,61 @@ __global__ __launch_bounds__(256, 2) void packed_dq128_kernel(PackArgs a) {
     }
 }
 
-// The key block of a dK, dV workgroup and its share [t0, t1) of the block's (query head, tile of BQ queries) pairs: nt
-// tiles a head, from query qs of the text on.
+// The (query head, tile of BQ queries) pairs that a block of keys from row `first` of n on walks, in a text of m queries: nt
+// tiles a head, from query qs on.
 template <int BQ>
+struct QueryTiles {
+  int qs, nt;
+  EDF_DEVICE QueryTiles(const PackArgs& a, int first, int n, int m) {
+    const int ahead = n - m;
+    qs = max(0, first - ahead);  // the first query that sees the block's first key
+    int end = m;
+    if (first >= a.sinks) end = (int)min((long)m, (long)first + PK_M - 1 + a.W - ahead);  // past the last key's window
+    nt = max(0, (end - qs + BQ - 1) / BQ);
+  }
+};
+
+// The key block of a dK, dV workgroup and its chunk [t0, t1) of the block's pairs; LEAST: of a chunk.
+template <int BQ, int LEAST>
 struct KeyBlock {
-  int head, share, krow, nk, first, qrow, nq, qs, nt, t0, t1;  // first: the block's first key within the text
+  int head, krow, nk, first, qrow, nq, qs, nt, t0, t1;  // first: the block's first key within the text
+  long slot;                                            // of one of several chunks: its place in part, or -1
   bool none;
   EDF_DEVICE int ahead() const { return nk - nq; }
-  EDF_DEVICE KeyBlock(const PackArgs& a, int id_x, int id_head, int share_) : head(id_head), share(share_) {
-    const TextTile t = a.by_work ? find_tile_by_work(a.ko, a.M, a.qo, a.N, a.S, 7, id_x, false)
-                                 : find_tile(a.ko, a.M, a.qo, a.N, a.S, 7, id_x);
+  // the first query of pairs i G .. (i + 1) G - 1: from a text's end backwards, so that the blocks that are under way meet in
+  // the same queries
+  EDF_DEVICE int query(int i) const { return qs + (nt - 1 - i) * BQ; }
+  // lds: 5 KB that the kernel uses later
+  EDF_DEVICE KeyBlock(const PackArgs& a, void* lds) : slot(-1) {
+    const int hkv = a.H / a.G;
+    int x, chunk = 0, len = 0;
+    none = !packed_block(hkv, a.items > 0 ? a.items : a.nx, x, head);
+    if (none) return;
+    TextTile t;
+    if (a.items > 0) {
+      const Item it = find_item(a.ko, a.M, a.qo, a.N, a.S, 7, hkv, LEAST, x, (int*)lds,
+                                [&](int first, int n, int m) { return QueryTiles<BQ>(a, first, n, m).nt * a.G; });
+      none = it.none;
+      if (none) return;
+      t = it.tile, chunk = it.chunk, len = it.len;
+      if (it.chunks > 1) slot = (long)head * a.items + x;
+      if (chunk == 0 && threadIdx.x == 0) {
+        int* p = a.plan + 2 * ((long)head * a.nx + it.x);
+        p[0] = x;
+        p[1] = it.chunks;
+      }
+    } else {
+      t = a.by_work ? find_tile_by_work(a.ko, a.M, a.qo, a.N, a.S, 7, x, false)
+                    : find_tile(a.ko, a.M, a.qo, a.N, a.S, 7, x);
+      none = t.first >= t.n;
+      if (none) return;
+    }
     krow = t.row0, nk = t.n, first = t.first;
-    none = first >= nk;
     qrow = t.other0, nq = t.m;
-    qs = max(0, first - ahead());  // the first query that sees the block's first key
-    int end = nq;
-    if (first >= a.sinks) end = (int)min((long)nq, (long)first + PK_M - 1 + a.W - ahead());  // past the last key's window
-    nt = max(0, (end - qs + BQ - 1) / BQ);
-    const long all = (long)nt * a.G;
-    t0 = (int)(all * share / a.shares);
-    t1 = (int)(all * (share + 1) / a.shares);
+    const QueryTiles<BQ> q(a, first, nk, nq);
+    qs = q.qs, nt = q.nt;
+    t0 = chunk * len;
+    t1 = a.items > 0 ? min(t0 + len, nt * a.G) : nt * a.G;
   }
 };
 
@@ -393,11 +428,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
   __shared__ __attribute__((aligned(16))) float sL[2][BQ], sD[2][BQ];
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
-  int x, head;  // of the key heads
-  if (!packed_block(a.H / a.G, a.nx * a.shares, x, head)) return;
-  const KeyBlock<BQ> kb(a, x / a.shares, head, x % a.shares);
+  const KeyBlock<BQ, sizeof(T) == 2 ? 2 : 1> kb(a, sQ);
   if (kb.none) return;
-  const int d = a.d, kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
+  const int head = kb.head;
+  const int d = a.d, kw = kb.first + 32 * w, mykey = kw + li, t0 = kb.t0, t1 = kb.t1;
   const long krow = (long)head * a.M + kb.krow + min(mykey, kb.nk - 1);
   WFrag<T> kf[NKK], vf[NKK];
 #pragma unroll
@@ -415,7 +449,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
   WFrag<T> rq[ld.N], ro[ld.N];
   float rl = 0.0f, rd = 0.0f;
   auto gload = [&](int t) {
-    const int h = t / nt, q0 = kb.qs + (t - h * nt) * BQ;
+    const int i = t / a.G, h = t - i * a.G, q0 = kb.query(i);
     const long base = (long)(head * a.G + h) * a.N + kb.qrow;
     ld.load((const T*)a.q + base * d, q0, rq);
     ld.load((const T*)a.go + base * d, q0, ro);
@@ -441,7 +475,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
   __syncthreads();
   for (int t = t0; t < t1; ++t) {
     const int buf = (t - t0) & 1;
-    const int p0 = kb.qs + t % nt * BQ + kb.ahead();  // position of the tile's first query
+    const int p0 = kb.query(t / a.G) + kb.ahead();  // position of the tile's first query
 #pragma unroll
     for (int sub = 0; sub < BQ / 32; ++sub) {
       const int pb = p0 + 32 * sub;
@@ -505,8 +539,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
     }
     __syncthreads();
   }
-  if (a.shares > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
-    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.shares) * (2L * PK_M * HD) + (32 * w + li) * HD;
+  if (mykey >= kb.nk) return;
+  if (kb.slot >= 0) {  // these sums are of a chunk: [key head][item][dK | dV][key][dim]
+    float* out = a.part + kb.slot * (2L * PK_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -522,7 +557,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 && HD <= 96 && VEC ? 2 : 1)) v
       }
     return;
   }
-  if (mykey >= kb.nk) return;
   T *kout = (T*)a.dk + krow * d, *vout = (T*)a.dv + krow * d;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
@@ -562,11 +596,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
 
   const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, g = l >> 5, li = l & 31;
   const int wu = __builtin_amdgcn_readfirstlane(w);
-  int x, head;  // of the key heads
-  if (!packed_block(a.H / a.G, a.nx * a.shares, x, head)) return;
-  const KeyBlock<BQ> kb(a, x / a.shares, head, x % a.shares);
+  const KeyBlock<BQ, 2> kb(a, sR0);
   if (kb.none) return;
-  const int kw = kb.first + 32 * w, mykey = kw + li, nt = kb.nt, t0 = kb.t0, t1 = kb.t1;
+  const int head = kb.head;
+  const int kw = kb.first + 32 * w, mykey = kw + li, t0 = kb.t0, t1 = kb.t1;
   const long kbase = (long)head * a.M + kb.krow, krow = kbase + min(mykey, kb.nk - 1);
 
   // keys past the text's end read zero rows of V: they only feed their own columns, never stored
@@ -586,7 +619,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
   // writes to LDS once the tile's loads have landed.
   auto issue = [&](auto bt, int t) {
     constexpr int B = decltype(bt)::value;
-    const int h = t / nt, q0 = kb.qs + (t - h * nt) * BQ;
+    const int i = t / a.G, h = t - i * a.G, q0 = kb.query(i);
     const long row = (long)(head * a.G + h) * a.N + kb.qrow;
     stage_hb<BQ>(make_rsrc((const bf16*)a.q + row * HD, (unsigned)kb.nq * HD * 2), B ? sR1 : sR0, q0, wu, l);
     stage_hb<BQ>(make_rsrc((const bf16*)a.go + row * HD, (unsigned)kb.nq * HD * 2), (B ? sR1 : sR0) + BQ * HD, q0, wu, l);
@@ -663,7 +696,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
   auto step = [&](auto bt, int t) {
     const std::integral_constant<int, 1 - decltype(bt)::value> ot{};
     if (t + 1 < t1) issue(ot, t + 1);
-    const int pb = kb.qs + t % nt * BQ + kb.ahead();  // position of the tile's first query
+    const int pb = kb.query(t / a.G) + kb.ahead();  // position of the tile's first query
     if (!(pb + 31 < kw || (pb > kw + 30 + a.W && kw >= a.sinks))) {  // some query sees a key of this wave
       if (pb >= kw + 31 && pb + 31 - kw < a.W) subtile(bt, pb, std::false_type{});
       else subtile(bt, pb, std::true_type{});
@@ -684,8 +717,9 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
     step(b0, t);
     if (t + 1 < t1) step(b1, t + 1);
   }
-  if (a.shares > 1) {  // these sums are a share: [share][key head][block][dK | dV][key][dim]
-    float* out = a.part + (((long)kb.share * (a.H / a.G) + head) * a.nx + x / a.shares) * (2L * PK_M * HD) + (32 * w + li) * HD;
+  if (mykey >= kb.nk) return;
+  if (kb.slot >= 0) {  // these sums are of a chunk: [key head][item][dK | dV][key][dim]
+    float* out = a.part + kb.slot * (2L * PK_M * HD) + (32 * w + li) * HD;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -701,7 +735,6 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
       }
     return;
   }
-  if (mykey >= kb.nk) return;
   const long row = krow * HD;
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt)
@@ -718,8 +751,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkdv128_kernel(PackArgs a) {
     }
 }
 
-// dK, dV of blocks whose sums are in shares, added in order, four elements a thread.  A workgroup takes one of the pieces
-// of a block's [dK | dV][key][dim].
+// dK, dV of blocks whose query tiles are in chunks, added in order, four elements a thread.  A workgroup takes one of the
+// pieces of a block's [dK | dV][key][dim].
 template <typename T, int HD>
 __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
   constexpr int PIECES = 2 * PK_M * HD / 1024;
@@ -728,13 +761,14 @@ __global__ __launch_bounds__(256) void packed_sum_kernel(PackArgs a) {
   const int e = (piece * 256 + threadIdx.x) * 4;
   const bool is_v = e >= PK_M * HD;
   const int key = t.first + e / HD % PK_M, c = e % HD;
-  if (key >= t.n || c >= a.d) return;
-  const int hkv = a.H / a.G;
-  const float* in = a.part + ((long)head * a.nx + x) * (2L * PK_M * HD) + e;
-  const long stride = (long)hkv * a.nx * (2L * PK_M * HD);
+  if (t.first >= t.n || key >= t.n || c >= a.d) return;
+  const int* p = a.plan + 2 * ((long)head * a.nx + x);
+  const int item = p[0], n = p[1];
+  if (n <= 1 || item < 0 || n > a.items - item) return;  // one chunk, or no plan (offsets that do not ascend)
+  const float* in = a.part + ((long)head * a.items + item) * (2L * PK_M * HD) + e;
   f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-  for (int i = 0; i < a.shares; ++i) s += *(const f32x4*)(in + i * stride);
+  for (int i = 0; i < n; ++i) s += *(const f32x4*)(in + i * (2L * PK_M * HD));
   if (!is_v) s *= a.scale;
   T* out = (T*)(is_v ? a.dv : a.dk) + ((long)head * a.M + t.row0 + key) * a.d + c;
 #pragma unroll
@@ -760,27 +794,26 @@ __global__ __launch_bounds__(256) void packed_dq_sum_kernel(PackArgs a) {
 
 constexpr int BQ_BF16 = 64, BQ_32 = 32;  // query tiles of dK, dV: bf16, and float32
 
-// Key blocks a head, and the shares of each block's query tiles: as many as bring the call to the GPU's 512 places, but no
-// more than leave each two tiles (float32, whose tiles take four times as long: one) of one text of all rows.  bf16, forward
-// and backward, with one tile a share, and two: 4 texts to 300, 8x64, 52.5 and 46.9 us; 8 to 100, 8(4)x64, 33.8 and 29.5; one
-// of 100 27.2 and 29.0.  float32: one text of 100, 8x64, 49.1 and 53.5.
+// Key blocks a head, and whether and into how many chunks their query tiles are cut: where the blocks would not fill the
+// GPU's 512 places, and query tiles are enough that chunks are worth the kernel that adds them.
 void backward_plan(PackArgs& a, int dtype) {
   a.nx = (int)packed_tiles(a.M, a.S, PK_M);
-  const int bq = dtype == EDF_BF16 ? 2 * BQ_BF16 : BQ_32;
-  const long wgs = (long)(a.H / a.G) * a.nx, tiles = (long)a.G * ((a.N + bq - 1) / bq);
-  a.shares = (int)std::max(1L, std::min(std::min(16L, tiles), 512 / wgs));
+  const long hkv = a.H / a.G, wgs = hkv * a.nx, queries = (long)a.N * a.G;
   a.by_work = order_by_work(a, wgs);
+  // (the plan's sum of tiles is an int)
+  const bool cut = wgs < PK_PLAN && queries > (dtype == EDF_BF16 ? 512 : 64) && queries < (1 << 25) && a.M < (1 << 24);
+  a.items = cut ? (int)((PK_ITEMS + hkv - 1) / hkv) + a.nx : 0;
 }
-size_t share_bytes(const PackArgs& a) {
-  return a.shares == 1 ? 0
-                       : (size_t)a.shares * (a.H / a.G) * a.nx * (2 * PK_M) * window_pad(a.d) * sizeof(float);
+size_t key_bytes(const PackArgs& a) {
+  const size_t hkv = a.H / a.G;
+  return a.items == 0 ? 0 : hkv * a.items * (2 * PK_M) * window_pad(a.d) * sizeof(float) + hkv * a.nx * 2 * sizeof(int);
 }
 // the larger of what the two kernels leave, one after the other
 size_t part_bytes(PackArgs a, int dtype) {
   query_plan(a, key_tile(dtype));
   const size_t queries = chunk_bytes(a, 0);
   backward_plan(a, dtype);
-  return std::max(queries, share_bytes(a));
+  return std::max(queries, key_bytes(a));
 }
 size_t row_bytes(long heads, long rows) { return ((size_t)heads * rows * sizeof(float) + 255) & ~(size_t)255; }
 
@@ -794,7 +827,7 @@ int launch_bwd(hipStream_t s, PackArgs a) {
   const long groups = a.H >> q.hs;
   const unsigned qgrid = (unsigned)packed_grid(groups, q.items > 0 ? q.items : q.nx);
   const int hkv = a.H / a.G;
-  const unsigned kgrid = (unsigned)packed_grid(hkv, (long)a.nx * a.shares);
+  const unsigned kgrid = (unsigned)packed_grid(hkv, a.items > 0 ? a.items : a.nx);
   if (fast) packed_dq128_kernel<<<qgrid, 256, 0, s>>>(q);
   else packed_dq_kernel<T, HD, BN, VEC><<<qgrid, 256, 0, s>>>(q);
   int rc = check_launch("packed attention dQ");
@@ -808,7 +841,7 @@ int launch_bwd(hipStream_t s, PackArgs a) {
   if (fast) packed_dkdv128_kernel<<<kgrid, 256, 0, s>>>(a);
   else packed_dkdv_kernel<T, HD, BQ, VEC><<<kgrid, 256, 0, s>>>(a);
   rc = check_launch("packed attention dK, dV");
-  if (rc || a.shares == 1) return rc;
+  if (rc || a.items == 0) return rc;
   packed_sum_kernel<T, HD><<<(unsigned)(2L * PK_M * HD / 1024 * a.nx * hkv), 256, 0, s>>>(a);
   return check_launch("packed attention dK, dV sums");
 }
@@ -858,6 +891,7 @@ int edf_packed_attention_backward(void* stream, const void* q, const void* k, co
   EDF_REQUIRE(workspace && workspace_bytes >= need, EDF_ERR_WORKSPACE, "workspace too small: need %zu bytes", need);
   a.dd = (float*)workspace;
   a.part = (float*)((char*)workspace + row_bytes(num_heads, rows));
+  a.plan = (int*)(a.part + (size_t)(a.H / a.G) * a.items * (2 * PK_M) * window_pad(a.d));
   const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)grad_out |
                          (uintptr_t)grad_q | (uintptr_t)grad_k | (uintptr_t)grad_v;
   const bool vec = (long)head_dim * (dtype == EDF_BF16 ? 2 : 4) % 16 == 0 && !(ptrs & 15) &&
