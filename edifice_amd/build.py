@@ -56,8 +56,8 @@ def sources():
 # The windowed attention's backward kernels hold two accumulators and scale P and dP with VALU
 # work (backward without and with the flag: bf16 4x16(4)x2000x96 window 500 239 -> 204 us,
 # float32 8x16(4)x1500x64 window 256 729 -> 640, 2x8(4)x1000x64 103 -> 96).  The same goes for those over packed
-# texts, whose bf16 kernels hardly change (forward and backward: float32 8 texts to 2000, 8(4)x64, 630 -> 576 us, 5 texts to
-# 700 98 -> 92; bf16 200 texts of 150, 16(4)x64, 256 -> 262; without it 24 registers of float32 at 128 are spilled).
+# texts, whose bf16 kernels hardly change (forward and backward: float32 8 texts to 2000, 8(4)x64, 473 -> 438 us, 5 texts to
+# 700 100 -> 92; bf16 200 texts of 150, 16(4)x64, 276 -> 273; without it 24 registers of float32 at 128 are spilled).
 PER_FILE_FLAGS = {
     "flash_attn_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "delta_rule_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
