@@ -380,7 +380,7 @@ struct KeyBlock {
   bool none;
   EDF_DEVICE int ahead() const { return nk - nq; }
   // the first query of pairs i G .. (i + 1) G - 1: from a text's end backwards, so that the blocks that are under way meet in
-  // the same queries
+  // the same queries (12 texts to 4096, 32(8)x128, and 8 to 2000, 8(4)x64: 1 to 2% of forward and backward)
   EDF_DEVICE int query(int i) const { return qs + (nt - 1 - i) * BQ; }
   // lds: 5 KB that the kernel uses later
   EDF_DEVICE KeyBlock(const PackArgs& a, void* lds) : slot(-1) {
