@@ -302,6 +302,12 @@ def _ragged(n, top):
     (_ragged(6, 1100), 4, 2, 128, 16, 0, 0, f32),    # cut, few and many
     (_ragged(90, 2300), 3, 3, 64, 64, 0, 0, bf16),
     (_ragged(3, 769), 2, 1, 256, 16, 700, 60, bf16),
+    (_ragged(5, 2000), 6, 2, 128, 64, 800, 20, bf16),
+    (_ragged(3, 1500), 40, 2, 64, 16, 0, 0, bf16),   # two query tiles
+    (_ragged(3, 1300), 4, 4, 80, 8, 1000, 0, bf16),
+    (_ragged(3, 900), 3, 1, 33, 5, 0, 0, bf16),      # rows by element
+    (_ragged(3, 1000), 7, 1, 100, 32, 770, 3, f32),
+    (_ragged(2, 800), 2, 2, 7, 1, 0, 0, f32),
 ], ids=lambda c: f"{len(c[0])}to{max(c[0])}-" + "-".join(str(x) for x in c[1:]))
 def test_attention_of_whole_and_cut_requests(case, code):
     test_attention(case, code)
