@@ -598,9 +598,9 @@ class SequenceModel(nn.Module):
             raise ValueError("tokens onto filled places need pages for all of them")
         slots, positions = cache.extend(x.shape[1], counts)
         real = torch.nonzero(positions.flatten() >= 0)[:, 0]
-        out = x.new_zeros(x.shape[0] * x.shape[1], blocks[0].attn.out_proj.weight.shape[0])
+        out = x.new_zeros(*x.shape[:2], blocks[0].attn.out_proj.weight.shape[0])
         if not real.numel():
-            return out.view(x.shape[0], x.shape[1], -1)
+            return out
         n = (positions >= 0).sum(1)
         ends = torch.stack([n, torch.where(n > 0, cache.lengths, 0)]).cumsum(1).to(torch.int32)
         offsets, key_offsets = F.pad(ends, (1, 0)).unbind(0)
@@ -611,8 +611,8 @@ class SequenceModel(nn.Module):
         for layer, blk in enumerate(blocks):
             h = blk.go_on(h, cache, layer, slots, positions, offsets, key_offsets, total)
         h = self.final_norm(h) if hasattr(self, "final_norm") else h
-        out[real] = h[0]
-        return out.view(x.shape[0], x.shape[1], -1)
+        out.flatten(0, 1)[real] = h[0]
+        return out
 
     def load_reference_weights(self, weights: dict):
         """Load a reference weight file's ``weight.<layer>.<param>`` tensors (PyTorch layout)."""

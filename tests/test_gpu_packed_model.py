@@ -149,3 +149,15 @@ def test_captured_step_on_an_eight_bit_cache():
         torch.cuda.synchronize()
         assert torch.equal(h, want) and torch.equal(a.table, b.table) and torch.equal(a.lengths, b.lengths)
         assert all(torch.equal(p, q) for p, q in zip(a.k_scale + a.k, b.k_scale + b.k))
+
+
+@pytest.mark.parametrize("kind", [None, torch.int8], ids=str)
+def test_no_places(kind):
+    """A cache of no places takes steps and prompts that go on, and answers with no states."""
+    announce("no places", kind=kind)
+    m = _model(f32, **OPTS)
+    cache = m.paged_cache(0, 24, block_size=4, **({} if kind is None else dict(dtype=kind)))
+    with torch.no_grad():
+        width = m.sequence(torch.zeros(1, 1, 48, device="cuda")).shape[2]
+    for method, n in (("go_on", 5), ("go_on", 1), ("step", 3), ("step", 1)):
+        assert getattr(m, method)(torch.zeros(0, n, 48, device="cuda"), cache).shape == (0, n, width)
