@@ -578,6 +578,8 @@ class SequenceModel(nn.Module):
         if x.shape[1] > 1 and bool(((cache.lengths > 0) & (True if counts is None else counts > 0)).any()):
             raise ValueError("several tokens at once go into empty places only (go_on takes them onto filled ones)")
         slots, positions = cache.extend(x.shape[1], counts)
+        if not x.shape[0]:
+            return x.new_zeros(*x.shape[:2], blocks[0].attn.out_proj.weight.shape[0])
         if x.shape[1] > 1 and counts is not None:  # whatever the padding holds, its keys and values are finite
             x = x.masked_fill((positions < 0)[..., None], 0.0)
         h = self.input_projection(x) if hasattr(self, "input_projection") else x

@@ -177,11 +177,12 @@ def test_sizes_whose_sums_pass_an_int(sizes):
 
 @pytest.mark.parametrize("opts", [{}, dict(dtype=torch.int8)], ids=["own type", "int8"])
 def test_no_places_go_on(opts, monkeypatch):
-    """No place, any number of tokens: no states, and the cache is as it was."""
+    """No place: no states, and the cache is as it was."""
     m, _ = _cache()
     c = m.paged_cache(0, 12, block_size=4, **opts)
     none = torch.zeros(0, 3, dtype=torch.int32)
     monkeypatch.setattr(fs, "paged_extend", lambda *a: (none, none, torch.zeros(1, dtype=torch.int32)))
     for counts in (None, torch.zeros(0, dtype=torch.int32)):
-        assert m.go_on(torch.zeros(0, 3, 32), c, counts).shape == (0, 3, m.final_norm.weight.numel())
+        for method in (m.go_on, m.step):
+            assert method(torch.zeros(0, 3, 32), c, counts).shape == (0, 3, m.final_norm.weight.numel())
     assert not c.lengths.numel() and int(c.taken) == 0
