@@ -11,8 +11,9 @@
 //   Keys go from memory to the matrix operand: a lane's 16 codes of each 64 of a row are 16 columns of the contraction,
 //   and the query has the same order.  A tile's rows are read whole by four lanes each.
 //   Values become float16 on their way into the wave's LDS tile, from where transposed reads take them.
-// Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, P vs by 2^15 over the largest vs so far (a power
-// of two that the running maximum's rescaling takes along), so that float16's range holds them to 2^-39 of the largest.
+// Queries are scaled by a power of two to a largest element of 2^14 .. 2^15, P vs by 2^15 over the query's largest so far (a
+// power of two that rises with it and falls as the running maximum leaves it behind), so that float16's range holds them to
+// 2^-39 of the largest, whatever the scales of pages that have next to no weight.
 // bf16 queries are exact in it; float32 ones, and P vs, go through the products in two parts, off by 2^-23 of themselves.
 // Tiles, chunks and joins are paged_attn.hip's, but that fewer requests are cut (whole_requests).
 #include <math.h>
@@ -57,6 +58,8 @@ EDF_DEVICE void half_parts(float x, F put) {
     x -= (float)y;
   }
 }
+// exponent of the least float32 above zero: no P vs is lost to a unit above it
+constexpr int LEAST_UNIT = -148;
 EDF_DEVICE f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // A wave's values in LDS, float16: a block for each 16 columns, of rows of 48 bytes (16 columns and padding), so that a
@@ -140,7 +143,7 @@ void paged_attn8_kernel(PagedArgs a) {
 #pragma unroll
   for (int dt = 0; dt < NDT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -INFINITY, lsum = 0.0f;
-  int ve = -100;  // o is in units of 2^(ve - 15), 2^ve the least power of two above every vs so far
+  int ve = LEAST_UNIT;  // o is in units of 2^(ve - 15): every P vs so far, at the present maximum, is below 2^ve
 
   // Page and head [num_blocks Hkv] of visible key n, or -1, and its row of the cache; one key a lane, repeated every KEYS
   // lanes.
@@ -227,7 +230,7 @@ void paged_attn8_kernel(PagedArgs a) {
     next = place_of(nb + 2 * STEP);
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    float mx = -INFINITY, vx = 0.0f;
+    float mx = -INFINITY;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       s[t] *= *(const f32x4*)(&sS[w][0][16 * t + 4 * g]) * qscale;
@@ -238,20 +241,27 @@ void paged_attn8_kernel(PagedArgs a) {
         for (int r = 0; r < 4; ++r) s[t][r] = mine & (1u << (16 * t + r)) ? s[t][r] : -INFINITY;
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        mx = fmaxf(mx, s[t][r]);
-        vx = fmaxf(vx, vs[t][r]);
-      }
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[t][r]);
     }
     mx = fmaxf(mx, __shfl_xor(mx, 16));
-    vx = fmaxf(vx, __shfl_xor(vx, 16));
     mx = fmaxf(mx, __shfl_xor(mx, 32));
-    vx = fmaxf(vx, __shfl_xor(vx, 32));
     const float mnew = fmaxf(m, mx);
     const float mns = mnew == -INFINITY ? 0.0f : mnew;
-    const int venew = vx > 0.0f ? max(ve, __builtin_amdgcn_frexp_expf(vx)) : ve;
+    float rs = 0.0f, wx = 0.0f, pv[4 * NT];  // pv: P vs
+#pragma unroll
+    for (int e = 0; e < 4 * NT; ++e) {
+      const float p = fast_exp2(s[e >> 2][e & 3] - mns);
+      rs += p;
+      pv[e] = p * vs[e >> 2][e & 3];
+      wx = fmaxf(wx, pv[e]);
+    }
+    wx = fmaxf(wx, __shfl_xor(wx, 16));
+    wx = fmaxf(wx, __shfl_xor(wx, 32));
+    // the unit falls with what the new maximum leaves of the old P vs
+    const int kept = ve + (int)ceilf(fmaxf(m - mnew, -1024.0f));
+    const int venew = max(max(kept, LEAST_UNIT), wx > 0.0f ? __builtin_amdgcn_frexp_expf(wx) : LEAST_UNIT);
     if (__any(mnew > m || venew > ve)) {
-      const float alpha = fast_exp2(m - mns), beta = ldexpf(alpha, ve - venew);
+      const float alpha = fast_exp2(m - mns), beta = fast_exp2(m - mns + (float)(ve - venew));
       lsum *= alpha;
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt)
@@ -260,14 +270,10 @@ void paged_attn8_kernel(PagedArgs a) {
     }
     m = mnew;
     ve = venew;
-    float rs = 0.0f;
     f16x4 pf[PP][NT];
 #pragma unroll
-    for (int e = 0; e < 4 * NT; ++e) {
-      const float p = fast_exp2(s[e >> 2][e & 3] - mns);
-      rs += p;
-      half_parts<PP>(p * ldexpf(vs[e >> 2][e & 3], 15 - ve), [&](int n, _Float16 y) { pf[n][e >> 2][e & 3] = y; });
-    }
+    for (int e = 0; e < 4 * NT; ++e)
+      half_parts<PP>(ldexpf(pv[e], 15 - ve), [&](int n, _Float16 y) { pf[n][e >> 2][e & 3] = y; });
     rs += __shfl_xor(rs, 16);
     lsum += rs + __shfl_xor(rs, 32);
 #pragma unroll

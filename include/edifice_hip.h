@@ -757,7 +757,8 @@ int edf_paged_attention(void* stream, const void* q, const void* k_cache, const 
  *   for, or, in a page that it begins, their codes.  A value that is not finite makes the scale NaN until the page is begun
  *   anew, and with it all that the page's head stands for.  No value is read back for a page that the call begins.
  * edf_paged_attention8: edf_paged_attention over such a cache; q and out in dtype.  The workspace is that of
- *   edf_paged_attention8_workspace_bytes().
+ *   edf_paged_attention8_workspace_bytes().  A key's probability times its v_scale is held to 2^-22 of itself and 2^-39 of the
+ *   query's largest.
  * edf_paged_cache_read: the first offsets[b + 1] - offsets[b] tokens of each request b as rows offsets[b] .. of k, v
  *   [num_kv_heads, total, d] in dtype, float32 or bf16 (offsets int32 [requests + 1], ascending); from a cache of dtype with
  *   code EDF_NO_CODE (the scales are not read).  Rows outside the texts, and tokens past the table's width or of pages
