@@ -11,9 +11,9 @@
 // range.  A value that is not finite makes the scale NaN, and with it what the page's head stands for.
 //
 // One group of threads (a wave, or four for pages of many elements) takes the tokens of one page, for keys or values of
-// one head: they are consecutive, here [tokens][d] and in the page, so the group reads them once, finds their largest and
-// writes the codes from the same registers.  Where a page's tokens begin is seen from the slots: a slot that does not
-// follow its predecessor's, or opens a page.  Bound by memory: 2 or 4 bytes read and one written a value; 8x2048x8x128 bf16,
+// one head: they follow one another in k, [tokens][d], so the group reads them once, finds their largest and, where their
+// slots follow one another too, writes the codes from the same registers; to slots in any other order it goes token by
+// token.  Where a page's tokens begin is seen from the slots: one whose predecessor's lies in another page.  Bound by memory: 2 or 4 bytes read and one written a value; 8x2048x8x128 bf16,
 // three quarters of them real, 21.4 us to int8 and 19.1 to e4m3 (3.5 and 3.9 TB/s): the slots, the values and the scale are
 // three loads that wait for one another.
 //
@@ -79,12 +79,12 @@ EDF_DEVICE float least_scale(float amax) {
 
 // G threads a run (64: the waves of a workgroup take a run each), which keep REG pieces of 8 values each between the maximum
 // and the codes and read what is more again; VEC: d a multiple of 8 and everything aligned to 16.  Four workgroups a CU: six
-// are no faster, and eight spill (float32 in eight pieces spills 3 registers at four).
+// are no faster, and eight spill.
 template <typename T, int C, int G, int REG, bool VEC>
 __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
   __shared__ float smax[4];
   const int lane = threadIdx.x & 63, tid = G == 64 ? lane : threadIdx.x;
-  const long unit = G == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const long unit = G == 64 ? (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
   const int which = (int)(unit & 1);
   const long rest = unit >> 1, bh = rest / a.nseg;
   const int h = (int)(bh % a.Hkv);
@@ -96,24 +96,29 @@ __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
     return s >= 0 && s < a.num_slots ? s : -1;
   };
   const int mine = slot_at(t0 + lane), before = slot_at(t0 + lane - 1);
+  const int mine0 = max(mine, 0) / a.block * a.block;  // the first slot of this lane's page (-1 lies in none)
   unsigned long long starts =
-      __ballot(lane < a.seg && mine >= 0 && !(before >= 0 && mine == before + 1 && mine % a.block != 0));
+      __ballot(lane < a.seg && mine >= 0 && !(before >= 0 && (unsigned)(before - mine0) < (unsigned)a.block));
   float* scales = a.scale[which];
   unsigned char* cache = (unsigned char*)a.cache[which];
   while (starts) {
     const int e = __builtin_ctzll(starts);
     starts &= starts - 1;
-    const int slot0 = __shfl(mine, e), page = slot0 / a.block, off = slot0 - page * a.block;
-    // the run: consecutive slots, to the page's end at most
+    const int slot0 = __builtin_amdgcn_readlane(mine, e), first = __builtin_amdgcn_readlane(mine0, e), page = first / a.block, off = slot0 - first;
+    // the run: tokens whose slots lie in the page
     int n = 0;
-    for (int base = 0;; base += 64) {  // lanes hold the slots of tokens t0 + base + lane
+    bool follow = true, fresh = false;  // the slots follow one another; the page's first one is among them
+    for (int base = 0;; base += 64) {   // lanes hold the slots of tokens t0 + base + lane
       const int v = base == 0 ? mine : slot_at(t0 + base + lane), pos = e + n - base;
-      const unsigned long long ends = ~(__ballot((unsigned)v == (unsigned)slot0 + base + lane - e) >> pos);
+      const unsigned long long ends = ~(__ballot(v >= 0 && (unsigned)(v - first) < (unsigned)a.block) >> pos);
       const int ones = ends ? __builtin_ctzll(ends) : 64;
+      const unsigned long long run = ones < 64 ? (1ull << ones) - 1 : ~0ull;
+      follow &= (~(__ballot((unsigned)v == (unsigned)slot0 + base + lane - e) >> pos) & run) == 0;
+      fresh |= (__ballot(v == first) >> pos & run) != 0;
       n += ones;
-      if (ones < 64 - pos || n >= a.block - off) break;
+      if (ones < 64 - pos || n >= a.block) break;
     }
-    n = min(n, a.block - off);
+    n = min(n, a.block);
     const int count = n * a.d;
     const T* x = (const T*)a.x[which] + (bh * a.T + t0 + e) * a.d;
     const long place = (long)page * a.Hkv + h;
@@ -152,18 +157,48 @@ __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
     }
     const float need = least_scale<C>(amax);
     float s = need, shrink = 1.0f;  // what the page's other codes are multiplied by
-    if (off != 0 && !(old <= 0.0f)) {
+    if (!fresh && !(old <= 0.0f)) {
       int e0, e1;
       const float m0 = frexpf(old, &e0), m1 = frexpf(need, &e1);
       const int k = need > 0.0f ? max(0, e1 - e0 + (m1 > m0)) : 0;
       s = old + need == old + need ? ldexpf(old, k) : __builtin_nanf("");  // NaN stays
       if (s == s) shrink = ldexpf(1.0f, -k);
-    } else if (off != 0) {
+    } else if (!fresh) {
       shrink = 0.0f;  // a page of zeros so far
     }
     if (tid == 0) scales[place] = s;
     const float inv = s > 0.0f ? 1.0f / s : 0.0f;
     unsigned char* codes = cache + place * a.block * a.d;
+    const int W = VEC ? 4 : 1, whole = a.block * a.d;
+    auto lower = [&](int p) {  // the codes from p on as the page's new scale has them
+      unsigned c = 0;
+      if (shrink != 0.0f) {
+        float f[4];
+        Codes<C>::unpack4(VEC ? *(const unsigned*)(codes + p) : codes[p], f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] *= shrink;
+        c = Codes<C>::pack4(f);
+      }
+      if constexpr (VEC) *(unsigned*)(codes + p) = c;
+      else codes[p] = (unsigned char)c;
+    };
+    if (!follow) {  // the page's codes first, the new ones over them
+      if (shrink != 1.0f)
+        for (int p = W * tid; p < whole; p += W * G) lower(p);
+      __threadfence();
+      if constexpr (G == 256) __syncthreads();
+      for (int p = W * tid; p < count; p += W * G) {
+        const int t = p / a.d, o = slots[t0 + e + t] - first;
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = i < W && inv > 0.0f ? to_f32(x[p + (i < W ? i : 0)]) * inv : 0.0f;
+        unsigned char* to = codes + (long)o * a.d + (p - t * a.d);
+        const unsigned c = Codes<C>::pack4(y);
+        if constexpr (VEC) *(unsigned*)to = c;
+        else *to = (unsigned char)c;
+      }
+      continue;
+    }
     auto store = [&](const Piece<T, VEC>& f, int p) {
       float y[8];
 #pragma unroll
@@ -188,22 +223,9 @@ __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
       f.load(x, p, count - p);
       store(f, p);
     }
-    if (shrink != 1.0f) {  // the slots of the page that this run does not write
-      const int first = off * a.d, whole = a.block * a.d, W = VEC ? 4 : 1;
-      for (int p = W * tid; p < whole; p += W * G) {
-        if (p >= first && p < first + count) continue;
-        unsigned c = 0;
-        if (shrink != 0.0f) {
-          float f[4];
-          Codes<C>::unpack4(VEC ? *(const unsigned*)(codes + p) : codes[p], f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] *= shrink;
-          c = Codes<C>::pack4(f);
-        }
-        if constexpr (VEC) *(unsigned*)(codes + p) = c;
-        else codes[p] = (unsigned char)c;
-      }
-    }
+    if (shrink != 1.0f)  // the slots of the page that this run does not write
+      for (int p = W * tid; p < whole; p += W * G)
+        if (p < off * a.d || p >= off * a.d + count) lower(p);
   }
 }
 

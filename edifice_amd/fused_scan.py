@@ -1359,8 +1359,8 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_c
     The cache is of k's type, or of int8 or float8_e4m3fn with k_scale, v_scale float32 [num_blocks, Hkv]: an 8-bit number
     stands for that many units of its page and head's scale.  The tokens of a page then share a scale that holds their
     largest value (int8: a 127th of it; e4m3: a power of two); a page whose first slot is written starts anew, any other
-    keeps its scale, or doubles it until it holds the new tokens, its numbers halved and rounded.  The slots of one page
-    have to be those of consecutive tokens of one row, in ascending order.  A value that is not finite makes its page's head
+    keeps its scale, or doubles it until it holds the new tokens, its numbers halved and rounded.  The tokens of one page
+    have to be consecutive ones of one row (their slots in it may be any, in any order).  A value that is not finite makes its page's head
     NaN until that page starts anew.  Scales and numbers of pages that hold nothing may be anything finite (zeros)."""
     if _wants_grad(k, v, k_cache, v_cache, k_scale, v_scale):
         raise EdificeHipError("paged_cache_write has no derivative: call it under torch.no_grad() and without tangents")

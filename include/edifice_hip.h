@@ -748,9 +748,9 @@ int edf_paged_attention(void* stream, const void* q, const void* k_cache, const 
 /* The same over a cache of 8-bit numbers, code EDF_INT8 or EDF_E4M3: k_cache, v_cache hold a byte a value, in units of
  * k_scale, v_scale, float32 [num_blocks, num_kv_heads], one for the tokens of a page and head.
  *
- * edf_paged_cache_write8: rows of k, v in dtype.  The slots of one page have to be those of tokens that follow one another
- *   in one row of k, in ascending order, as edf_paged_extend gives them.  The written tokens of a page and head need
- *   a scale n = max |x| / 127 (int8: times the float32 nearest to 1 / 127) or the least power of two from max |x| / 448 on
+ * edf_paged_cache_write8: rows of k, v in dtype.  The tokens that go into one page have to follow one another in one row of
+ *   k, with no other token between them (their slots may be any of the page's, in any order): a page of two rows, or of
+ *   tokens apart, would have its scale written twice, in no order.  The written tokens of a page and head need a scale n = max |x| / 127 (int8: times the float32 nearest to 1 / 127) or the least power of two from max |x| / 448 on
  *   (e4m3), at least 2^-100, or 0 where every x is 0.  A page whose first slot is written takes s = n; any other keeps its
  *   scale, doubled until it is n at least, and its codes, halved as often and rounded (a scale of 0 or less: s = n, codes
  *   0).  A value is held as x (1 / s), rounded to even; slots of the page that the call does not write keep what they stand
