@@ -14,7 +14,8 @@ typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 
-// C: the code's kind.  unpack4: four codes as float32, exactly; pack4: four values to codes, ties to even, saturated.
+// C: the code's kind.  unpack4: four codes as float32, exactly; pack4: four values to codes, ties to even, whole
+// numbers saturated, e4m3 for values up to 448 (what a scale leaves).
 template <int C> struct Codes;
 template <> struct Codes<EDF_INT8> {
   EDF_DEVICE static void unpack4(unsigned c, float* x) {

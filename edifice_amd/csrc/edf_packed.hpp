@@ -187,8 +187,8 @@ struct BlockTiles {
 // they and the tiles' last, shorter ones are as many as the GPU's places (a chunk more than those waits for a whole one to
 // end), numbered from tile to tile.  Item `item` of a head group's; threads look at two tiles of 2^ms rows each, of which
 // there are fewer than 512; count(first, n, m): the tiles that the one from row `first` on walks.
-// Queries uncut, and cut: 8 texts of up to 64 queries on 28563 keys, 32(8)x128, 80 and 46 us; 500 queries on 30000 keys 224
-// and 163.  Keys (forward and backward) with an equal number of shares of each block's query tiles, and with such chunks: 8
+// Queries uncut, and cut: 8 texts of up to 64 queries on 28563 keys, 32(8)x128, 80 and 44 us; 247 queries on 30000 keys 550
+// and 147.  Keys (forward and backward) with an equal number of shares of each block's query tiles, and with such chunks: 8
 // texts to 2000, 8(4)x128, 244 and 175 us, one of 4000, 16(4)x128, 548 and 420, 4 to 1500, 32(8)x128, 262 and 191, 12 to 4096,
 // 8(1)x128, 1189 and 700; float32 8 to 2000, 8(4)x64, 636 and 450.  As many chunks as 576 to 1536 places are slower at most of
 // these, and a search for the shortest len costs 1 to 4 us more than it saves.

@@ -3,10 +3,10 @@
 // model's type:
 //   s_j = (q . c_j) ks / sqrt(d),  o = sum_j softmax_j(s) vs c'_j,   codes c, c', scales ks, vs of key j's page.
 //
-// Half the bytes of a bf16 cache, and bound by them: 64 requests, 32(8)x128, 115000 tokens in pages of 16, int8: 52 us (4.56
-// TB/s; a copy reaches 4.89) and 4.2 for the join; 3 requests, 16(2)x128, 237000 tokens in pages of 64, e4m3: 27 (4.4 TB/s)
-// and 5.8 for the join of up to 255 chunks.  Without its arithmetic the first took 66 us a pass where the whole took
-// 70.  The codes are exact in float16, so the matrix products run on float16 operands and the scales multiply scores and
+// Half the bytes of a bf16 cache, and bound by them: 64 requests, 32(8)x128, 115000 tokens in pages of 16, int8: 51 us (4.6
+// TB/s; a copy reaches 4.89) and 4.0 for the join; 3 requests, 16(2)x128, 237000 tokens in pages of 64, e4m3: 27 (4.4 TB/s)
+// and 5.8 for the join of up to 255 chunks.  Float32 queries, which go through the first product in two parts, take 8% more
+// (64 requests to 4096 68.6 and 74.0 us a pass).  The codes are exact in float16, so the matrix products run on float16 operands and the scales multiply scores and
 // probabilities, one of each a key; no dequantised value is formed.
 //   Keys go from memory to the matrix operand: a lane's 16 codes of each 64 of a row are 16 columns of the contraction,
 //   and the query has the same order.  A tile's rows are read whole by four lanes each.

@@ -13,13 +13,13 @@
 // One group of threads (a wave, or four for pages of many elements) takes the tokens of one page, for keys or values of
 // one head: they follow one another in k, [tokens][d], so the group reads them once, finds their largest and, where their
 // slots follow one another too, writes the codes from the same registers; to slots in any other order it goes token by
-// token.  Where a page's tokens begin is seen from the slots: one whose predecessor's lies in another page.  Bound by memory: 2 or 4 bytes read and one written a value; 8x2048x8x128 bf16,
-// three quarters of them real, 21.4 us to int8 and 19.1 to e4m3 (3.5 and 3.9 TB/s): the slots, the values and the scale are
-// three loads that wait for one another.
+// token.  Where a page's tokens begin is seen from the slots: one whose predecessor's lies in another page.  Bound by memory: 2 or 4 bytes read and one written a value; 8x2048x8x128 in pages of
+// 16, three quarters of them real, bf16 to int8 20.1 us, to e4m3 17.5 (3.7 and 4.4 TB/s), float32 to int8 29.5 (4.3): the
+// slots, the values and the scale are three loads that wait for one another.
 //
 // Read.  A workgroup takes 64 rows of the packed texts of one head; each row's page and scales are looked up once (the
-// text by binary search over the offsets), then all threads copy.  Bound by memory: 28563 tokens of 8x128 e4m3 to bf16
-// 42.6 us (5.2 TB/s), int8 to float32 86 (4.2).
+// text by binary search over the offsets), then all threads copy.  Bound by memory: 35858 tokens of 8x128 e4m3 to bf16
+// 42.6 us (5.2 TB/s), int8 to float32 86 (4.2); a cache of the result's type, bf16 48 and float32 121.
 #include <math.h>
 #include <stdint.h>
 
@@ -232,8 +232,8 @@ __global__ __launch_bounds__(256, 4) void paged_write8_kernel(Write8Args a) {
 template <typename T, int C>
 int launch_write8(hipStream_t s, Write8Args a, bool vec) {
   // a wave keeps up to 8 pieces a lane; the runs of pages that hold more take four waves, but for single tokens: few large
-  // pages are then not left to few waves (8x2048x8x128 in pages of 128, where there are enough of them: 29.7 us, by waves
-  // alone 31.1)
+  // pages are then not left to few waves (8x2048x8x128 in pages of 128, where there are enough of them: float32 41.4 us, by
+  // waves alone 43.1; bf16 33.9 and 33.7)
   const long runs = 2L * a.B * a.Hkv * a.nseg, page = (long)a.block * a.d;
   const bool wide = page > 8L * 64 * 8 && a.T > 1;
   const long grid = wide ? runs : (runs + 3) / 4;
